@@ -288,6 +288,70 @@ int pnfx_flash_bwd_noalloc(const void* q, int64_t qsb, int64_t qsh, int64_t qsn,
                            float scale, float gamma, int has_gamma, int causal, int dtype,
                            void* stream);
 
+/*
+ * The gated feed-forward block, y = (act(x Wg^T) * (x Wu^T)) Wd^T, and its backward pass.  No counterpart in
+ * the reference.
+ *   x      : [T, D], row stride x_rs;   y : contiguous [T, Do]
+ *   w_in   : [2 F, D], row stride win_rs: the F rows of Wg, then the F rows of Wu
+ *   w_down : [Do, F], row stride wd_rs
+ * keep: what the forward leaves for the backward pass in `gu` (16-byte aligned; Fp: F rounded up to a
+ * multiple of 8, the columns past F are zero):
+ *   PNFX_KEEP_NONE  nothing (gu and scales may be null)
+ *   PNFX_KEEP_FULL  fp32 operands: [T][2][Fp] fp32, g = x Wg^T and u = x Wu^T (scales may be null).  bf16: [T][2][Fp]
+ *                   in half precision, value / s, and in `scales` [T][2][ceil(F / 32)] bytes, of each block of 32
+ *                   columns the exponent + 127 of a power of two s for which its finite values are below 2^15 s
+ *   PNFX_KEEP_E4M3  (bf16 operands) the same in [T][2][Fp] bytes: value / s in e4m3 with the smallest s for which
+ *                   the finite values are at most 448 s (an infinity or a NaN becomes NaN)
+ * The backward takes gu and scales as the forward with the same keep wrote them and writes the gradients that
+ * are not null: dx [T, D], dw_in [2 F, D], dw_down [Do, F], contiguous, 16-byte aligned.
+ * Operands whose columns are not a multiple of 8, or whose base or rows are not 16-byte aligned, are copied
+ * into the workspace first.  T < 2^29; D, F, Do <= 2^18.  Workspace: 16-byte aligned, as large as
+ * pnfx_ffn_*_workspace_size says, with `copies` not 0 where an operand has to be copied (F not a multiple of 8,
+ * too).  Bitwise repeatable.
+ */
+#define PNFX_ACT_SILU 0
+#define PNFX_ACT_GELU 1 /* g Phi(g), the error-function form */
+#define PNFX_KEEP_NONE 0
+#define PNFX_KEEP_FULL 1
+#define PNFX_KEEP_E4M3 2
+int64_t pnfx_ffn_fwd_workspace_size(int64_t T, int64_t D, int64_t F, int64_t Do, int copies, int dtype);
+int pnfx_ffn_fwd(const void* x, int64_t x_rs, const void* w_in, int64_t win_rs, const void* w_down,
+                 int64_t wd_rs, void* y, void* gu, uint8_t* scales, int64_t T, int64_t D, int64_t F,
+                 int64_t Do, int act, int keep, int dtype, void* workspace, int64_t workspace_bytes,
+                 void* stream);
+int64_t pnfx_ffn_bwd_workspace_size(int64_t T, int64_t D, int64_t F, int64_t Do, int copies, int dtype);
+int pnfx_ffn_bwd(const void* dy, int64_t dy_rs, const void* x, int64_t x_rs, const void* w_in,
+                 int64_t win_rs, const void* w_down, int64_t wd_rs, const void* gu, const uint8_t* scales,
+                 void* dx, void* dw_in, void* dw_down, int64_t T, int64_t D, int64_t F, int64_t Do, int act,
+                 int keep, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Softmax cross entropy of the logits x W^T against target tokens, without the logits, and its gradients.  No
+ * counterpart in the reference (its LM takes torch's, experiments/exp4_wikitext2_lm.py:334-348).
+ *   x      : [T, D], row stride x_rs;   w : [V, D], row stride w_rs
+ *   target : int64 [T].  Rows whose target is ignore_index have loss 0 and gradient 0 whatever they hold and
+ *            reach no other result; a row with any other target outside 0 .. V - 1 has a NaN loss and NaN gradients
+ *   loss   : fp32 [T] (PNFX_REDUCE_NONE) or one value: the sum, or the mean over the rows that are not
+ *            ignored (NaN if there is none)
+ *   loss_rows, lse : fp32 [T], each row's loss and log-sum-exp (0 in ignored rows), for the backward
+ * The backward takes dloss like loss and writes the gradients that are not null: dx [T, D], dw [V, D], contiguous,
+ * 16-byte aligned.  T, V <= 2^24; D <= 2^18.  Workspace as above (`copies` not 0 where D is not a multiple of
+ * 8 or w's base or rows are not 16-byte aligned).  Bitwise repeatable.
+ */
+#define PNFX_REDUCE_NONE 0
+#define PNFX_REDUCE_SUM 1
+#define PNFX_REDUCE_MEAN 2
+int64_t pnfx_xent_fwd_workspace_size(int64_t T, int64_t D, int64_t V, int copies, int dtype);
+int pnfx_xent_fwd(const void* x, int64_t x_rs, const void* w, int64_t w_rs, const int64_t* target,
+                  int64_t ignore_index, float* loss, float* loss_rows, float* lse, int64_t T, int64_t D,
+                  int64_t V, int reduction, int dtype, void* workspace, int64_t workspace_bytes,
+                  void* stream);
+int64_t pnfx_xent_bwd_workspace_size(int64_t T, int64_t D, int64_t V, int copies, int dtype);
+int pnfx_xent_bwd(const float* dloss, const void* x, int64_t x_rs, const void* w, int64_t w_rs,
+                  const int64_t* target, int64_t ignore_index, const float* loss_rows, const float* lse,
+                  void* dx, void* dw, int64_t T, int64_t D, int64_t V, int reduction, int dtype,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

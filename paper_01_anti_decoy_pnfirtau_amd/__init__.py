@@ -28,6 +28,8 @@ __all__ = [
     "flash_pn_fir_tau_attention",
     "triton_causal_fir",
     "triton_pn_fir_tau_scores",
+    "gated_ffn",
+    "linear_cross_entropy",
 ]
 
 
@@ -38,4 +40,8 @@ def __getattr__(name):
         from . import hip_pnfirtau
 
         return getattr(hip_pnfirtau, name)
+    if name in ("gated_ffn", "linear_cross_entropy"):
+        from . import hip_lm
+
+        return getattr(hip_lm, name)
     raise AttributeError(name)

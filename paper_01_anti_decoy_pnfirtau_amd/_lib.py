@@ -14,6 +14,9 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libpnfx.so"
 ABI_VERSION = 3
 PNFX_F32 = 0
 PNFX_BF16 = 1
+PNFX_ACT = {"silu": 0, "gelu": 1}
+PNFX_KEEP = {"none": 0, "full": 1, "e4m3": 2}
+PNFX_REDUCE = {"none": 0, "sum": 1, "mean": 2}
 PNFX_BWD_PREPARE, PNFX_BWD_DKDV, PNFX_BWD_DQ, PNFX_BWD_ALL = 1, 2, 4, 7
 PNFX_NOALLOC_SCRATCH_BYTES = 128 << 20
 
@@ -65,6 +68,16 @@ def _declare(lib: ctypes.CDLL) -> None:
     sig["pnfx_flash_bwd_stages"] = ([i32] + sig["pnfx_flash_bwd"][0], i32)
     bwd = sig["pnfx_flash_bwd"][0]  # pnfx_flash_bwd without (workspace, workspace_bytes)
     sig["pnfx_flash_bwd_noalloc"] = (bwd[:37] + bwd[39:], i32)
+    for name in ("pnfx_ffn_fwd_workspace_size", "pnfx_ffn_bwd_workspace_size"):
+        sig[name] = ([i64] * 4 + [i32, i32], i64)
+    for name in ("pnfx_xent_fwd_workspace_size", "pnfx_xent_bwd_workspace_size"):
+        sig[name] = ([i64] * 3 + [i32, i32], i64)
+    sig["pnfx_ffn_fwd"] = ([vp, i64] * 3 + [vp] * 3 + [i64] * 4 + [i32] * 3 + [vp, i64, vp], i32)
+    sig["pnfx_ffn_bwd"] = ([vp, i64] * 4 + [vp] * 5 + [i64] * 4 + [i32] * 3 + [vp, i64, vp], i32)
+    sig["pnfx_xent_fwd"] = ([vp, i64] * 2 + [vp, i64, vp, vp, vp] + [i64] * 3 + [i32] * 2
+                            + [vp, i64, vp], i32)
+    sig["pnfx_xent_bwd"] = ([vp] + [vp, i64] * 2 + [vp, i64, vp, vp, vp, vp] + [i64] * 3 + [i32] * 2
+                            + [vp, i64, vp], i32)
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
         fn.argtypes = args
@@ -103,4 +116,7 @@ def exported_symbols() -> list[str]:
         "pnfx_flash_bwd_noalloc", "pnfx_flash_fwd_any", "pnfx_flash_bwd_any",
         "pnfx_sum_f64_workspace_size", "pnfx_sum_f64",
         "pnfx_linear_wgrad_workspace_size", "pnfx_linear_wgrad", "pnfx_fir_bwd_into",
+        "pnfx_ffn_fwd_workspace_size", "pnfx_ffn_fwd", "pnfx_ffn_bwd_workspace_size", "pnfx_ffn_bwd",
+        "pnfx_xent_fwd_workspace_size", "pnfx_xent_fwd", "pnfx_xent_bwd_workspace_size",
+        "pnfx_xent_bwd",
     ]

@@ -1,0 +1,633 @@
+// The gated feed-forward block, y = h Wd^T with h = act(g) u, g = x Wg^T, u = x Wu^T, and its backward pass.
+//
+// Forward, two kernels: one computes both projections of a tile of rows (their weights' rows alternate in its
+// second operand, 32 of each, so that a lane holds g and u of the same eight columns), applies the activation
+// and the product in registers and writes h and, for the backward pass, g and u; the other is h Wd^T.
+//
+// Backward: dh = dy Wd is formed tile by tile and never written: its epilogue reads g and u, and writes
+// dg = dh u act'(g), du = dh act(g) and h again; then dx = [dg du] [Wg; Wu], d[Wg; Wu] = [dg du]^T x and
+// dWd = dy^T h are plain products (product.hip).
+//
+// bf16 operands: g, u and dh are fp32 sums; h, dg and du are rounded to bf16 once, because they are operands of
+// the next bf16 product (2^-8 of each at most, as y itself is rounded).  What is kept of g and u is in blocks of
+// 32 columns of a row that share a power of two s: 16 bits (value / s in half precision, 2^-11 of the value; in
+// bf16 their rounding was half of the gradients' error, 3.4e-3 of the norm against 2.4e-3), or 8 bits (value / s in
+// e4m3, with the smallest s for which |value| <= 448 s).  The backward pass computes with what they stand for.
+//
+// Up to 64 rows (single tokens of a batch) the time is that of reading the weights once, and a 128-row tile
+// would leave most of the chip idle: ffn_rows_kernel gives 16 weight rows to a workgroup, whose waves split
+// k among them and read the weights from global memory into registers.
+#include <algorithm>
+
+#include "product.h"
+
+namespace pnfx {
+namespace {
+
+template <int ACT>
+__device__ __forceinline__ float act_of(float g) {
+  if constexpr (ACT == PNFX_ACT_SILU) return g * __builtin_amdgcn_rcpf(1.f + __expf(-g));
+  return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
+}
+// act(g) and act'(g)
+template <int ACT>
+__device__ __forceinline__ void act_both(float g, float& a, float& d) {
+  if constexpr (ACT == PNFX_ACT_SILU) {
+    const float p = __builtin_amdgcn_rcpf(1.f + __expf(-g));
+    a = g * p;
+    d = p * (1.f + g * (1.f - p));
+  } else {
+    const float p = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+    a = g * p;
+    d = p + g * 0.39894228040143268f * __expf(-0.5f * g * g);
+  }
+}
+
+// -------------------------------------------------------------------- blocks of 32
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+// The largest finite |v| of the lane's eight values and the other three lanes' of the row's 32.
+__device__ __forceinline__ float block_top(const float* v) {
+  float t = 0.f;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    const float a = fabsf(v[r]);
+    t = fmaxf(t, a < INFINITY ? a : 0.f);
+  }
+  t = fmaxf(t, __shfl_xor(t, 16, 64));
+  return fmaxf(t, __shfl_xor(t, 32, 64));
+}
+// Exponent of the power of two that brings a block into half precision's range: values below 2^15.
+__device__ __forceinline__ int half_exp(float top) { return max((int)(__float_as_uint(top) >> 23) - 127 - 14, -126); }
+// Exponent of the smallest power of two s with top <= 448 s (448 = 1.75 2^8), at least -126.
+__device__ __forceinline__ int scale_exp(float top) {
+  const unsigned b = __float_as_uint(top);
+  const int e = (int)(b >> 23) - 127 - 8 + ((b & 0x7fffff) > 0x600000);
+  return max(e, -126);
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
+// Four values over s as e4m3.
+__device__ __forceinline__ uint32_t pack_e4m3(const float* v, float inv) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, w, true);
+}
+__device__ __forceinline__ void unpack_e4m3(uint32_t w, float s, float* v) {
+  v[0] = __builtin_amdgcn_cvt_f32_fp8((int)w, 0) * s;
+  v[1] = __builtin_amdgcn_cvt_f32_fp8((int)w, 1) * s;
+  v[2] = __builtin_amdgcn_cvt_f32_fp8((int)w, 2) * s;
+  v[3] = __builtin_amdgcn_cvt_f32_fp8((int)w, 3) * s;
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float* v) {
+  if constexpr (sizeof(T) == 2) {
+    *reinterpret_cast<bf16x8*>(p) = pack8(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
+  } else {
+    *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4f(T* p, const float* v) {
+  if constexpr (sizeof(T) == 2) *reinterpret_cast<bf16x4*>(p) = bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
+  else *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+}
+template <typename T>
+__device__ __forceinline__ void load4f(const T* p, float* v) {
+  if constexpr (sizeof(T) == 2) {
+    const bf16x4 b = *reinterpret_cast<const bf16x4*>(p);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = (float)b[r];
+  } else {
+    const f32x4 b = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = b[r];
+  }
+}
+
+// Fp: F rounded up to a multiple of 8, the columns of h, of either half of g | u and of either half of dg | du;
+// those past F are zero.
+struct GluArgs {
+  const void* x;    // [T][ldx], or dy
+  const void* wg;   // [F][ldw], or Wd [Do][ldw]
+  const void* wu;
+  void* h;          // [T][Fp]
+  void* gu;         // [T][2 Fp]: fp32, or half precision or bytes in blocks; null: not kept
+  uint8_t* scales;  // [T][2 nb]: exponent + 127 of each block's power of two
+  void* dgu;        // [T][2 Fp]
+  int64_t ldx, ldw, K;
+  int T, F, Fp, nb, tm, tn;
+  int keep;
+};
+
+template <typename T, int ACT, class C>
+__global__ __launch_bounds__(threads_of<C>, 2) void glu_fwd_kernel(GluArgs a) {
+  typedef Product<T, ROW, PAIR, C> P;
+  extern __shared__ __align__(16) char sm[];
+  int tm, tn;
+  tile_of(blockIdx.x, a.tm, a.tn, tm, tn);
+  const int m0 = tm * C::TM, f0 = tn * (C::TN / 2);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  typename P::StageA sa;
+  typename P::StageB sb;
+  sa.init(static_cast<const T*>(a.x) + m0 * a.ldx, a.ldx, a.T - m0, a.K, threadIdx.x);
+  sb.init(static_cast<const T*>(a.wg) + f0 * a.ldw, a.ldw, a.F - f0, a.K, threadIdx.x,
+          static_cast<const T*>(a.wu) + f0 * a.ldw);
+  f32x4 acc[P::MI][P::NJ] = {};
+  P::run(sa, sb, (int)((a.K + k_step<T> - 1) / k_step<T>), reinterpret_cast<T*>(sm), wave, lane, acc);
+  const int wm = wave / C::WN * P::MI, wn = wave % C::WN * P::NJ, ag = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < P::MI; ++i) {
+    const int m = m0 + stage_row<ROW>(wm + i, lane & 15);
+#pragma unroll
+    for (int s = 0; s < P::NJ / 4; ++s) {
+      const int fb = f0 + 32 * (wn / 4 + s), f = fb + 8 * ag;  // the 32 columns' first, the lane's first of 8
+      float g[8], u[8], h[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        g[r] = acc[i][4 * s + (r >> 2)][r & 3];
+        u[r] = acc[i][4 * s + 2 + (r >> 2)][r & 3];
+        h[r] = act_of<ACT>(g[r]) * u[r];
+      }
+      const bool in = m < a.T && f < a.Fp;
+      if (in) store8(static_cast<T*>(a.h) + (int64_t)m * a.Fp + f, h);
+      if (a.keep == PNFX_KEEP_NONE) continue;
+      const int64_t at = (int64_t)m * 2 * a.Fp + f;
+      if constexpr (sizeof(T) == 4) {
+        if (in) {
+          store8(static_cast<float*>(a.gu) + at, g);
+          store8(static_cast<float*>(a.gu) + at + a.Fp, u);
+        }
+      } else {
+        // columns past F are zero and change no maximum
+        const float tg = block_top(g), tu = block_top(u);
+        const bool half = a.keep == PNFX_KEEP_FULL;
+        const int eg = half ? half_exp(tg) : scale_exp(tg), eu = half ? half_exp(tu) : scale_exp(tu);
+        const float ig = pow2(-eg), iu = pow2(-eu);
+        if (!in) continue;
+        if (half) {
+          f16x8 hg, hu;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            hg[r] = (_Float16)(g[r] * ig);
+            hu[r] = (_Float16)(u[r] * iu);
+          }
+          _Float16* gu = static_cast<_Float16*>(a.gu) + at;
+          *reinterpret_cast<f16x8*>(gu) = hg;
+          *reinterpret_cast<f16x8*>(gu + a.Fp) = hu;
+        } else {
+          uint8_t* gu = static_cast<uint8_t*>(a.gu) + at;
+          *reinterpret_cast<uint2*>(gu) = uint2{pack_e4m3(g, ig), pack_e4m3(g + 4, ig)};
+          *reinterpret_cast<uint2*>(gu + a.Fp) = uint2{pack_e4m3(u, iu), pack_e4m3(u + 4, iu)};
+        }
+        if (ag == 0) {
+          uint8_t* sc = a.scales + (int64_t)m * 2 * a.nb + fb / 32;
+          sc[0] = (uint8_t)(eg + 127);
+          sc[a.nb] = (uint8_t)(eu + 127);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int ACT, class C>
+__global__ __launch_bounds__(threads_of<C>, 2) void glu_bwd_kernel(GluArgs a) {
+  typedef Product<T, ROW, COL, C> P;
+  extern __shared__ __align__(16) char sm[];
+  int tm, tn;
+  tile_of(blockIdx.x, a.tm, a.tn, tm, tn);
+  const int m0 = tm * C::TM, n0 = tn * C::TN;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  typename P::StageA sa;
+  typename P::StageB sb;
+  sa.init(static_cast<const T*>(a.x) + m0 * a.ldx, a.ldx, a.T - m0, a.K, threadIdx.x);
+  sb.init(static_cast<const T*>(a.wg) + n0, a.ldw, a.F - n0, a.K, threadIdx.x);
+  f32x4 acc[P::MI][P::NJ] = {};
+  P::run(sa, sb, (int)((a.K + k_step<T> - 1) / k_step<T>), reinterpret_cast<T*>(sm), wave, lane, acc);
+  const int wm = wave / C::WN * P::MI, wn = wave % C::WN * P::NJ;
+#pragma unroll
+  for (int i = 0; i < P::MI; ++i) {
+    const int m = m0 + stage_row<ROW>(wm + i, lane & 15);
+    if (m >= a.T) continue;
+#pragma unroll
+    for (int j = 0; j < P::NJ; ++j) {
+      const int f = n0 + stage_row<COL>(wn + j, 4 * (lane >> 4));
+      if (f >= a.Fp) continue;
+      const int64_t at = (int64_t)m * 2 * a.Fp + f;
+      float g[4], u[4], dg[4], du[4], h[4];
+      if constexpr (sizeof(T) == 4) {
+        load4f(static_cast<const float*>(a.gu) + at, g);
+        load4f(static_cast<const float*>(a.gu) + at + a.Fp, u);
+      } else {
+        const uint8_t* sc = a.scales + (int64_t)m * 2 * a.nb + f / 32;
+        const float sg = pow2((int)sc[0] - 127), su = pow2((int)sc[a.nb] - 127);
+        if (a.keep == PNFX_KEEP_FULL) {
+          const _Float16* gu = static_cast<const _Float16*>(a.gu) + at;
+          const f16x4 hg = *reinterpret_cast<const f16x4*>(gu), hu = *reinterpret_cast<const f16x4*>(gu + a.Fp);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            g[r] = (float)hg[r] * sg;
+            u[r] = (float)hu[r] * su;
+          }
+        } else {
+          const uint8_t* gu = static_cast<const uint8_t*>(a.gu) + at;
+          unpack_e4m3(*reinterpret_cast<const uint32_t*>(gu), sg, g);
+          unpack_e4m3(*reinterpret_cast<const uint32_t*>(gu + a.Fp), su, u);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float s, d;
+        act_both<ACT>(g[r], s, d);
+        // columns between F and Fp are of zero weights: zero for any dy, an infinite one too
+        const float dh = f + r < a.F ? acc[i][j][r] : 0.f;
+        dg[r] = dh * u[r] * d;
+        du[r] = dh * s;
+        h[r] = s * u[r];
+      }
+      store4f(static_cast<T*>(a.dgu) + at, dg);
+      store4f(static_cast<T*>(a.dgu) + at + a.Fp, du);
+      store4f(static_cast<T*>(a.h) + (int64_t)m * a.Fp + f, h);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------ few rows
+constexpr int kFewRows = 64;
+
+struct RowsArgs {
+  const void* x;   // [T][ldx]
+  const void* w;   // [N][ldw]
+  const void* w2;  // PAIRED: the up projection
+  void* y;         // [T][ldy]
+  int64_t ldx, ldw, ldy;
+  int T, N, K, cols;  // cols: columns of y to write, those past N as zeros
+};
+
+// y[t][n] = sum_k x[t][k] w[n][k], or with PAIRED act(that) times the same with w2: 16 n per workgroup, MB blocks of
+// 16 rows t; wave w takes the 128-byte pieces of k number w, w + W, ...  Buffer loads give zeros past N and K.
+// ffn_token (1 row, D = 1024, F = 4096, bf16): see the measured figures at ffn_fwd.
+template <typename T, int ACT, bool PAIRED, int MB, int W>
+__global__ __launch_bounds__(64 * W) void ffn_rows_kernel(RowsArgs a) {
+  typedef typename Elem<T>::Frag F;
+  constexpr int ES = (int)sizeof(T);
+  constexpr int NM = PAIRED ? 2 : 1;
+  __shared__ f32x4 part[W > 1 ? W - 1 : 1][NM * MB][64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int r16 = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;
+  const unsigned rows = (unsigned)min(a.N - n0, 16), kb = (unsigned)a.K * ES;
+  const unsigned ldw = (unsigned)(a.ldw * ES), ldx = (unsigned)(a.ldx * ES);
+  typedef __amdgpu_buffer_rsrc_t Rsrc;
+  const auto rsrc = [](const void* p, unsigned bytes) -> Rsrc {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00027000);
+  };
+  const Rsrc rw = rsrc(static_cast<const T*>(a.w) + n0 * a.ldw, (rows - 1) * ldw + kb);
+  const Rsrc ru = PAIRED ? rsrc(static_cast<const T*>(a.w2) + n0 * a.ldw, (rows - 1) * ldw + kb) : rw;
+  const Rsrc rx = rsrc(a.x, (unsigned)(a.T - 1) * ldx + kb);
+  const auto load = [&](Rsrc d, unsigned row_at, unsigned k) -> F {  // k: byte within the row
+    return __builtin_bit_cast(F, __builtin_amdgcn_raw_buffer_load_b128(d, k < kb ? row_at + k : 0x80000000u, 0, 0));
+  };
+  f32x4 acc[NM][MB] = {};
+  // lane group g: bytes 32 g .. 32 g + 31 of each 128-byte piece, two fragments
+  constexpr int U = MB <= 2 ? 4 : 2;  // pieces in flight
+  const unsigned pieces = (kb + 127) / 128;
+  for (unsigned p0 = wave; p0 < pieces; p0 += W * U) {
+    F w[U][2], u[U][2], x[U][MB][2];
+#pragma unroll
+    for (int q = 0; q < U; ++q)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const unsigned k = (p0 + q * W) * 128 + 32 * g + 16 * e;
+        w[q][e] = load(rw, r16 * ldw, k);
+        if (PAIRED) u[q][e] = load(ru, r16 * ldw, k);
+#pragma unroll
+        for (int b = 0; b < MB; ++b) x[q][b][e] = load(rx, (16 * b + r16) * ldx, k);
+      }
+#pragma unroll
+    for (int q = 0; q < U; ++q)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int b = 0; b < MB; ++b) {
+          acc[0][b] = mma(w[q][e], x[q][b][e], acc[0][b]);
+          if (PAIRED) acc[NM - 1][b] = mma(u[q][e], x[q][b][e], acc[NM - 1][b]);
+        }
+  }
+  // the waves' sums, added in wave order
+  if constexpr (W > 1) {
+    if (wave) {
+#pragma unroll
+      for (int m = 0; m < NM; ++m)
+#pragma unroll
+        for (int b = 0; b < MB; ++b) part[wave - 1][m * MB + b][lane] = acc[m][b];
+    }
+    __syncthreads();
+    if (wave) return;
+    for (int v = 0; v < W - 1; ++v)
+#pragma unroll
+      for (int m = 0; m < NM; ++m)
+#pragma unroll
+        for (int b = 0; b < MB; ++b) acc[m][b] += part[v][m * MB + b][lane];
+  }
+#pragma unroll
+  for (int b = 0; b < MB; ++b) {
+    const int t = 16 * b + r16;
+    if (t >= a.T) continue;
+    T* y = static_cast<T*>(a.y) + t * a.ldy;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int n = n0 + 4 * g + r;
+      if (n < a.cols) y[n] = from_f32<T>(PAIRED ? act_of<ACT>(acc[0][b][r]) * acc[NM - 1][b][r] : acc[0][b][r]);
+    }
+  }
+}
+
+template <typename T, int ACT, bool PAIRED, int MB, int W>
+int rows_launch(const RowsArgs& a, hipStream_t st) {
+  return launch<ffn_rows_kernel<T, ACT, PAIRED, MB, W>>(ceil_div(a.cols, 16), 64 * W, 0, a, st, "ffn rows");
+}
+// Waves per workgroup: the down projection has F to reduce over and a quarter of the rows.
+template <typename T, int ACT, bool PAIRED>
+int rows_any(const RowsArgs& a, hipStream_t st) {
+  constexpr int W = PAIRED ? 4 : 8;
+  if (a.T <= 16) return rows_launch<T, ACT, PAIRED, 1, W>(a, st);
+  if (a.T <= 32) return rows_launch<T, ACT, PAIRED, 2, W>(a, st);
+  return rows_launch<T, ACT, PAIRED, 4, W>(a, st);
+}
+
+// ------------------------------------------------------------------------ host side
+struct Sizes {
+  int64_t T, D, F, Do, Dp, Fp, Dop, nb;
+  int es, dtype;
+};
+Sizes sizes_of(int64_t T, int64_t D, int64_t F, int64_t Do, int dtype) {
+  Sizes z;
+  z.T = T, z.D = D, z.F = F, z.Do = Do;
+  z.Dp = round_up(D, 8), z.Fp = round_up(F, 8), z.Dop = round_up(Do, 8);
+  z.nb = ceil_div(F, 32);
+  z.es = dtype == PNFX_F32 ? 4 : 2;
+  z.dtype = dtype;
+  return z;
+}
+
+// Workspace handed out in pieces of 256 bytes; null: only counted.
+struct Arena {
+  char* p;
+  int64_t used;
+  void* take(int64_t bytes) {
+    char* r = p ? p + used : nullptr;
+    used += round_up(bytes, 256);
+    return r;
+  }
+};
+
+// An operand as the kernels take it: in place, or a padded copy.
+struct In {
+  const void* p;
+  int64_t ld;
+};
+bool in_place(const void* p, int64_t ld, int64_t cols, const Sizes& z) {
+  return cols % 8 == 0 && operand_ok(p, ld, z.es);
+}
+
+int check_sizes(const char* what, int64_t T, int64_t D, int64_t F, int64_t Do, int act, int dtype) {
+  PNFX_REQUIRE(dtype == PNFX_F32 || dtype == PNFX_BF16, "%s: unsupported dtype %d", what, dtype);
+  PNFX_REQUIRE(act == PNFX_ACT_SILU || act == PNFX_ACT_GELU, "%s: unknown activation %d", what, act);
+  PNFX_REQUIRE(T >= 1 && D >= 1 && F >= 1 && Do >= 1 && T < (1 << 29) && D <= (1 << 18) && F <= (1 << 18) &&
+                   Do <= (1 << 18),
+               "%s: bad shape T=%lld D=%lld F=%lld Do=%lld", what, (long long)T, (long long)D, (long long)F,
+               (long long)Do);
+  return PNFX_OK;
+}
+
+// The padded copies that a call makes of what it cannot take in place.
+struct Operands {
+  PadItem pads[4];
+  int n = 0;
+  In take(Arena& ar, const void* p, int64_t ld, int64_t rows, int64_t cols, const Sizes& z) {
+    if (in_place(p, ld, cols, z)) return In{p, ld};
+    const int64_t cp = round_up(cols, 8);
+    void* d = ar.take(rows * cp * z.es);
+    pads[n++] = PadItem{p, d, ld, rows, cols, rows, cp, 1};
+    return In{d, cp};
+  }
+  // both halves of w_in, Fp rows apart
+  In take_in(Arena& ar, const void* p, int64_t ld, const Sizes& z) {
+    if (z.F == z.Fp && in_place(p, ld, z.D, z)) return In{p, ld};
+    void* d = ar.take(2 * z.Fp * z.Dp * z.es);
+    pads[n++] = PadItem{p, d, ld, z.F, z.D, z.Fp, z.Dp, 2};
+    return In{d, z.Dp};
+  }
+};
+
+template <typename T, int ACT>
+int glu_fwd(GluArgs& a, bool big, hipStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (big) {
+      a.tm = (int)ceil_div(a.T, Big::TM), a.tn = (int)ceil_div(a.Fp, Big::TN / 2);
+      return launch<glu_fwd_kernel<T, ACT, Big>>((int64_t)a.tm * a.tn, threads_of<Big>, lds_of<Big>, a, st, "glu_fwd");
+    }
+  }
+  a.tm = (int)ceil_div(a.T, Mid::TM), a.tn = (int)ceil_div(a.Fp, Mid::TN / 2);
+  return launch<glu_fwd_kernel<T, ACT, Mid>>((int64_t)a.tm * a.tn, threads_of<Mid>, lds_of<Mid>, a, st, "glu_fwd");
+}
+template <typename T, int ACT>
+int glu_bwd(GluArgs& a, bool big, hipStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (big) {
+      a.tm = (int)ceil_div(a.T, Big::TM), a.tn = (int)ceil_div(a.Fp, Big::TN);
+      return launch<glu_bwd_kernel<T, ACT, Big>>((int64_t)a.tm * a.tn, threads_of<Big>, lds_of<Big>, a, st, "glu_bwd");
+    }
+  }
+  a.tm = (int)ceil_div(a.T, Mid::TM), a.tn = (int)ceil_div(a.Fp, Mid::TN);
+  return launch<glu_bwd_kernel<T, ACT, Mid>>((int64_t)a.tm * a.tn, threads_of<Mid>, lds_of<Mid>, a, st, "glu_bwd");
+}
+
+struct FwdArgs {
+  const void *x, *w_in, *w_down;
+  int64_t x_rs, win_rs, wd_rs;
+  void *y, *gu;
+  uint8_t* scales;
+  int act, keep;
+};
+
+// Workspace of the forward pass, with or without padded copies of its operands.
+int64_t fwd_bytes(const Sizes& z, bool copies) {
+  Arena ar{nullptr, 0};
+  if (copies) {
+    ar.take(z.T * z.Dp * z.es);
+    ar.take(2 * z.Fp * z.Dp * z.es);
+    ar.take(z.Do * z.Fp * z.es);
+  }
+  ar.take(z.T * z.Fp * z.es);
+  ar.take(product_workspace(cut_of(z.T, z.Do, z.Fp, z.dtype, true), z.T, z.Do));
+  return ar.used;
+}
+
+template <typename T, int ACT>
+int ffn_fwd(const FwdArgs& f, const Sizes& z, void* ws, hipStream_t st) {
+  Arena ar{static_cast<char*>(ws), 0};
+  Operands ops;
+  const In x = ops.take(ar, f.x, f.x_rs, z.T, z.D, z);
+  const In win = ops.take_in(ar, f.w_in, f.win_rs, z);
+  const In wd = ops.take(ar, f.w_down, f.wd_rs, z.Do, z.F, z);
+  void* h = ar.take(z.T * z.Fp * z.es);
+  PNFX_TRY(pad(ops.pads, ops.n, z.dtype, st));
+  const T* wg = static_cast<const T*>(win.p);
+  const T* wu = wg + z.Fp * win.ld;
+  if (z.T <= kFewRows && f.keep == PNFX_KEEP_NONE) {
+    RowsArgs r{x.p, wg, wu, h, x.ld, win.ld, z.Fp, (int)z.T, (int)z.F, (int)z.Dp, (int)z.Fp};
+    PNFX_TRY((rows_any<T, ACT, true>(r, st)));
+    RowsArgs d{h, wd.p, nullptr, f.y, z.Fp, wd.ld, z.Do, (int)z.T, (int)z.Do, (int)z.Fp, (int)z.Do};
+    return rows_any<T, ACT, false>(d, st);
+  }
+  GluArgs a = {};
+  a.x = x.p, a.wg = wg, a.wu = wu, a.h = h, a.gu = f.gu, a.scales = f.scales;
+  a.ldx = x.ld, a.ldw = win.ld, a.K = z.Dp;
+  a.T = (int)z.T, a.F = (int)z.F, a.Fp = (int)z.Fp, a.nb = (int)z.nb, a.keep = f.keep;
+  PNFX_TRY((glu_fwd<T, ACT>(a, cut_of(z.T, 2 * z.Fp, z.Dp, z.dtype, false).big, st)));
+  const Cut cut = cut_of(z.T, z.Do, z.Fp, z.dtype, true);
+  ProductArgs p = {};
+  p.a = h, p.b = wd.p, p.c = f.y, p.lda = z.Fp, p.ldb = wd.ld, p.ldc = z.Do;
+  p.M = z.T, p.N = z.Do, p.K = z.Fp;
+  return product(ROW, ROW, p, cut, z.dtype, ar.take(product_workspace(cut, z.T, z.Do)), st);
+}
+
+int64_t bwd_bytes(const Sizes& z, bool copies) {
+  Arena ar{nullptr, 0};
+  if (copies) {
+    ar.take(z.T * z.Dop * z.es);
+    ar.take(z.T * z.Dp * z.es);
+    ar.take(2 * z.Fp * z.Dp * z.es);
+    ar.take(z.Do * z.Fp * z.es);
+  }
+  ar.take(z.T * 2 * z.Fp * z.es);
+  ar.take(z.T * z.Fp * z.es);
+  int64_t most = product_workspace(cut_of(z.T, z.D, 2 * z.Fp, z.dtype, true), z.T, z.D);
+  most = std::max(most, product_workspace(cut_of(2 * z.Fp, z.D, z.T, z.dtype, true), 2 * z.Fp, z.D));
+  most = std::max(most, product_workspace(cut_of(z.Do, z.F, z.T, z.dtype, true), z.Do, z.F));
+  ar.take(most);
+  return ar.used;
+}
+
+struct BwdArgs {
+  const void *dy, *x, *w_in, *w_down, *gu;
+  const uint8_t* scales;
+  int64_t dy_rs, x_rs, win_rs, wd_rs;
+  void *dx, *dw_in, *dw_down;
+  int act, keep;
+};
+
+template <typename T, int ACT>
+int ffn_bwd(const BwdArgs& f, const Sizes& z, void* ws, hipStream_t st) {
+  Arena ar{static_cast<char*>(ws), 0};
+  Operands ops;
+  const In dy = ops.take(ar, f.dy, f.dy_rs, z.T, z.Do, z);
+  const In x = ops.take(ar, f.x, f.x_rs, z.T, z.D, z);
+  const In win = ops.take_in(ar, f.w_in, f.win_rs, z);
+  const In wd = ops.take(ar, f.w_down, f.wd_rs, z.Do, z.F, z);
+  void* dgu = ar.take(z.T * 2 * z.Fp * z.es);
+  void* h = ar.take(z.T * z.Fp * z.es);
+  void* rest = ar.take(0);
+  PNFX_TRY(pad(ops.pads, ops.n, z.dtype, st));
+  GluArgs a = {};
+  a.x = dy.p, a.wg = wd.p, a.h = h, a.gu = const_cast<void*>(f.gu), a.scales = const_cast<uint8_t*>(f.scales);
+  a.dgu = dgu, a.ldx = dy.ld, a.ldw = wd.ld, a.K = z.Do;
+  a.T = (int)z.T, a.F = (int)z.F, a.Fp = (int)z.Fp, a.nb = (int)z.nb, a.keep = f.keep;
+  PNFX_TRY((glu_bwd<T, ACT>(a, cut_of(z.T, z.Fp, z.Do, z.dtype, false).big, st)));
+  if (f.dx) {
+    ProductArgs p = {};
+    p.a = dgu, p.b = win.p, p.c = f.dx, p.lda = 2 * z.Fp, p.ldb = win.ld, p.ldc = z.D;
+    p.M = z.T, p.N = z.D, p.K = 2 * z.Fp;
+    PNFX_TRY(product(ROW, COL, p, cut_of(p.M, p.N, p.K, z.dtype, true), z.dtype, rest, st));
+  }
+  if (f.dw_in) {
+    ProductArgs p = {};
+    p.a = dgu, p.b = x.p, p.c = f.dw_in, p.lda = 2 * z.Fp, p.ldb = x.ld, p.ldc = z.D;
+    p.M = 2 * z.Fp, p.N = z.D, p.K = z.T, p.gap_at = z.F, p.gap = z.Fp - z.F;
+    // the columns from Fp + F on are the second gap: the last rows
+    p.M -= p.gap;
+    PNFX_TRY(product(COL, COL, p, cut_of(2 * z.Fp, p.N, p.K, z.dtype, true), z.dtype, rest, st));
+  }
+  if (f.dw_down) {
+    ProductArgs p = {};
+    p.a = dy.p, p.b = h, p.c = f.dw_down, p.lda = dy.ld, p.ldb = z.Fp, p.ldc = z.F;
+    p.M = z.Do, p.N = z.F, p.K = z.T;
+    PNFX_TRY(product(COL, COL, p, cut_of(p.M, p.N, p.K, z.dtype, true), z.dtype, rest, st));
+  }
+  return PNFX_OK;
+}
+
+}  // namespace
+}  // namespace pnfx
+
+extern "C" int64_t pnfx_ffn_fwd_workspace_size(int64_t T, int64_t D, int64_t F, int64_t Do, int copies, int dtype) {
+  using namespace pnfx;
+  if (check_sizes("ffn", T, D, F, Do, PNFX_ACT_SILU, dtype) != PNFX_OK) return 0;
+  return fwd_bytes(sizes_of(T, D, F, Do, dtype), copies);
+}
+
+extern "C" int pnfx_ffn_fwd(const void* x, int64_t x_rs, const void* w_in, int64_t win_rs, const void* w_down,
+                            int64_t wd_rs, void* y, void* gu, uint8_t* scales, int64_t T, int64_t D, int64_t F,
+                            int64_t Do, int act, int keep, int dtype, void* workspace, int64_t workspace_bytes,
+                            void* stream) {
+  using namespace pnfx;
+  PNFX_REQUIRE(x && w_in && w_down && y, "ffn_fwd: null pointer");
+  PNFX_TRY(check_sizes("ffn_fwd", T, D, F, Do, act, dtype));
+  PNFX_REQUIRE(keep == PNFX_KEEP_NONE || keep == PNFX_KEEP_FULL || (keep == PNFX_KEEP_E4M3 && dtype == PNFX_BF16),
+               "ffn_fwd: keep %d of dtype %d", keep, dtype);
+  PNFX_REQUIRE(keep == PNFX_KEEP_NONE || (gu && (dtype == PNFX_F32 || scales)), "ffn_fwd: nowhere to keep g and u");
+  PNFX_REQUIRE(x_rs >= D && win_rs >= D && wd_rs >= F, "ffn_fwd: row strides %lld, %lld, %lld", (long long)x_rs,
+               (long long)win_rs, (long long)wd_rs);
+  const Sizes z = sizes_of(T, D, F, Do, dtype);
+  PNFX_REQUIRE(((reinterpret_cast<uintptr_t>(gu) | reinterpret_cast<uintptr_t>(workspace) |
+                 reinterpret_cast<uintptr_t>(y)) & 15) == 0,
+               "ffn_fwd: results and workspace must be 16-byte aligned");
+  const bool copies = !(in_place(x, x_rs, D, z) && z.F == z.Fp && in_place(w_in, win_rs, D, z) &&
+                        in_place(w_down, wd_rs, F, z));
+  const int64_t need = fwd_bytes(z, copies);
+  PNFX_REQUIRE(workspace && workspace_bytes >= need, "ffn_fwd: workspace needs %lld bytes", (long long)need);
+  const FwdArgs f{x, w_in, w_down, x_rs, win_rs, wd_rs, y, gu, scales, act, keep};
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (dtype == PNFX_F32)
+    return act == PNFX_ACT_SILU ? ffn_fwd<float, PNFX_ACT_SILU>(f, z, workspace, st)
+                                : ffn_fwd<float, PNFX_ACT_GELU>(f, z, workspace, st);
+  return act == PNFX_ACT_SILU ? ffn_fwd<bf16, PNFX_ACT_SILU>(f, z, workspace, st)
+                              : ffn_fwd<bf16, PNFX_ACT_GELU>(f, z, workspace, st);
+}
+
+extern "C" int64_t pnfx_ffn_bwd_workspace_size(int64_t T, int64_t D, int64_t F, int64_t Do, int copies, int dtype) {
+  using namespace pnfx;
+  if (check_sizes("ffn", T, D, F, Do, PNFX_ACT_SILU, dtype) != PNFX_OK) return 0;
+  return bwd_bytes(sizes_of(T, D, F, Do, dtype), copies);
+}
+
+extern "C" int pnfx_ffn_bwd(const void* dy, int64_t dy_rs, const void* x, int64_t x_rs, const void* w_in,
+                            int64_t win_rs, const void* w_down, int64_t wd_rs, const void* gu, const uint8_t* scales,
+                            void* dx, void* dw_in, void* dw_down, int64_t T, int64_t D, int64_t F, int64_t Do, int act,
+                            int keep, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace pnfx;
+  PNFX_REQUIRE(dy && x && w_in && w_down && gu, "ffn_bwd: null pointer");
+  PNFX_TRY(check_sizes("ffn_bwd", T, D, F, Do, act, dtype));
+  PNFX_REQUIRE(dtype == PNFX_F32 ? keep == PNFX_KEEP_FULL
+                                 : (keep == PNFX_KEEP_FULL || keep == PNFX_KEEP_E4M3) && scales,
+               "ffn_bwd: keep %d of dtype %d", keep, dtype);
+  PNFX_REQUIRE(dy_rs >= Do && x_rs >= D && win_rs >= D && wd_rs >= F, "ffn_bwd: row strides %lld, %lld, %lld, %lld",
+               (long long)dy_rs, (long long)x_rs, (long long)win_rs, (long long)wd_rs);
+  const Sizes z = sizes_of(T, D, F, Do, dtype);
+  PNFX_REQUIRE(((reinterpret_cast<uintptr_t>(gu) | reinterpret_cast<uintptr_t>(workspace) |
+                 reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw_in) |
+                 reinterpret_cast<uintptr_t>(dw_down)) & 15) == 0,
+               "ffn_bwd: results, g and u and the workspace must be 16-byte aligned");
+  const bool copies = !(in_place(dy, dy_rs, Do, z) && in_place(x, x_rs, D, z) && z.F == z.Fp &&
+                        in_place(w_in, win_rs, D, z) && in_place(w_down, wd_rs, F, z));
+  const int64_t need = bwd_bytes(z, copies);
+  PNFX_REQUIRE(workspace && workspace_bytes >= need, "ffn_bwd: workspace needs %lld bytes", (long long)need);
+  const BwdArgs f{dy, x, w_in, w_down, gu, scales, dy_rs, x_rs, win_rs, wd_rs, dx, dw_in, dw_down, act, keep};
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (dtype == PNFX_F32)
+    return act == PNFX_ACT_SILU ? ffn_bwd<float, PNFX_ACT_SILU>(f, z, workspace, st)
+                                : ffn_bwd<float, PNFX_ACT_GELU>(f, z, workspace, st);
+  return act == PNFX_ACT_SILU ? ffn_bwd<bf16, PNFX_ACT_SILU>(f, z, workspace, st)
+                              : ffn_bwd<bf16, PNFX_ACT_GELU>(f, z, workspace, st);
+}

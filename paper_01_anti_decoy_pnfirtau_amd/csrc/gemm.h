@@ -1,0 +1,359 @@
+// The matrix product C[m][n] = sum_k A(m, k) B(n, k) that the feed-forward and cross-entropy kernels are built
+// on: operand staging, tile loop and the choice of tiles.  Each kernel adds its own epilogue on the fp32
+// accumulators.
+//
+// Operands go from global memory straight to LDS (buffer loads with LDS as destination, whose bounds check
+// supplies the zeros past an edge), two tiles of 128 bytes of k deep, and from there to registers as MFMA
+// fragments one phase ahead of the products that use them.  The loads of the tile after next are issued in two
+// parts, A's behind the step's only barrier and B's a phase later, so that they do not queue up in front of
+// the fragments' reads: 8192^3 in bf16 877 -> 838 us.
+//
+// Measured on MI355X, bf16, 8192^3 with 256 x 256 tiles: both operands as rows of k 795-840 us (1310-1380
+// TFLOP/s; the library's product 766 us), rows by columns 815 us (872), columns by columns 837 us (984).
+// 128 x 128 tiles of four waves 990-1025 us (1075-1110 TFLOP/s), two of which share a CU.  Bound by the LDS,
+// which has to supply 192 KB of fragments and take 64 KB of tiles for every 2048 cycles of products.
+#pragma once
+
+#include <atomic>
+
+#include "tiles_bf16.h"
+
+namespace pnfx {
+namespace {
+
+// Wait until at most N of this wave's vector-memory operations (direct-to-LDS loads among them) and no
+// LDS operation are outstanding.
+template <int N>
+__device__ __forceinline__ void wait_vm_lgkm() {
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x70);
+}
+
+// A buffer descriptor over `bytes` bytes from p (both wave-uniform): loads past its end return zero.
+__device__ __forceinline__ u32x4 buffer_of(const void* p, unsigned bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  u32x4 d;
+  d[0] = __builtin_amdgcn_readfirstlane((unsigned)a);
+  d[1] = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32) & 0xffff);
+  d[2] = __builtin_amdgcn_readfirstlane(bytes);
+  d[3] = 0x00027000;
+  return d;
+}
+// 16 bytes per lane from buffer d at byte offset `off` to LDS bytes `lds` + 16 * lane.  In inline assembly:
+// the compiler cannot tell the two LDS buffers of a pipelined loop apart and would wait for every such
+// load before the next LDS read.  It has no output register; Product::run waits for the loads itself.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved: named all the same, as it is written
+__device__ __forceinline__ void lds_dma16(u32x4 d, unsigned off, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :: "s"(lds), "v"(off), "s"(d)
+               : "m0", "memory");
+}
+#pragma clang diagnostic pop
+__device__ __forceinline__ unsigned lds_addr(const void* p) {
+  return (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)p);
+}
+
+// Element types.  A step covers 128 bytes of k; a fragment is 16 bytes of k of one row.
+template <typename T>
+struct Elem;
+template <>
+struct Elem<bf16> {
+  typedef bf16x8 Frag;
+};
+template <>
+struct Elem<float> {
+  typedef f32x4 Frag;
+};
+template <typename T>
+constexpr int k_step = 128 / (int)sizeof(T);
+template <typename T>
+constexpr int per16 = 16 / (int)sizeof(T);  // elements in 16 bytes
+
+// acc[r] += sum_k b(row 4 (lane / 16) + r, k) a(row lane % 16, k).
+__device__ __forceinline__ f32x4 mma(bf16x8 b, bf16x8 a, f32x4 acc) { return mfma16x16x32(b, a, acc); }
+__device__ __forceinline__ f32x4 mma(f32x4 b, f32x4 a, f32x4 acc) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(b[t], a[t], acc, 0, 0, 0);
+  return acc;
+}
+
+// Operands.  ROW: rows of k (element (r, k) at p[r ld + k]), staged as sub-tiles of 64 rows and read 16 bytes
+// per lane.  COL: element (r, k) at p[k ld + r], staged as sub-tiles of 64 columns and read transposed.  PAIR:
+// ROW from two matrices (the gate and the up projection), 32 rows of each in turn.
+enum Kind { ROW, COL, PAIR };
+
+// A sub-tile is 64 slots of 128 bytes; 16-byte chunk c of slot s lies at position c ^ stage_swz(s).  The
+// swizzles depend on the slot's low four bits only, so that a fragment's block is a constant offset.  ROW: 16
+// lanes read 16 consecutive slots at one chunk, which with two slots to the 64 banks lands on all of them.
+// COL, bf16: a half wave reads 32 bytes of 8 slots; fp32: a wave 64 bytes of 4 slots.
+template <typename T, Kind KIND>
+__device__ __forceinline__ int stage_swz(int slot) {
+  if (KIND != COL) return slot >> 1 & 7;
+  if (sizeof(T) == 4) return 4 * (slot >> 1 & 1);
+  return 2 * ((slot >> 1 & 1) | (((slot >> 2) ^ (slot >> 3)) & 1) << 1);
+}
+
+// Stages tiles of R rows of one operand, NT threads, 16 bytes per thread and load.  Past `rows` and past K come
+// zeros, or other elements of the same matrix where they only reach results that are not stored; past K
+// zeros in both operands.  An operand's memory goes on to a whole 16-byte chunk of its inner dimension, which
+// for ROW holds zeros there.
+template <typename T, Kind KIND, int R, int NT>
+struct Stage {
+  static constexpr int NI = R * 8 / NT;  // loads per thread and step
+  static constexpr int SPL = NT / 8;     // slots per load
+  static_assert(SPL == 32 || SPL == 64, "a load fills half a sub-tile or a whole one");
+  static constexpr int ES = (int)sizeof(T), KS = k_step<T>;
+  const char* base[KIND == PAIR ? 2 : 1];  // element (first row, k0)
+  int64_t left;    // k left
+  unsigned ldb;    // bytes from row to row
+  unsigned limit;  // ROW, PAIR: bytes to the last row in reach; COL: bytes of a row in reach
+  unsigned off;    // the lane's byte offset in load 0
+  int ch;          // ROW: the lane's chunk of the step's k
+
+  // p (PAIR: and p2): the tile's first row; rows >= 1: how many there are from it on (PAIR: in each); K: its k.
+  __device__ __forceinline__ void init(const T* p, int64_t ld, int rows, int64_t K, int tid,
+                                       const T* p2 = nullptr) {
+    ldb = (unsigned)(ES * ld);
+    left = K;
+    base[0] = reinterpret_cast<const char*>(p);
+    const int slot = tid / 8;
+    ch = (tid % 8) ^ stage_swz<T, KIND>(slot);
+    if constexpr (KIND == PAIR) base[1] = reinterpret_cast<const char*>(p2);
+    if constexpr (KIND == COL) {
+      limit = (unsigned)(ES * min(rows, R) + 15) & ~15u;
+      // fp32: slot 32 h + 16 f + 4 t + g holds k = 16 f + 4 g + t of columns 32 h .. 32 h + 31
+      const int k = ES == 4 ? (slot & 16) + 4 * (slot & 3) + (slot >> 2 & 3) : row_of_slot(slot);
+      off = k * ldb + 16 * ch + (ES == 4 ? (slot >> 5) * 128 : 0);
+    } else {
+      const int row = row_of_slot(slot);
+      limit = (unsigned)(min(rows, KIND == PAIR ? R / 2 : R) - 1) * ldb;
+      off = (KIND == PAIR ? row & 31 : row) * ldb + 16 * ch;
+    }
+  }
+  // The next step's tile to LDS byte address lds.
+  __device__ __forceinline__ void load(unsigned lds, int wave) {
+    const unsigned ks = (unsigned)max<int64_t>(0, min<int64_t>(left, KS));
+    const unsigned dst = lds + wave * 1024;
+    if constexpr (KIND == COL) {
+      const u32x4 d = buffer_of(base[0], ks ? (ks - 1) * ldb + limit : 0u);
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const unsigned o = ES == 4 ? j * SPL * 4
+                                   : SPL == 64 ? 128 * j : (j & 1) * 32 * ldb + 128 * (j >> 1);
+        lds_dma16(d, off + o, dst + j * NT * 16);
+      }
+      base[0] += (int64_t)KS * ldb;
+    } else {
+      // lanes past K read far out of the buffer
+      const unsigned o0 = (unsigned)(per16<T> * ch) < ks ? off : 0x80000000u;
+      const unsigned bytes = ks ? limit + ((ES * ks + 15) & ~15u) : 0u;
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        if constexpr (KIND == PAIR) {
+          const int half = SPL == 64 ? wave >> 2 : j & 1, g = SPL == 64 ? j : j >> 1;
+          lds_dma16(buffer_of(half ? base[1] : base[0], bytes), o0 + g * 32 * ldb, dst + j * NT * 16);
+        } else {
+          lds_dma16(buffer_of(base[0], bytes), o0 + j * SPL * ldb, dst + j * NT * 16);
+        }
+      }
+      base[0] += 128;
+      if constexpr (KIND == PAIR) base[1] += 128;
+    }
+    left -= KS;
+  }
+};
+
+// Fragments of a staged tile, in two halves of a step's k: lane group g of half hf holds, in bf16, k = 32 hf +
+// 8 g + 0..7 and, in fp32, k = 16 hf + 4 g + 0..3.
+template <typename T, Kind KIND>
+struct Frags {
+  typedef typename Elem<T>::Frag F;
+  static constexpr int SUB = 64 * 128 / (int)sizeof(T);  // elements of a sub-tile
+  const T* p[KIND == COL && sizeof(T) == 2 ? 4 : 2];
+  // tile: the wave's first sub-tile in buffer 0
+  __device__ __forceinline__ Frags(const T* tile, int lane) {
+    const int r16 = lane & 15, g = lane >> 4;
+    if constexpr (KIND == COL && sizeof(T) == 4) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        p[b] = tile + g * 32 + 4 * ((4 * b + (r16 >> 2)) ^ stage_swz<T, COL>(g)) + (r16 & 3);
+    } else if constexpr (KIND == COL) {
+      const int e = (lane >> 2) & 3, q = lane & 3, sl = 4 * g + e;
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        p[b] = tile + sl * 64 + 8 * ((2 * b + (q >> 1)) ^ stage_swz<T, COL>(sl)) + 4 * (q & 1);
+    } else {
+      constexpr int C = per16<T>;
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+        p[hf] = tile + r16 * 8 * C + C * ((g + 4 * hf) ^ stage_swz<T, ROW>(r16));
+    }
+  }
+  // 16-row block blk of the wave, `at` elements further on.
+  __device__ __forceinline__ F get(int blk, int hf, int at) const {
+    if constexpr (KIND == COL && sizeof(T) == 4) {
+      const T* t = p[blk & 1] + at + (blk >> 2) * SUB + (blk >> 1 & 1) * (SUB / 2) + 16 * hf * 32;
+      return F{t[0], t[4 * 32], t[8 * 32], t[12 * 32]};
+    } else if constexpr (KIND == COL) {
+      const T* t = p[blk & 3] + at + (blk >> 2) * SUB + 32 * hf * 64;
+      return __builtin_shufflevector(ld_tr(t), ld_tr(t + 16 * 64), 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      return *reinterpret_cast<const F*>(p[hf] + at + blk * (SUB / 4));
+    }
+  }
+};
+// Row of the tile that index r (0..15) of block blk is.  PAIR: of 64 such rows the first 32 are 32 rows of the
+// first matrix, the others the same rows of the second.
+template <Kind KIND>
+__device__ __forceinline__ int stage_row(int blk, int r) {
+  return KIND == COL ? 16 * blk + r : 64 * (blk >> 2) + perm_row(blk & 3, r);
+}
+
+// Tiles of TM x TN by WM x WN waves.  Big for products with tiles enough for every CU, two waves per SIMD;
+// Mid, two workgroups per CU, for the others and for fp32.
+struct Big {
+  static constexpr int TM = 256, TN = 256, WM = 2, WN = 4, PER_CU = 1;
+};
+struct Mid {
+  static constexpr int TM = 128, TN = 128, WM = 2, WN = 2, PER_CU = 2;
+};
+template <class C>
+constexpr int threads_of = 64 * C::WM * C::WN;
+template <class C>
+constexpr int lds_of = 2 * (C::TM + C::TN) * 128;
+
+// acc[i][j][r] of a wave (wm, wn): row m = stage_row<KA>(wm MI + i, lane % 16), column n =
+// stage_row<KB>(wn NJ + j, 4 (lane / 16) + r) of the tile.
+template <typename T, Kind KA, Kind KB, class C>
+struct Product {
+  static constexpr int TM = C::TM, TN = C::TN, NT = threads_of<C>;
+  static constexpr int MI = TM / C::WM / 16, NJ = TN / C::WN / 16;
+  static_assert(MI % 4 == 0 && NJ % 4 == 0, "a wave's share is whole sub-tiles");
+  typedef Stage<T, KA, TM, NT> StageA;
+  typedef Stage<T, KB, TN, NT> StageB;
+  typedef typename Elem<T>::Frag F;
+
+  // sm: lds_of<C> bytes, free; every wave's reads of it are done when run returns (its writes too).
+  __device__ __forceinline__ static void run(StageA& sa, StageB& sb, int steps, T* sm, int wave, int lane,
+                                             f32x4 (&acc)[MI][NJ]) {
+    if (steps <= 0) return;
+    // both buffers of A, then both of B: an operand's fragments are within the 64 KB of an LDS load's offset
+    constexpr int SA = TM * k_step<T>, SB = TN * k_step<T>, ES = (int)sizeof(T);
+    const unsigned la = __builtin_amdgcn_readfirstlane(lds_addr(sm));
+    const auto load_a = [&](int b) { sa.load(la + ES * b * SA, wave); };
+    const auto load_b = [&](int b) { sb.load(la + ES * (2 * SA + b * SB), wave); };
+    const Frags<T, KA> fa(sm + wave / C::WN * MI * 16 * k_step<T>, lane);
+    const Frags<T, KB> fb(sm + 2 * SA + wave % C::WN * NJ * 16 * k_step<T>, lane);
+    // Four phases per step, (k-half, half of the row blocks): while one phase's products run, the
+    // fragments of the next are read.
+    constexpr int MH = MI / 2;
+    F a[2][MH], b[2][NJ];
+    const auto read_a = [&](int buf, int hf, int ih) {
+#pragma unroll
+      for (int i = 0; i < MH; ++i) a[ih][i] = fa.get(ih * MH + i, hf, buf * SA);
+    };
+    const auto read_b = [&](int buf, int hf) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) b[hf][j] = fb.get(j, hf, buf * SB);
+    };
+    const auto products = [&](int hf, int ih) {
+#pragma unroll
+      for (int i = 0; i < MH; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+          acc[ih * MH + i][j] = mma(b[hf][j], a[ih][i], acc[ih * MH + i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    load_a(0);
+    load_b(0);
+    if (steps > 1) {
+      load_a(1);
+      load_b(1);
+      wait_vm_lgkm<StageA::NI + StageB::NI>();
+    } else {
+      wait_vm_lgkm<0>();
+    }
+    __builtin_amdgcn_s_barrier();
+    read_b(0, 0);
+    read_a(0, 0, 0);
+    const auto step = [&](int s, int buf) {
+      if (s && s + 1 < steps) load_b(buf ^ 1);
+      __builtin_amdgcn_sched_barrier(0);
+      read_a(buf, 0, 1);
+      products(0, 0);
+      read_b(buf, 1);
+      read_a(buf, 1, 0);
+      products(0, 1);
+      read_a(buf, 1, 1);
+      products(1, 0);
+      // the next tile is here, and every wave has read this one
+      wait_vm_lgkm<0>();
+      __builtin_amdgcn_s_barrier();
+      if (s + 2 < steps) load_a(buf);
+      __builtin_amdgcn_sched_barrier(0);
+      read_b(buf ^ 1, 0);
+      read_a(buf ^ 1, 0, 0);
+      products(1, 1);
+    };
+    int s = 0;
+    for (; s + 1 < steps; s += 2) {
+      step(s, 0);
+      step(s + 1, 1);
+    }
+    if (s < steps) step(s, 0);
+    wait_vm_lgkm<0>();
+    __builtin_amdgcn_s_barrier();
+  }
+};
+
+// Workgroup `id` of tm x tn tiles.  Consecutive ids go to the eight XCDs in turn: each XCD takes a range of
+// tiles of its own, column by column over bands of four tile rows, so that its L2 holds what they share.
+__device__ __forceinline__ void tile_of(int id, int tm, int tn, int& m, int& n) {
+  const int total = tm * tn, q = total / 8, r = total % 8, x = id % 8, y = id / 8;
+  id = x < r ? x * (q + 1) + y : r * (q + 1) + (x - r) * q + y;
+  const int band = id / (4 * tn), first = 4 * band, high = min(tm - first, 4), in = id - band * 4 * tn;
+  m = first + in % high;
+  n = in / high;
+}
+
+// Sizes that the staging's 32-bit byte offsets cover.
+constexpr int64_t kMaxLd = 1 << 20;
+inline bool operand_ok(const void* p, int64_t ld, int es) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * es % 16 == 0 && ld <= kMaxLd;
+}
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+
+// Launch with `lds` bytes of dynamic LDS; above 64 KB the kernel is told so, once on each device.
+template <auto KERNEL, typename Arg>
+int launch(int64_t grid, int threads, int lds, const Arg& a, hipStream_t st, const char* what) {
+  if (grid <= 0) return PNFX_OK;
+  PNFX_REQUIRE(grid < (1ll << 31), "%s: %lld workgroups", what, (long long)grid);
+  if (lds > 65536) {
+    static std::atomic<uint64_t> told{0};
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (e == hipSuccess && !(told.load(std::memory_order_relaxed) & bit)) {
+      e = hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      told.fetch_or(bit, std::memory_order_relaxed);
+    }
+    if (e != hipSuccess) {
+      set_error("%s: %s", what, hipGetErrorString(e));
+      return PNFX_ELAUNCH;
+    }
+  }
+  hipLaunchKernelGGL(KERNEL, dim3((unsigned)grid), dim3(threads), lds, st, a);
+  return launch_status(what);
+}
+
+#define PNFX_TRY(call)             \
+  do {                             \
+    const int rc_ = (call);        \
+    if (rc_ != PNFX_OK) return rc_; \
+  } while (0)
+
+}  // namespace
+}  // namespace pnfx

@@ -1,0 +1,50 @@
+// Products of two matrices with plain results, shared by the feed-forward and the cross-entropy entries
+// (kernels in product.hip).
+#pragma once
+
+#include "gemm.h"
+
+namespace pnfx {
+
+// C[m][n] = sum_k A(m, k) B(n, k), M x N over K; A and B of one type, 16-byte aligned with rows in whole 16-byte
+// chunks, ROW operands zero up to a whole chunk of k.  Only the combinations ROW ROW, ROW COL and COL COL.
+struct ProductArgs {
+  const void* a;
+  const void* b;
+  void* c;              // [*][ldc], the operands' type
+  int64_t lda, ldb, ldc;
+  int64_t M, N, K;
+  // Rows of the product that are no rows of C: gap_at .. gap_at + gap - 1; those behind them move up.
+  int64_t gap_at, gap;
+  // Number of rows (m_count) or of k (k_count) in device memory, at most M or K; null: M, K.
+  const int* m_count;
+  const int* k_count;
+  // Not null: fp32 sums [splits][M][N] instead of C, added to what is there (add) or written.
+  float* sums;
+  bool add;
+  const float* alpha;  // one fp32 value in device memory that C is scaled by before it is rounded, or null
+};
+
+// How a product is cut: tiles of 256 or 128 and splits of its k over workgroups.
+struct Cut {
+  bool big;
+  int splits;
+  int64_t steps;  // steps of a split
+};
+Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool can_split);
+
+// Workspace of product() for C (not sums) at this cut, in bytes.
+int64_t product_workspace(const Cut& cut, int64_t M, int64_t N);
+int product(int ka, int kb, const ProductArgs& p, const Cut& cut, int dtype, void* workspace, hipStream_t stream);
+
+// Copies of matrices with their columns zero-padded to whole 16-byte chunks, in one launch.
+struct PadItem {
+  const void* src;
+  void* dst;         // [halves][rows_out][cols_out]
+  int64_t ld;        // src elements from row to row
+  int64_t rows, cols, rows_out, cols_out;
+  int halves;        // matrices below each other in src
+};
+int pad(const PadItem* items, int n, int dtype, hipStream_t stream);
+
+}  // namespace pnfx

@@ -14,6 +14,8 @@
 // pnfx::flash_fwd_fir       (none: the FIR fused into the forward's key-tile load)
 // pnfx::attn_rows / _bwd    (none: key FIR and flash on projection rows, one autograd node)
 // pnfx::linear / _wgrad     (none: x W^T with its weight gradient's fp32 sums)
+// pnfx::gated_ffn / _bwd    (none: the gated feed-forward block, both projections in one kernel)
+// pnfx::linear_xent / _bwd  (none: cross entropy over the vocabulary without the logits)
 // pnfx::sum_f64             the fp64 sum of tau's row gradients  :784
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
@@ -208,6 +210,214 @@ Tensor linear_cuda(const Tensor& x, const Tensor& w) {
   TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16, "linear: x is ", x.scalar_type(),
                    " (bfloat16)");
   return at::linear(x, w.to(at::kBFloat16));
+}
+
+// ------------------------------------------------- feed-forward block and cross entropy
+// A matrix's rows as the C ABI takes them: unit inner stride and a row stride of at least a row.
+struct Rows {
+  Tensor t;  // [rows, cols]
+  int64_t rs;
+  void* ptr() const { return t.data_ptr(); }
+  int64_t rows() const { return t.size(0); }
+  int64_t cols() const { return t.size(1); }
+  // Whether the kernels read it in place: whole 16-byte chunks, 16-byte aligned.
+  bool aligned() const {
+    return cols() % 8 == 0 && rs * t.element_size() % 16 == 0 && rs <= (1 << 20) &&
+           reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  }
+};
+Rows rows_of(const Tensor& in) {
+  Tensor t = in.dim() == 2 ? in : in.reshape({-1, in.size(-1)});
+  if (t.size(0) == 1 && (t.stride(1) == 1 || t.size(1) == 1)) return {t, t.size(1)};
+  if (t.stride(1) != 1 || t.stride(0) < t.size(1)) t = t.clone(at::MemoryFormat::Contiguous);
+  return {t, t.stride(0)};
+}
+void check_like(const char* what, const char* name, const Tensor& t, const Tensor& x) {
+  TORCH_CHECK_TYPE(t.scalar_type() == x.scalar_type(), what, ": ", name, " is ", t.scalar_type(),
+                   ", x is ", x.scalar_type());
+  TORCH_CHECK_VALUE(t.device() == x.device(), what, ": ", name, " is on ", t.device(), ", x on ",
+                    x.device());
+}
+Tensor workspace(int64_t bytes, const Tensor& like) {
+  return at::empty({bytes}, like.options().dtype(at::kByte));
+}
+
+struct FfnSizes {
+  int64_t T, D, F, Do, Fp, nb;
+  int code;
+};
+FfnSizes ffn_check(const Tensor& x, const Tensor& w_in, const Tensor& w_down, int64_t act,
+                   int64_t keep) {
+  FfnSizes z;
+  z.code = dtype_code(x, "gated_ffn");
+  check_like("gated_ffn", "w_in", w_in, x);
+  check_like("gated_ffn", "w_down", w_down, x);
+  TORCH_CHECK_VALUE(x.dim() >= 1 && w_in.dim() == 2 && w_down.dim() == 2 &&
+                        x.size(-1) == w_in.size(1) && w_in.size(0) == 2 * w_down.size(1) &&
+                        w_in.numel() > 0 && w_down.numel() > 0,
+                    "gated_ffn: x ", x.sizes(), ", w_in ", w_in.sizes(), " and w_down ",
+                    w_down.sizes(), " must be [..., D], [2 F, D] and [D_out, F]");
+  TORCH_CHECK_VALUE(act == PNFX_ACT_SILU || act == PNFX_ACT_GELU, "gated_ffn: activation ", act);
+  TORCH_CHECK_VALUE(keep >= PNFX_KEEP_NONE && keep <= PNFX_KEEP_E4M3, "gated_ffn: checkpoint ", keep);
+  TORCH_CHECK_VALUE(keep != PNFX_KEEP_E4M3 || z.code == PNFX_BF16,
+                    "gated_ffn: 8-bit checkpoints are of bfloat16 operands, x is ", x.scalar_type());
+  z.D = x.size(-1);
+  z.T = x.numel() / z.D;
+  z.F = w_down.size(1);
+  z.Do = w_down.size(0);
+  z.Fp = (z.F + 7) / 8 * 8;
+  z.nb = (z.F + 31) / 32;
+  return z;
+}
+// Type of what a forward keeps of its projections.
+at::ScalarType kept_type(int64_t keep, int code) {
+  if (code == PNFX_F32) return at::kFloat;
+  return keep == PNFX_KEEP_E4M3 ? at::kByte : at::kHalf;
+}
+std::vector<int64_t> with_last(const Tensor& x, int64_t last) {
+  auto s = x.sizes().vec();
+  s.back() = last;
+  return s;
+}
+
+std::tuple<Tensor, Tensor, Tensor> gated_ffn_cuda(const Tensor& x_in, const Tensor& w_in_,
+                                                  const Tensor& w_down_, int64_t act, int64_t keep) {
+  const FfnSizes z = ffn_check(x_in, w_in_, w_down_, act, keep);
+  const auto bytes = x_in.options().dtype(at::kByte);
+  Tensor y = at::empty(with_last(x_in, z.Do), x_in.options());
+  const auto kept = x_in.options().dtype(kept_type(keep, z.code));
+  Tensor gu = keep == PNFX_KEEP_NONE ? at::empty({0}, kept) : at::empty({z.T, 2, z.Fp}, kept);
+  const bool blocks = keep != PNFX_KEEP_NONE && z.code == PNFX_BF16;
+  Tensor scales = blocks ? at::empty({z.T, 2, z.nb}, bytes) : at::empty({0}, bytes);
+  if (z.T == 0) return {y, gu, scales};
+  const c10::DeviceGuard guard(x_in.device());
+  const Rows x = rows_of(x_in), w_in = rows_of(w_in_), w_down = rows_of(w_down_);
+  const bool copies = !(x.aligned() && w_in.aligned() && w_down.aligned());
+  const int64_t wsb = pnfx_ffn_fwd_workspace_size(z.T, z.D, z.F, z.Do, copies, z.code);
+  Tensor ws = workspace(wsb, x_in);
+  check_rc(pnfx_ffn_fwd(x.ptr(), x.rs, w_in.ptr(), w_in.rs, w_down.ptr(), w_down.rs, y.data_ptr(),
+                        keep ? gu.data_ptr() : nullptr,
+                        blocks ? scales.data_ptr<uint8_t>() : nullptr, z.T, z.D, z.F, z.Do, (int)act,
+                        (int)keep, z.code, ws.data_ptr(), wsb, stream_of(x_in)),
+           "pnfx_ffn_fwd");
+  return {y, gu, scales};
+}
+
+std::tuple<Tensor, Tensor, Tensor> gated_ffn_bwd_cuda(const Tensor& dy_in, const Tensor& x_in,
+                                                      const Tensor& w_in_, const Tensor& w_down_,
+                                                      const Tensor& gu, const Tensor& scales,
+                                                      int64_t act, int64_t keep,
+                                                      std::array<bool, 3> mask) {
+  const FfnSizes z = ffn_check(x_in, w_in_, w_down_, act, keep);
+  TORCH_CHECK_VALUE(keep != PNFX_KEEP_NONE, "gated_ffn_bwd: the forward kept nothing");
+  check_like("gated_ffn_bwd", "dy", dy_in, x_in);
+  TORCH_CHECK_VALUE(dy_in.sizes() == with_last(x_in, z.Do), "gated_ffn_bwd: dy has shape ",
+                    dy_in.sizes(), ", x ", x_in.sizes());
+  check_saved(gu, "gated_ffn_bwd", "gu", z.T * 2 * z.Fp, kept_type(keep, z.code), x_in);
+  if (z.code == PNFX_BF16)
+    check_saved(scales, "gated_ffn_bwd", "scales", z.T * 2 * z.nb, at::kByte, x_in);
+  const auto out = [&](bool wanted, at::IntArrayRef shape) {
+    return at::empty(wanted ? shape : at::IntArrayRef{0}, x_in.options());
+  };
+  Tensor dx = out(mask[0], x_in.sizes()), dw_in = out(mask[1], w_in_.sizes()),
+         dw_down = out(mask[2], w_down_.sizes());
+  if (z.T == 0) return {dx, dw_in.zero_(), dw_down.zero_()};
+  const c10::DeviceGuard guard(x_in.device());
+  const Rows dy = rows_of(dy_in), x = rows_of(x_in), w_in = rows_of(w_in_), w_down = rows_of(w_down_);
+  const Tensor gu16 = reinterpret_cast<uintptr_t>(gu.data_ptr()) % 16 ? gu.clone() : gu;
+  const bool copies = !(dy.aligned() && x.aligned() && w_in.aligned() && w_down.aligned());
+  const int64_t wsb = pnfx_ffn_bwd_workspace_size(z.T, z.D, z.F, z.Do, copies, z.code);
+  Tensor ws = workspace(wsb, x_in);
+  check_rc(pnfx_ffn_bwd(dy.ptr(), dy.rs, x.ptr(), x.rs, w_in.ptr(), w_in.rs, w_down.ptr(), w_down.rs,
+                        gu16.data_ptr(),
+                        z.code == PNFX_BF16 ? scales.data_ptr<uint8_t>() : nullptr,
+                        mask[0] ? dx.data_ptr() : nullptr, mask[1] ? dw_in.data_ptr() : nullptr,
+                        mask[2] ? dw_down.data_ptr() : nullptr, z.T, z.D, z.F, z.Do, (int)act,
+                        (int)keep, z.code, ws.data_ptr(), wsb, stream_of(x_in)),
+           "pnfx_ffn_bwd");
+  return {dx, dw_in, dw_down};
+}
+
+struct XentSizes {
+  int64_t T, D, V;
+  int code;
+};
+XentSizes xent_check(const Tensor& x, const Tensor& w, const Tensor& target, int64_t reduction) {
+  XentSizes z;
+  z.code = dtype_code(x, "linear_xent");
+  check_like("linear_xent", "weight", w, x);
+  TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1) && w.numel() > 0,
+                    "linear_xent: x ", x.sizes(), " and weight ", w.sizes(),
+                    " must be [..., D] and [V, D]");
+  TORCH_CHECK_TYPE(target.scalar_type() == at::kLong, "linear_xent: target is ",
+                   target.scalar_type(), " (int64)");
+  TORCH_CHECK_VALUE(target.sizes() == x.sizes().slice(0, x.dim() - 1), "linear_xent: target ",
+                    target.sizes(), " must have x's rows, ", x.sizes());
+  TORCH_CHECK_VALUE(target.device() == x.device(), "linear_xent: target is on ", target.device(),
+                    ", x on ", x.device());
+  TORCH_CHECK_VALUE(reduction >= PNFX_REDUCE_NONE && reduction <= PNFX_REDUCE_MEAN,
+                    "linear_xent: reduction ", reduction);
+  z.D = x.size(-1);
+  z.V = w.size(0);
+  z.T = x.numel() / z.D;
+  return z;
+}
+
+std::tuple<Tensor, Tensor, Tensor> linear_xent_cuda(const Tensor& x_in, const Tensor& w_in,
+                                                    const Tensor& target, int64_t ignore_index,
+                                                    int64_t reduction) {
+  const XentSizes z = xent_check(x_in, w_in, target, reduction);
+  const auto f32 = x_in.options().dtype(at::kFloat);
+  const bool none = reduction == PNFX_REDUCE_NONE;
+  Tensor loss = none ? at::empty(target.sizes(), f32) : at::empty({}, f32);
+  Tensor rows = at::empty({z.T}, f32), lse = at::empty({z.T}, f32);
+  if (z.T == 0) {  // no rows: the sum is 0, the mean 0 / 0
+    if (!none) loss.fill_(reduction == PNFX_REDUCE_MEAN ? NAN : 0.0);
+    return {loss, rows, lse};
+  }
+  const c10::DeviceGuard guard(x_in.device());
+  const Rows x = rows_of(x_in), w = rows_of(w_in);
+  const Tensor t = target.contiguous();
+  const int64_t wsb = pnfx_xent_fwd_workspace_size(z.T, z.D, z.V, !w.aligned(), z.code);
+  Tensor ws = workspace(wsb, x_in);
+  check_rc(pnfx_xent_fwd(x.ptr(), x.rs, w.ptr(), w.rs, t.data_ptr<int64_t>(), ignore_index,
+                         loss.data_ptr<float>(), rows.data_ptr<float>(), lse.data_ptr<float>(), z.T,
+                         z.D, z.V, (int)reduction, z.code, ws.data_ptr(), wsb, stream_of(x_in)),
+           "pnfx_xent_fwd");
+  return {loss, rows, lse};
+}
+
+std::tuple<Tensor, Tensor> linear_xent_bwd_cuda(const Tensor& dloss_in, const Tensor& x_in,
+                                                const Tensor& w_in, const Tensor& target,
+                                                const Tensor& rows, const Tensor& lse,
+                                                int64_t ignore_index, int64_t reduction,
+                                                std::array<bool, 2> mask) {
+  const XentSizes z = xent_check(x_in, w_in, target, reduction);
+  TORCH_CHECK_VALUE(reduction == PNFX_REDUCE_NONE ? dloss_in.sizes() == target.sizes()
+                                                  : dloss_in.numel() == 1,
+                    "linear_xent_bwd: dloss has shape ", dloss_in.sizes());
+  TORCH_CHECK_VALUE(dloss_in.device() == x_in.device(), "linear_xent_bwd: dloss is on ",
+                    dloss_in.device(), ", x on ", x_in.device());
+  check_saved(rows, "linear_xent_bwd", "rows", z.T, at::kFloat, x_in);
+  check_saved(lse, "linear_xent_bwd", "lse", z.T, at::kFloat, x_in);
+  const auto out = [&](bool wanted, at::IntArrayRef shape) {
+    return at::empty(wanted ? shape : at::IntArrayRef{0}, x_in.options());
+  };
+  Tensor dx = out(mask[0], x_in.sizes()), dw = out(mask[1], w_in.sizes());
+  if (z.T == 0) return {dx, dw.zero_()};
+  const c10::DeviceGuard guard(x_in.device());
+  const Tensor dloss = dloss_in.to(at::kFloat).contiguous();
+  const Rows x = rows_of(x_in), w = rows_of(w_in);
+  const Tensor t = target.contiguous();
+  const int64_t wsb = pnfx_xent_bwd_workspace_size(z.T, z.D, z.V, !w.aligned(), z.code);
+  Tensor ws = workspace(wsb, x_in);
+  check_rc(pnfx_xent_bwd(dloss.data_ptr<float>(), x.ptr(), x.rs, w.ptr(), w.rs,
+                         t.data_ptr<int64_t>(), ignore_index, rows.data_ptr<float>(),
+                         lse.data_ptr<float>(), mask[0] ? dx.data_ptr() : nullptr,
+                         mask[1] ? dw.data_ptr() : nullptr, z.T, z.D, z.V, (int)reduction, z.code,
+                         ws.data_ptr(), wsb, stream_of(x_in)),
+           "pnfx_xent_bwd");
+  return {dx, dw};
 }
 
 // ------------------------------------------------------------------------------ flash
@@ -775,6 +985,116 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> attn_rows_autograd(
   return {r[0], r[1], r[2], r[3], r[4], r[5]};
 }
 
+// The backward passes below are kernels that autograd cannot follow: a second derivative is refused.
+void check_first_order(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what, ": second derivatives (create_graph) are not supported");
+}
+
+const auto& gated_ffn_op() {
+  static auto h = op("pnfx::gated_ffn")
+                      .typed<std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&,
+                                                                const Tensor&, int64_t, int64_t)>();
+  return h;
+}
+
+class GatedFfnFn : public torch::autograd::Function<GatedFfnFn> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_in,
+                               const Tensor& w_down, int64_t act, int64_t keep) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [y, gu, scales] = gated_ffn_op().call(x, w_in, w_down, act, keep);
+    ctx->mark_non_differentiable({gu, scales});
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, w_in, w_down, gu, scales});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["keep"] = keep;
+    return {y, gu, scales};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    static auto bwd = op("pnfx::gated_ffn_bwd")
+                          .typed<std::tuple<Tensor, Tensor, Tensor>(
+                              const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                              const Tensor&, int64_t, int64_t, std::array<bool, 3>)>();
+    variable_list grads(5);
+    if (!g[0].defined()) return grads;
+    check_first_order("gated_ffn");
+    const auto s = ctx->get_saved_variables();
+    const std::array<bool, 3> mask = {ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+                                      ctx->needs_input_grad(2)};
+    auto [dx, dw_in, dw_down] =
+        bwd.call(g[0], s[0], s[1], s[2], s[3], s[4], ctx->saved_data["act"].toInt(),
+                 ctx->saved_data["keep"].toInt(), mask);
+    if (mask[0]) grads[0] = dx;
+    if (mask[1]) grads[1] = dw_in;
+    if (mask[2]) grads[2] = dw_down;
+    return grads;
+  }
+};
+
+// Without a gradient to come nothing is kept, whatever `keep` says.
+std::tuple<Tensor, Tensor, Tensor> gated_ffn_autograd(const Tensor& x, const Tensor& w_in,
+                                                      const Tensor& w_down, int64_t act,
+                                                      int64_t keep) {
+  if (keep == PNFX_KEEP_NONE || !records({&x, &w_in, &w_down})) {
+    TORCH_CHECK_VALUE(!records({&x, &w_in, &w_down}),
+                      "gated_ffn: a call that keeps nothing has no gradients");
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return gated_ffn_op().call(x, w_in, w_down, act, keep);
+  }
+  auto r = GatedFfnFn::apply(x, w_in, w_down, act, keep);
+  return {r[0], r[1], r[2]};
+}
+
+const auto& linear_xent_op() {
+  static auto h = op("pnfx::linear_xent")
+                      .typed<std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&,
+                                                                const Tensor&, int64_t, int64_t)>();
+  return h;
+}
+
+class LinearXentFn : public torch::autograd::Function<LinearXentFn> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w,
+                               const Tensor& target, int64_t ignore_index, int64_t reduction) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [loss, rows, lse] = linear_xent_op().call(x, w, target, ignore_index, reduction);
+    ctx->mark_non_differentiable({rows, lse});
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, w, target, rows, lse});
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["reduction"] = reduction;
+    return {loss, rows, lse};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    static auto bwd = op("pnfx::linear_xent_bwd")
+                          .typed<std::tuple<Tensor, Tensor>(
+                              const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                              const Tensor&, int64_t, int64_t, std::array<bool, 2>)>();
+    variable_list grads(5);
+    if (!g[0].defined()) return grads;
+    check_first_order("linear_xent");
+    const auto s = ctx->get_saved_variables();
+    const std::array<bool, 2> mask = {ctx->needs_input_grad(0), ctx->needs_input_grad(1)};
+    auto [dx, dw] = bwd.call(g[0], s[0], s[1], s[2], s[3], s[4],
+                             ctx->saved_data["ignore_index"].toInt(),
+                             ctx->saved_data["reduction"].toInt(), mask);
+    if (mask[0]) grads[0] = dx;
+    if (mask[1]) grads[1] = dw;
+    return grads;
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor> linear_xent_autograd(const Tensor& x, const Tensor& w,
+                                                        const Tensor& target, int64_t ignore_index,
+                                                        int64_t reduction) {
+  if (!records({&x, &w})) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return linear_xent_op().call(x, w, target, ignore_index, reduction);
+  }
+  auto r = LinearXentFn::apply(x, w, target, ignore_index, reduction);
+  return {r[0], r[1], r[2]};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(pnfx, m) {
@@ -787,6 +1107,14 @@ TORCH_LIBRARY(pnfx, m) {
   m.def("sum_f64(Tensor x, bool wide) -> Tensor");
   m.def("linear(Tensor x, Tensor w) -> Tensor");
   m.def("linear_wgrad(Tensor dy, Tensor x, bool wide) -> Tensor");
+  m.def("gated_ffn(Tensor x, Tensor w_in, Tensor w_down, int act, int keep) -> "
+        "(Tensor, Tensor, Tensor)");
+  m.def("gated_ffn_bwd(Tensor dy, Tensor x, Tensor w_in, Tensor w_down, Tensor gu, Tensor scales, "
+        "int act, int keep, bool[3] mask) -> (Tensor, Tensor, Tensor)");
+  m.def("linear_xent(Tensor x, Tensor w, Tensor target, int ignore_index, int reduction) -> "
+        "(Tensor, Tensor, Tensor)");
+  m.def("linear_xent_bwd(Tensor dloss, Tensor x, Tensor w, Tensor target, Tensor rows, Tensor lse, "
+        "int ignore_index, int reduction, bool[2] mask) -> (Tensor, Tensor)");
   m.def("flash_fwd(Tensor q, Tensor k, Tensor v, Tensor tau, float scale, float gamma, "
         "bool has_gamma, bool causal, bool o_bnhd, bool with_nmax) -> "
         "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
@@ -811,6 +1139,10 @@ TORCH_LIBRARY_IMPL(pnfx, CUDA, m) {
   m.impl("sum_f64", sum_f64_cuda);
   m.impl("linear", linear_cuda);
   m.impl("linear_wgrad", linear_wgrad_cuda);
+  m.impl("gated_ffn", gated_ffn_cuda);
+  m.impl("gated_ffn_bwd", gated_ffn_bwd_cuda);
+  m.impl("linear_xent", linear_xent_cuda);
+  m.impl("linear_xent_bwd", linear_xent_bwd_cuda);
   m.impl("flash_fwd", flash_fwd_cuda);
   m.impl("flash_bwd", flash_bwd_cuda);
   m.impl("attn_rows", attn_rows_cuda);
@@ -823,5 +1155,7 @@ TORCH_LIBRARY_IMPL(pnfx, Autograd, m) {
   m.impl("pn_rows_fwd", pn_rows_fwd_autograd);
   m.impl("linear", linear_autograd);
   m.impl("attn_rows", attn_rows_autograd);
+  m.impl("gated_ffn", gated_ffn_autograd);
+  m.impl("linear_xent", linear_xent_autograd);
   m.impl("flash_fwd", flash_fwd_autograd);
 }

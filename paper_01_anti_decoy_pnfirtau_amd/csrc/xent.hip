@@ -1,0 +1,627 @@
+// Softmax cross entropy of the logits z = x W^T (x [T, D], W [V, D]) against target tokens, without the logits:
+//   lse_t = log sum_v exp z_tv,  loss_t = lse_t - z_t,target,  d_tv = (exp(z_tv - lse_t) - [v = target_t]) s_t,
+//   dx = d W,  dW = d^T x,
+// with s_t the loss's gradient of row t (1 / kept rows of it for a mean).
+//
+// Rows whose target is ignore_index are left out before anything else: xent_rows_kernel copies the others to
+// the front of a buffer, so they cost no products, and what they hold, infinities included, reaches no sum.
+//
+// Forward: workgroups of one tile of rows each run over a range of the vocabulary and keep, in registers, the
+// running maximum and the sum of exponentials of what each lane has seen; xent_loss_kernel joins them.  The
+// target's logit is a dot product of its own.
+//
+// Backward: z is computed again for a piece of the vocabulary at a time (a piece's d, in the operands' type,
+// stays in the 256 MB last-level cache while both gradients read it) and d is written in place of the
+// logits; then dx += d W over the piece, in fp32, and the piece's rows of dW = d^T x.  bf16 operands: d is
+// rounded to bf16 once, 2^-8 of each of its elements at most, as it is an operand of bf16 products.  It is
+// rounded without s_t: the target's element, close to -1 for most rows, would otherwise be off by the same
+// amount in each of them, and a frequent token's sum with it (0.4 % where 1 / rows rounds badly).  s_t enters the
+// fp32 results where it is one value, and for a loss per row dx's rows and the x of dW = d^T (s x).  The target's
+// own element is expm1(-loss_t), which keeps its digits where the softmax is close to one.
+//
+// Exponentials are taken in base 2, exp2(z L - m L) with L = log2 e as one fma per logit.  The rounding of m L is
+// the same for a whole row and comes out again as the factor unround(m) = exp2(round(m L) - m L): without it logits
+// around 5e4 would be 4e-3 off.
+#include <algorithm>
+
+#include "product.h"
+
+namespace pnfx {
+namespace {
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float unround(float m) { return exp2_fast(-__builtin_fmaf(m, kLog2e, -(m * kLog2e))); }
+// Joins (top, sum) with (top2, sum2): maxima of logits and sums of exponentials beside them.  While nothing but
+// -infinity was seen there is nothing to scale.
+__device__ __forceinline__ void join(float& top, float& sum, float top2, float sum2) {
+  const float next = fmaxf(top, top2), ref = next == -INFINITY ? 0.f : next;
+  sum = sum * exp2_fast((top - ref) * kLog2e) + sum2 * exp2_fast((top2 - ref) * kLog2e);
+  top = next;
+}
+
+// -------------------------------------------------------------------------- kept rows
+constexpr int kRowsBlocks = 512;
+
+struct RowsArgs {
+  const void* x;
+  const int64_t* target;
+  void* xc;         // [T][Dp] kept rows, zero-padded
+  int* pos;         // [T] place of a row among the kept ones, or -1
+  int* src;         // [kept] row
+  int* tgt;         // [kept] target, or -1 where it is no token
+  int* count;
+  int64_t x_rs, ignore;
+  int T, D, Dp, V, per;  // per: rows of a workgroup
+  // backward only: row constants {lse, s_t, loss_t, 1 or NaN}; s_t where it is one value; s_t x_t where not
+  const float* lse;
+  const float* loss;
+  const float* dloss;
+  float4* rowc;
+  float* alpha;
+  void* xs;
+  int reduction;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs a) {
+  __shared__ int red[4];
+  __shared__ int list[256];
+  __shared__ float scale[256];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int r0 = blockIdx.x * a.per, r1 = min(r0 + a.per, a.T);
+  // kept rows before this workgroup's, and (backward, for the mean) behind them
+  int before = 0, total = 0;
+  const int to = a.rowc ? a.T : r0;
+  for (int r = tid; r < to; r += 256) {
+    const int k = a.target[r] != a.ignore;
+    total += k;
+    if (r < r0) before += k;
+  }
+  const auto block_sum = [&](int v) {
+    v = wave_sum_i(v);
+    __syncthreads();
+    if (lane == 0) red[wave] = v;
+    __syncthreads();
+    return red[0] + red[1] + red[2] + red[3];
+  };
+  before = block_sum(before);
+  if (a.rowc) total = block_sum(total);
+  float row_scale = 1.f;
+  if (a.rowc && a.reduction != PNFX_REDUCE_NONE) {
+    row_scale = a.reduction == PNFX_REDUCE_SUM ? a.dloss[0]
+                : total ? a.dloss[0] / (float)total : 0.f;  // no rows: no gradients
+    if (blockIdx.x == 0 && tid == 0) *a.alpha = row_scale;
+  }
+  for (int c0 = r0; c0 < r1; c0 += 256) {
+    const int r = c0 + tid;
+    const int64_t t = r < r1 ? a.target[r] : a.ignore;
+    const bool keep = r < r1 && t != a.ignore;
+    const uint64_t mask = __ballot(keep);
+    __syncthreads();
+    if (lane == 0) red[wave] = __popcll(mask);
+    __syncthreads();
+    int at = __popcll(mask & ((1ull << lane) - 1));
+    for (int w = 0; w < wave; ++w) at += red[w];
+    const int n = red[0] + red[1] + red[2] + red[3];
+    if (keep) {
+      const int i = before + at;
+      const bool valid = t >= 0 && t < a.V;
+      list[at] = r;
+      a.src[i] = r;
+      a.tgt[i] = valid ? (int)t : -1;
+      if (a.rowc) {
+        const float s = a.reduction == PNFX_REDUCE_NONE ? a.dloss[r] : row_scale;
+        // a target that is no token: its loss is NaN, and so are its gradients
+        a.rowc[i] = float4{a.lse[r], s, a.loss[r], valid ? 1.f : __builtin_nanf("")};
+        scale[at] = s;
+      }
+    }
+    if (r < r1) a.pos[r] = keep ? before + at : -1;
+    __syncthreads();
+    for (int i = wave; i < n; i += 4) {
+      const T* x = static_cast<const T*>(a.x) + (int64_t)list[i] * a.x_rs;
+      T* y = static_cast<T*>(a.xc) + (int64_t)(before + i) * a.Dp;
+      if (a.xs) {
+        T* ys = static_cast<T*>(a.xs) + (int64_t)(before + i) * a.Dp;
+        const float s = scale[i];
+        for (int c = lane; c < a.Dp; c += 64) {
+          const T v = c < a.D ? x[c] : (T)0.f;
+          y[c] = v;
+          ys[c] = from_f32<T>(to_f32(v) * s);
+        }
+      } else {
+        for (int c = lane; c < a.Dp; c += 64) y[c] = c < a.D ? x[c] : (T)0.f;
+      }
+    }
+    before += n;
+  }
+  if (r1 == a.T && tid == 0) *a.count = before;
+}
+
+// -------------------------------------------------------------------------- forward
+struct FwdArgs {
+  const void* xc;
+  const void* w;
+  float2* part;  // [splits * WN][T] running maximum and sum
+  const int* count;
+  int64_t ldx, ldw, K;
+  int T, V, tm, tn, splits, per;  // per: vocabulary tiles of a split
+};
+
+template <typename T, class C>
+__global__ __launch_bounds__(threads_of<C>, 2) void xent_fwd_kernel(FwdArgs a) {
+  typedef Product<T, ROW, ROW, C> P;
+  extern __shared__ __align__(16) char sm[];
+  int tm, split;
+  tile_of(blockIdx.x, a.tm, a.splits, tm, split);
+  const int M = *a.count, m0 = tm * C::TM;
+  if (m0 >= M) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wm = wave / C::WN * P::MI, wn = wave % C::WN * P::NJ;
+  float top[P::MI], sum[P::MI];
+#pragma unroll
+  for (int i = 0; i < P::MI; ++i) top[i] = -INFINITY, sum[i] = 0.f;
+  const int t1 = min(a.tn, (split + 1) * a.per);
+  for (int t = split * a.per; t < t1; ++t) {
+    const int n0 = t * C::TN;
+    typename P::StageA sa;
+    typename P::StageB sb;
+    sa.init(static_cast<const T*>(a.xc) + m0 * a.ldx, a.ldx, M - m0, a.K, threadIdx.x);
+    sb.init(static_cast<const T*>(a.w) + n0 * a.ldw, a.ldw, a.V - n0, a.K, threadIdx.x);
+    f32x4 acc[P::MI][P::NJ] = {};
+    P::run(sa, sb, (int)((a.K + k_step<T> - 1) / k_step<T>), reinterpret_cast<T*>(sm), wave, lane, acc);
+    if (n0 + C::TN > a.V) {  // past the vocabulary
+#pragma unroll
+      for (int j = 0; j < P::NJ; ++j) {
+        const int n = n0 + stage_row<ROW>(wn + j, 4 * (lane >> 4));
+#pragma unroll
+        for (int i = 0; i < P::MI; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (n + r >= a.V) acc[i][j][r] = -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < P::MI; ++i) {
+      float m = acc[i][0][0];
+#pragma unroll
+      for (int j = 0; j < P::NJ; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[i][j][r]);
+      const float ref = m == -INFINITY ? 0.f : m;
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < P::NJ; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s += exp2_fast(__builtin_fmaf(acc[i][j][r], kLog2e, -(ref * kLog2e)));
+      join(top[i], sum[i], m, s * unround(ref));
+    }
+  }
+  // over the four lanes of a row
+#pragma unroll
+  for (int i = 0; i < P::MI; ++i) {
+#pragma unroll
+    for (int o = 16; o <= 32; o <<= 1)
+      join(top[i], sum[i], __shfl_xor(top[i], o, 64), __shfl_xor(sum[i], o, 64));
+    const int m = m0 + stage_row<ROW>(wm + i, lane & 15);
+    if (lane < 16 && m < M) a.part[(int64_t)(split * C::WN + wave % C::WN) * a.T + m] = float2{top[i], sum[i]};
+  }
+}
+
+struct LossArgs {
+  const void* xc;
+  const void* w;
+  const float2* part;
+  const int *pos, *tgt, *count;
+  float *rows, *lse;   // [T] loss and log-sum-exp of every row (ignored: 0)
+  float* out;          // reduction none: [T]
+  double* sums;        // per workgroup
+  int64_t ldx, ldw;
+  int T, K, parts, reduction, per;  // per: rows of a workgroup
+};
+// One wave per row: joins the row's partial statistics, forms the target's logit and the loss.
+template <typename T>
+__global__ __launch_bounds__(256) void xent_loss_kernel(LossArgs a) {
+  __shared__ double red[4];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int r0 = blockIdx.x * a.per, r1 = min(r0 + a.per, a.T);
+  double total = 0;
+  for (int r = r0 + wave; r < r1; r += 4) {
+    const int i = a.pos[r];
+    float loss = 0.f, lse = 0.f;
+    if (i >= 0) {
+      float top = -INFINITY, sum = 0.f;
+      for (int p = lane; p < a.parts; p += 64) {
+        const float2 v = a.part[(int64_t)p * a.T + i];
+        join(top, sum, v.x, v.y);
+      }
+      const int t = a.tgt[i];
+      float dot = 0.f;
+      if (t >= 0) {
+        const T* x = static_cast<const T*>(a.xc) + i * a.ldx;
+        const T* w = static_cast<const T*>(a.w) + t * a.ldw;
+        for (int k = lane; k < a.K; k += 64) dot = __builtin_fmaf(to_f32(x[k]), to_f32(w[k]), dot);
+      }
+      const float m = wave_max(top), ref = m == -INFINITY ? 0.f : m;
+      sum = wave_sum(sum * exp2_fast((top - ref) * kLog2e));
+      dot = wave_sum(dot);
+      const float log_sum = __builtin_amdgcn_logf(sum) * kLn2;
+      lse = m + log_sum;
+      // of a softmax close to one the difference may round to below zero
+      loss = t >= 0 ? (m - dot) + log_sum : __builtin_nanf("");
+      loss = loss < 0.f ? 0.f : loss;
+    }
+    if (lane == 0) {
+      a.rows[r] = loss;
+      a.lse[r] = lse;
+      if (a.reduction == PNFX_REDUCE_NONE) a.out[r] = loss;
+    }
+    total += loss;
+  }
+  if (a.reduction == PNFX_REDUCE_NONE) return;
+  if (lane == 0) red[wave] = total;
+  __syncthreads();
+  if (threadIdx.x == 0) a.sums[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+// The workgroups' sums in a fixed order.
+__global__ __launch_bounds__(64) void xent_total_kernel(const double* sums, int n, const int* count, float* out,
+                                                        int reduction) {
+  double v = 0;
+  for (int i = threadIdx.x; i < n; i += 64) v += sums[i];
+  v = wave_sum_d(v);
+  if (threadIdx.x == 0) *out = (float)(reduction == PNFX_REDUCE_MEAN ? v / *count : v);
+}
+
+// -------------------------------------------------------------------------- backward
+struct GradArgs {
+  const void* xc;
+  const void* w;      // the piece's first row
+  void* d;            // [T][ldd]
+  const float4* rowc;
+  const int *tgt, *count;
+  int64_t ldx, ldw, K, ldd;
+  int v0, P, tm, tn;  // the piece's first token, its tokens
+};
+
+template <typename T, class C>
+__global__ __launch_bounds__(threads_of<C>, 2) void xent_grad_kernel(GradArgs a) {
+  typedef Product<T, ROW, ROW, C> P;
+  extern __shared__ __align__(16) char sm[];
+  int tm, tn;
+  tile_of(blockIdx.x, a.tm, a.tn, tm, tn);
+  const int M = *a.count, m0 = tm * C::TM, n0 = tn * C::TN;
+  if (m0 >= M) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wm = wave / C::WN * P::MI, wn = wave % C::WN * P::NJ;
+  typename P::StageA sa;
+  typename P::StageB sb;
+  sa.init(static_cast<const T*>(a.xc) + m0 * a.ldx, a.ldx, M - m0, a.K, threadIdx.x);
+  sb.init(static_cast<const T*>(a.w) + n0 * a.ldw, a.ldw, a.P - n0, a.K, threadIdx.x);
+  f32x4 acc[P::MI][P::NJ] = {};
+  P::run(sa, sb, (int)((a.K + k_step<T> - 1) / k_step<T>), reinterpret_cast<T*>(sm), wave, lane, acc);
+  const int Pc = (a.P + 7) & ~7;  // columns past the piece, up to a whole chunk, are zero
+#pragma unroll
+  for (int i = 0; i < P::MI; ++i) {
+    const int m = m0 + stage_row<ROW>(wm + i, lane & 15);
+    if (m >= M) continue;
+    const float4 c = a.rowc[m];
+    const float lse = c.x * kLog2e, factor = c.w * unround(c.x);
+    T* row = static_cast<T*>(a.d) + m * a.ldd;
+    // two blocks: eight columns of a lane
+#pragma unroll
+    for (int j = 0; j < P::NJ; j += 2) {
+      const int n = n0 + stage_row<ROW>(wn + j, 4 * (lane >> 4));
+      if (n >= Pc) continue;
+      float v[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        v[r] = exp2_fast(__builtin_fmaf(acc[i][j + (r >> 2)][r & 3], kLog2e, -lse)) * factor;
+        if (n + r >= a.P) v[r] = 0.f;
+      }
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<bf16x8*>(row + n) = pack8(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
+      } else {
+        *reinterpret_cast<f32x4*>(row + n) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4*>(row + n + 4) = f32x4{v[4], v[5], v[6], v[7]};
+      }
+    }
+  }
+  // the targets of this tile's rows that are in its columns, once the tile's stores are done
+  __builtin_amdgcn_s_waitcnt(0x0F70);
+  __syncthreads();
+  for (int r = threadIdx.x; r < C::TM && m0 + r < M; r += threads_of<C>) {
+    const int m = m0 + r, t = a.tgt[m] - a.v0;
+    if (t >= n0 && t < min(n0 + C::TN, a.P)) {
+      static_cast<T*>(a.d)[m * a.ldd + t] = from_f32<T>(expm1f(-a.rowc[m].z));
+    }
+  }
+}
+
+struct DxArgs {
+  const float* sums;  // [splits][T][D]
+  const float4* rowc;
+  const int* pos;
+  void* dx;           // [T][D]
+  int64_t TD;
+  int D, splits;
+};
+// dx in the operands' type: s_t times the splits' sums of a kept row, in split order, zeros for the others.
+template <typename T>
+__global__ __launch_bounds__(256) void xent_dx_kernel(DxArgs a) {
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int per = a.D % 4 == 0 ? 4 : 1;
+  if (e * per >= a.TD) return;
+  const int row = (int)(e * per / a.D), col = (int)(e * per % a.D), i = a.pos[row];
+  T* dx = static_cast<T*>(a.dx) + e * per;
+  const float* s = a.sums + (int64_t)i * a.D + col;
+  if (per == 4) {
+    f32x4 v = {};
+    if (i >= 0)
+      for (int p = 0; p < a.splits; ++p) v += *reinterpret_cast<const f32x4*>(s + p * a.TD);
+    if (i >= 0) v *= a.rowc[i].y;
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<bf16x4*>(dx) = bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
+    else *reinterpret_cast<f32x4*>(dx) = v;
+  } else {
+    float v = 0.f;
+    if (i >= 0)
+      for (int p = 0; p < a.splits; ++p) v += s[p * a.TD];
+    if (i >= 0) v *= a.rowc[i].y;
+    *dx = from_f32<T>(v);
+  }
+}
+
+// -------------------------------------------------------------------------- host side
+struct Sizes {
+  int64_t T, D, V, Dp;
+  int es, dtype;
+};
+Sizes sizes_of(int64_t T, int64_t D, int64_t V, int dtype) {
+  return Sizes{T, D, V, round_up(D, 8), dtype == PNFX_F32 ? 4 : 2, dtype};
+}
+struct Arena {
+  char* p;
+  int64_t used;
+  template <typename U>
+  U* take(int64_t n) {
+    char* r = p ? p + used : nullptr;
+    used += round_up(n * (int64_t)sizeof(U), 256);
+    return reinterpret_cast<U*>(r);
+  }
+};
+
+// The forward's cut: tiles of rows by ranges of the vocabulary, two or more workgroups for each place on the chip.
+struct FwdCut {
+  bool big;
+  int64_t tm, tn, splits, per;
+};
+FwdCut fwd_cut(const Sizes& z) {
+  FwdCut c;
+  // The exponentials of a 256-tile are not hidden by a neighbour's products (128-tiles share a CU), so a large
+  // tile pays only where the products take several times as long.
+  c.big = z.dtype == PNFX_BF16 && z.D >= 768 && ceil_div(z.T, 256) * ceil_div(z.V, 256) >= 512;
+  c.tm = ceil_div(z.T, c.big ? 256 : 128);
+  c.tn = ceil_div(z.V, c.big ? 256 : 128);
+  const int64_t want = ceil_div(c.big ? 1024 : 2048, c.tm);
+  c.per = ceil_div(c.tn, std::min(want, c.tn));
+  c.splits = ceil_div(c.tn, c.per);
+  return c;
+}
+// Rows of d that stay in the last-level cache with their piece's weights: 64 MB.
+int64_t piece_of(const Sizes& z) {
+  const int64_t most = std::min(round_up(std::max<int64_t>((64ll << 20) / (z.T * z.es), 2048), 256), kMaxLd / 2);
+  const int64_t n = ceil_div(z.V, most);
+  return round_up(ceil_div(z.V, n), 256);
+}
+
+struct Kept {
+  void* xc;
+  int *pos, *src, *tgt, *count;
+  void* w;  // padded copy, or null
+};
+Kept take_kept(Arena& ar, const Sizes& z, bool copy) {
+  Kept k;
+  k.xc = ar.take<char>(z.T * z.Dp * z.es);
+  k.pos = ar.take<int>(z.T);
+  k.src = ar.take<int>(z.T);
+  k.tgt = ar.take<int>(z.T);
+  k.count = ar.take<int>(1);
+  k.w = copy ? ar.take<char>(z.V * z.Dp * z.es) : nullptr;
+  return k;
+}
+int loss_rows_per(const Sizes& z) { return (int)std::max<int64_t>(4, ceil_div(z.T, 2048)); }
+int64_t loss_blocks(const Sizes& z) { return ceil_div(z.T, loss_rows_per(z)); }
+
+int64_t fwd_bytes(const Sizes& z, bool copy) {
+  Arena ar{nullptr, 0};
+  take_kept(ar, z, copy);
+  const FwdCut c = fwd_cut(z);
+  ar.take<float2>(c.splits * 4 * z.T);
+  ar.take<double>(loss_blocks(z));
+  return ar.used;
+}
+struct BwdCut {
+  int64_t P;
+  Cut dx, dw;
+};
+BwdCut bwd_cut(const Sizes& z) {
+  BwdCut c;
+  c.P = std::min(piece_of(z), round_up(z.V, 8));
+  c.dx = cut_of(z.T, z.D, c.P, z.dtype, true);
+  c.dw = cut_of(c.P, z.D, z.T, z.dtype, true);
+  return c;
+}
+int64_t bwd_bytes(const Sizes& z, bool copy) {
+  Arena ar{nullptr, 0};
+  take_kept(ar, z, copy);
+  ar.take<float>(1);
+  ar.take<char>(z.T * z.Dp * z.es);  // s x, of a loss per row
+  const BwdCut c = bwd_cut(z);
+  ar.take<float4>(z.T);
+  ar.take<char>(z.T * c.P * z.es);
+  ar.take<float>(c.dx.splits * z.T * z.D);
+  ar.take<char>(product_workspace(c.dw, c.P, z.D));
+  return ar.used;
+}
+
+template <typename T>
+int keep_rows(const Kept& k, const void* x, int64_t x_rs, const int64_t* target, int64_t ignore, const Sizes& z,
+              RowsArgs a, hipStream_t st) {
+  a.x = x, a.target = target, a.xc = k.xc, a.pos = k.pos, a.src = k.src, a.tgt = k.tgt, a.count = k.count;
+  a.x_rs = x_rs, a.ignore = ignore;
+  a.T = (int)z.T, a.D = (int)z.D, a.Dp = (int)z.Dp, a.V = (int)z.V;
+  a.per = (int)std::max<int64_t>(16, ceil_div(z.T, kRowsBlocks));
+  return launch<xent_rows_kernel<T>>(ceil_div(z.T, a.per), 256, 0, a, st, "xent rows");
+}
+// W in place, or its padded copy.
+int take_w(const Kept& k, const void*& w, int64_t& w_rs, const Sizes& z, hipStream_t st) {
+  if (!k.w) return PNFX_OK;
+  const PadItem p{w, k.w, w_rs, z.V, z.D, z.V, z.Dp, 1};
+  PNFX_TRY(pad(&p, 1, z.dtype, st));
+  w = k.w, w_rs = z.Dp;
+  return PNFX_OK;
+}
+
+template <typename T>
+int xent_fwd(const void* x, int64_t x_rs, const void* w, int64_t w_rs, const int64_t* target, int64_t ignore,
+             float* out, float* rows, float* lse, int reduction, const Sizes& z, bool copy, void* ws, hipStream_t st) {
+  Arena ar{static_cast<char*>(ws), 0};
+  const Kept k = take_kept(ar, z, copy);
+  const FwdCut c = fwd_cut(z);
+  float2* part = ar.take<float2>(c.splits * 4 * z.T);
+  double* sums = ar.take<double>(loss_blocks(z));
+  PNFX_TRY(take_w(k, w, w_rs, z, st));
+  PNFX_TRY(keep_rows<T>(k, x, x_rs, target, ignore, z, RowsArgs{}, st));
+  FwdArgs f{k.xc, w, part, k.count, z.Dp, w_rs, z.Dp, (int)z.T, (int)z.V, (int)c.tm, (int)c.tn, (int)c.splits, (int)c.per};
+  int wn = Mid::WN;
+  if constexpr (sizeof(T) == 2) {
+    if (c.big) {
+      wn = Big::WN;
+      PNFX_TRY((launch<xent_fwd_kernel<T, Big>>(c.tm * c.splits, threads_of<Big>, lds_of<Big>, f, st, "xent_fwd")));
+    }
+  }
+  if (!c.big)
+    PNFX_TRY((launch<xent_fwd_kernel<T, Mid>>(c.tm * c.splits, threads_of<Mid>, lds_of<Mid>, f, st, "xent_fwd")));
+  LossArgs l{k.xc, w, part, k.pos, k.tgt, k.count, rows, lse, out, sums, z.Dp, w_rs,
+             (int)z.T, (int)z.D, (int)c.splits * wn, reduction, loss_rows_per(z)};
+  PNFX_TRY((launch<xent_loss_kernel<T>>(loss_blocks(z), 256, 0, l, st, "xent_loss")));
+  if (reduction == PNFX_REDUCE_NONE) return PNFX_OK;
+  hipLaunchKernelGGL(xent_total_kernel, dim3(1), dim3(64), 0, st, sums, (int)loss_blocks(z), k.count, out, reduction);
+  return launch_status("xent_total");
+}
+
+template <typename T>
+int xent_bwd(const float* dloss, const void* x, int64_t x_rs, const void* w, int64_t w_rs, const int64_t* target,
+             int64_t ignore, const float* rows, const float* lse, void* dx, void* dw, int reduction, const Sizes& z,
+             bool copy, void* ws, hipStream_t st) {
+  Arena ar{static_cast<char*>(ws), 0};
+  const Kept k = take_kept(ar, z, copy);
+  const BwdCut c = bwd_cut(z);
+  RowsArgs r = {};
+  r.lse = lse, r.loss = rows, r.dloss = dloss, r.reduction = reduction;
+  r.alpha = ar.take<float>(1);
+  void* xs = ar.take<char>(z.T * z.Dp * z.es);
+  if (reduction == PNFX_REDUCE_NONE) r.xs = xs;
+  r.rowc = ar.take<float4>(z.T);
+  T* d = reinterpret_cast<T*>(ar.take<char>(z.T * c.P * z.es));
+  float* sums = ar.take<float>(c.dx.splits * z.T * z.D);
+  void* dw_ws = ar.take<char>(product_workspace(c.dw, c.P, z.D));
+  PNFX_TRY(take_w(k, w, w_rs, z, st));
+  PNFX_TRY(keep_rows<T>(k, x, x_rs, target, ignore, z, r, st));
+  for (int64_t v0 = 0; v0 < z.V; v0 += c.P) {
+    const int64_t n = std::min(c.P, z.V - v0);
+    const T* wp = static_cast<const T*>(w) + v0 * w_rs;
+    GradArgs g{k.xc, wp, d, r.rowc, k.tgt, k.count, z.Dp, w_rs, z.Dp, c.P, (int)v0, (int)n, 0, 0};
+    const bool big = cut_of(z.T, n, z.Dp, z.dtype, false).big && z.D >= 768;
+    g.tm = (int)ceil_div(z.T, big ? 256 : 128), g.tn = (int)ceil_div(round_up(n, 8), big ? 256 : 128);
+    if constexpr (sizeof(T) == 2) {
+      if (big)
+        PNFX_TRY((launch<xent_grad_kernel<T, Big>>((int64_t)g.tm * g.tn, threads_of<Big>, lds_of<Big>, g, st, "xent_grad")));
+    }
+    if (!big)
+      PNFX_TRY((launch<xent_grad_kernel<T, Mid>>((int64_t)g.tm * g.tn, threads_of<Mid>, lds_of<Mid>, g, st, "xent_grad")));
+    if (dx) {
+      ProductArgs p = {};
+      p.a = d, p.b = wp, p.lda = c.P, p.ldb = w_rs, p.M = z.T, p.N = z.D, p.K = n;
+      p.m_count = k.count, p.sums = sums, p.add = v0 > 0;
+      PNFX_TRY(product(ROW, COL, p, c.dx, z.dtype, nullptr, st));
+    }
+    if (dw) {
+      ProductArgs p = {};
+      p.a = d, p.b = r.xs ? xs : k.xc, p.c = static_cast<T*>(dw) + v0 * z.D, p.lda = c.P, p.ldb = z.Dp, p.ldc = z.D;
+      p.M = n, p.N = z.D, p.K = z.T, p.k_count = k.count;
+      p.alpha = r.xs ? nullptr : r.alpha;
+      PNFX_TRY(product(COL, COL, p, c.dw, z.dtype, dw_ws, st));
+    }
+  }
+  if (!dx) return PNFX_OK;
+  const DxArgs x1{sums, r.rowc, k.pos, dx, z.T * z.D, (int)z.D, c.dx.splits};
+  return launch<xent_dx_kernel<T>>(ceil_div(x1.TD, z.D % 4 == 0 ? 1024 : 256), 256, 0, x1, st, "xent_dx");
+}
+
+int check_sizes(const char* what, int64_t T, int64_t D, int64_t V, int reduction, int dtype) {
+  PNFX_REQUIRE(dtype == PNFX_F32 || dtype == PNFX_BF16, "%s: unsupported dtype %d", what, dtype);
+  PNFX_REQUIRE(reduction == PNFX_REDUCE_NONE || reduction == PNFX_REDUCE_SUM || reduction == PNFX_REDUCE_MEAN,
+               "%s: unknown reduction %d", what, reduction);
+  PNFX_REQUIRE(T >= 1 && D >= 1 && V >= 1 && T <= (1 << 24) && D <= (1 << 18) && V <= (1 << 24),
+               "%s: bad shape T=%lld D=%lld V=%lld", what, (long long)T, (long long)D, (long long)V);
+  return PNFX_OK;
+}
+bool copies_w(const void* w, int64_t w_rs, const Sizes& z) { return !(z.D == z.Dp && operand_ok(w, w_rs, z.es)); }
+
+}  // namespace
+}  // namespace pnfx
+
+extern "C" int64_t pnfx_xent_fwd_workspace_size(int64_t T, int64_t D, int64_t V, int copies, int dtype) {
+  using namespace pnfx;
+  if (check_sizes("xent", T, D, V, PNFX_REDUCE_NONE, dtype) != PNFX_OK) return 0;
+  return fwd_bytes(sizes_of(T, D, V, dtype), copies);
+}
+extern "C" int64_t pnfx_xent_bwd_workspace_size(int64_t T, int64_t D, int64_t V, int copies, int dtype) {
+  using namespace pnfx;
+  if (check_sizes("xent", T, D, V, PNFX_REDUCE_NONE, dtype) != PNFX_OK) return 0;
+  return bwd_bytes(sizes_of(T, D, V, dtype), copies);
+}
+
+extern "C" int pnfx_xent_fwd(const void* x, int64_t x_rs, const void* w, int64_t w_rs, const int64_t* target,
+                             int64_t ignore_index, float* loss, float* loss_rows, float* lse, int64_t T, int64_t D,
+                             int64_t V, int reduction, int dtype, void* workspace, int64_t workspace_bytes,
+                             void* stream) {
+  using namespace pnfx;
+  PNFX_REQUIRE(x && w && target && loss && loss_rows && lse, "xent_fwd: null pointer");
+  PNFX_TRY(check_sizes("xent_fwd", T, D, V, reduction, dtype));
+  PNFX_REQUIRE(x_rs >= D && w_rs >= D, "xent_fwd: row strides %lld, %lld", (long long)x_rs, (long long)w_rs);
+  const Sizes z = sizes_of(T, D, V, dtype);
+  const bool copy = copies_w(w, w_rs, z);
+  const int64_t need = fwd_bytes(z, copy);
+  PNFX_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= need,
+               "xent_fwd: workspace needs %lld bytes", (long long)need);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  return dtype == PNFX_F32 ? xent_fwd<float>(x, x_rs, w, w_rs, target, ignore_index, loss, loss_rows, lse, reduction, z,
+                                             copy, workspace, st)
+                           : xent_fwd<bf16>(x, x_rs, w, w_rs, target, ignore_index, loss, loss_rows, lse, reduction, z,
+                                            copy, workspace, st);
+}
+
+extern "C" int pnfx_xent_bwd(const float* dloss, const void* x, int64_t x_rs, const void* w, int64_t w_rs,
+                             const int64_t* target, int64_t ignore_index, const float* loss_rows, const float* lse,
+                             void* dx, void* dw, int64_t T, int64_t D, int64_t V, int reduction, int dtype,
+                             void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace pnfx;
+  PNFX_REQUIRE(dloss && x && w && target && loss_rows && lse, "xent_bwd: null pointer");
+  PNFX_TRY(check_sizes("xent_bwd", T, D, V, reduction, dtype));
+  PNFX_REQUIRE(x_rs >= D && w_rs >= D, "xent_bwd: row strides %lld, %lld", (long long)x_rs, (long long)w_rs);
+  PNFX_REQUIRE(((reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw)) & 15) == 0,
+               "xent_bwd: gradients must be 16-byte aligned");
+  const Sizes z = sizes_of(T, D, V, dtype);
+  const bool copy = copies_w(w, w_rs, z);
+  const int64_t need = bwd_bytes(z, copy);
+  PNFX_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= need,
+               "xent_bwd: workspace needs %lld bytes", (long long)need);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  return dtype == PNFX_F32 ? xent_bwd<float>(dloss, x, x_rs, w, w_rs, target, ignore_index, loss_rows, lse, dx, dw,
+                                             reduction, z, copy, workspace, st)
+                           : xent_bwd<bf16>(dloss, x, x_rs, w, w_rs, target, ignore_index, loss_rows, lse, dx, dw,
+                                            reduction, z, copy, workspace, st);
+}

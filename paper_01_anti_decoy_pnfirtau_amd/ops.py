@@ -16,6 +16,8 @@ pnfx::flash_fwd_fir    (none: the key FIR fused into the forward's key-tile load
 pnfx::attn_rows/_bwd   (none: key FIR and flash on projection rows [B, N, 3 D], one autograd node)
 pnfx::linear           (none: x W^T whose weight gradient is linear_wgrad)
 pnfx::linear_wgrad     (none: dY^T X of bf16 rows, fp32 sums)
+pnfx::gated_ffn/_bwd   (none: the gated feed-forward block, both projections in one kernel)
+pnfx::linear_xent/_bwd (none: cross entropy over the vocabulary without the logits)
 pnfx::sum_f64          the fp64 sum of tau's row gradients  :784
 """
 from __future__ import annotations
@@ -191,3 +193,32 @@ def _(q, k_raw, v, tau, taps, scale, gamma, has_gamma, causal, o_bnhd=False):
     f = lambda: q.new_empty((B, H, N), dtype=torch.float32)  # noqa: E731
     return (_new_o(q, o_bnhd), _new_o(q, o_bnhd), f(), f(),
             q.new_empty(_mask_shape(B, H, N), dtype=torch.uint8))
+
+
+@torch.library.register_fake("pnfx::gated_ffn")
+def _(x, w_in, w_down, act, keep):
+    T, F = math.prod(x.shape[:-1]), w_down.shape[1]
+    y = x.new_empty((*x.shape[:-1], w_down.shape[0]))
+    none = keep == _lib.PNFX_KEEP["none"]
+    kept = (torch.float32 if x.dtype == torch.float32 else
+            torch.uint8 if keep == _lib.PNFX_KEEP["e4m3"] else torch.float16)
+    gu = x.new_empty(0 if none else (T, 2, (F + 7) // 8 * 8), dtype=kept)
+    blocks = not none and x.dtype != torch.float32
+    return y, gu, x.new_empty((T, 2, (F + 31) // 32) if blocks else 0, dtype=torch.uint8)
+
+
+@torch.library.register_fake("pnfx::gated_ffn_bwd")
+def _(dy, x, w_in, w_down, gu, scales, act, keep, mask):
+    return tuple(x.new_empty(t.shape if m else (0,)) for t, m in zip((x, w_in, w_down), mask))
+
+
+@torch.library.register_fake("pnfx::linear_xent")
+def _(x, w, target, ignore_index, reduction):
+    f = lambda shape: x.new_empty(shape, dtype=torch.float32)  # noqa: E731
+    rows = math.prod(x.shape[:-1])
+    return f(target.shape if reduction == _lib.PNFX_REDUCE["none"] else ()), f(rows), f(rows)
+
+
+@torch.library.register_fake("pnfx::linear_xent_bwd")
+def _(dloss, x, w, target, rows, lse, ignore_index, reduction, mask):
+    return tuple(x.new_empty(t.shape if m else (0,)) for t, m in zip((x, w), mask))

@@ -1,0 +1,274 @@
+"""Cross entropy over the vocabulary (pnfx::linear_xent and its backward) against its formulas in 64 bits.
+
+The tolerances bound the kernels' roundings elementwise: H = 2^-8 of a value that is rounded to bf16, E = 2^-24 of
+one fp32 operation, (n + 2) E of the absolute sum for an fp32 sum of n products.
+"""
+import pytest
+import torch
+
+from paper_01_anti_decoy_pnfirtau_amd import linear_cross_entropy, ops  # noqa: F401  (loads the ops)
+from tests.helpers import seeded
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -24
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def make(T, D, V, dtype, dev, ignored=0.0, seed=0):
+    x, w = seeded((T, D), seed, dtype, dev), seeded((V, D), seed + 1, dtype, dev, 2 * D ** -0.5)
+    g = torch.Generator().manual_seed(seed + 2)
+    target = torch.randint(0, V, (T,), generator=g)
+    target[torch.rand(T, generator=g) < ignored] = -100
+    return x, w, target.to(dev)
+
+
+def reference(x, w, target, H, s=None, ignore=-100, per_row=False):
+    """(losses, bound), and with row factors s (dx, bound), (dw, bound), in 64 bits.  per_row: s differs from row
+    to row, and dw is the product with s x, rounded to the operands' type."""
+    T, D = x.shape
+    V = w.shape[0]
+    x, w = x.double(), w.double()
+    kept = target != ignore
+    at = torch.where(kept, target, 0)[:, None]
+    z = x @ w.T
+    ez = (D + 2) * E * (x.abs() @ w.abs().T).amax(1, keepdim=True)  # of any logit of the row
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    # exponentials of differences in base 2: a rounding of each product with log2 e, of the difference and
+    # of the exponential; V sums of positive terms; the same once more where the parts are joined
+    e_exp = ez + 8 * E * (z.abs().amax(1, keepdim=True) + lse.abs() + 2)
+    e_lse = 2 * e_exp + (V + 64) * E
+    losses = torch.where(kept, (lse - z.gather(1, at))[:, 0], 0.0)
+    out = [(losses, (e_lse + ez + 4 * E * (lse.abs() + z.abs().amax(1, keepdim=True)))[:, 0])]
+    if s is None:
+        return out
+    s = torch.where(kept, s, 0.0)[:, None]
+    p = torch.exp(z - lse)
+    d = p.clone()
+    d.scatter_add_(1, at, -torch.ones_like(lse))
+    # p is off by its exponent's error; the target's own element is of the loss, off by out[0][1]
+    ed = p * (e_exp + e_lse) + 4 * E * p
+    ed.scatter_(1, at, out[0][1][:, None] + 4 * E)
+    ed = ed + H * (d.abs() + ed)
+    # s: a quotient, and one more factor
+    d, ed = d * s, (ed + 2 * E * (d.abs() + ed)) * s.abs()
+
+    def mm(p, ep, q, n):
+        v = p @ q
+        e = ep @ q.abs() + (n + 66) * E * ((p.abs() + ep) @ q.abs())
+        return v, e + H * (v.abs() + e)
+
+    x = torch.where(kept[:, None], x, 0.0)
+    return [*out, mm(d, ed, w, V), mm(d.T, (ed + (H * (d.abs() + ed) if per_row else 0)).T, x, T)]
+
+
+def close(got, want, what):
+    (v, e), got = want, got.double()
+    assert got.shape == v.shape, (what, got.shape, v.shape)
+    over = (got - v).abs() - e
+    assert bool((over <= 0).all()), (what, float(over.max()), float((got - v).norm()), float(v.norm()))
+
+
+CASES = [
+    # T, D, V
+    (1, 1, 1), (1, 8, 2), (3, 5, 7), (5, 64, 300), (64, 16, 129), (100, 33, 1000), (129, 72, 257),
+    (260, 64, 2500), (300, 250, 511), (700, 96, 4100), (40, 1000, 777),
+]
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T,D,V", CASES)
+def test_loss_and_gradients(dev, T, D, V, dtype, reduction):
+    print(f"[xent {T} {D} {V} {dtype} {reduction}]", flush=True)
+    x, w, target = make(T, D, V, dtype, dev, 0.3 if T > 4 else 0.0)
+    H = torch.finfo(dtype).eps / 2
+    kept = int((target != -100).sum())
+    dloss = seeded((T,) if reduction == "none" else (), 5, F32, dev)
+    s = dloss.double().expand(T) / (kept if reduction == "mean" else 1)
+    (losses, el), *grads = reference(x, w, target, H, s, per_row=reduction == "none")
+    if reduction != "none":
+        n = kept if reduction == "mean" else 1
+        losses, el = losses.sum() / n, el.sum() / n + 2 * E * losses.sum() / n
+    leaves = [t.clone().requires_grad_() for t in (x, w)]
+    loss = linear_cross_entropy(*leaves, target, reduction=reduction)
+    assert loss.dtype == F32
+    close(loss.detach(), (losses, el), "loss")
+    assert torch.equal(loss.detach(), linear_cross_entropy(x, w, target, reduction=reduction))
+    for name, a, want in zip(("dx", "dw"), torch.autograd.grad(loss, leaves, dloss), grads):
+        assert a.dtype == dtype
+        close(a, want, name)
+
+
+def test_several_pieces_of_the_vocabulary(dev, monkeypatch):
+    """More tokens than a piece holds (64 MB of logits' gradients): 17000 rows take pieces of 2048."""
+    print("[xent pieces]", flush=True)
+    T, D, V = 17000, 24, 5000
+    x, w, target = make(T, D, V, BF16, dev, 0.1, 7)
+    leaves = [t.clone().requires_grad_() for t in (x, w)]
+    loss = linear_cross_entropy(*leaves, target, reduction="sum")
+    got = torch.autograd.grad(loss, leaves)
+    (losses, el), *want = reference(x, w, target, 2.0 ** -8, torch.ones(T, dtype=torch.float64, device=dev))
+    close(loss.detach(), (losses.sum(), el.sum() + 2 * E * losses.sum()), "loss")
+    for name, a, b in zip(("dx", "dw"), got, want):
+        close(a, b, name)
+
+
+def test_gradients_against_differences(dev):
+    x, w, target = make(90, 40, 333, F32, dev, 0.2, 9)
+    leaves = [t.clone().requires_grad_() for t in (x, w)]
+    grads = torch.autograd.grad(linear_cross_entropy(*leaves, target, reduction="sum"), leaves)
+    eps = 2.0 ** -6
+    for i, g in enumerate(grads):
+        v = seeded(g.shape, 30 + i, F32, dev)
+        v /= v.norm()
+        f = lambda s: linear_cross_entropy(*[t + s * eps * v if j == i else t  # noqa: E731
+                                             for j, t in enumerate((x, w))], target, reduction="none").double().sum()
+        num, ana = float((f(1.0) - f(-1.0)) / (2 * eps)), float((g.double() * v.double()).sum())
+        assert abs(num - ana) <= 2e-3 * float(g.double().norm()), (i, num, ana)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_ignored_rows_reach_nothing(dev, dtype):
+    """Rows that are ignored may hold anything: the results are those of the batch without them, their loss
+    and gradients are zero.  Runs of ignored rows at the front, in the middle and at the end."""
+    T, D, V = 600, 40, 500
+    x, w, target = make(T, D, V, dtype, dev, 0.0, 11)
+    for a, b in ((0, 130), (200, 201), (300, 420), (590, 600)):
+        target[a:b] = 7  # the ignored token
+    target[target == 7] = 7
+    kept = target != 7
+    x[~kept] = float("nan")
+    x[1], x[595] = float("inf"), torch.finfo(dtype).min
+    leaves = [t.clone().requires_grad_() for t in (x, w)]
+    loss = linear_cross_entropy(*leaves, target, ignore_index=7, reduction="none")
+    dloss = seeded((T,), 12, F32, dev)
+    dx, dw = torch.autograd.grad(loss, leaves, dloss)
+    dense = [x[kept].clone().requires_grad_(), w.clone().requires_grad_()]
+    ref = linear_cross_entropy(*dense, target[kept], reduction="none")
+    rdx, rdw = torch.autograd.grad(ref, dense, dloss[kept])
+    assert not bool(loss[~kept].any()) and not bool(dx[~kept].any())
+    assert torch.equal(loss[kept], ref) and torch.equal(dx[kept], rdx)
+    # (sums over another number of rows may be cut otherwise: a rounding of 2^-8 each in bf16)
+    assert bool(((dw - rdw).double().abs() <= 2.0 ** -7 * rdw.double().abs().amax()).all())
+
+
+def test_all_rows_ignored_and_no_rows(dev):
+    x, w, _ = make(50, 16, 30, BF16, dev)
+    target = torch.full((50,), -100, device=dev)
+    for reduction, want in (("sum", 0.0), ("mean", None), ("none", 0.0)):
+        leaves = [t.clone().requires_grad_() for t in (x, w)]
+        loss = linear_cross_entropy(*leaves, target, reduction=reduction)
+        assert bool(loss.isnan()) if want is None else not bool(loss.any())
+        for g in torch.autograd.grad(loss.sum(), leaves):
+            assert not bool(g.any())
+    none = x[:0].requires_grad_()
+    for reduction in ("sum", "mean", "none"):
+        loss = linear_cross_entropy(none, w, target[:0], reduction=reduction)
+        assert loss.numel() == (0 if reduction == "none" else 1)
+    assert float(linear_cross_entropy(x[:0], w, target[:0], reduction="sum")) == 0.0
+    assert bool(linear_cross_entropy(none, w, target[:0]).isnan())
+
+
+def test_targets_that_are_no_tokens(dev):
+    """Outside 0 .. V - 1 and not ignored: that row's loss and gradient are NaN, the others' losses stay."""
+    x, w, target = make(140, 32, 100, BF16, dev, 0.1, 13)
+    ref = linear_cross_entropy(x, w, target, reduction="none")
+    bad = target.clone()
+    bad[3], bad[139], bad[70] = 100, -1, 1 << 40
+    leaf = x.clone().requires_grad_()
+    loss = linear_cross_entropy(leaf, w, bad, reduction="none")
+    rows = torch.zeros(140, dtype=torch.bool, device=dev)
+    rows[[3, 139, 70]] = True
+    assert bool(loss[rows].isnan().all()) and torch.equal(loss[~rows], ref[~rows])
+    dx = torch.autograd.grad(loss, leaf, torch.ones_like(loss))[0]
+    assert bool(dx[rows].isnan().all()) and not bool(dx[~rows].isnan().any())
+
+
+def test_extreme_logits(dev):
+    """Logits far apart and equal, a vocabulary of one, a row of infinities: as log_softmax has them."""
+    D, V = 8, 70
+    x = torch.zeros(4, D, device=dev)
+    w = torch.zeros(V, D, device=dev)
+    x[0, 0], x[1, 0], x[2, 1] = 1.0, -1.0, 1.0
+    w[:, 0] = torch.linspace(-5e4, 5e4, V, device=dev)
+    w[5, 1] = float("inf")
+    target = torch.tensor([V - 1, V - 1, 5, 3], device=dev)
+    loss = linear_cross_entropy(x[[0, 1, 3]], torch.where(w.isfinite(), w, 0), target[[0, 1, 3]], reduction="none")
+    want = torch.tensor([0.0, 1e5, torch.tensor(float(V)).log().item()], device=dev)
+    assert torch.allclose(loss, want, rtol=1e-6, atol=1e-6)
+    assert bool(linear_cross_entropy(x[2:3], w, target[2:3]).isnan())
+    assert float(linear_cross_entropy(x[:1], w[:1], target[:1] * 0)) == 0.0
+    # a certain row's gradient: expm1 of a tiny loss, not a rounded one minus one
+    sure = torch.zeros(2, D, device=dev)
+    sure[1, 0] = 16.0
+    row = torch.ones(1, D, device=dev)
+    row[0, 0] = 1.0
+    leaf = sure.clone().requires_grad_()
+    loss = linear_cross_entropy(row, leaf, torch.tensor([1], device=dev))
+    dw = torch.autograd.grad(loss, leaf)[0]
+    p = torch.sigmoid(torch.tensor(-16.0, dtype=torch.float64)).item()
+    assert abs(float(dw[0, 0]) - p) <= 1e-3 * p and abs(float(dw[1, 0]) + p) <= 2 * 2.0 ** -20
+
+
+def test_views_and_shapes(dev):
+    """[B, N, D] rows that are views, a strided weight, expanded gradients: the bits of their contiguous copies."""
+    B, N, D, V = 3, 50, 40, 210
+    x = seeded((B, N + 2, D + 8), 14, BF16, dev)[:, 1:-1, 8:]
+    w = seeded((V, D + 3), 15, BF16, dev)[:, 3:]
+    target = torch.randint(0, V, (N, B), generator=torch.Generator().manual_seed(1)).to(dev).t()
+    leaves = [t.detach().requires_grad_() for t in (x, w)]
+    flat = [t.detach().contiguous().requires_grad_() for t in leaves]
+    a = linear_cross_entropy(*leaves, target, reduction="none")
+    b = linear_cross_entropy(*flat, target.contiguous(), reduction="none")
+    assert a.shape == (B, N) and torch.equal(a, b)
+    for u, v, t in zip(torch.autograd.grad(a.sum(), leaves), torch.autograd.grad(b.sum(), flat), leaves):
+        assert u.shape == t.shape and torch.equal(u, v)
+
+
+def test_repeatable_on_a_side_stream_and_in_a_graph(dev):
+    x, w, target = make(900, 64, 3001, BF16, dev, 0.2, 16)
+    leaves = [t.clone().requires_grad_() for t in (x, w)]
+
+    def call():
+        loss = linear_cross_entropy(*leaves, target)
+        return [loss.detach(), *torch.autograd.grad(loss, leaves)]
+
+    ref = call()
+    torch.cuda.synchronize()
+    got, side = [], [torch.cuda.Stream() for _ in range(2)]
+    for s in side:
+        with torch.cuda.stream(s):
+            got.append(call())
+    torch.cuda.synchronize()
+    for outs in got:
+        assert all(torch.equal(a, b) for a, b in zip(outs, ref))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = call()
+    for i in range(3):
+        with torch.no_grad():
+            leaves[0].copy_(seeded(x.shape, 80 + i, BF16, dev))
+        target[i::5] = -100  # another number of kept rows
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(static, call()):
+            assert torch.equal(a, b)
+        torch.cuda.synchronize()
+
+
+def test_refusals(dev):
+    x, w, target = make(6, 16, 20, BF16, dev)
+    with pytest.raises(TypeError):
+        linear_cross_entropy(x, w.float(), target)
+    with pytest.raises(TypeError):
+        linear_cross_entropy(x, w, target.int())
+    with pytest.raises(TypeError):
+        linear_cross_entropy(x.half(), w.half(), target)
+    for bad in ((x, w[:, :8], target), (x, w, target[:5]), (x, w[0], target), (x, w, target.cpu()),
+                (x, w.cpu(), target), (x, w[:0], target)):
+        with pytest.raises(ValueError):
+            linear_cross_entropy(*bad)
+    leaf = x.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        torch.autograd.grad(linear_cross_entropy(leaf, w, target), leaf, create_graph=True)
