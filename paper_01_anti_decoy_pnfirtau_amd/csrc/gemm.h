@@ -15,6 +15,7 @@
 #pragma once
 
 #include <atomic>
+#include <type_traits>
 
 #include "tiles_bf16.h"
 
@@ -69,11 +70,17 @@ constexpr int k_step = 128 / (int)sizeof(T);
 template <typename T>
 constexpr int per16 = 16 / (int)sizeof(T);  // elements in 16 bytes
 
-// acc[r] += sum_k b(row 4 (lane / 16) + r, k) a(row lane % 16, k).
-__device__ __forceinline__ f32x4 mma(bf16x8 b, bf16x8 a, f32x4 acc) { return mfma16x16x32(b, a, acc); }
-__device__ __forceinline__ f32x4 mma(f32x4 b, f32x4 a, f32x4 acc) {
+// acc[r] += sum_k b(row 4 (lane / 16) + r, k) a(row lane % 16, k), in mma_parts<T> instructions.
+template <typename T>
+constexpr int mma_parts = sizeof(T) == 4 ? 4 : 1;
+__device__ __forceinline__ f32x4 mma_part(bf16x8 b, bf16x8 a, f32x4 acc, int) { return mfma16x16x32(b, a, acc); }
+__device__ __forceinline__ f32x4 mma_part(f32x4 b, f32x4 a, f32x4 acc, int t) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(b[t], a[t], acc, 0, 0, 0);
+}
+template <typename F>
+__device__ __forceinline__ f32x4 mma(F b, F a, f32x4 acc) {
 #pragma unroll
-  for (int t = 0; t < 4; ++t) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(b[t], a[t], acc, 0, 0, 0);
+  for (int t = 0; t < (sizeof(a[0]) == 4 ? 4 : 1); ++t) acc = mma_part(b, a, acc, t);
   return acc;
 }
 
@@ -85,12 +92,12 @@ enum Kind { ROW, COL, PAIR };
 // A sub-tile is 64 slots of 128 bytes; 16-byte chunk c of slot s lies at position c ^ stage_swz(s).  The
 // swizzles depend on the slot's low four bits only, so that a fragment's block is a constant offset.  ROW: 16
 // lanes read 16 consecutive slots at one chunk, which with two slots to the 64 banks lands on all of them.
-// COL, bf16: a half wave reads 32 bytes of 8 slots; fp32: a wave 64 bytes of 4 slots.
+// COL, bf16: a half wave reads 32 bytes, two chunks, of 8 consecutive slots: all banks too, with the same
+// swizzle.  COL, fp32: a wave reads 64 bytes of 4 slots.
 template <typename T, Kind KIND>
 __device__ __forceinline__ int stage_swz(int slot) {
-  if (KIND != COL) return slot >> 1 & 7;
-  if (sizeof(T) == 4) return 4 * (slot >> 1 & 1);
-  return 2 * ((slot >> 1 & 1) | (((slot >> 2) ^ (slot >> 3)) & 1) << 1);
+  if (KIND == COL && sizeof(T) == 4) return 4 * (slot >> 1 & 1);
+  return (slot >> 1 & 3) << 1 | (slot >> 3 & 1);
 }
 
 // Stages tiles of R rows of one operand, NT threads, 16 bytes per thread and load.  Past `rows` and past K come
@@ -104,17 +111,19 @@ struct Stage {
   static_assert(SPL == 32 || SPL == 64, "a load fills half a sub-tile or a whole one");
   static constexpr int ES = (int)sizeof(T), KS = k_step<T>;
   const char* base[KIND == PAIR ? 2 : 1];  // element (first row, k0)
-  int64_t left;    // k left
+  int64_t K, left;  // k of a tile, and those left of it
+  int rows;        // rows from the tile's first on
   unsigned ldb;    // bytes from row to row
   unsigned limit;  // ROW, PAIR: bytes to the last row in reach; COL: bytes of a row in reach
   unsigned off;    // the lane's byte offset in load 0
   int ch;          // ROW: the lane's chunk of the step's k
 
-  // p (PAIR: and p2): the tile's first row; rows >= 1: how many there are from it on (PAIR: in each); K: its k.
-  __device__ __forceinline__ void init(const T* p, int64_t ld, int rows, int64_t K, int tid,
+  // p (PAIR: and p2): the tile's first row; nrows >= 1: how many there are from it on (PAIR: in each); k: its k.
+  __device__ __forceinline__ void init(const T* p, int64_t ld, int nrows, int64_t k, int tid,
                                        const T* p2 = nullptr) {
     ldb = (unsigned)(ES * ld);
-    left = K;
+    K = left = k;
+    rows = nrows;
     base[0] = reinterpret_cast<const char*>(p);
     const int slot = tid / 8;
     ch = (tid % 8) ^ stage_swz<T, KIND>(slot);
@@ -126,9 +135,20 @@ struct Stage {
       off = k * ldb + 16 * ch + (ES == 4 ? (slot >> 5) * 128 : 0);
     } else {
       const int row = row_of_slot(slot);
-      limit = (unsigned)(min(rows, KIND == PAIR ? R / 2 : R) - 1) * ldb;
+      set_limit();
       off = (KIND == PAIR ? row & 31 : row) * ldb + 16 * ch;
     }
+  }
+  __device__ __forceinline__ void set_limit() {
+    limit = (unsigned)(min(rows, KIND == PAIR ? R / 2 : R) - 1) * ldb;
+  }
+  // ROW: the next steps are of the tile `by` rows further on, from its first k.
+  __device__ __forceinline__ void move(int by, int steps) {
+    static_assert(KIND == ROW, "");
+    base[0] += (int64_t)by * ldb - 128 * steps;
+    left = K;
+    rows -= by;
+    if (by) set_limit();
   }
   // The next step's tile to LDS byte address lds.
   __device__ __forceinline__ void load(unsigned lds, int wave) {
@@ -236,12 +256,35 @@ struct Product {
   // sm: lds_of<C> bytes, free; every wave's reads of it are done when run returns (its writes too).
   __device__ __forceinline__ static void run(StageA& sa, StageB& sb, int steps, T* sm, int wave, int lane,
                                              f32x4 (&acc)[MI][NJ]) {
-    if (steps <= 0) return;
+    loop<false>(sa, sb, steps, 1, sm, wave, lane, acc, [](int) {});
+  }
+  // `tiles` tiles of TN rows of B below each other against the same rows of A: done(t) is called with tile t's
+  // sums in acc, while the first steps of the next tile are on their way.
+  template <class Done>
+  __device__ __forceinline__ static void run_tiles(StageA& sa, StageB& sb, int steps, int tiles, T* sm, int wave,
+                                                   int lane, f32x4 (&acc)[MI][NJ], Done done) {
+    loop<true>(sa, sb, steps, tiles, sm, wave, lane, acc, done);
+  }
+
+ private:
+  template <bool MANY, class Done>
+  __device__ __forceinline__ static void loop(StageA& sa, StageB& sb, int steps, int tiles, T* sm, int wave, int lane,
+                                              f32x4 (&acc)[MI][NJ], Done done) {
+    if (steps <= 0 || tiles <= 0) return;
+    const int total = MANY ? steps * tiles : steps;
     // both buffers of A, then both of B: an operand's fragments are within the 64 KB of an LDS load's offset
     constexpr int SA = TM * k_step<T>, SB = TN * k_step<T>, ES = (int)sizeof(T);
     const unsigned la = __builtin_amdgcn_readfirstlane(lds_addr(sm));
-    const auto load_a = [&](int b) { sa.load(la + ES * b * SA, wave); };
-    const auto load_b = [&](int b) { sb.load(la + ES * (2 * SA + b * SB), wave); };
+    const auto load_a = [&](int b) {
+      sa.load(la + ES * b * SA, wave);
+      if constexpr (MANY)
+        if (sa.left <= 0) sa.move(0, steps);
+    };
+    const auto load_b = [&](int b) {
+      sb.load(la + ES * (2 * SA + b * SB), wave);
+      if constexpr (MANY)
+        if (sb.left <= 0) sb.move(TN, steps);
+    };
     const Frags<T, KA> fa(sm + wave / C::WN * MI * 16 * k_step<T>, lane);
     const Frags<T, KB> fb(sm + 2 * SA + wave % C::WN * NJ * 16 * k_step<T>, lane);
     // Four phases per step, (k-half, half of the row blocks): while one phase's products run, the
@@ -257,16 +300,19 @@ struct Product {
       for (int j = 0; j < NJ; ++j) b[hf][j] = fb.get(j, hf, buf * SB);
     };
     const auto products = [&](int hf, int ih) {
+      // (fp32: four products for each element of the fragment, no two in a row on the same sums)
 #pragma unroll
-      for (int i = 0; i < MH; ++i)
+      for (int t = 0; t < mma_parts<T>; ++t)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
-          acc[ih * MH + i][j] = mma(b[hf][j], a[ih][i], acc[ih * MH + i][j]);
+        for (int i = 0; i < MH; ++i)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+            acc[ih * MH + i][j] = mma_part(b[hf][j], a[ih][i], acc[ih * MH + i][j], t);
       __builtin_amdgcn_sched_barrier(0);
     };
     load_a(0);
     load_b(0);
-    if (steps > 1) {
+    if (total > 1) {
       load_a(1);
       load_b(1);
       wait_vm_lgkm<StageA::NI + StageB::NI>();
@@ -276,8 +322,9 @@ struct Product {
     __builtin_amdgcn_s_barrier();
     read_b(0, 0);
     read_a(0, 0, 0);
+    int k = 0, tile = 0;
     const auto step = [&](int s, int buf) {
-      if (s && s + 1 < steps) load_b(buf ^ 1);
+      if (s && s + 1 < total) load_b(buf ^ 1);
       __builtin_amdgcn_sched_barrier(0);
       read_a(buf, 0, 1);
       products(0, 0);
@@ -289,18 +336,112 @@ struct Product {
       // the next tile is here, and every wave has read this one
       wait_vm_lgkm<0>();
       __builtin_amdgcn_s_barrier();
-      if (s + 2 < steps) load_a(buf);
+      if (s + 2 < total) load_a(buf);
       __builtin_amdgcn_sched_barrier(0);
       read_b(buf ^ 1, 0);
       read_a(buf ^ 1, 0, 0);
       products(1, 1);
+      if constexpr (MANY) {
+        if (++k == steps) {
+          done(tile++);
+          k = 0;
+#pragma unroll
+          for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{};
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
     };
     int s = 0;
-    for (; s + 1 < steps; s += 2) {
+    for (; s + 1 < total; s += 2) {
       step(s, 0);
       step(s + 1, 1);
     }
-    if (s < steps) step(s, 0);
+    if (s < total) step(s, 0);
+    wait_vm_lgkm<0>();
+    __builtin_amdgcn_s_barrier();
+  }
+};
+
+// Product::run_tiles for at most KS <= 4 steps of k: A's fragments stay in registers over all the tiles, which
+// halves what the LDS has to supply (with 4 steps or fewer of products between two epilogues a tile's loop
+// is otherwise bound by it), and B's steps go through a ring of four buffers, three of them ahead.  STORES: global
+// stores that every done() issues (it may issue more); the loop does not wait for the latest ones.
+template <typename T, int KS, class C, int STORES>
+struct Thin {
+  static constexpr int TM = C::TM, TN = C::TN, NT = threads_of<C>;
+  static constexpr int MI = TM / C::WM / 16, NJ = TN / C::WN / 16;
+  static constexpr int RING = 4;
+  static constexpr int LDS = RING * TN * 128;
+  static_assert(TM == TN, "A passes through the ring's buffers");
+  typedef Stage<T, ROW, TM, NT> StageA;
+  typedef Stage<T, ROW, TN, NT> StageB;
+  typedef typename Elem<T>::Frag F;
+
+  template <class Done>
+  __device__ __forceinline__ static void run_tiles(StageA& sa, StageB& sb, int tiles, T* sm, int wave, int lane,
+                                                   f32x4 (&acc)[MI][NJ], Done done) {
+    if (tiles <= 0) return;
+    constexpr int SB = TN * k_step<T>, ES = (int)sizeof(T);
+    const unsigned la = __builtin_amdgcn_readfirstlane(lds_addr(sm));
+    F a[KS][2][MI];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) sa.load(la + ES * k * SB, wave);
+    wait_vm_lgkm<0>();
+    __builtin_amdgcn_s_barrier();
+    const Frags<T, ROW> fa(sm + wave / C::WN * MI * 16 * k_step<T>, lane);
+    const Frags<T, ROW> fb(sm + wave % C::WN * NJ * 16 * k_step<T>, lane);
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int i = 0; i < MI; ++i) a[k][hf][i] = fa.get(i, hf, k * SB);
+    wait_vm_lgkm<0>();
+    __builtin_amdgcn_s_barrier();
+    const int total = KS * tiles;
+    const auto load = [&](int s) {
+      sb.load(la + ES * (s % RING) * SB, wave);
+      if (sb.left <= 0) sb.move(TN, KS);
+    };
+    load(0);
+    if (total > 1) load(1);
+    if (total > 2) load(2);
+    // Step s = KS t + k.  Its loads were issued in step s - 3, so that the loads of two steps may be outstanding
+    // behind them, and the stores of the tiles that ended with step s - 3, s - 2 or s - 1 (from the fourth tile on).
+    const auto step = [&](auto kc, int t) {
+      constexpr int k = decltype(kc)::value;
+      constexpr int ended = ((k + 2 * KS) % KS == 0) + ((k + 2 * KS - 1) % KS == 0) + ((k + 2 * KS - 2) % KS == 0);
+      const int s = KS * t + k, buf = KS == RING ? k : s % RING;
+      if (s + 2 >= total) wait_vm_lgkm<0>();
+      else if (STORES && t >= 3) wait_vm_lgkm<2 * StageB::NI + STORES * ended>();
+      else wait_vm_lgkm<2 * StageB::NI>();
+      // and every wave has read step s - 1
+      __builtin_amdgcn_s_barrier();
+      if (s + 3 < total) load(s + 3);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        F b[NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) b[j] = fb.get(j, hf, buf * SB);
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) acc[i][j] = mma(b[j], a[k][hf][i], k + hf ? acc[i][j] : f32x4{});
+        if (KS == 4) __builtin_amdgcn_sched_barrier(0);  // no registers for both halves' fragments
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    for (int t = 0; t < tiles; ++t) {
+      step(std::integral_constant<int, 0>{}, t);
+      if constexpr (KS > 1) step(std::integral_constant<int, 1>{}, t);
+      if constexpr (KS > 2) step(std::integral_constant<int, 2>{}, t);
+      if constexpr (KS > 3) step(std::integral_constant<int, 3>{}, t);
+      done(t);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     wait_vm_lgkm<0>();
     __builtin_amdgcn_s_barrier();
   }

@@ -174,7 +174,7 @@ Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool can_split) {
       const int64_t per = ceil_div(steps, s), slots = 256 * per_cu;
       const int64_t full = tiles * s / slots, rest = tiles * s % slots;
       // a last round that leaves CUs with one tile of two runs it faster
-      const double last = !rest ? 0 : per_cu == 2 && rest <= 256 ? 0.6 : 1;
+      const double last = !rest ? 0 : per_cu == 2 && rest <= 256 ? 0.9 : 1;
       double us = (full + last) * (per * step_us + 2.0);
       if (s > 1) us += 4.0 + s * M * N * 8 / 4e6;
       if (us < best_us) {

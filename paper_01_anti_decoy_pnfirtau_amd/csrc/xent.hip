@@ -19,10 +19,11 @@
 // fp32 results where it is one value, and for a loss per row dx's rows and the x of dW = d^T (s x).  The target's
 // own element is expm1(-loss_t), which keeps its digits where the softmax is close to one.
 //
-// Exponentials are taken in base 2, exp2(z L - m L) with L = log2 e as one fma per logit.  The rounding of m L is
-// the same for a whole row and comes out again as the factor unround(m) = exp2(round(m L) - m L): without it logits
-// around 5e4 would be 4e-3 off.
+// Exponentials are taken in base 2.  The forward's are exp2(z L - m L) with L = log2 e as one fma per logit; the
+// rounding of m L is the same for a whole row and comes out again as the factor unround(m) = exp2(round(m L) - m L):
+// without it logits around 5e4 would be 4e-3 off.
 #include <algorithm>
+#include <type_traits>
 
 #include "product.h"
 
@@ -54,7 +55,7 @@ struct RowsArgs {
   int* count;
   int64_t x_rs, ignore;
   int T, D, Dp, V, per;  // per: rows of a workgroup
-  // backward only: row constants {lse, s_t, loss_t, 1 or NaN}; s_t where it is one value; s_t x_t where not
+  // backward only: row constants {lse, s_t, expm1(-loss_t), -}; s_t where it is one value; s_t x_t where not
   const float* lse;
   const float* loss;
   const float* dloss;
@@ -62,6 +63,7 @@ struct RowsArgs {
   float* alpha;
   void* xs;
   int reduction;
+  bool vec;  // rows in whole, aligned 16-byte chunks
 };
 
 template <typename T>
@@ -74,10 +76,11 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs a) {
   // kept rows before this workgroup's, and (backward, for the mean) behind them
   int before = 0, total = 0;
   const int to = a.rowc ? a.T : r0;
+#pragma unroll 8
   for (int r = tid; r < to; r += 256) {
     const int k = a.target[r] != a.ignore;
     total += k;
-    if (r < r0) before += k;
+    before += r < r0 ? k : 0;
   }
   const auto block_sum = [&](int v) {
     v = wave_sum_i(v);
@@ -114,7 +117,7 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs a) {
       if (a.rowc) {
         const float s = a.reduction == PNFX_REDUCE_NONE ? a.dloss[r] : row_scale;
         // a target that is no token: its loss is NaN, and so are its gradients
-        a.rowc[i] = float4{a.lse[r], s, a.loss[r], valid ? 1.f : __builtin_nanf("")};
+        a.rowc[i] = float4{valid ? a.lse[r] : __builtin_nanf(""), s, expm1f(-a.loss[r]), 0.f};
         scale[at] = s;
       }
     }
@@ -123,16 +126,27 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs a) {
     for (int i = wave; i < n; i += 4) {
       const T* x = static_cast<const T*>(a.x) + (int64_t)list[i] * a.x_rs;
       T* y = static_cast<T*>(a.xc) + (int64_t)(before + i) * a.Dp;
-      if (a.xs) {
-        T* ys = static_cast<T*>(a.xs) + (int64_t)(before + i) * a.Dp;
-        const float s = scale[i];
+      T* ys = a.xs ? static_cast<T*>(a.xs) + (int64_t)(before + i) * a.Dp : nullptr;
+      const float s = scale[i];
+      if (a.vec) {  // 16 bytes at a time
+        typedef typename Elem<T>::Frag F;
+#pragma unroll 4
+        for (int c = lane * per16<T>; c < a.D; c += 64 * per16<T>) {
+          F v = *reinterpret_cast<const F*>(x + c);
+          *reinterpret_cast<F*>(y + c) = v;
+          if (ys) {
+#pragma unroll
+            for (int e = 0; e < per16<T>; ++e) v[e] = from_f32<T>(to_f32(v[e]) * s);
+            *reinterpret_cast<F*>(ys + c) = v;
+          }
+        }
+      } else {
+#pragma unroll 8
         for (int c = lane; c < a.Dp; c += 64) {
           const T v = c < a.D ? x[c] : (T)0.f;
           y[c] = v;
-          ys[c] = from_f32<T>(to_f32(v) * s);
+          if (ys) ys[c] = from_f32<T>(to_f32(v) * s);
         }
-      } else {
-        for (int c = lane; c < a.Dp; c += 64) y[c] = c < a.D ? x[c] : (T)0.f;
       }
     }
     before += n;
@@ -150,9 +164,31 @@ struct FwdArgs {
   int T, V, tm, tn, splits, per;  // per: vocabulary tiles of a split
 };
 
-template <typename T, class C>
-__global__ __launch_bounds__(threads_of<C>, 2) void xent_fwd_kernel(FwdArgs a) {
+// The tiles' product: KS > 0: of that many steps of k at most, A's fragments in registers.
+template <typename T, class C, int KS, int STORES>
+struct Tiles : Thin<T, KS, C, STORES> {
+  static constexpr int LDS = Thin<T, KS, C, STORES>::LDS;
+  typedef Thin<T, KS, C, STORES> P;
+  template <class Done>
+  __device__ __forceinline__ static void go(typename P::StageA& sa, typename P::StageB& sb, int64_t, int tiles, T* sm,
+                                            int wave, int lane, f32x4 (&acc)[P::MI][P::NJ], Done done) {
+    P::run_tiles(sa, sb, tiles, sm, wave, lane, acc, done);
+  }
+};
+template <typename T, class C, int STORES>
+struct Tiles<T, C, 0, STORES> : Product<T, ROW, ROW, C> {
+  static constexpr int LDS = lds_of<C>;
   typedef Product<T, ROW, ROW, C> P;
+  template <class Done>
+  __device__ __forceinline__ static void go(typename P::StageA& sa, typename P::StageB& sb, int64_t K, int tiles, T* sm,
+                                            int wave, int lane, f32x4 (&acc)[P::MI][P::NJ], Done done) {
+    P::run_tiles(sa, sb, (int)((K + k_step<T> - 1) / k_step<T>), tiles, sm, wave, lane, acc, done);
+  }
+};
+
+template <typename T, class C, int KS>
+__global__ __launch_bounds__(threads_of<C>, 2) void xent_fwd_kernel(FwdArgs a) {
+  typedef Tiles<T, C, KS, 0> P;
   extern __shared__ __align__(16) char sm[];
   int tm, split;
   tile_of(blockIdx.x, a.tm, a.splits, tm, split);
@@ -163,15 +199,14 @@ __global__ __launch_bounds__(threads_of<C>, 2) void xent_fwd_kernel(FwdArgs a) {
   float top[P::MI], sum[P::MI];
 #pragma unroll
   for (int i = 0; i < P::MI; ++i) top[i] = -INFINITY, sum[i] = 0.f;
-  const int t1 = min(a.tn, (split + 1) * a.per);
-  for (int t = split * a.per; t < t1; ++t) {
-    const int n0 = t * C::TN;
-    typename P::StageA sa;
-    typename P::StageB sb;
-    sa.init(static_cast<const T*>(a.xc) + m0 * a.ldx, a.ldx, M - m0, a.K, threadIdx.x);
-    sb.init(static_cast<const T*>(a.w) + n0 * a.ldw, a.ldw, a.V - n0, a.K, threadIdx.x);
-    f32x4 acc[P::MI][P::NJ] = {};
-    P::run(sa, sb, (int)((a.K + k_step<T> - 1) / k_step<T>), reinterpret_cast<T*>(sm), wave, lane, acc);
+  const int t0 = split * a.per, tiles = min(a.tn - t0, a.per);
+  typename P::StageA sa;
+  typename P::StageB sb;
+  sa.init(static_cast<const T*>(a.xc) + m0 * a.ldx, a.ldx, M - m0, a.K, threadIdx.x);
+  sb.init(static_cast<const T*>(a.w) + (int64_t)t0 * C::TN * a.ldw, a.ldw, a.V - t0 * C::TN, a.K, threadIdx.x);
+  f32x4 acc[P::MI][P::NJ] = {};
+  P::go(sa, sb, a.K, tiles, reinterpret_cast<T*>(sm), wave, lane, acc, [&](int t) {
+    const int n0 = (t0 + t) * C::TN;
     if (n0 + C::TN > a.V) {  // past the vocabulary
 #pragma unroll
       for (int j = 0; j < P::NJ; ++j) {
@@ -198,7 +233,7 @@ __global__ __launch_bounds__(threads_of<C>, 2) void xent_fwd_kernel(FwdArgs a) {
         for (int r = 0; r < 4; ++r) s += exp2_fast(__builtin_fmaf(acc[i][j][r], kLog2e, -(ref * kLog2e)));
       join(top[i], sum[i], m, s * unround(ref));
     }
-  }
+  });
   // over the four lanes of a row
 #pragma unroll
   for (int i = 0; i < P::MI; ++i) {
@@ -242,6 +277,7 @@ __global__ __launch_bounds__(256) void xent_loss_kernel(LossArgs a) {
       if (t >= 0) {
         const T* x = static_cast<const T*>(a.xc) + i * a.ldx;
         const T* w = static_cast<const T*>(a.w) + t * a.ldw;
+#pragma unroll 8
         for (int k = lane; k < a.K; k += 64) dot = __builtin_fmaf(to_f32(x[k]), to_f32(w[k]), dot);
       }
       const float m = wave_max(top), ref = m == -INFINITY ? 0.f : m;
@@ -266,11 +302,16 @@ __global__ __launch_bounds__(256) void xent_loss_kernel(LossArgs a) {
   if (threadIdx.x == 0) a.sums[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
 }
 // The workgroups' sums in a fixed order.
-__global__ __launch_bounds__(64) void xent_total_kernel(const double* sums, int n, const int* count, float* out,
-                                                        int reduction) {
+__global__ __launch_bounds__(256) void xent_total_kernel(const double* sums, int n, const int* count, float* out,
+                                                         int reduction) {
+  __shared__ double red[4];
   double v = 0;
-  for (int i = threadIdx.x; i < n; i += 64) v += sums[i];
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += 256) v += sums[i];
   v = wave_sum_d(v);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = red[0] + red[1] + red[2] + red[3];
   if (threadIdx.x == 0) *out = (float)(reduction == PNFX_REDUCE_MEAN ? v / *count : v);
 }
 
@@ -282,61 +323,88 @@ struct GradArgs {
   const float4* rowc;
   const int *tgt, *count;
   int64_t ldx, ldw, K, ldd;
-  int v0, P, tm, tn;  // the piece's first token, its tokens
+  int v0, P, tm, tn, splits, per;  // the piece's first token, its tokens; column tiles of a workgroup
 };
 
-template <typename T, class C>
+__device__ __forceinline__ void store16(__amdgpu_buffer_rsrc_t d, unsigned at, u32x4 v) {
+  __builtin_amdgcn_raw_buffer_store_b128(v, d, at, 0, 0);
+}
+
+template <typename T, class C, int KS>
 __global__ __launch_bounds__(threads_of<C>, 2) void xent_grad_kernel(GradArgs a) {
-  typedef Product<T, ROW, ROW, C> P;
+  // 16-byte stores of a lane and tile
+  constexpr int STORES = (C::TM / C::WM / 16) * (C::TN / C::WN / 16) * 4 / per16<T>;
+  typedef Tiles<T, C, KS, STORES> P;
   extern __shared__ __align__(16) char sm[];
-  int tm, tn;
-  tile_of(blockIdx.x, a.tm, a.tn, tm, tn);
-  const int M = *a.count, m0 = tm * C::TM, n0 = tn * C::TN;
+  int tm, split;
+  tile_of(blockIdx.x, a.tm, a.splits, tm, split);
+  const int M = *a.count, m0 = tm * C::TM;
   if (m0 >= M) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave / C::WN * P::MI, wn = wave % C::WN * P::NJ;
+  const int Pc = (a.P + 7) & ~7;  // columns past the piece, up to a whole chunk, are zero
+  // of each row its log-sum-exp and its target's column in the piece, if it has one there (in LDS: there are
+  // no registers left for them beside A's fragments); published by the loop's first barrier
+  __shared__ float2 rows[C::TM];
+  for (int r = threadIdx.x; r < C::TM; r += threads_of<C>) {
+    const int m = min(m0 + r, M - 1);
+    rows[r] = float2{a.rowc[m].x, __int_as_float(a.tgt[m] - a.v0)};
+  }
+  const auto out = __builtin_amdgcn_make_buffer_rsrc(static_cast<T*>(a.d) + m0 * a.ldd, 0,
+                                                     (int)(min(M - m0, C::TM) * a.ldd * sizeof(T)), 0x00027000);
+  const unsigned ldb = (unsigned)(a.ldd * sizeof(T)), row = stage_row<ROW>(wm, lane & 15) * ldb;
+  const int t0 = split * a.per, tiles = min(a.tn - t0, a.per);
   typename P::StageA sa;
   typename P::StageB sb;
   sa.init(static_cast<const T*>(a.xc) + m0 * a.ldx, a.ldx, M - m0, a.K, threadIdx.x);
-  sb.init(static_cast<const T*>(a.w) + n0 * a.ldw, a.ldw, a.P - n0, a.K, threadIdx.x);
+  sb.init(static_cast<const T*>(a.w) + (int64_t)t0 * C::TN * a.ldw, a.ldw, a.P - t0 * C::TN, a.K, threadIdx.x);
   f32x4 acc[P::MI][P::NJ] = {};
-  P::run(sa, sb, (int)((a.K + k_step<T> - 1) / k_step<T>), reinterpret_cast<T*>(sm), wave, lane, acc);
-  const int Pc = (a.P + 7) & ~7;  // columns past the piece, up to a whole chunk, are zero
+  P::go(sa, sb, a.K, tiles, reinterpret_cast<T*>(sm), wave, lane, acc, [&](int t) {
+    // the lane's first column; block j's are col(j) .. col(j) + 3 behind it
+    const int n0 = (t0 + t) * C::TN, nl = n0 + 16 * wn + 8 * (lane >> 4);
+    const auto col = [](int j) { return stage_row<ROW>(j, 0); };
+    const bool edge = n0 + C::TN > a.P;
 #pragma unroll
-  for (int i = 0; i < P::MI; ++i) {
-    const int m = m0 + stage_row<ROW>(wm + i, lane & 15);
-    if (m >= M) continue;
-    const float4 c = a.rowc[m];
-    const float lse = c.x * kLog2e, factor = c.w * unround(c.x);
-    T* row = static_cast<T*>(a.d) + m * a.ldd;
-    // two blocks: eight columns of a lane
+    for (int i = 0; i < P::MI; ++i) {
+      const float2 c = rows[stage_row<ROW>(wm + i, lane & 15)];
 #pragma unroll
-    for (int j = 0; j < P::NJ; j += 2) {
-      const int n = n0 + stage_row<ROW>(wn + j, 4 * (lane >> 4));
-      if (n >= Pc) continue;
-      float v[8];
+      for (int j = 0; j < P::NJ; ++j)
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        v[r] = exp2_fast(__builtin_fmaf(acc[i][j + (r >> 2)][r & 3], kLog2e, -lse)) * factor;
-        if (n + r >= a.P) v[r] = 0.f;
+        for (int r = 0; r < 4; ++r)
+          acc[i][j][r] = exp2_fast((acc[i][j][r] - c.x) * kLog2e);
+      // 16 bytes at a time; the buffer's bounds drop the rows past M, a far offset the columns past the piece
+      const unsigned at = row + stage_row<ROW>(i, 0) * ldb + nl * (unsigned)sizeof(T);
+#pragma unroll
+      for (int j = 0; j < P::NJ; j += 2) {
+        float v[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) v[r] = acc[i][j + (r >> 2)][r & 3];
+        unsigned o = at + col(j) * (unsigned)sizeof(T);
+        if (edge) {
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            if (nl + col(j) + r >= a.P) v[r] = 0.f;
+          if (nl + col(j) >= Pc) o = 0x80000000u;
+        }
+        if constexpr (sizeof(T) == 2) {
+          store16(out, o, __builtin_bit_cast(u32x4, pack8(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7])));
+        } else {
+          store16(out, o, __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]}));
+          store16(out, o + 16, __builtin_bit_cast(u32x4, f32x4{v[4], v[5], v[6], v[7]}));
+        }
       }
-      if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<bf16x8*>(row + n) = pack8(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
-      } else {
-        *reinterpret_cast<f32x4*>(row + n) = f32x4{v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<f32x4*>(row + n + 4) = f32x4{v[4], v[5], v[6], v[7]};
+      // seldom: the row's target is among the lane's columns; this store is the same thread's and comes later
+      const int own = __float_as_int(c.y) - nl;
+      if ((unsigned)own < 16u * P::NJ && (own & 24) == 0) {
+        const T v = from_f32<T>(a.rowc[min(m0 + stage_row<ROW>(wm + i, lane & 15), M - 1)].z);
+        if constexpr (sizeof(T) == 2)
+          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), out, at + own * 2, 0, 0);
+        else
+          __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), out, at + own * 4, 0, 0);
       }
+      __builtin_amdgcn_sched_barrier(0);  // one row block at a time: no registers for more
     }
-  }
-  // the targets of this tile's rows that are in its columns, once the tile's stores are done
-  __builtin_amdgcn_s_waitcnt(0x0F70);
-  __syncthreads();
-  for (int r = threadIdx.x; r < C::TM && m0 + r < M; r += threads_of<C>) {
-    const int m = m0 + r, t = a.tgt[m] - a.v0;
-    if (t >= n0 && t < min(n0 + C::TN, a.P)) {
-      static_cast<T*>(a.d)[m * a.ldd + t] = from_f32<T>(expm1f(-a.rowc[m].z));
-    }
-  }
+  });
 }
 
 struct DxArgs {
@@ -408,11 +476,26 @@ FwdCut fwd_cut(const Sizes& z) {
   c.splits = ceil_div(c.tn, c.per);
   return c;
 }
-// Rows of d that stay in the last-level cache with their piece's weights: 64 MB.
+// Tokens of a piece: 256 MB of d, the last-level cache's size.  Smaller pieces write and read dx's fp32 sums
+// more often and give the products fewer k or rows (xent_lm 2102 us at 64 MB, 1830 at 128, 1711 at 256, 1739 at 512;
+// xent_narrow 914, 743, 685, 741; xent_large 7018, 6461, 6362, 6246).
 int64_t piece_of(const Sizes& z) {
-  const int64_t most = std::min(round_up(std::max<int64_t>((64ll << 20) / (z.T * z.es), 2048), 256), kMaxLd / 2);
+  const int64_t most = std::min(round_up(std::max<int64_t>((256ll << 20) / (z.T * z.es), 2048), 256), kMaxLd / 2);
   const int64_t n = ceil_div(z.V, most);
   return round_up(ceil_div(z.V, n), 256);
+}
+
+// Calls f(tile, steps) with the kernels' variant for this width: bf16 rows of up to 256 take Thin's.
+template <typename T, class Fn>
+int by_width(bool big, const Sizes& z, Fn f) {
+  if constexpr (sizeof(T) == 2) {
+    if (big) return f(Big{}, std::integral_constant<int, 0>{});
+    if (z.Dp <= 64) return f(Mid{}, std::integral_constant<int, 1>{});
+    if (z.Dp <= 128) return f(Mid{}, std::integral_constant<int, 2>{});
+    if (z.Dp <= 192) return f(Mid{}, std::integral_constant<int, 3>{});
+    if (z.Dp <= 256) return f(Mid{}, std::integral_constant<int, 4>{});
+  }
+  return f(Mid{}, std::integral_constant<int, 0>{});
 }
 
 struct Kept {
@@ -430,7 +513,7 @@ Kept take_kept(Arena& ar, const Sizes& z, bool copy) {
   k.w = copy ? ar.take<char>(z.V * z.Dp * z.es) : nullptr;
   return k;
 }
-int loss_rows_per(const Sizes& z) { return (int)std::max<int64_t>(4, ceil_div(z.T, 2048)); }
+int loss_rows_per(const Sizes& z) { return (int)std::max<int64_t>(4, ceil_div(z.T, 1024)); }
 int64_t loss_blocks(const Sizes& z) { return ceil_div(z.T, loss_rows_per(z)); }
 
 int64_t fwd_bytes(const Sizes& z, bool copy) {
@@ -471,7 +554,8 @@ int keep_rows(const Kept& k, const void* x, int64_t x_rs, const int64_t* target,
   a.x = x, a.target = target, a.xc = k.xc, a.pos = k.pos, a.src = k.src, a.tgt = k.tgt, a.count = k.count;
   a.x_rs = x_rs, a.ignore = ignore;
   a.T = (int)z.T, a.D = (int)z.D, a.Dp = (int)z.Dp, a.V = (int)z.V;
-  a.per = (int)std::max<int64_t>(16, ceil_div(z.T, kRowsBlocks));
+  a.per = (int)std::max<int64_t>(4, ceil_div(z.T, kRowsBlocks));
+  a.vec = z.D == z.Dp && operand_ok(x, x_rs, z.es);
   return launch<xent_rows_kernel<T>>(ceil_div(z.T, a.per), 256, 0, a, st, "xent rows");
 }
 // W in place, or its padded copy.
@@ -494,20 +578,17 @@ int xent_fwd(const void* x, int64_t x_rs, const void* w, int64_t w_rs, const int
   PNFX_TRY(take_w(k, w, w_rs, z, st));
   PNFX_TRY(keep_rows<T>(k, x, x_rs, target, ignore, z, RowsArgs{}, st));
   FwdArgs f{k.xc, w, part, k.count, z.Dp, w_rs, z.Dp, (int)z.T, (int)z.V, (int)c.tm, (int)c.tn, (int)c.splits, (int)c.per};
-  int wn = Mid::WN;
-  if constexpr (sizeof(T) == 2) {
-    if (c.big) {
-      wn = Big::WN;
-      PNFX_TRY((launch<xent_fwd_kernel<T, Big>>(c.tm * c.splits, threads_of<Big>, lds_of<Big>, f, st, "xent_fwd")));
-    }
-  }
-  if (!c.big)
-    PNFX_TRY((launch<xent_fwd_kernel<T, Mid>>(c.tm * c.splits, threads_of<Mid>, lds_of<Mid>, f, st, "xent_fwd")));
+  const int wn = c.big ? Big::WN : Mid::WN;
+  PNFX_TRY((by_width<T>(c.big, z, [&](auto cfg, auto ks) {
+    typedef decltype(cfg) C;
+    constexpr int KS = decltype(ks)::value;
+    return launch<xent_fwd_kernel<T, C, KS>>(c.tm * c.splits, threads_of<C>, Tiles<T, C, KS, 0>::LDS, f, st, "xent_fwd");
+  })));
   LossArgs l{k.xc, w, part, k.pos, k.tgt, k.count, rows, lse, out, sums, z.Dp, w_rs,
              (int)z.T, (int)z.D, (int)c.splits * wn, reduction, loss_rows_per(z)};
   PNFX_TRY((launch<xent_loss_kernel<T>>(loss_blocks(z), 256, 0, l, st, "xent_loss")));
   if (reduction == PNFX_REDUCE_NONE) return PNFX_OK;
-  hipLaunchKernelGGL(xent_total_kernel, dim3(1), dim3(64), 0, st, sums, (int)loss_blocks(z), k.count, out, reduction);
+  hipLaunchKernelGGL(xent_total_kernel, dim3(1), dim3(256), 0, st, sums, (int)loss_blocks(z), k.count, out, reduction);
   return launch_status("xent_total");
 }
 
@@ -532,15 +613,18 @@ int xent_bwd(const float* dloss, const void* x, int64_t x_rs, const void* w, int
   for (int64_t v0 = 0; v0 < z.V; v0 += c.P) {
     const int64_t n = std::min(c.P, z.V - v0);
     const T* wp = static_cast<const T*>(w) + v0 * w_rs;
-    GradArgs g{k.xc, wp, d, r.rowc, k.tgt, k.count, z.Dp, w_rs, z.Dp, c.P, (int)v0, (int)n, 0, 0};
+    GradArgs g{k.xc, wp, d, r.rowc, k.tgt, k.count, z.Dp, w_rs, z.Dp, c.P, (int)v0, (int)n, 0, 0, 0, 0};
     const bool big = cut_of(z.T, n, z.Dp, z.dtype, false).big && z.D >= 768;
     g.tm = (int)ceil_div(z.T, big ? 256 : 128), g.tn = (int)ceil_div(round_up(n, 8), big ? 256 : 128);
-    if constexpr (sizeof(T) == 2) {
-      if (big)
-        PNFX_TRY((launch<xent_grad_kernel<T, Big>>((int64_t)g.tm * g.tn, threads_of<Big>, lds_of<Big>, g, st, "xent_grad")));
-    }
-    if (!big)
-      PNFX_TRY((launch<xent_grad_kernel<T, Mid>>((int64_t)g.tm * g.tn, threads_of<Mid>, lds_of<Mid>, g, st, "xent_grad")));
+    const int64_t want = ceil_div(big ? 1024 : 2048, g.tm);
+    g.per = (int)ceil_div(g.tn, std::min<int64_t>(want, g.tn));
+    g.splits = (int)ceil_div(g.tn, g.per);
+    PNFX_TRY((by_width<T>(big, z, [&](auto cfg, auto ks) {
+      typedef decltype(cfg) C;
+      constexpr int KS = decltype(ks)::value;
+      return launch<xent_grad_kernel<T, C, KS>>((int64_t)g.tm * g.splits, threads_of<C>, Tiles<T, C, KS, 0>::LDS, g, st,
+                                                "xent_grad");
+    })));
     if (dx) {
       ProductArgs p = {};
       p.a = d, p.b = wp, p.lda = c.P, p.ldb = w_rs, p.M = z.T, p.N = z.D, p.K = n;
