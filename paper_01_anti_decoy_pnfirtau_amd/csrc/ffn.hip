@@ -24,10 +24,23 @@
 namespace pnfx {
 namespace {
 
+// Phi(g), the normal distribution, and e = exp(-g^2 / 2): Phi by formula 7.1.26 of Abramowitz and Stegun's
+// Handbook of Mathematical Functions for erf, which is within 1.5e-7, of |g| / sqrt 2; it uses the same e.
+__device__ __forceinline__ float phi(float g, float& e) {
+  const float x = fabsf(g) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.f));
+  e = __expf(-x * x);
+  float q = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+  q = __builtin_fmaf(q, t, 1.421413741f);
+  q = __builtin_fmaf(q, t, -0.284496736f);
+  q = __builtin_fmaf(q, t, 0.254829592f);
+  q *= 0.5f * t * e;
+  return g >= 0.f ? 1.f - q : q;
+}
 template <int ACT>
 __device__ __forceinline__ float act_of(float g) {
   if constexpr (ACT == PNFX_ACT_SILU) return g * __builtin_amdgcn_rcpf(1.f + __expf(-g));
-  return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
+  float e;
+  return g * phi(g, e);
 }
 // act(g) and act'(g)
 template <int ACT>
@@ -37,14 +50,14 @@ __device__ __forceinline__ void act_both(float g, float& a, float& d) {
     a = g * p;
     d = p * (1.f + g * (1.f - p));
   } else {
-    const float p = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+    float e;
+    const float p = phi(g, e);
     a = g * p;
-    d = p + g * 0.39894228040143268f * __expf(-0.5f * g * g);
+    d = p + g * 0.39894228040143268f * e;
   }
 }
 
 // -------------------------------------------------------------------- blocks of 32
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 // The largest finite |v| of the lane's eight values and the other three lanes' of the row's 32.
 __device__ __forceinline__ float block_top(const float* v) {
@@ -76,33 +89,6 @@ __device__ __forceinline__ void unpack_e4m3(uint32_t w, float s, float* v) {
   v[1] = __builtin_amdgcn_cvt_f32_fp8((int)w, 1) * s;
   v[2] = __builtin_amdgcn_cvt_f32_fp8((int)w, 2) * s;
   v[3] = __builtin_amdgcn_cvt_f32_fp8((int)w, 3) * s;
-}
-
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float* v) {
-  if constexpr (sizeof(T) == 2) {
-    *reinterpret_cast<bf16x8*>(p) = pack8(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
-  } else {
-    *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-    *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
-  }
-}
-template <typename T>
-__device__ __forceinline__ void store4f(T* p, const float* v) {
-  if constexpr (sizeof(T) == 2) *reinterpret_cast<bf16x4*>(p) = bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
-  else *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-}
-template <typename T>
-__device__ __forceinline__ void load4f(const T* p, float* v) {
-  if constexpr (sizeof(T) == 2) {
-    const bf16x4 b = *reinterpret_cast<const bf16x4*>(p);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = (float)b[r];
-  } else {
-    const f32x4 b = *reinterpret_cast<const f32x4*>(p);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = b[r];
-  }
 }
 
 // Fp: F rounded up to a multiple of 8, the columns of h, of either half of g | u and of either half of dg | du;
@@ -190,6 +176,59 @@ __global__ __launch_bounds__(threads_of<C>, 2) void glu_fwd_kernel(GluArgs a) {
   }
 }
 
+// Eight columns of g and u as they were kept, from memory and as fp32.
+template <typename T>
+struct KeptPart;
+template <>
+struct KeptPart<float> {
+  f32x4 g[2], u[2];
+  __device__ __forceinline__ void load(const GluArgs& a, int m, int f, int) {
+    const float* p = static_cast<const float*>(a.gu) + (int64_t)m * 2 * a.Fp + f;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      g[r] = *reinterpret_cast<const f32x4*>(p + 4 * r);
+      u[r] = *reinterpret_cast<const f32x4*>(p + a.Fp + 4 * r);
+    }
+  }
+  __device__ __forceinline__ void get(int, float* vg, float* vu) const {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) vg[r] = g[r >> 2][r & 3], vu[r] = u[r >> 2][r & 3];
+  }
+};
+template <>
+struct KeptPart<bf16> {
+  uint4 g, u;  // e4m3: the first half of each
+  uint8_t sg, su;
+  __device__ __forceinline__ void load(const GluArgs& a, int m, int f, int block) {
+    const int64_t at = (int64_t)m * 2 * a.Fp + f;
+    if (a.keep == PNFX_KEEP_FULL) {
+      const _Float16* p = static_cast<const _Float16*>(a.gu) + at;
+      g = *reinterpret_cast<const uint4*>(p);
+      u = *reinterpret_cast<const uint4*>(p + a.Fp);
+    } else {
+      const uint8_t* p = static_cast<const uint8_t*>(a.gu) + at;
+      const uint2 g2 = *reinterpret_cast<const uint2*>(p), u2 = *reinterpret_cast<const uint2*>(p + a.Fp);
+      g.x = g2.x, g.y = g2.y, u.x = u2.x, u.y = u2.y;
+    }
+    const uint8_t* sc = a.scales + (int64_t)m * 2 * a.nb + block;
+    sg = sc[0];
+    su = sc[a.nb];
+  }
+  __device__ __forceinline__ void get(int keep, float* vg, float* vu) const {
+    const float fg = pow2((int)sg - 127), fu = pow2((int)su - 127);
+    if (keep == PNFX_KEEP_FULL) {
+      const f16x8 hg = __builtin_bit_cast(f16x8, g), hu = __builtin_bit_cast(f16x8, u);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) vg[r] = (float)hg[r] * fg, vu[r] = (float)hu[r] * fu;
+    } else {
+      unpack_e4m3(g.x, fg, vg);
+      unpack_e4m3(g.y, fg, vg + 4);
+      unpack_e4m3(u.x, fu, vu);
+      unpack_e4m3(u.y, fu, vu + 4);
+    }
+  }
+};
+
 template <typename T, int ACT, class C>
 __global__ __launch_bounds__(threads_of<C>, 2) void glu_bwd_kernel(GluArgs a) {
   typedef Product<T, ROW, COL, C> P;
@@ -205,50 +244,47 @@ __global__ __launch_bounds__(threads_of<C>, 2) void glu_bwd_kernel(GluArgs a) {
   f32x4 acc[P::MI][P::NJ] = {};
   P::run(sa, sb, (int)((a.K + k_step<T> - 1) / k_step<T>), reinterpret_cast<T*>(sm), wave, lane, acc);
   const int wm = wave / C::WN * P::MI, wn = wave % C::WN * P::NJ;
+  // g and u of one row block are read while the block before is worked on
+  typedef KeptPart<T> Part;
+  constexpr int NP = P::NJ / 2;  // pairs of blocks: eight columns of a lane, 32 of a wave
+  Part part[2][NP];
+  const auto fetch = [&](int i) {
+    const int m = min(m0 + stage_row<ROW>(wm + i, lane & 15), a.T - 1);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const int f = n0 + pair_col<COL>(wn + 2 * p, lane);
+      part[i & 1][p].load(a, m, min(f, a.Fp - 8), min((n0 + 16 * (wn + 2 * p)) / 32, a.nb - 1));
+    }
+  };
+  fetch(0);
 #pragma unroll
   for (int i = 0; i < P::MI; ++i) {
+    if (i + 1 < P::MI) fetch(i + 1);
+    __builtin_amdgcn_sched_barrier(0);
     const int m = m0 + stage_row<ROW>(wm + i, lane & 15);
-    if (m >= a.T) continue;
 #pragma unroll
-    for (int j = 0; j < P::NJ; ++j) {
-      const int f = n0 + stage_row<COL>(wn + j, 4 * (lane >> 4));
-      if (f >= a.Fp) continue;
-      const int64_t at = (int64_t)m * 2 * a.Fp + f;
-      float g[4], u[4], dg[4], du[4], h[4];
-      if constexpr (sizeof(T) == 4) {
-        load4f(static_cast<const float*>(a.gu) + at, g);
-        load4f(static_cast<const float*>(a.gu) + at + a.Fp, u);
-      } else {
-        const uint8_t* sc = a.scales + (int64_t)m * 2 * a.nb + f / 32;
-        const float sg = pow2((int)sc[0] - 127), su = pow2((int)sc[a.nb] - 127);
-        if (a.keep == PNFX_KEEP_FULL) {
-          const _Float16* gu = static_cast<const _Float16*>(a.gu) + at;
-          const f16x4 hg = *reinterpret_cast<const f16x4*>(gu), hu = *reinterpret_cast<const f16x4*>(gu + a.Fp);
+    for (int p = 0; p < NP; ++p) {
+      const int f = n0 + pair_col<COL>(wn + 2 * p, lane);
+      float dh[8], g[8], u[8], dg[8], du[8], h[8];
+      pair8<COL>(acc[i][2 * p], acc[i][2 * p + 1], dh);
+      part[i & 1][p].get(a.keep, g, u);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            g[r] = (float)hg[r] * sg;
-            u[r] = (float)hu[r] * su;
-          }
-        } else {
-          const uint8_t* gu = static_cast<const uint8_t*>(a.gu) + at;
-          unpack_e4m3(*reinterpret_cast<const uint32_t*>(gu), sg, g);
-          unpack_e4m3(*reinterpret_cast<const uint32_t*>(gu + a.Fp), su, u);
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
+      for (int r = 0; r < 8; ++r) {
         float s, d;
         act_both<ACT>(g[r], s, d);
         // columns between F and Fp are of zero weights: zero for any dy, an infinite one too
-        const float dh = f + r < a.F ? acc[i][j][r] : 0.f;
-        dg[r] = dh * u[r] * d;
-        du[r] = dh * s;
+        const float v = f + r < a.F ? dh[r] : 0.f;
+        dg[r] = v * u[r] * d;
+        du[r] = v * s;
         h[r] = s * u[r];
       }
-      store4f(static_cast<T*>(a.dgu) + at, dg);
-      store4f(static_cast<T*>(a.dgu) + at + a.Fp, du);
-      store4f(static_cast<T*>(a.h) + (int64_t)m * a.Fp + f, h);
+      if (m >= a.T || f >= a.Fp) continue;
+      T* o = static_cast<T*>(a.dgu) + (int64_t)m * 2 * a.Fp + f;
+      store8(o, dg);
+      store8(o + a.Fp, du);
+      store8(static_cast<T*>(a.h) + (int64_t)m * a.Fp + f, h);
     }
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
@@ -485,7 +521,7 @@ int ffn_fwd(const FwdArgs& f, const Sizes& z, void* ws, hipStream_t st) {
   a.x = x.p, a.wg = wg, a.wu = wu, a.h = h, a.gu = f.gu, a.scales = f.scales;
   a.ldx = x.ld, a.ldw = win.ld, a.K = z.Dp;
   a.T = (int)z.T, a.F = (int)z.F, a.Fp = (int)z.Fp, a.nb = (int)z.nb, a.keep = f.keep;
-  PNFX_TRY((glu_fwd<T, ACT>(a, cut_of(z.T, 2 * z.Fp, z.Dp, z.dtype, false).big, st)));
+  PNFX_TRY((glu_fwd<T, ACT>(a, cut_of(z.T, 2 * z.Fp, z.Dp, z.dtype, false).big(), st)));
   const Cut cut = cut_of(z.T, z.Do, z.Fp, z.dtype, true);
   ProductArgs p = {};
   p.a = h, p.b = wd.p, p.c = f.y, p.lda = z.Fp, p.ldb = wd.ld, p.ldc = z.Do;
@@ -534,7 +570,7 @@ int ffn_bwd(const BwdArgs& f, const Sizes& z, void* ws, hipStream_t st) {
   a.x = dy.p, a.wg = wd.p, a.h = h, a.gu = const_cast<void*>(f.gu), a.scales = const_cast<uint8_t*>(f.scales);
   a.dgu = dgu, a.ldx = dy.ld, a.ldw = wd.ld, a.K = z.Do;
   a.T = (int)z.T, a.F = (int)z.F, a.Fp = (int)z.Fp, a.nb = (int)z.nb, a.keep = f.keep;
-  PNFX_TRY((glu_bwd<T, ACT>(a, cut_of(z.T, z.Fp, z.Do, z.dtype, false).big, st)));
+  PNFX_TRY((glu_bwd<T, ACT>(a, cut_of(z.T, z.Fp, z.Do, z.dtype, false).big(), st)));
   if (f.dx) {
     ProductArgs p = {};
     p.a = dgu, p.b = win.p, p.c = f.dx, p.lda = 2 * z.Fp, p.ldb = win.ld, p.ldc = z.D;

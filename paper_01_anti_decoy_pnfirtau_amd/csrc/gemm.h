@@ -229,24 +229,63 @@ __device__ __forceinline__ int stage_row(int blk, int r) {
   return KIND == COL ? 16 * blk + r : 64 * (blk >> 2) + perm_row(blk & 3, r);
 }
 
-// Tiles of TM x TN by WM x WN waves.  Big for products with tiles enough for every CU, two waves per SIMD;
-// Mid, two workgroups per CU, for the others and for fp32.
+// The eight consecutive columns that a lane holds of one row after pair8 of the sums of blocks blk and blk + 1 (blk
+// even).  ROW: those that perm_row gives the two blocks.  COL: the first four of a block are exchanged with
+// the neighbouring lane group's, so that even groups hold columns of the first block and odd ones of the second.
+template <Kind KB>
+__device__ __forceinline__ int pair_col(int blk, int lane) {
+  const int a = lane >> 4;
+  return KB == COL ? 16 * (blk + (a & 1)) + 8 * (a >> 1) : stage_row<ROW>(blk, 4 * a);
+}
+template <Kind KB>
+__device__ __forceinline__ void pair8(const f32x4& x, const f32x4& y, float* v) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    if constexpr (KB == COL) {
+      const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x[r]), __float_as_uint(y[r]), false, false);
+      v[r] = __uint_as_float(s[0]);
+      v[r + 4] = __uint_as_float(s[1]);
+    } else {
+      v[r] = x[r];
+      v[r + 4] = y[r];
+    }
+  }
+}
+// Eight values to memory that is aligned to an element: gfx950 takes 16 bytes at any address.
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float* v) {
+  if constexpr (sizeof(T) == 2) {
+    typedef bf16x8 V __attribute__((aligned(2)));
+    *reinterpret_cast<V*>(p) = pack8(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
+  } else {
+    typedef f32x4 V __attribute__((aligned(4)));
+    *reinterpret_cast<V*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<V*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+  }
+}
+
+// Tiles of TM x TN by WM x WN waves, KG such groups of waves with a share of k each.  Big for products with tiles
+// enough for every CU, two waves per SIMD; Mid, two workgroups per CU, for the others and for fp32; Duo, a CU's two
+// Mid workgroups on the two halves of one tile's k, where there are fewer tiles than places for them.
 struct Big {
-  static constexpr int TM = 256, TN = 256, WM = 2, WN = 4, PER_CU = 1;
+  static constexpr int TM = 256, TN = 256, WM = 2, WN = 4, KG = 1;
 };
 struct Mid {
-  static constexpr int TM = 128, TN = 128, WM = 2, WN = 2, PER_CU = 2;
+  static constexpr int TM = 128, TN = 128, WM = 2, WN = 2, KG = 1;
+};
+struct Duo {
+  static constexpr int TM = 128, TN = 128, WM = 2, WN = 2, KG = 2;
 };
 template <class C>
-constexpr int threads_of = 64 * C::WM * C::WN;
+constexpr int threads_of = 64 * C::WM * C::WN * C::KG;
 template <class C>
-constexpr int lds_of = 2 * (C::TM + C::TN) * 128;
+constexpr int lds_of = C::KG * 2 * (C::TM + C::TN) * 128;
 
 // acc[i][j][r] of a wave (wm, wn): row m = stage_row<KA>(wm MI + i, lane % 16), column n =
 // stage_row<KB>(wn NJ + j, 4 (lane / 16) + r) of the tile.
 template <typename T, Kind KA, Kind KB, class C>
 struct Product {
-  static constexpr int TM = C::TM, TN = C::TN, NT = threads_of<C>;
+  static constexpr int TM = C::TM, TN = C::TN, NT = threads_of<C> / C::KG;  // of a group of waves
   static constexpr int MI = TM / C::WM / 16, NJ = TN / C::WN / 16;
   static_assert(MI % 4 == 0 && NJ % 4 == 0, "a wave's share is whole sub-tiles");
   typedef Stage<T, KA, TM, NT> StageA;
@@ -449,6 +488,7 @@ struct Thin {
 
 // Workgroup `id` of tm x tn tiles.  Consecutive ids go to the eight XCDs in turn: each XCD takes a range of
 // tiles of its own, column by column over bands of four tile rows, so that its L2 holds what they share.
+// (Where the number of rows is on the device, tm is of those, so that no XCD is left with tiles of none.)
 __device__ __forceinline__ void tile_of(int id, int tm, int tn, int& m, int& n) {
   const int total = tm * tn, q = total / 8, r = total % 8, x = id % 8, y = id / 8;
   id = x < r ? x * (q + 1) + y : r * (q + 1) + (x - r) * q + y;

@@ -25,13 +25,15 @@ struct ProductArgs {
   const float* alpha;  // one fp32 value in device memory that C is scaled by before it is rounded, or null
 };
 
-// How a product is cut: tiles of 256 or 128 and splits of its k over workgroups.
+// How a product is cut: its tiles (gemm.h's Mid, Duo or Big) and the splits of its k over workgroups.
 struct Cut {
-  bool big;
+  enum Kind { MID, DUO, BIG } kind;
   int splits;
   int64_t steps;  // steps of a split
+  bool big() const { return kind == BIG; }
 };
-Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool can_split);
+// can_split: whether k may be divided, over workgroups or a workgroup's waves; sums: fp32 sums are wanted anyway.
+Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool can_split, bool sums = false);
 
 // Workspace of product() for C (not sums) at this cut, in bytes.
 int64_t product_workspace(const Cut& cut, int64_t M, int64_t N);

@@ -1,5 +1,7 @@
 // Plain matrix products, the sum of their splits, and zero-padded copies.  What bounds the products and how they
 // are staged: gemm.h.
+#include <algorithm>
+
 #include "product.h"
 
 namespace pnfx {
@@ -14,7 +16,7 @@ struct MmArgs {
   int gap_at, gap;
   const int *m_count, *k_count;
   const float* alpha;
-  bool add;
+  bool add, by_xcd;
 };
 
 // Row of C of product row m, or -1.
@@ -23,69 +25,111 @@ __device__ __forceinline__ int out_row(int m, int gap_at, int gap) {
   return m < gap_at + gap ? -1 : m - gap;
 }
 
-// Four columns from n on of a row of `N`, vectors where the row allows them.
+// The first `n` of eight elements (eight, where there are more).
 template <typename T>
-__device__ __forceinline__ void store4(T* row, int n, int N, bool aligned, f32x4 v) {
-  if (aligned && n + 4 <= N) {
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<f32x4*>(row + n) = v;
-    } else {
-      *reinterpret_cast<bf16x4*>(row + n) = bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
-    }
-  } else {
+__device__ __forceinline__ void store_upto8(T* p, int n, const float* v) {
+  if (n >= 8) return store8(p, v);
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (n + r < N) row[n + r] = from_f32<T>(v[r]);
+  for (int r = 0; r < 7; ++r)
+    if (r < n) p[r] = from_f32<T>(v[r]);
+}
+__device__ __forceinline__ void load8(const float* p, int n, float* v) {
+  typedef f32x4 V __attribute__((aligned(4)));
+  if (n >= 8) {
+    const f32x4 x = *reinterpret_cast<const V*>(p), y = *reinterpret_cast<const V*>(p + 4);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = x[r], v[r + 4] = y[r];
+    return;
   }
+#pragma unroll
+  for (int r = 0; r < 8; ++r) v[r] = r < n ? p[r] : 0.f;
 }
 
 template <typename T, Kind KA, Kind KB, class C>
 __global__ __launch_bounds__(threads_of<C>, 2) void mm_kernel(MmArgs g) {
   typedef Product<T, KA, KB, C> P;
   extern __shared__ __align__(16) char sm[];
-  const int split = blockIdx.x / (g.tm * g.tn);
-  int tm, tn;
-  tile_of(blockIdx.x - split * g.tm * g.tn, g.tm, g.tn, tm, tn);
-  const int m0 = tm * C::TM, n0 = tn * C::TN;
   const int M = g.m_count ? min(g.M, *g.m_count) : g.M;
-  if (m0 >= M) return;
+  const int tms = (M + C::TM - 1) / C::TM, tiles = tms * g.tn;
+  if ((int)blockIdx.x >= tiles * g.splits) return;
+  int split = blockIdx.x / tiles, id = blockIdx.x % tiles;
+  if (g.by_xcd) {
+    // the tiles of a split read the same k: all on one XCD (workgroup id % 8), which so reads it once
+    split = (int)blockIdx.x / 8 / tiles * 8 + (int)blockIdx.x % 8;
+    id = (int)blockIdx.x / 8 % tiles;
+  }
+  int tm, tn;
+  if (g.by_xcd) tn = id % g.tn, tm = id / g.tn;
+  else tile_of(id, tms, g.tn, tm, tn);
+  const int m0 = tm * C::TM, n0 = tn * C::TN;
   const int64_t K = g.k_count ? min<int64_t>(g.K, *g.k_count) : g.K;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int64_t k0 = split * g.steps * k_step<T>;
-  const int64_t ks = min<int64_t>(K - k0, g.steps * k_step<T>);
+  const int all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  constexpr int WAVES = C::WM * C::WN;
+  const int group = all / WAVES, wave = all % WAVES;
+  int64_t k0 = split * g.steps * k_step<T>;
+  int64_t ks = min<int64_t>(K - k0, g.steps * k_step<T>);
+  int steps = (int)((ks + k_step<T> - 1) / k_step<T>);
+  if constexpr (C::KG == 2) {  // as many steps for either group; past the end they read zeros
+    steps = (steps + 1) / 2;
+    const int64_t half = (int64_t)steps * k_step<T>;
+    k0 += group * half;
+    ks = group ? ks - half : min(ks, half);
+  }
   typename P::StageA sa;
   typename P::StageB sb;
   const T* a = static_cast<const T*>(g.a) + (KA == COL ? k0 * g.lda + m0 : m0 * g.lda + k0);
   const T* b = static_cast<const T*>(g.b) + (KB == COL ? k0 * g.ldb + n0 : n0 * g.ldb + k0);
-  sa.init(a, g.lda, M - m0, ks, threadIdx.x);
-  sb.init(b, g.ldb, g.N - n0, ks, threadIdx.x);
+  sa.init(a, g.lda, M - m0, ks, threadIdx.x % P::NT);
+  sb.init(b, g.ldb, g.N - n0, ks, threadIdx.x % P::NT);
   f32x4 acc[P::MI][P::NJ] = {};
-  P::run(sa, sb, (int)((ks + k_step<T> - 1) / k_step<T>), reinterpret_cast<T*>(sm), wave, lane, acc);
+  P::run(sa, sb, steps, reinterpret_cast<T*>(sm + group * (lds_of<C> / C::KG)), wave, lane, acc);
+  int i0 = 0, i1 = P::MI;
+  if constexpr (C::KG == 2) {
+    // each group adds up and stores half of the tile: the other half's sums go to the other group
+    constexpr int H = P::MI / 2;
+    f32x4* other = reinterpret_cast<f32x4*>(sm + group * (lds_of<C> / 2)) + wave * (H * P::NJ * 64) + lane;
+    const f32x4* mine = reinterpret_cast<f32x4*>(sm + (group ^ 1) * (lds_of<C> / 2)) + wave * (H * P::NJ * 64) + lane;
+#pragma unroll
+    for (int i = 0; i < H; ++i)
+#pragma unroll
+      for (int j = 0; j < P::NJ; ++j) other[(i * P::NJ + j) * 64] = group ? acc[i][j] : acc[H + i][j];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < H; ++i)
+#pragma unroll
+      for (int j = 0; j < P::NJ; ++j) {
+        if (group) acc[H + i][j] += mine[(i * P::NJ + j) * 64];
+        else acc[i][j] += mine[(i * P::NJ + j) * 64];
+      }
+    i0 = group * H, i1 = i0 + H;
+  }
   const int wm = wave / C::WN * P::MI, wn = wave % C::WN * P::NJ;
   float* sums = g.sums ? g.sums + (int64_t)split * g.M * g.N : nullptr;
-  const bool aligned = g.ldc % 4 == 0;
   const float alpha = g.alpha ? *g.alpha : 1.f;
 #pragma unroll
   for (int i = 0; i < P::MI; ++i) {
+    if (C::KG == 2 && (i < i0 || i >= i1)) continue;
     const int m = m0 + stage_row<KA>(wm + i, lane & 15);
-    if (m >= M) continue;
     const int row = out_row(m, g.gap_at, g.gap);
 #pragma unroll
-    for (int j = 0; j < P::NJ; ++j) {
-      const int n = n0 + stage_row<KB>(wn + j, 4 * (lane >> 4));
-      if (n >= g.N) continue;
+    for (int j = 0; j < P::NJ; j += 2) {
+      const int n = n0 + pair_col<KB>(wn + j, lane);
+      float v[8];
+      pair8<KB>(acc[i][j], acc[i][j + 1], v);
+      if (m >= M || n >= g.N) continue;
       if (sums) {
         float* s = sums + (int64_t)m * g.N + n;
-        if (g.N % 4 == 0) {
-          f32x4* s4 = reinterpret_cast<f32x4*>(s);
-          *s4 = g.add ? *s4 + acc[i][j] : acc[i][j];
-        } else {
+        if (g.add) {
+          float old[8];
+          load8(s, g.N - n, old);
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (n + r < g.N) s[r] = g.add ? s[r] + acc[i][j][r] : acc[i][j][r];
+          for (int r = 0; r < 8; ++r) v[r] += old[r];
         }
+        store_upto8(s, g.N - n, v);
       } else if (row >= 0) {
-        store4<T>(static_cast<T*>(g.c) + row * g.ldc, n, g.N, aligned, acc[i][j] * alpha);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) v[r] *= alpha;
+        store_upto8(static_cast<T*>(g.c) + row * g.ldc + n, g.N - n, v);
       }
     }
   }
@@ -96,50 +140,56 @@ struct SumArgs {
   void* c;
   const float* alpha;
   int64_t MN, ldc;
-  int N, splits, gap_at, gap;
+  int M, N, groups, splits, gap_at, gap;  // groups: of eight columns, in a row
 };
-// C from the splits' sums, added in split order: four elements per thread.
+// C from the splits' sums, added in split order: eight columns per thread.
 template <typename T>
 __global__ __launch_bounds__(256) void mm_sum_kernel(SumArgs g) {
-  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (e >= g.MN) return;
-  const float alpha = g.alpha ? *g.alpha : 1.f;
-  if (g.N % 4 == 0) {
-    f32x4 acc = *reinterpret_cast<const f32x4*>(g.sums + e);
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int m = (int)(id / g.groups), n = (int)(id % g.groups) * 8;
+  if (m >= g.M) return;
+  const int row = out_row(m, g.gap_at, g.gap);
+  if (row < 0) return;
+  const float* s = g.sums + (int64_t)m * g.N + n;
+  float v[8] = {};
 #pragma unroll 4
-    for (int s = 1; s < g.splits; ++s) acc += *reinterpret_cast<const f32x4*>(g.sums + s * g.MN + e);
-    const int row = out_row((int)(e / g.N), g.gap_at, g.gap);
-    if (row >= 0)
-      store4<T>(static_cast<T*>(g.c) + row * g.ldc, (int)(e % g.N), g.N, g.ldc % 4 == 0, acc * alpha);
-    return;
+  for (int p = 0; p < g.splits; ++p) {
+    float x[8];
+    load8(s + p * g.MN, g.N - n, x);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) v[r] += x[r];
   }
-  for (int64_t i = e; i < min<int64_t>(e + 4, g.MN); ++i) {
-    float acc = g.sums[i];
-    for (int s = 1; s < g.splits; ++s) acc += g.sums[s * g.MN + i];
-    const int row = out_row((int)(i / g.N), g.gap_at, g.gap);
-    if (row >= 0) static_cast<T*>(g.c)[row * g.ldc + i % g.N] = from_f32<T>(acc * alpha);
-  }
+  const float alpha = g.alpha ? *g.alpha : 1.f;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) v[r] *= alpha;
+  store_upto8(static_cast<T*>(g.c) + row * g.ldc + n, g.N - n, v);
 }
 
 constexpr int kMaxPads = 4;
 struct PadArgs {
   PadItem item[kMaxPads];
-  int64_t first[kMaxPads + 1];  // workgroups of 4 rows each
+  int64_t first[kMaxPads + 1];  // workgroups
   int n;
 };
-// One wave per row.
+// Eight columns per thread, read at any alignment.
 template <typename T>
 __global__ __launch_bounds__(256) void pad_kernel(PadArgs g) {
   int i = 0;
   while (i + 1 < g.n && (int64_t)blockIdx.x >= g.first[i + 1]) ++i;
   const PadItem& p = g.item[i];
-  const int64_t r = (blockIdx.x - g.first[i]) * 4 + (threadIdx.x >> 6);
+  const int64_t id = (blockIdx.x - g.first[i]) * 256 + threadIdx.x, groups = p.cols_out / 8;
+  const int64_t r = id / groups, c = id % groups * 8;
   if (r >= p.rows_out * p.halves) return;
   const int64_t half = r / p.rows_out, in = r % p.rows_out;
-  const T* src = static_cast<const T*>(p.src) + (half * p.rows + in) * p.ld;
-  T* dst = static_cast<T*>(p.dst) + r * p.cols_out;
-  for (int64_t c = threadIdx.x & 63; c < p.cols_out; c += 64)
-    dst[c] = in < p.rows && c < p.cols ? src[c] : (T)0.f;
+  const T* src = static_cast<const T*>(p.src) + (half * p.rows + in) * p.ld + c;
+  T v[8];
+  if (in < p.rows && c + 8 <= p.cols) {
+    __builtin_memcpy(v, src, sizeof(v));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = in < p.rows && c + e < p.cols ? src[e] : (T)0.f;
+  }
+  __builtin_memcpy(__builtin_assume_aligned(static_cast<T*>(p.dst) + r * p.cols_out + c, 16), v, sizeof(v));
 }
 
 template <typename T, Kind KA, Kind KB, class C>
@@ -157,29 +207,37 @@ int mm_kinds(int ka, int kb, const MmArgs& g, hipStream_t st) {
 }  // namespace
 
 // The cut that is expected to be done first.  A tile's step takes, with one of its kind on every CU, the time of
-// its products at the rate that gemm.h's figures give; a split adds its fp32 sums' way to memory and back.
-Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool can_split) {
+// its products at the rate that gemm.h's figures give, or half a microsecond if the step's loads are not hidden by
+// another workgroup's products; a split adds its fp32 sums' way to memory and back.
+Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool can_split, bool sums) {
   const int es = dtype == PNFX_F32 ? 4 : 2;
   const int64_t steps = ceil_div(K, 128 / es);
-  Cut best{false, 1, steps};
+  Cut best{Cut::MID, 1, steps};
   double best_us = 1e30;
-  for (int big = 0; big < (dtype == PNFX_BF16 ? 2 : 1); ++big) {
-    const int64_t T = big ? 256 : 128, tiles = ceil_div(M, T) * ceil_div(N, T);
-    // us of one step of a tile alone on its CU, and of the CU's tiles together
-    const double rate = dtype == PNFX_F32 ? 110e6 : big ? 1300e6 : 1050e6;  // operations per us on 256 CUs
-    const int per_cu = big ? 1 : 2;
-    const double step_us = 2.0 * T * T * (128 / es) / (rate / 256) * per_cu;
+  for (int kind = 0; kind < 3; ++kind) {
+    if (kind == Cut::BIG && dtype == PNFX_F32) continue;
+    if (kind == Cut::DUO && !can_split) continue;
+    const int64_t T = kind == Cut::BIG ? 256 : 128, tiles = ceil_div(M, T) * ceil_div(N, T);
+    const double rate = dtype == PNFX_F32 ? 120e6 : kind == Cut::BIG ? 1300e6 : 1050e6;  // operations per us, 256 CUs
+    const double step_us = 2.0 * T * T * (128 / es) / (rate / 256);  // of one tile that has the CU to itself
     for (int64_t s = 1; s <= 64; s *= 2) {
       if (s > 1 && (!can_split || steps / s < 4)) break;
-      const int64_t per = ceil_div(steps, s), slots = 256 * per_cu;
-      const int64_t full = tiles * s / slots, rest = tiles * s % slots;
-      // a last round that leaves CUs with one tile of two runs it faster
-      const double last = !rest ? 0 : per_cu == 2 && rest <= 256 ? 0.9 : 1;
-      double us = (full + last) * (per * step_us + 2.0);
-      if (s > 1) us += 4.0 + s * M * N * 8 / 4e6;
+      const int64_t per = ceil_div(steps, s), work = tiles * s;
+      double us = 3.0;
+      if (kind == Cut::MID) {
+        // pairs on a CU; the last round may have CUs with one, whose step is not hidden
+        const int64_t full = work / 512, rest = work % 512;
+        us += full * (per * 2 * step_us + 1.5);
+        if (rest) us += per * (rest > 256 ? 2 * step_us : std::max(1.75 * step_us, 0.45)) + 1.5;
+      } else if (kind == Cut::DUO) {
+        us += ceil_div(work, 256) * (ceil_div(per, 2) * std::max(2 * step_us, 0.45) + 2.0);
+      } else {
+        us += ceil_div(work, 256) * (per * step_us + 3.0);
+      }
+      us += (s > 1 || sums ? s * M * N * 4 / 4e6 : 0) + (s > 1 && !sums ? 4.0 + s * M * N * 4 / 4e6 : 0);
       if (us < best_us) {
         best_us = us;
-        best = Cut{big != 0, (int)ceil_div(steps, per), per};
+        best = Cut{(Cut::Kind)kind, (int)ceil_div(steps, per), per};
       }
     }
   }
@@ -198,7 +256,7 @@ int product(int ka, int kb, const ProductArgs& p, const Cut& cut, int dtype, voi
                (long long)p.M, (long long)p.N, (long long)p.K);
   const bool summed = !p.sums && cut.splits > 1;
   PNFX_REQUIRE(!summed || workspace, "product: no workspace");
-  const int64_t T = cut.big ? 256 : 128;
+  const int64_t T = cut.kind == Cut::BIG ? 256 : 128;
   MmArgs g;
   g.a = p.a;
   g.b = p.b;
@@ -220,15 +278,17 @@ int product(int ka, int kb, const ProductArgs& p, const Cut& cut, int dtype, voi
   g.k_count = p.k_count;
   g.add = p.add;
   g.alpha = summed ? nullptr : p.alpha;
+  g.by_xcd = cut.splits % 8 == 0;
   if (dtype == PNFX_F32)
-    PNFX_TRY((mm_kinds<float, Mid>(ka, kb, g, st)));
-  else if (cut.big)
-    PNFX_TRY((mm_kinds<bf16, Big>(ka, kb, g, st)));
+    PNFX_TRY((cut.kind == Cut::DUO ? mm_kinds<float, Duo>(ka, kb, g, st) : mm_kinds<float, Mid>(ka, kb, g, st)));
   else
-    PNFX_TRY((mm_kinds<bf16, Mid>(ka, kb, g, st)));
+    PNFX_TRY((cut.kind == Cut::BIG   ? mm_kinds<bf16, Big>(ka, kb, g, st)
+              : cut.kind == Cut::DUO ? mm_kinds<bf16, Duo>(ka, kb, g, st)
+                                     : mm_kinds<bf16, Mid>(ka, kb, g, st)));
   if (!summed) return PNFX_OK;
-  SumArgs s{g.sums, p.c, p.alpha, p.M * p.N, p.ldc, g.N, cut.splits, g.gap_at, g.gap};
-  const int64_t grid = ceil_div(s.MN, 1024);
+  const int64_t groups = ceil_div(p.N, 8);
+  SumArgs s{g.sums, p.c, p.alpha, p.M * p.N, p.ldc, g.M, g.N, (int)groups, cut.splits, g.gap_at, g.gap};
+  const int64_t grid = ceil_div(p.M * groups, 256);
   return dtype == PNFX_F32 ? launch<mm_sum_kernel<float>>(grid, 256, 0, s, st, "product sums")
                            : launch<mm_sum_kernel<bf16>>(grid, 256, 0, s, st, "product sums");
 }
@@ -240,7 +300,7 @@ int pad(const PadItem* items, int n, int dtype, hipStream_t st) {
   g.first[0] = 0;
   for (int i = 0; i < n; ++i) {
     g.item[i] = items[i];
-    g.first[i + 1] = g.first[i] + ceil_div(items[i].rows_out * items[i].halves, 4);
+    g.first[i + 1] = g.first[i] + ceil_div(items[i].rows_out * items[i].halves * (items[i].cols_out / 8), 256);
   }
   return dtype == PNFX_F32 ? launch<pad_kernel<float>>(g.first[n], 256, 0, g, st, "pad")
                            : launch<pad_kernel<bf16>>(g.first[n], 256, 0, g, st, "pad");

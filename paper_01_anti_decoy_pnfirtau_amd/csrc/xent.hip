@@ -158,10 +158,10 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs a) {
 struct FwdArgs {
   const void* xc;
   const void* w;
-  float2* part;  // [splits * WN][T] running maximum and sum
+  float2* part;  // [T][splits * WN] running maximum and sum
   const int* count;
   int64_t ldx, ldw, K;
-  int T, V, tm, tn, splits, per;  // per: vocabulary tiles of a split
+  int T, V, tn, splits, per;  // per: vocabulary tiles of a split
 };
 
 // The tiles' product: KS > 0: of that many steps of k at most, A's fragments in registers.
@@ -190,10 +190,11 @@ template <typename T, class C, int KS>
 __global__ __launch_bounds__(threads_of<C>, 2) void xent_fwd_kernel(FwdArgs a) {
   typedef Tiles<T, C, KS, 0> P;
   extern __shared__ __align__(16) char sm[];
+  const int M = *a.count, tms = (M + C::TM - 1) / C::TM;
+  if ((int)blockIdx.x >= tms * a.splits) return;
   int tm, split;
-  tile_of(blockIdx.x, a.tm, a.splits, tm, split);
-  const int M = *a.count, m0 = tm * C::TM;
-  if (m0 >= M) return;
+  tile_of(blockIdx.x, tms, a.splits, tm, split);
+  const int m0 = tm * C::TM;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave / C::WN * P::MI, wn = wave % C::WN * P::NJ;
   float top[P::MI], sum[P::MI];
@@ -241,7 +242,7 @@ __global__ __launch_bounds__(threads_of<C>, 2) void xent_fwd_kernel(FwdArgs a) {
     for (int o = 16; o <= 32; o <<= 1)
       join(top[i], sum[i], __shfl_xor(top[i], o, 64), __shfl_xor(sum[i], o, 64));
     const int m = m0 + stage_row<ROW>(wm + i, lane & 15);
-    if (lane < 16 && m < M) a.part[(int64_t)(split * C::WN + wave % C::WN) * a.T + m] = float2{top[i], sum[i]};
+    if (lane < 16 && m < M) a.part[(int64_t)m * (a.splits * C::WN) + split * C::WN + wave % C::WN] = float2{top[i], sum[i]};
   }
 }
 
@@ -269,7 +270,7 @@ __global__ __launch_bounds__(256) void xent_loss_kernel(LossArgs a) {
     if (i >= 0) {
       float top = -INFINITY, sum = 0.f;
       for (int p = lane; p < a.parts; p += 64) {
-        const float2 v = a.part[(int64_t)p * a.T + i];
+        const float2 v = a.part[(int64_t)i * a.parts + p];
         join(top, sum, v.x, v.y);
       }
       const int t = a.tgt[i];
@@ -323,7 +324,7 @@ struct GradArgs {
   const float4* rowc;
   const int *tgt, *count;
   int64_t ldx, ldw, K, ldd;
-  int v0, P, tm, tn, splits, per;  // the piece's first token, its tokens; column tiles of a workgroup
+  int v0, P, tn, splits, per;  // the piece's first token, its tokens; column tiles of a workgroup
 };
 
 __device__ __forceinline__ void store16(__amdgpu_buffer_rsrc_t d, unsigned at, u32x4 v) {
@@ -336,10 +337,11 @@ __global__ __launch_bounds__(threads_of<C>, 2) void xent_grad_kernel(GradArgs a)
   constexpr int STORES = (C::TM / C::WM / 16) * (C::TN / C::WN / 16) * 4 / per16<T>;
   typedef Tiles<T, C, KS, STORES> P;
   extern __shared__ __align__(16) char sm[];
+  const int M = *a.count, tms = (M + C::TM - 1) / C::TM;
+  if ((int)blockIdx.x >= tms * a.splits) return;
   int tm, split;
-  tile_of(blockIdx.x, a.tm, a.splits, tm, split);
-  const int M = *a.count, m0 = tm * C::TM;
-  if (m0 >= M) return;
+  tile_of(blockIdx.x, tms, a.splits, tm, split);
+  const int m0 = tm * C::TM;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave / C::WN * P::MI, wn = wave % C::WN * P::NJ;
   const int Pc = (a.P + 7) & ~7;  // columns past the piece, up to a whole chunk, are zero
@@ -464,6 +466,12 @@ struct FwdCut {
   bool big;
   int64_t tm, tn, splits, per;
 };
+// Vocabulary tiles that a workgroup goes through: 64 steps of k to pay for its start, less where that leaves
+// fewer than four workgroups for each place on the chip.
+int64_t tiles_per(const Sizes& z, int64_t tm, int64_t tn) {
+  const int64_t steps = ceil_div(z.D * z.es, 128), most = std::max<int64_t>(1, tm * tn / 2048);
+  return std::min(ceil_div(64, steps), most);
+}
 FwdCut fwd_cut(const Sizes& z) {
   FwdCut c;
   // The exponentials of a 256-tile are not hidden by a neighbour's products (128-tiles share a CU), so a large
@@ -471,8 +479,7 @@ FwdCut fwd_cut(const Sizes& z) {
   c.big = z.dtype == PNFX_BF16 && z.D >= 768 && ceil_div(z.T, 256) * ceil_div(z.V, 256) >= 512;
   c.tm = ceil_div(z.T, c.big ? 256 : 128);
   c.tn = ceil_div(z.V, c.big ? 256 : 128);
-  const int64_t want = ceil_div(c.big ? 1024 : 2048, c.tm);
-  c.per = ceil_div(c.tn, std::min(want, c.tn));
+  c.per = tiles_per(z, c.tm, c.tn);
   c.splits = ceil_div(c.tn, c.per);
   return c;
 }
@@ -531,7 +538,7 @@ struct BwdCut {
 BwdCut bwd_cut(const Sizes& z) {
   BwdCut c;
   c.P = std::min(piece_of(z), round_up(z.V, 8));
-  c.dx = cut_of(z.T, z.D, c.P, z.dtype, true);
+  c.dx = cut_of(z.T, z.D, c.P, z.dtype, true, true);
   c.dw = cut_of(c.P, z.D, z.T, z.dtype, true);
   return c;
 }
@@ -577,7 +584,7 @@ int xent_fwd(const void* x, int64_t x_rs, const void* w, int64_t w_rs, const int
   double* sums = ar.take<double>(loss_blocks(z));
   PNFX_TRY(take_w(k, w, w_rs, z, st));
   PNFX_TRY(keep_rows<T>(k, x, x_rs, target, ignore, z, RowsArgs{}, st));
-  FwdArgs f{k.xc, w, part, k.count, z.Dp, w_rs, z.Dp, (int)z.T, (int)z.V, (int)c.tm, (int)c.tn, (int)c.splits, (int)c.per};
+  FwdArgs f{k.xc, w, part, k.count, z.Dp, w_rs, z.Dp, (int)z.T, (int)z.V, (int)c.tn, (int)c.splits, (int)c.per};
   const int wn = c.big ? Big::WN : Mid::WN;
   PNFX_TRY((by_width<T>(c.big, z, [&](auto cfg, auto ks) {
     typedef decltype(cfg) C;
@@ -613,16 +620,16 @@ int xent_bwd(const float* dloss, const void* x, int64_t x_rs, const void* w, int
   for (int64_t v0 = 0; v0 < z.V; v0 += c.P) {
     const int64_t n = std::min(c.P, z.V - v0);
     const T* wp = static_cast<const T*>(w) + v0 * w_rs;
-    GradArgs g{k.xc, wp, d, r.rowc, k.tgt, k.count, z.Dp, w_rs, z.Dp, c.P, (int)v0, (int)n, 0, 0, 0, 0};
-    const bool big = cut_of(z.T, n, z.Dp, z.dtype, false).big && z.D >= 768;
-    g.tm = (int)ceil_div(z.T, big ? 256 : 128), g.tn = (int)ceil_div(round_up(n, 8), big ? 256 : 128);
-    const int64_t want = ceil_div(big ? 1024 : 2048, g.tm);
-    g.per = (int)ceil_div(g.tn, std::min<int64_t>(want, g.tn));
+    GradArgs g{k.xc, wp, d, r.rowc, k.tgt, k.count, z.Dp, w_rs, z.Dp, c.P, (int)v0, (int)n, 0, 0, 0};
+    const bool big = cut_of(z.T, n, z.Dp, z.dtype, false).big() && z.D >= 768;
+    const int64_t tm = ceil_div(z.T, big ? 256 : 128);
+    g.tn = (int)ceil_div(round_up(n, 8), big ? 256 : 128);
+    g.per = (int)tiles_per(z, tm, g.tn);
     g.splits = (int)ceil_div(g.tn, g.per);
     PNFX_TRY((by_width<T>(big, z, [&](auto cfg, auto ks) {
       typedef decltype(cfg) C;
       constexpr int KS = decltype(ks)::value;
-      return launch<xent_grad_kernel<T, C, KS>>((int64_t)g.tm * g.splits, threads_of<C>, Tiles<T, C, KS, 0>::LDS, g, st,
+      return launch<xent_grad_kernel<T, C, KS>>(tm * g.splits, threads_of<C>, Tiles<T, C, KS, 0>::LDS, g, st,
                                                 "xent_grad");
     })));
     if (dx) {
