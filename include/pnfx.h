@@ -314,7 +314,8 @@ int pnfx_flash_bwd_noalloc(const void* q, int64_t qsb, int64_t qsh, int64_t qsn,
 #define PNFX_KEEP_NONE 0
 #define PNFX_KEEP_FULL 1
 #define PNFX_KEEP_E4M3 2
-int64_t pnfx_ffn_fwd_workspace_size(int64_t T, int64_t D, int64_t F, int64_t Do, int copies, int dtype);
+int64_t pnfx_ffn_fwd_workspace_size(int64_t T, int64_t D, int64_t F, int64_t Do, int keep, int copies,
+                                    int dtype);
 int pnfx_ffn_fwd(const void* x, int64_t x_rs, const void* w_in, int64_t win_rs, const void* w_down,
                  int64_t wd_rs, void* y, void* gu, uint8_t* scales, int64_t T, int64_t D, int64_t F,
                  int64_t Do, int act, int keep, int dtype, void* workspace, int64_t workspace_bytes,

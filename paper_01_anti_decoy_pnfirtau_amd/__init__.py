@@ -43,5 +43,6 @@ def __getattr__(name):
     if name in ("gated_ffn", "linear_cross_entropy"):
         from . import hip_lm
 
-        return getattr(hip_lm, name)
+        globals()[name] = getattr(hip_lm, name)  # found directly from now on
+        return globals()[name]
     raise AttributeError(name)

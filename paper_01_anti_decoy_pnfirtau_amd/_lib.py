@@ -68,8 +68,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     sig["pnfx_flash_bwd_stages"] = ([i32] + sig["pnfx_flash_bwd"][0], i32)
     bwd = sig["pnfx_flash_bwd"][0]  # pnfx_flash_bwd without (workspace, workspace_bytes)
     sig["pnfx_flash_bwd_noalloc"] = (bwd[:37] + bwd[39:], i32)
-    for name in ("pnfx_ffn_fwd_workspace_size", "pnfx_ffn_bwd_workspace_size"):
-        sig[name] = ([i64] * 4 + [i32, i32], i64)
+    sig["pnfx_ffn_fwd_workspace_size"] = ([i64] * 4 + [i32] * 3, i64)
+    sig["pnfx_ffn_bwd_workspace_size"] = ([i64] * 4 + [i32] * 2, i64)
     for name in ("pnfx_xent_fwd_workspace_size", "pnfx_xent_bwd_workspace_size"):
         sig[name] = ([i64] * 3 + [i32, i32], i64)
     sig["pnfx_ffn_fwd"] = ([vp, i64] * 3 + [vp] * 3 + [i64] * 4 + [i32] * 3 + [vp, i64, vp], i32)

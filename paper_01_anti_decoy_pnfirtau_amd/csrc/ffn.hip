@@ -15,8 +15,7 @@
 // e4m3, with the smallest s for which |value| <= 448 s).  The backward pass computes with what they stand for.
 //
 // Up to 64 rows (single tokens of a batch) the time is that of reading the weights once, and a 128-row tile
-// would leave most of the chip idle: ffn_rows_kernel gives 16 weight rows to a workgroup, whose waves split
-// k among them and read the weights from global memory into registers.
+// would leave most of the chip idle: ffn_rows_kernel gives 16 weight rows to a workgroup, whose waves split k.
 #include <algorithm>
 
 #include "product.h"
@@ -301,70 +300,96 @@ struct RowsArgs {
 };
 
 // y[t][n] = sum_k x[t][k] w[n][k], or with PAIRED act(that) times the same with w2: 16 n per workgroup, MB blocks of
-// 16 rows t; wave w takes the 128-byte pieces of k number w, w + W, ...  Buffer loads give zeros past N and K.
-// ffn_token (1 row, D = 1024, F = 4096, bf16): see the measured figures at ffn_fwd.
-template <typename T, int ACT, bool PAIRED, int MB, int W>
-__global__ __launch_bounds__(64 * W) void ffn_rows_kernel(RowsArgs a) {
+// 16 rows t; wave w takes the 128-byte pieces of k number w, w + W, ...  Each wave brings its pieces of the weights
+// and of x to LDS of its own, S pieces ahead and without a barrier, eight lanes to a row: read straight into
+// registers in the products' layout, 16 rows side by side, every lane is a cache access of its own (39 for each load
+// of 1 KB, and the address unit busy throughout).  Zeros past N, T and K.
+template <bool PAIRED, int MB>
+struct FewRows {
+  static constexpr int W = PAIRED ? 4 : 8;                      // waves
+  static constexpr int PARTS = (PAIRED ? 2 : 1) + MB;           // 16-row parts of a piece, 2 KB each
+  static constexpr int S = PARTS <= (PAIRED ? 3 : 2) ? 4 : PARTS <= (PAIRED ? 4 : 3) ? 3 : 2;  // pieces on their way
+  static constexpr int LDS = W * S * PARTS * 2048;
+  static_assert(LDS <= 160 * 1024, "a CU's LDS");
+};
+template <typename T, int ACT, bool PAIRED, int MB>
+__global__ __launch_bounds__((64 * FewRows<PAIRED, MB>::W), 2) void ffn_rows_kernel(RowsArgs a) {
   typedef typename Elem<T>::Frag F;
-  constexpr int ES = (int)sizeof(T);
-  constexpr int NM = PAIRED ? 2 : 1;
-  __shared__ f32x4 part[W > 1 ? W - 1 : 1][NM * MB][64];
+  typedef FewRows<PAIRED, MB> R;
+  constexpr int ES = (int)sizeof(T), W = R::W, S = R::S, PARTS = R::PARTS, NM = PAIRED ? 2 : 1;
+  constexpr int PART = 2048 / ES;  // elements
+  extern __shared__ __align__(16) char sm[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int r16 = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;
   const unsigned rows = (unsigned)min(a.N - n0, 16), kb = (unsigned)a.K * ES;
   const unsigned ldw = (unsigned)(a.ldw * ES), ldx = (unsigned)(a.ldx * ES);
-  typedef __amdgpu_buffer_rsrc_t Rsrc;
-  const auto rsrc = [](const void* p, unsigned bytes) -> Rsrc {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00027000);
+  const u32x4 dw = buffer_of(static_cast<const T*>(a.w) + n0 * a.ldw, (rows - 1) * ldw + kb);
+  const u32x4 du = PAIRED ? buffer_of(static_cast<const T*>(a.w2) + n0 * a.ldw, (rows - 1) * ldw + kb) : dw;
+  const u32x4 dx = buffer_of(a.x, (unsigned)(a.T - 1) * ldx + kb);
+  // a load fills eight slots: lane l the chunk that belongs at position l % 8 of slot l / 8 (and slot + 8)
+  const int slot = lane >> 3, c0 = (lane & 7) ^ stage_swz<T, ROW>(slot), c1 = (lane & 7) ^ stage_swz<T, ROW>(slot + 8);
+  T* const ring = reinterpret_cast<T*>(sm) + wave * (S * PARTS * PART);
+  const unsigned at = __builtin_amdgcn_readfirstlane(lds_addr(ring));
+  const auto fetch = [&](int stage, unsigned piece) {
+    const unsigned k0 = piece * 128 + 16 * c0, k1 = piece * 128 + 16 * c1;
+    const auto part = [&](u32x4 d, unsigned ld, int first, int p) {
+      const unsigned to = at + (stage * PARTS + p) * 2048;
+      lds_dma16(d, k0 < kb ? (first + slot) * ld + k0 : 0x80000000u, to);
+      lds_dma16(d, k1 < kb ? (first + slot + 8) * ld + k1 : 0x80000000u, to + 1024);
+    };
+    part(dw, ldw, 0, 0);
+    if constexpr (PAIRED) part(du, ldw, 0, 1);
+#pragma unroll
+    for (int b = 0; b < MB; ++b) part(dx, ldx, 16 * b, NM + b);
   };
-  const Rsrc rw = rsrc(static_cast<const T*>(a.w) + n0 * a.ldw, (rows - 1) * ldw + kb);
-  const Rsrc ru = PAIRED ? rsrc(static_cast<const T*>(a.w2) + n0 * a.ldw, (rows - 1) * ldw + kb) : rw;
-  const Rsrc rx = rsrc(a.x, (unsigned)(a.T - 1) * ldx + kb);
-  const auto load = [&](Rsrc d, unsigned row_at, unsigned k) -> F {  // k: byte within the row
-    return __builtin_bit_cast(F, __builtin_amdgcn_raw_buffer_load_b128(d, k < kb ? row_at + k : 0x80000000u, 0, 0));
-  };
+  const T* frag[2];
+#pragma unroll
+  for (int hf = 0; hf < 2; ++hf)
+    frag[hf] = ring + r16 * (128 / ES) + per16<T> * ((g + 4 * hf) ^ stage_swz<T, ROW>(r16));
   f32x4 acc[NM][MB] = {};
-  // lane group g: bytes 32 g .. 32 g + 31 of each 128-byte piece, two fragments
-  constexpr int U = MB <= 2 ? 4 : 2;  // pieces in flight
   const unsigned pieces = (kb + 127) / 128;
-  for (unsigned p0 = wave; p0 < pieces; p0 += W * U) {
-    F w[U][2], u[U][2], x[U][MB][2];
 #pragma unroll
-    for (int q = 0; q < U; ++q)
+  for (int s = 0; s < S; ++s) fetch(s, wave + s * W);
+  int stage = 0;
+  for (unsigned p = wave; p < pieces; p += W) {
+    wait_vm_lgkm<(S - 1) * PARTS * 2>();
+    F f[2][PARTS];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const unsigned k = (p0 + q * W) * 128 + 32 * g + 16 * e;
-        w[q][e] = load(rw, r16 * ldw, k);
-        if (PAIRED) u[q][e] = load(ru, r16 * ldw, k);
+    for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-        for (int b = 0; b < MB; ++b) x[q][b][e] = load(rx, (16 * b + r16) * ldx, k);
-      }
+      for (int q = 0; q < PARTS; ++q)
+        f[hf][q] = *reinterpret_cast<const F*>(frag[hf] + (stage * PARTS + q) * PART);
+    wait_vm_lgkm<63>();
+    __builtin_amdgcn_sched_barrier(0);
+    fetch(stage, p + S * W);  // past the last piece: zeros, so that the count of loads is the same
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int q = 0; q < U; ++q)
+    for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+      for (int b = 0; b < MB; ++b)
 #pragma unroll
-        for (int b = 0; b < MB; ++b) {
-          acc[0][b] = mma(w[q][e], x[q][b][e], acc[0][b]);
-          if (PAIRED) acc[NM - 1][b] = mma(u[q][e], x[q][b][e], acc[NM - 1][b]);
-        }
+        for (int m = 0; m < NM; ++m) acc[m][b] = mma(f[hf][m], f[hf][NM + b], acc[m][b]);
+    stage = stage + 1 == S ? 0 : stage + 1;
   }
+  wait_vm_lgkm<0>();
+  __syncthreads();
+  f32x4(*const part)[NM * MB][64] = reinterpret_cast<f32x4(*)[NM * MB][64]>(sm);
+  static_assert((W - 1) * NM * MB * 1024 <= R::LDS, "");
   // the waves' sums, added in wave order
-  if constexpr (W > 1) {
-    if (wave) {
+  if (wave) {
 #pragma unroll
-      for (int m = 0; m < NM; ++m)
+    for (int m = 0; m < NM; ++m)
 #pragma unroll
-        for (int b = 0; b < MB; ++b) part[wave - 1][m * MB + b][lane] = acc[m][b];
-    }
-    __syncthreads();
-    if (wave) return;
-    for (int v = 0; v < W - 1; ++v)
-#pragma unroll
-      for (int m = 0; m < NM; ++m)
-#pragma unroll
-        for (int b = 0; b < MB; ++b) acc[m][b] += part[v][m * MB + b][lane];
+      for (int b = 0; b < MB; ++b) part[wave - 1][m * MB + b][lane] = acc[m][b];
   }
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int v = 0; v < W - 1; ++v)
+#pragma unroll
+    for (int m = 0; m < NM; ++m)
+#pragma unroll
+      for (int b = 0; b < MB; ++b) acc[m][b] += part[v][m * MB + b][lane];
 #pragma unroll
   for (int b = 0; b < MB; ++b) {
     const int t = 16 * b + r16;
@@ -378,17 +403,17 @@ __global__ __launch_bounds__(64 * W) void ffn_rows_kernel(RowsArgs a) {
   }
 }
 
-template <typename T, int ACT, bool PAIRED, int MB, int W>
+template <typename T, int ACT, bool PAIRED, int MB>
 int rows_launch(const RowsArgs& a, hipStream_t st) {
-  return launch<ffn_rows_kernel<T, ACT, PAIRED, MB, W>>(ceil_div(a.cols, 16), 64 * W, 0, a, st, "ffn rows");
+  typedef FewRows<PAIRED, MB> R;
+  return launch<ffn_rows_kernel<T, ACT, PAIRED, MB>>(ceil_div(a.cols, 16), 64 * R::W, R::LDS, a, st, "ffn rows");
 }
-// Waves per workgroup: the down projection has F to reduce over and a quarter of the rows.
 template <typename T, int ACT, bool PAIRED>
 int rows_any(const RowsArgs& a, hipStream_t st) {
-  constexpr int W = PAIRED ? 4 : 8;
-  if (a.T <= 16) return rows_launch<T, ACT, PAIRED, 1, W>(a, st);
-  if (a.T <= 32) return rows_launch<T, ACT, PAIRED, 2, W>(a, st);
-  return rows_launch<T, ACT, PAIRED, 4, W>(a, st);
+  if (a.T <= 16) return rows_launch<T, ACT, PAIRED, 1>(a, st);
+  if (a.T <= 32) return rows_launch<T, ACT, PAIRED, 2>(a, st);
+  if (a.T <= 48) return rows_launch<T, ACT, PAIRED, 3>(a, st);
+  return rows_launch<T, ACT, PAIRED, 4>(a, st);
 }
 
 // ------------------------------------------------------------------------ host side
@@ -488,7 +513,8 @@ struct FwdArgs {
 };
 
 // Workspace of the forward pass, with or without padded copies of its operands.
-int64_t fwd_bytes(const Sizes& z, bool copies) {
+bool few_rows(const Sizes& z, int keep) { return z.T <= kFewRows && keep == PNFX_KEEP_NONE; }
+int64_t fwd_bytes(const Sizes& z, int keep, bool copies) {
   Arena ar{nullptr, 0};
   if (copies) {
     ar.take(z.T * z.Dp * z.es);
@@ -496,7 +522,7 @@ int64_t fwd_bytes(const Sizes& z, bool copies) {
     ar.take(z.Do * z.Fp * z.es);
   }
   ar.take(z.T * z.Fp * z.es);
-  ar.take(product_workspace(cut_of(z.T, z.Do, z.Fp, z.dtype, true), z.T, z.Do));
+  if (!few_rows(z, keep)) ar.take(product_workspace(cut_of(z.T, z.Do, z.Fp, z.dtype, true), z.T, z.Do));
   return ar.used;
 }
 
@@ -511,7 +537,7 @@ int ffn_fwd(const FwdArgs& f, const Sizes& z, void* ws, hipStream_t st) {
   PNFX_TRY(pad(ops.pads, ops.n, z.dtype, st));
   const T* wg = static_cast<const T*>(win.p);
   const T* wu = wg + z.Fp * win.ld;
-  if (z.T <= kFewRows && f.keep == PNFX_KEEP_NONE) {
+  if (few_rows(z, f.keep)) {
     RowsArgs r{x.p, wg, wu, h, x.ld, win.ld, z.Fp, (int)z.T, (int)z.F, (int)z.Dp, (int)z.Fp};
     PNFX_TRY((rows_any<T, ACT, true>(r, st)));
     RowsArgs d{h, wd.p, nullptr, f.y, z.Fp, wd.ld, z.Do, (int)z.T, (int)z.Do, (int)z.Fp, (int)z.Do};
@@ -597,10 +623,11 @@ int ffn_bwd(const BwdArgs& f, const Sizes& z, void* ws, hipStream_t st) {
 }  // namespace
 }  // namespace pnfx
 
-extern "C" int64_t pnfx_ffn_fwd_workspace_size(int64_t T, int64_t D, int64_t F, int64_t Do, int copies, int dtype) {
+extern "C" int64_t pnfx_ffn_fwd_workspace_size(int64_t T, int64_t D, int64_t F, int64_t Do, int keep, int copies,
+                                               int dtype) {
   using namespace pnfx;
   if (check_sizes("ffn", T, D, F, Do, PNFX_ACT_SILU, dtype) != PNFX_OK) return 0;
-  return fwd_bytes(sizes_of(T, D, F, Do, dtype), copies);
+  return fwd_bytes(sizes_of(T, D, F, Do, dtype), keep, copies);
 }
 
 extern "C" int pnfx_ffn_fwd(const void* x, int64_t x_rs, const void* w_in, int64_t win_rs, const void* w_down,
@@ -621,7 +648,7 @@ extern "C" int pnfx_ffn_fwd(const void* x, int64_t x_rs, const void* w_in, int64
                "ffn_fwd: results and workspace must be 16-byte aligned");
   const bool copies = !(in_place(x, x_rs, D, z) && z.F == z.Fp && in_place(w_in, win_rs, D, z) &&
                         in_place(w_down, wd_rs, F, z));
-  const int64_t need = fwd_bytes(z, copies);
+  const int64_t need = fwd_bytes(z, keep, copies);
   PNFX_REQUIRE(workspace && workspace_bytes >= need, "ffn_fwd: workspace needs %lld bytes", (long long)need);
   const FwdArgs f{x, w_in, w_down, x_rs, win_rs, wd_rs, y, gu, scales, act, keep};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);

@@ -221,7 +221,7 @@ Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool can_split, bool sums
     const double rate = dtype == PNFX_F32 ? 120e6 : kind == Cut::BIG ? 1300e6 : 1050e6;  // operations per us, 256 CUs
     const double step_us = 2.0 * T * T * (128 / es) / (rate / 256);  // of one tile that has the CU to itself
     for (int64_t s = 1; s <= 64; s *= 2) {
-      if (s > 1 && (!can_split || steps / s < 4)) break;
+      if (s > 1 && (!can_split || steps / s < 4 || tiles * s > 2048)) break;
       const int64_t per = ceil_div(steps, s), work = tiles * s;
       double us = 3.0;
       if (kind == Cut::MID) {

@@ -293,7 +293,8 @@ std::tuple<Tensor, Tensor, Tensor> gated_ffn_cuda(const Tensor& x_in, const Tens
   const c10::DeviceGuard guard(x_in.device());
   const Rows x = rows_of(x_in), w_in = rows_of(w_in_), w_down = rows_of(w_down_);
   const bool copies = !(x.aligned() && w_in.aligned() && w_down.aligned());
-  const int64_t wsb = pnfx_ffn_fwd_workspace_size(z.T, z.D, z.F, z.Do, copies, z.code);
+  const int64_t wsb = pnfx_ffn_fwd_workspace_size(z.T, z.D, z.F, z.Do, (int)keep, copies,
+                                                  z.code);
   Tensor ws = workspace(wsb, x_in);
   check_rc(pnfx_ffn_fwd(x.ptr(), x.rs, w_in.ptr(), w_in.rs, w_down.ptr(), w_down.rs, y.data_ptr(),
                         keep ? gu.data_ptr() : nullptr,

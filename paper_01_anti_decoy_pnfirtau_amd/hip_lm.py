@@ -12,6 +12,8 @@ Under autocast both compute in the autocast type, as ``nn.Linear`` does.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 import torch.nn.functional as F
 
@@ -22,16 +24,23 @@ CHECKPOINTS = ("full", "e4m3")
 REDUCTIONS = ("mean", "sum", "none")
 
 
+@functools.cache
+def _op(name: str):
+    """The operator pnfx::name (importing ops loads the library, which CPU tensors do without)."""
+    from . import ops  # noqa: F401
+
+    return getattr(torch.ops.pnfx, name).default
+
+
 def _one_of(what: str, value: str, choices: tuple[str, ...]) -> None:
     if value not in choices:
         raise ValueError(f"{what} {value!r}: one of {', '.join(choices)}")
 
 
 def _autocast(*tensors: torch.Tensor) -> tuple[torch.Tensor, ...]:
-    device = tensors[0].device.type
-    if not torch.is_autocast_enabled(device):
+    if not torch.is_autocast_enabled("cuda" if tensors[0].is_cuda else "cpu"):
         return tensors
-    dtype = torch.get_autocast_dtype(device)
+    dtype = torch.get_autocast_dtype(tensors[0].device.type)
     return tuple(t.to(dtype) if t.is_floating_point() and t.dtype != torch.float64 else t
                  for t in tensors)
 
@@ -60,12 +69,9 @@ def gated_ffn(x: torch.Tensor, w_in: torch.Tensor, w_down: torch.Tensor, activat
     if not x.is_cuda:
         g, u = F.linear(x, w_in).chunk(2, -1)
         return F.linear((F.silu(g) if activation == "silu" else F.gelu(g)) * u, w_down)
-    from . import ops  # noqa: F401  (registers the pnfx:: ops)
-
-    keep = checkpoint if torch.is_grad_enabled() and any(
-        t.requires_grad for t in (x, w_in, w_down)) else "none"
-    return torch.ops.pnfx.gated_ffn.default(x, w_in, w_down, _lib.PNFX_ACT[activation],
-                                            _lib.PNFX_KEEP[keep])[0]
+    keep = checkpoint if torch.is_grad_enabled() and (
+        x.requires_grad or w_in.requires_grad or w_down.requires_grad) else "none"
+    return _op("gated_ffn")(x, w_in, w_down, _lib.PNFX_ACT[activation], _lib.PNFX_KEEP[keep])[0]
 
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor,
@@ -88,7 +94,4 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
         loss = F.cross_entropy(F.linear(x, weight).reshape(-1, V).float(), target.reshape(-1),
                                ignore_index=ignore_index, reduction=reduction)
         return loss.view(target.shape) if reduction == "none" else loss
-    from . import ops  # noqa: F401
-
-    return torch.ops.pnfx.linear_xent.default(x, weight, target, int(ignore_index),
-                                              _lib.PNFX_REDUCE[reduction])[0]
+    return _op("linear_xent")(x, weight, target, int(ignore_index), _lib.PNFX_REDUCE[reduction])[0]
