@@ -9,6 +9,10 @@ Mirrors the reference's WikiText-2 model and step (``experiments/exp4_wikitext2_
 * ``train_step`` :334-348 -- zero_grad, bf16 autocast forward, next-token cross-entropy,
   backward, AdamW (betas 0.9/0.95).
 
+Beside the reference's model, ``WikiLMConfig`` offers two choices that it does not have: a gated
+feed-forward block (``ffn="swiglu"`` or ``"geglu"``: ``GatedFFN``, whose activations may be kept in
+8 bits) and the loss without materialised logits (``fused_loss``).
+
 ``GraphedStep`` captures that whole step (including the optimizer update) in one HIP graph,
 as the reference's ``experiments/exp4c_cuda_graphs.py:81-108`` does for the attention stack:
 the eager stack is launch-bound at these sizes.
@@ -21,6 +25,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .hip_lm import gated_ffn, linear_cross_entropy
 from .pnfirtau_attention import PnFirConfig, PnFirTauFlashMHA, PnFirTauMHA, PnFirTauTritonMHA
 
 ATTENTION = {
@@ -30,9 +35,17 @@ ATTENTION = {
 }
 
 
+GATED_FFN = {"swiglu": "silu", "geglu": "gelu"}  # WikiLMConfig.ffn: the gate's activation
+
+
 @dataclass
 class WikiLMConfig:
-    """Model shape and optimiser settings (defaults of experiments/exp4_wikitext2_lm.py:67-88)."""
+    """Model shape and optimiser settings (defaults of experiments/exp4_wikitext2_lm.py:67-88).
+
+    ``ffn``: "gelu", the reference's two-layer FFN, or a gated one, "swiglu" or "geglu" (d_ff columns
+    each for the gate and the up projection); ``ffn_checkpoint``: how a gated FFN keeps its
+    projections for the backward pass, "full" or "e4m3" (hip_lm.gated_ffn).  ``fused_loss``: lm_loss
+    computes the loss with hip_lm.linear_cross_entropy instead of materialised logits."""
 
     d_model: int = 64
     n_heads: int = 4
@@ -46,19 +59,45 @@ class WikiLMConfig:
     silence_gamma: float = 0.5
     tau_init: float = 0.0
     fir_k: int = 7
+    ffn: str = "gelu"
+    ffn_checkpoint: str = "full"
+    fused_loss: bool = False
+
+
+class GatedFFN(nn.Module):
+    """Bias-free gated feed-forward block with dropout on its output: ``gate_up.weight`` holds the gate's
+    d_ff rows, then the up projection's (hip_lm.gated_ffn)."""
+
+    def __init__(self, d_model: int, d_ff: int, activation: str = "silu", dropout: float = 0.0,
+                 checkpoint: str = "full"):
+        super().__init__()
+        self.gate_up = nn.Linear(d_model, 2 * d_ff, bias=False)
+        self.down = nn.Linear(d_ff, d_model, bias=False)
+        self.drop = nn.Dropout(dropout)
+        self.activation, self.checkpoint = activation, checkpoint
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return self.drop(gated_ffn(x, self.gate_up.weight, self.down.weight, self.activation,
+                                   self.checkpoint))
 
 
 class Block(nn.Module):
     """Pre-LN residual block (experiments/exp4_wikitext2_lm.py:183-201)."""
 
-    def __init__(self, d_model: int, attn: nn.Module, dropout: float, d_ff: int):
+    def __init__(self, d_model: int, attn: nn.Module, dropout: float, d_ff: int, ffn: str = "gelu",
+                 ffn_checkpoint: str = "full"):
         super().__init__()
         self.ln1 = nn.LayerNorm(d_model)
         self.attn = attn
         self.ln2 = nn.LayerNorm(d_model)
-        self.ffn = nn.Sequential(
-            nn.Linear(d_model, d_ff), nn.GELU(), nn.Linear(d_ff, d_model), nn.Dropout(dropout)
-        )
+        if ffn in GATED_FFN:
+            self.ffn = GatedFFN(d_model, d_ff, GATED_FFN[ffn], dropout, ffn_checkpoint)
+        elif ffn == "gelu":
+            self.ffn = nn.Sequential(
+                nn.Linear(d_model, d_ff), nn.GELU(), nn.Linear(d_ff, d_model), nn.Dropout(dropout)
+            )
+        else:
+            raise ValueError(f"Unknown ffn: {ffn}")
         self.drop = nn.Dropout(dropout)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
@@ -89,20 +128,25 @@ class WikiLM(nn.Module):
             bias=False,
         )
         self.blocks = nn.ModuleList(
-            Block(cfg.d_model, ATTENTION[variant](acfg), cfg.dropout, cfg.d_ff)
+            Block(cfg.d_model, ATTENTION[variant](acfg), cfg.dropout, cfg.d_ff, cfg.ffn,
+                  cfg.ffn_checkpoint)
             for _ in range(cfg.n_layers)
         )
         self.ln_f = nn.LayerNorm(cfg.d_model)
         self.head = nn.Linear(cfg.d_model, vocab, bias=False)
         self.head.weight = self.embed.weight
 
-    def forward(self, idx: torch.Tensor) -> torch.Tensor:
+    def hidden(self, idx: torch.Tensor) -> torch.Tensor:
+        """The rows [B, N, d_model] that the head projects to logits."""
         _, n = idx.shape
         pos = torch.arange(n, device=idx.device).unsqueeze(0)
         h = self.drop(self.embed(idx) + self.pos(pos))
         for blk in self.blocks:
             h = blk(h)
-        return self.head(self.ln_f(h))
+        return self.ln_f(h)
+
+    def forward(self, idx: torch.Tensor) -> torch.Tensor:
+        return self.head(self.hidden(idx))
 
 
 def zipf_tokens(batch: int, seq: int, vocab: int, seed: int, s: float = 1.1) -> torch.Tensor:
@@ -132,9 +176,14 @@ def make_optimizer(model: nn.Module, cfg: WikiLMConfig, capturable: bool = False
 
 
 def lm_loss(model: nn.Module, x: torch.Tensor, amp: bool) -> torch.Tensor:
-    """Next-token cross-entropy over the sequence, under bf16 autocast when ``amp``."""
+    """Next-token cross-entropy over the sequence, under bf16 autocast when ``amp``; without the logits
+    where the model's config has ``fused_loss`` (each sequence's last row, which has no next token, is
+    ignored there)."""
     vocab = model.head.weight.shape[0]
     with torch.autocast(device_type=x.device.type, dtype=torch.bfloat16, enabled=amp):
+        if getattr(getattr(model, "cfg", None), "fused_loss", False):
+            target = torch.cat([x[:, 1:], x.new_full((x.shape[0], 1), -100)], 1)
+            return linear_cross_entropy(model.hidden(x), model.head.weight, target)
         logits = model(x)
         return F.cross_entropy(logits[:, :-1].reshape(-1, vocab), x[:, 1:].reshape(-1))
 
