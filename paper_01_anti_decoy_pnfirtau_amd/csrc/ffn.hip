@@ -552,9 +552,17 @@ int ffn_fwd(const FwdArgs& f, const Sizes& z, void* ws, hipStream_t st) {
   ProductArgs p = {};
   p.a = h, p.b = wd.p, p.c = f.y, p.lda = z.Fp, p.ldb = wd.ld, p.ldc = z.Do;
   p.M = z.T, p.N = z.Do, p.K = z.Fp;
-  return product(ROW, ROW, p, cut, z.dtype, ar.take(product_workspace(cut, z.T, z.Do)), st);
+  const Job job{ROW, ROW, p, cut, ar.take(product_workspace(cut, z.T, z.Do))};
+  return products(&job, 1, z.dtype, st);
 }
 
+// dx, dw_in, dw_down
+void bwd_cuts(const Sizes& z, Shape* s, Cut* cuts) {
+  s[0] = Shape{z.T, z.D, 2 * z.Fp, false};
+  s[1] = Shape{z.Fp + z.F, z.D, z.T, false};
+  s[2] = Shape{z.Do, z.F, z.T, false};
+  cut_group(s, 3, z.dtype, cuts);
+}
 int64_t bwd_bytes(const Sizes& z, bool copies) {
   Arena ar{nullptr, 0};
   if (copies) {
@@ -565,10 +573,10 @@ int64_t bwd_bytes(const Sizes& z, bool copies) {
   }
   ar.take(z.T * 2 * z.Fp * z.es);
   ar.take(z.T * z.Fp * z.es);
-  int64_t most = product_workspace(cut_of(z.T, z.D, 2 * z.Fp, z.dtype, true), z.T, z.D);
-  most = std::max(most, product_workspace(cut_of(2 * z.Fp, z.D, z.T, z.dtype, true), 2 * z.Fp, z.D));
-  most = std::max(most, product_workspace(cut_of(z.Do, z.F, z.T, z.dtype, true), z.Do, z.F));
-  ar.take(most);
+  Shape s[3];
+  Cut cuts[3];
+  bwd_cuts(z, s, cuts);
+  for (int i = 0; i < 3; ++i) ar.take(product_workspace(cuts[i], s[i].M, s[i].N));
   return ar.used;
 }
 
@@ -590,34 +598,31 @@ int ffn_bwd(const BwdArgs& f, const Sizes& z, void* ws, hipStream_t st) {
   const In wd = ops.take(ar, f.w_down, f.wd_rs, z.Do, z.F, z);
   void* dgu = ar.take(z.T * 2 * z.Fp * z.es);
   void* h = ar.take(z.T * z.Fp * z.es);
-  void* rest = ar.take(0);
+  Shape s[3];
+  Cut cuts[3];
+  bwd_cuts(z, s, cuts);
   PNFX_TRY(pad(ops.pads, ops.n, z.dtype, st));
   GluArgs a = {};
   a.x = dy.p, a.wg = wd.p, a.h = h, a.gu = const_cast<void*>(f.gu), a.scales = const_cast<uint8_t*>(f.scales);
   a.dgu = dgu, a.ldx = dy.ld, a.ldw = wd.ld, a.K = z.Do;
   a.T = (int)z.T, a.F = (int)z.F, a.Fp = (int)z.Fp, a.nb = (int)z.nb, a.keep = f.keep;
   PNFX_TRY((glu_bwd<T, ACT>(a, cut_of(z.T, z.Fp, z.Do, z.dtype, false).big(), st)));
-  if (f.dx) {
+  Job jobs[3];
+  int n = 0;
+  const auto job = [&](int i, int ka, const void* pa, int64_t lda, const void* pb, int64_t ldb, void* c, int64_t ldc) {
+    void* sums = ar.take(product_workspace(cuts[i], s[i].M, s[i].N));
+    if (!c) return;
     ProductArgs p = {};
-    p.a = dgu, p.b = win.p, p.c = f.dx, p.lda = 2 * z.Fp, p.ldb = win.ld, p.ldc = z.D;
-    p.M = z.T, p.N = z.D, p.K = 2 * z.Fp;
-    PNFX_TRY(product(ROW, COL, p, cut_of(p.M, p.N, p.K, z.dtype, true), z.dtype, rest, st));
-  }
-  if (f.dw_in) {
-    ProductArgs p = {};
-    p.a = dgu, p.b = x.p, p.c = f.dw_in, p.lda = 2 * z.Fp, p.ldb = x.ld, p.ldc = z.D;
-    p.M = 2 * z.Fp, p.N = z.D, p.K = z.T, p.gap_at = z.F, p.gap = z.Fp - z.F;
-    // the columns from Fp + F on are the second gap: the last rows
-    p.M -= p.gap;
-    PNFX_TRY(product(COL, COL, p, cut_of(2 * z.Fp, p.N, p.K, z.dtype, true), z.dtype, rest, st));
-  }
-  if (f.dw_down) {
-    ProductArgs p = {};
-    p.a = dy.p, p.b = h, p.c = f.dw_down, p.lda = dy.ld, p.ldb = z.Fp, p.ldc = z.F;
-    p.M = z.Do, p.N = z.F, p.K = z.T;
-    PNFX_TRY(product(COL, COL, p, cut_of(p.M, p.N, p.K, z.dtype, true), z.dtype, rest, st));
-  }
-  return PNFX_OK;
+    p.a = pa, p.b = pb, p.c = c, p.lda = lda, p.ldb = ldb, p.ldc = ldc;
+    p.M = s[i].M, p.N = s[i].N, p.K = s[i].K;
+    // dw_in: the columns of dg behind F are no rows of it (those of du behind F are left out as the last ones)
+    if (i == 1) p.gap_at = z.F, p.gap = z.Fp - z.F;
+    jobs[n++] = Job{ka, COL, p, cuts[i], sums};
+  };
+  job(0, ROW, dgu, 2 * z.Fp, win.p, win.ld, f.dx, z.D);
+  job(1, COL, dgu, 2 * z.Fp, x.p, x.ld, f.dw_in, z.D);
+  job(2, COL, dy.p, dy.ld, h, z.Fp, f.dw_down, z.F);
+  return n ? products(jobs, n, z.dtype, st) : PNFX_OK;
 }
 
 }  // namespace

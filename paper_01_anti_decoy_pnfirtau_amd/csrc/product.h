@@ -35,9 +35,25 @@ struct Cut {
 // can_split: whether k may be divided, over workgroups or a workgroup's waves; sums: fp32 sums are wanted anyway.
 Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool can_split, bool sums = false);
 
-// Workspace of product() for C (not sums) at this cut, in bytes.
+// The cuts of products that run in one launch.
+struct Shape {
+  int64_t M, N, K;
+  bool sums;
+};
+void cut_group(const Shape* shapes, int n, int dtype, Cut* cuts);
+
+// Workspace of a product with a C (not sums) at this cut, in bytes.
 int64_t product_workspace(const Cut& cut, int64_t M, int64_t N);
-int product(int ka, int kb, const ProductArgs& p, const Cut& cut, int dtype, void* workspace, hipStream_t stream);
+
+// Up to three products that do not depend on each other: in one launch if the first is ROW COL, the others COL COL
+// and their tiles of one kind.
+struct Job {
+  int ka, kb;  // operand kinds
+  ProductArgs p;
+  Cut cut;
+  void* ws;
+};
+int products(const Job* jobs, int n, int dtype, hipStream_t stream);
 
 // Copies of matrices with their columns zero-padded to whole 16-byte chunks, in one launch.
 struct PadItem {

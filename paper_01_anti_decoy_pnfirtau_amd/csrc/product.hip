@@ -45,18 +45,18 @@ __device__ __forceinline__ void load8(const float* p, int n, float* v) {
   for (int r = 0; r < 8; ++r) v[r] = r < n ? p[r] : 0.f;
 }
 
+// Workgroup `block` of a product.
 template <typename T, Kind KA, Kind KB, class C>
-__global__ __launch_bounds__(threads_of<C>, 2) void mm_kernel(MmArgs g) {
+__device__ __forceinline__ void mm_tile(const MmArgs& g, int block, char* sm) {
   typedef Product<T, KA, KB, C> P;
-  extern __shared__ __align__(16) char sm[];
   const int M = g.m_count ? min(g.M, *g.m_count) : g.M;
   const int tms = (M + C::TM - 1) / C::TM, tiles = tms * g.tn;
-  if ((int)blockIdx.x >= tiles * g.splits) return;
-  int split = blockIdx.x / tiles, id = blockIdx.x % tiles;
+  if (block >= tiles * g.splits) return;
+  int split = block / tiles, id = block % tiles;
   if (g.by_xcd) {
     // the tiles of a split read the same k: all on one XCD (workgroup id % 8), which so reads it once
-    split = (int)blockIdx.x / 8 / tiles * 8 + (int)blockIdx.x % 8;
-    id = (int)blockIdx.x / 8 % tiles;
+    split = block / 8 / tiles * 8 + block % 8;
+    id = block / 8 % tiles;
   }
   int tm, tn;
   if (g.by_xcd) tn = id % g.tn, tm = id / g.tn;
@@ -135,6 +135,25 @@ __global__ __launch_bounds__(threads_of<C>, 2) void mm_kernel(MmArgs g) {
   }
 }
 
+template <typename T, Kind KA, Kind KB, class C>
+__global__ __launch_bounds__(threads_of<C>, 2) void mm_kernel(MmArgs g) {
+  extern __shared__ __align__(16) char sm[];
+  mm_tile<T, KA, KB, C>(g, blockIdx.x, sm);
+}
+// The products of a backward pass in one launch, none of which fills the chip by itself: first workgroups of each.
+struct GroupArgs {
+  MmArgs rc, cc[2];  // ROW COL, then COL COL
+  int first[2];      // workgroups, a multiple of eight each
+};
+template <typename T, class C>
+__global__ __launch_bounds__(threads_of<C>, 2) void mm_group_kernel(GroupArgs g) {
+  extern __shared__ __align__(16) char sm[];
+  const int block = blockIdx.x;
+  if (block < g.first[0]) return mm_tile<T, ROW, COL, C>(g.rc, block, sm);
+  const bool last = block >= g.first[1];
+  mm_tile<T, COL, COL, C>(g.cc[last], block - g.first[last], sm);
+}
+
 struct SumArgs {
   const float* sums;
   void* c;
@@ -142,10 +161,19 @@ struct SumArgs {
   int64_t MN, ldc;
   int M, N, groups, splits, gap_at, gap;  // groups: of eight columns, in a row
 };
+constexpr int kMaxGroup = 3;
+struct SumsArgs {
+  SumArgs item[kMaxGroup];
+  int64_t first[kMaxGroup + 1];  // workgroups
+  int n;
+};
 // C from the splits' sums, added in split order: eight columns per thread.
 template <typename T>
-__global__ __launch_bounds__(256) void mm_sum_kernel(SumArgs g) {
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(256) void mm_sum_kernel(SumsArgs all) {
+  int i = 0;
+  while (i + 1 < all.n && (int64_t)blockIdx.x >= all.first[i + 1]) ++i;
+  const SumArgs& g = all.item[i];
+  const int64_t id = (blockIdx.x - all.first[i]) * 256 + threadIdx.x;
   const int m = (int)(id / g.groups), n = (int)(id % g.groups) * 8;
   if (m >= g.M) return;
   const int row = out_row(m, g.gap_at, g.gap);
@@ -209,7 +237,7 @@ int mm_kinds(int ka, int kb, const MmArgs& g, hipStream_t st) {
 // The cut that is expected to be done first.  A tile's step takes, with one of its kind on every CU, the time of
 // its products at the rate that gemm.h's figures give, or half a microsecond if the step's loads are not hidden by
 // another workgroup's products; a split adds its fp32 sums' way to memory and back.
-Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool can_split, bool sums) {
+static Cut cut_kind(int64_t M, int64_t N, int64_t K, int dtype, bool can_split, bool sums, int only, double* cost) {
   const int es = dtype == PNFX_F32 ? 4 : 2;
   const int64_t steps = ceil_div(K, 128 / es);
   Cut best{Cut::MID, 1, steps};
@@ -217,6 +245,7 @@ Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool can_split, bool sums
   for (int kind = 0; kind < 3; ++kind) {
     if (kind == Cut::BIG && dtype == PNFX_F32) continue;
     if (kind == Cut::DUO && !can_split) continue;
+    if (only >= 0 && kind != only) continue;
     const int64_t T = kind == Cut::BIG ? 256 : 128, tiles = ceil_div(M, T) * ceil_div(N, T);
     const double rate = dtype == PNFX_F32 ? 120e6 : kind == Cut::BIG ? 1300e6 : 1050e6;  // operations per us, 256 CUs
     const double step_us = 2.0 * T * T * (128 / es) / (rate / 256);  // of one tile that has the CU to itself
@@ -241,27 +270,47 @@ Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool can_split, bool sums
       }
     }
   }
+  if (cost) *cost = best_us;
   return best;
+}
+Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool can_split, bool sums) {
+  return cut_kind(M, N, K, dtype, can_split, sums, -1, nullptr);
+}
+// One kind of tile for all of a group: that with the least sum of times.
+void cut_group(const Shape* shapes, int n, int dtype, Cut* cuts) {
+  double best = 1e30;
+  for (int kind = 0; kind < 3; ++kind) {
+    if (kind == Cut::BIG && dtype == PNFX_F32) continue;
+    Cut got[kMaxGroup];
+    double total = 0;
+    for (int i = 0; i < n; ++i) {
+      double us;
+      got[i] = cut_kind(shapes[i].M, shapes[i].N, shapes[i].K, dtype, true, shapes[i].sums, kind, &us);
+      total += us;
+    }
+    if (total < best) {
+      best = total;
+      for (int i = 0; i < n; ++i) cuts[i] = got[i];
+    }
+  }
 }
 
 int64_t product_workspace(const Cut& cut, int64_t M, int64_t N) {
   return cut.splits > 1 ? cut.splits * M * N * 4 : 0;
 }
 
-int product(int ka, int kb, const ProductArgs& p, const Cut& cut, int dtype, void* workspace, hipStream_t st) {
-  if (p.M < 1 || p.N < 1) return PNFX_OK;
-  const int es = dtype == PNFX_F32 ? 4 : 2;
+// The kernel's arguments of a product; `ws`: where its splits' sums go, if it has any.
+static int mm_args(const ProductArgs& p, const Cut& cut, int es, void* ws, MmArgs& g) {
   PNFX_REQUIRE(operand_ok(p.a, p.lda, es) && operand_ok(p.b, p.ldb, es), "product: operand alignment");
   PNFX_REQUIRE(p.M < (1 << 30) && p.N < (1 << 30) && p.K < (1ll << 31), "product: %lld x %lld over %lld",
                (long long)p.M, (long long)p.N, (long long)p.K);
   const bool summed = !p.sums && cut.splits > 1;
-  PNFX_REQUIRE(!summed || workspace, "product: no workspace");
+  PNFX_REQUIRE(!summed || ws, "product: no workspace");
   const int64_t T = cut.kind == Cut::BIG ? 256 : 128;
-  MmArgs g;
   g.a = p.a;
   g.b = p.b;
   g.c = p.c;
-  g.sums = summed ? static_cast<float*>(workspace) : p.sums;
+  g.sums = summed ? static_cast<float*>(ws) : p.sums;
   g.lda = p.lda;
   g.ldb = p.ldb;
   g.ldc = p.ldc;
@@ -279,18 +328,73 @@ int product(int ka, int kb, const ProductArgs& p, const Cut& cut, int dtype, voi
   g.add = p.add;
   g.alpha = summed ? nullptr : p.alpha;
   g.by_xcd = cut.splits % 8 == 0;
-  if (dtype == PNFX_F32)
-    PNFX_TRY((cut.kind == Cut::DUO ? mm_kinds<float, Duo>(ka, kb, g, st) : mm_kinds<float, Mid>(ka, kb, g, st)));
-  else
-    PNFX_TRY((cut.kind == Cut::BIG   ? mm_kinds<bf16, Big>(ka, kb, g, st)
-              : cut.kind == Cut::DUO ? mm_kinds<bf16, Duo>(ka, kb, g, st)
-                                     : mm_kinds<bf16, Mid>(ka, kb, g, st)));
-  if (!summed) return PNFX_OK;
-  const int64_t groups = ceil_div(p.N, 8);
-  SumArgs s{g.sums, p.c, p.alpha, p.M * p.N, p.ldc, g.M, g.N, (int)groups, cut.splits, g.gap_at, g.gap};
-  const int64_t grid = ceil_div(p.M * groups, 256);
-  return dtype == PNFX_F32 ? launch<mm_sum_kernel<float>>(grid, 256, 0, s, st, "product sums")
-                           : launch<mm_sum_kernel<bf16>>(grid, 256, 0, s, st, "product sums");
+  return PNFX_OK;
+}
+
+static int sum_up(const Job* jobs, const MmArgs* g, int n, int dtype, hipStream_t st) {
+  SumsArgs s;
+  s.n = 0;
+  s.first[0] = 0;
+  for (int i = 0; i < n; ++i) {
+    const ProductArgs& p = jobs[i].p;
+    if (p.M < 1 || p.N < 1 || p.sums || jobs[i].cut.splits == 1) continue;
+    const int64_t groups = ceil_div(p.N, 8);
+    s.item[s.n] = SumArgs{g[i].sums, p.c, p.alpha, p.M * p.N, p.ldc, g[i].M, g[i].N, (int)groups, jobs[i].cut.splits,
+                          g[i].gap_at, g[i].gap};
+    s.first[s.n + 1] = s.first[s.n] + ceil_div(p.M * groups, 256);
+    ++s.n;
+  }
+  if (!s.n) return PNFX_OK;
+  return dtype == PNFX_F32 ? launch<mm_sum_kernel<float>>(s.first[s.n], 256, 0, s, st, "product sums")
+                           : launch<mm_sum_kernel<bf16>>(s.first[s.n], 256, 0, s, st, "product sums");
+}
+
+template <typename T, class C>
+static int group_launch(const GroupArgs& g, int64_t grid, hipStream_t st) {
+  return launch<mm_group_kernel<T, C>>(grid, threads_of<C>, lds_of<C>, g, st, "products");
+}
+
+int products(const Job* jobs, int n, int dtype, hipStream_t st) {
+  const int es = dtype == PNFX_F32 ? 4 : 2;
+  PNFX_REQUIRE(n >= 1 && n <= kMaxGroup, "products: %d", n);
+  MmArgs g[kMaxGroup] = {};
+  bool group = n > 1 && jobs[0].ka == ROW && jobs[0].kb == COL;
+  for (int i = 0; i < n; ++i) {
+    PNFX_TRY(mm_args(jobs[i].p, jobs[i].cut, es, jobs[i].ws, g[i]));
+    group = group && jobs[i].cut.kind == jobs[0].cut.kind && (i == 0 || (jobs[i].ka == COL && jobs[i].kb == COL));
+  }
+  if (group) {
+    GroupArgs a = {};
+    a.rc = g[0];
+    a.cc[0] = g[1];
+    a.cc[1] = g[n - 1];
+    int64_t grid = 0;
+    for (int i = 0; i < n; ++i) {
+      // a multiple of eight: workgroup id % 8 is the XCD for every product (those left over end at once)
+      grid += round_up((int64_t)g[i].tm * g[i].tn * g[i].splits, 8);
+      PNFX_REQUIRE(grid < (1ll << 31), "products: %lld workgroups", (long long)grid);
+      if (i < 2) a.first[i] = (int)grid;
+    }
+    const Cut::Kind kind = jobs[0].cut.kind;
+    if (dtype == PNFX_F32)
+      PNFX_TRY((kind == Cut::DUO ? group_launch<float, Duo>(a, grid, st) : group_launch<float, Mid>(a, grid, st)));
+    else
+      PNFX_TRY((kind == Cut::BIG   ? group_launch<bf16, Big>(a, grid, st)
+                : kind == Cut::DUO ? group_launch<bf16, Duo>(a, grid, st)
+                                   : group_launch<bf16, Mid>(a, grid, st)));
+  } else {
+    for (int i = 0; i < n; ++i) {
+      const Job& j = jobs[i];
+      if (dtype == PNFX_F32)
+        PNFX_TRY((j.cut.kind == Cut::DUO ? mm_kinds<float, Duo>(j.ka, j.kb, g[i], st)
+                                         : mm_kinds<float, Mid>(j.ka, j.kb, g[i], st)));
+      else
+        PNFX_TRY((j.cut.kind == Cut::BIG   ? mm_kinds<bf16, Big>(j.ka, j.kb, g[i], st)
+                  : j.cut.kind == Cut::DUO ? mm_kinds<bf16, Duo>(j.ka, j.kb, g[i], st)
+                                           : mm_kinds<bf16, Mid>(j.ka, j.kb, g[i], st)));
+    }
+  }
+  return sum_up(jobs, g, n, dtype, st);
 }
 
 int pad(const PadItem* items, int n, int dtype, hipStream_t st) {

@@ -538,8 +538,10 @@ struct BwdCut {
 BwdCut bwd_cut(const Sizes& z) {
   BwdCut c;
   c.P = std::min(piece_of(z), round_up(z.V, 8));
-  c.dx = cut_of(z.T, z.D, c.P, z.dtype, true, true);
-  c.dw = cut_of(c.P, z.D, z.T, z.dtype, true);
+  const Shape s[2] = {{z.T, z.D, c.P, true}, {c.P, z.D, z.T, false}};
+  Cut cuts[2];
+  cut_group(s, 2, z.dtype, cuts);
+  c.dx = cuts[0], c.dw = cuts[1];
   return c;
 }
 int64_t bwd_bytes(const Sizes& z, bool copy) {
@@ -632,19 +634,22 @@ int xent_bwd(const float* dloss, const void* x, int64_t x_rs, const void* w, int
       return launch<xent_grad_kernel<T, C, KS>>(tm * g.splits, threads_of<C>, Tiles<T, C, KS, 0>::LDS, g, st,
                                                 "xent_grad");
     })));
+    Job jobs[2];
+    int nj = 0;
     if (dx) {
       ProductArgs p = {};
       p.a = d, p.b = wp, p.lda = c.P, p.ldb = w_rs, p.M = z.T, p.N = z.D, p.K = n;
       p.m_count = k.count, p.sums = sums, p.add = v0 > 0;
-      PNFX_TRY(product(ROW, COL, p, c.dx, z.dtype, nullptr, st));
+      jobs[nj++] = Job{ROW, COL, p, c.dx, nullptr};
     }
     if (dw) {
       ProductArgs p = {};
       p.a = d, p.b = r.xs ? xs : k.xc, p.c = static_cast<T*>(dw) + v0 * z.D, p.lda = c.P, p.ldb = z.Dp, p.ldc = z.D;
       p.M = n, p.N = z.D, p.K = z.T, p.k_count = k.count;
       p.alpha = r.xs ? nullptr : r.alpha;
-      PNFX_TRY(product(COL, COL, p, c.dw, z.dtype, dw_ws, st));
+      jobs[nj++] = Job{COL, COL, p, c.dw, dw_ws};
     }
+    if (nj) PNFX_TRY(products(jobs, nj, z.dtype, st));
   }
   if (!dx) return PNFX_OK;
   const DxArgs x1{sums, r.rowc, k.pos, dx, z.T * z.D, (int)z.D, c.dx.splits};
