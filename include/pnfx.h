@@ -347,7 +347,8 @@ int pnfx_xent_fwd(const void* x, int64_t x_rs, const void* w, int64_t w_rs, cons
                   int64_t ignore_index, float* loss, float* loss_rows, float* lse, int64_t T, int64_t D,
                   int64_t V, int reduction, int dtype, void* workspace, int64_t workspace_bytes,
                   void* stream);
-int64_t pnfx_xent_bwd_workspace_size(int64_t T, int64_t D, int64_t V, int copies, int dtype);
+int64_t pnfx_xent_bwd_workspace_size(int64_t T, int64_t D, int64_t V, int reduction, int copies,
+                                     int dtype);
 int pnfx_xent_bwd(const float* dloss, const void* x, int64_t x_rs, const void* w, int64_t w_rs,
                   const int64_t* target, int64_t ignore_index, const float* loss_rows, const float* lse,
                   void* dx, void* dw, int64_t T, int64_t D, int64_t V, int reduction, int dtype,

@@ -70,8 +70,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     sig["pnfx_flash_bwd_noalloc"] = (bwd[:37] + bwd[39:], i32)
     sig["pnfx_ffn_fwd_workspace_size"] = ([i64] * 4 + [i32] * 3, i64)
     sig["pnfx_ffn_bwd_workspace_size"] = ([i64] * 4 + [i32] * 2, i64)
-    for name in ("pnfx_xent_fwd_workspace_size", "pnfx_xent_bwd_workspace_size"):
-        sig[name] = ([i64] * 3 + [i32, i32], i64)
+    sig["pnfx_xent_fwd_workspace_size"] = ([i64] * 3 + [i32] * 2, i64)
+    sig["pnfx_xent_bwd_workspace_size"] = ([i64] * 3 + [i32] * 3, i64)
     sig["pnfx_ffn_fwd"] = ([vp, i64] * 3 + [vp] * 3 + [i64] * 4 + [i32] * 3 + [vp, i64, vp], i32)
     sig["pnfx_ffn_bwd"] = ([vp, i64] * 4 + [vp] * 5 + [i64] * 4 + [i32] * 3 + [vp, i64, vp], i32)
     sig["pnfx_xent_fwd"] = ([vp, i64] * 2 + [vp, i64, vp, vp, vp] + [i64] * 3 + [i32] * 2

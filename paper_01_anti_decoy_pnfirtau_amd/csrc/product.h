@@ -55,6 +55,10 @@ struct Job {
 };
 int products(const Job* jobs, int n, int dtype, hipStream_t stream);
 
+// C [M][N] = alpha times the sum of `splits` fp32 matrices [M][N] in `sums`, in their order (alpha null: 1).
+int sum_splits(const float* sums, int splits, int64_t M, int64_t N, void* c, const float* alpha, int dtype,
+               hipStream_t stream);
+
 // Copies of matrices with their columns zero-padded to whole 16-byte chunks, in one launch.
 struct PadItem {
   const void* src;

@@ -349,6 +349,18 @@ static int sum_up(const Job* jobs, const MmArgs* g, int n, int dtype, hipStream_
                            : launch<mm_sum_kernel<bf16>>(s.first[s.n], 256, 0, s, st, "product sums");
 }
 
+int sum_splits(const float* sums, int splits, int64_t M, int64_t N, void* c, const float* alpha, int dtype,
+               hipStream_t st) {
+  const int64_t groups = ceil_div(N, 8);
+  SumsArgs s;
+  s.n = 1;
+  s.item[0] = SumArgs{sums, c, alpha, M * N, N, (int)M, (int)N, (int)groups, splits, (int)M, 0};
+  s.first[0] = 0;
+  s.first[1] = ceil_div(M * groups, 256);
+  return dtype == PNFX_F32 ? launch<mm_sum_kernel<float>>(s.first[1], 256, 0, s, st, "sum of splits")
+                           : launch<mm_sum_kernel<bf16>>(s.first[1], 256, 0, s, st, "sum of splits");
+}
+
 template <typename T, class C>
 static int group_launch(const GroupArgs& g, int64_t grid, hipStream_t st) {
   return launch<mm_group_kernel<T, C>>(grid, threads_of<C>, lds_of<C>, g, st, "products");

@@ -410,7 +410,8 @@ std::tuple<Tensor, Tensor> linear_xent_bwd_cuda(const Tensor& dloss_in, const Te
   const Tensor dloss = dloss_in.to(at::kFloat).contiguous();
   const Rows x = rows_of(x_in), w = rows_of(w_in);
   const Tensor t = target.contiguous();
-  const int64_t wsb = pnfx_xent_bwd_workspace_size(z.T, z.D, z.V, !w.aligned(), z.code);
+  const int64_t wsb = pnfx_xent_bwd_workspace_size(z.T, z.D, z.V, (int)reduction, !w.aligned(),
+                                                   z.code);
   Tensor ws = workspace(wsb, x_in);
   check_rc(pnfx_xent_bwd(dloss.data_ptr<float>(), x.ptr(), x.rs, w.ptr(), w.rs,
                          t.data_ptr<int64_t>(), ignore_index, rows.data_ptr<float>(),

@@ -55,7 +55,7 @@ struct RowsArgs {
   int* count;
   int64_t x_rs, ignore;
   int T, D, Dp, V, per;  // per: rows of a workgroup
-  // backward only: row constants {lse, s_t, expm1(-loss_t), -}; s_t where it is one value; s_t x_t where not
+  // backward only: row constants {lse, s_t, expm1(-loss_t), target or -1}; s_t where it is one value; s_t x_t where not
   const float* lse;
   const float* loss;
   const float* dloss;
@@ -117,7 +117,8 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs a) {
       if (a.rowc) {
         const float s = a.reduction == PNFX_REDUCE_NONE ? a.dloss[r] : row_scale;
         // a target that is no token: its loss is NaN, and so are its gradients
-        a.rowc[i] = float4{valid ? a.lse[r] : __builtin_nanf(""), s, expm1f(-a.loss[r]), 0.f};
+        a.rowc[i] = float4{valid ? a.lse[r] : __builtin_nanf(""), s, expm1f(-a.loss[r]),
+                           __int_as_float(valid ? (int)t : -1)};
         scale[at] = s;
       }
     }
@@ -409,6 +410,204 @@ __global__ __launch_bounds__(threads_of<C>, 2) void xent_grad_kernel(GradArgs a)
   });
 }
 
+// Rows of at most 64 columns: the gradients without d in memory.  There the products are so short that writing d and
+// reading it twice would be most of the time (xent_narrow, per 7936 tokens: 61 us for d, 105 for the two products).
+// A workgroup keeps 128 rows of one operand, as fragments in registers, and goes through tiles of 128 rows
+// of the other: the tile's logits, their exponentials, rounded to bf16 in the registers that are the next product's
+// operand, and the product with the same tile, read transposed from where it lies in LDS.  For dx the rows kept are
+// x's and the tiles W's; for dW the other way round, with the rows' log-sum-exps along the tile.
+struct NarrowArgs {
+  const void* a;    // rows kept, of lda
+  const void* b;    // tiles, of ldb
+  float* sums;      // [splits][M][N]: of a's rows
+  const float4* rowc;
+  const int *tgt, *count;
+  int64_t lda, ldb, K;
+  int M, N, nb;     // rows of a and columns of the result (all of the array's); rows of b
+  int V, splits, per;
+};
+template <bool DW>
+__global__ __launch_bounds__(256, 2) void xent_narrow_kernel(NarrowArgs a) {
+  typedef Stage<bf16, ROW, 128, 256> St;
+  constexpr int SB = 128 * 64, RING = 4;
+  extern __shared__ __align__(16) char smem[];
+  bf16* const sm = reinterpret_cast<bf16*>(smem);
+  float4* const cols = reinterpret_cast<float4*>(smem + RING * SB * 2);  // DW: [RING][wave][64] of the tile's rows
+  float2* const rowl = reinterpret_cast<float2*>(smem + RING * SB * 2);  // dx: [128] of the rows kept
+  const int count = *a.count;
+  const int rows = DW ? a.M : count, nb = DW ? count : a.nb;
+  const int tms = (rows + 127) / 128;
+  if ((int)blockIdx.x >= tms * a.splits) return;
+  int tm, split;
+  tile_of(blockIdx.x, tms, a.splits, tm, split);
+  const int m0 = tm * 128, t0 = split * a.per, tiles = max(0, min((nb + 127) / 128 - t0, a.per));
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wm = wave >> 1, wn = wave & 1, r16 = lane & 15, g = lane >> 4;
+  f32x4 out[4][4] = {};  // [row block][block of 16 columns of the result]
+  const unsigned la = __builtin_amdgcn_readfirstlane(lds_addr(sm));
+  if (tiles) {
+    St sa, sb;
+    sa.init(static_cast<const bf16*>(a.a) + m0 * a.lda, a.lda, rows - m0, a.K, threadIdx.x);
+    sb.init(static_cast<const bf16*>(a.b) + (int64_t)t0 * 128 * a.ldb, a.ldb, nb - t0 * 128, a.K, threadIdx.x);
+    const u32x4 dc = buffer_of(a.rowc, (unsigned)nb * 16u);
+    const auto load = [&](int s) {
+      sb.load(la + 2 * (s % RING) * SB, wave);
+      sb.move(128, 1);
+      if constexpr (DW)
+        lds_dma16(dc, ((t0 + s) * 128 + 64 * wn + lane) * 16u, la + 2 * RING * SB + ((s % RING) * 4 + wave) * 1024);
+    };
+    constexpr int NI = St::NI + (DW ? 1 : 0);
+    sa.load(la, wave);
+    wait_vm_lgkm<0>();
+    __builtin_amdgcn_s_barrier();
+    bf16x8 fa[2][4];
+    {
+      const Frags<bf16, ROW> f(sm + wm * 64 * 64, lane);
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fa[hf][i] = f.get(i, hf, 0);
+    }
+    wait_vm_lgkm<0>();
+    __builtin_amdgcn_s_barrier();
+    // dx: each row's log-sum-exp and target, as a column of the first tile; published by the loop's first barrier
+    if constexpr (!DW) {
+      if (threadIdx.x < 128) {
+        const int m = min(m0 + (int)threadIdx.x, rows - 1);
+        rowl[threadIdx.x] = float2{a.rowc[m].x, __int_as_float(a.tgt[m] - t0 * 128)};
+      }
+      wait_vm_lgkm<0>();
+    }
+    const Frags<bf16, ROW> fb(sm + wn * 64 * 64, lane);
+    const Frags<bf16, COL> ft(sm + wn * 64 * 64, lane);
+    load(0);
+    if (tiles > 1) load(1);
+    if (tiles > 2) load(2);
+    for (int t = 0; t < tiles; ++t) {
+      const int buf = t % RING;
+      if (t + 2 < tiles) wait_vm_lgkm<2 * NI>();
+      else wait_vm_lgkm<0>();
+      __builtin_amdgcn_s_barrier();
+      if (t + 3 < tiles) load(t + 3);
+      __builtin_amdgcn_sched_barrier(0);
+      f32x4 z[4][4];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        bf16x8 b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] = fb.get(j, hf, buf * SB);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) z[i][j] = mma(b[j], fa[hf][i], hf ? z[i][j] : f32x4{});
+      }
+      const auto col = [](int j) { return stage_row<ROW>(j, 0); };  // block j's first column of the lane's
+      const float4* const c = cols + (buf * 4 + wave) * 64;
+      bool hit;
+      if constexpr (DW) {
+        // (the log-sum-exps of the lane's 16 columns)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float l = c[8 * g + col(j) + r].x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z[i][j][r] = exp2_fast((z[i][j][r] - l) * kLog2e);
+          }
+        hit = (unsigned)(__float_as_int(c[lane].w) - m0 - 64 * wm) < 64u;
+      } else {
+        hit = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 c = rowl[stage_row<ROW>(4 * wm + i, r16)];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) z[i][j][r] = exp2_fast((z[i][j][r] - c.x) * kLog2e);
+          hit = hit || (unsigned)(__float_as_int(c.y) - 128 * t - 64 * wn - 8 * g) < 40u;
+        }
+      }
+      if (__any(hit)) {  // seldom: a target's own element
+        if constexpr (DW) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float4 e = c[8 * g + col(j) + r];
+              const int own = __float_as_int(e.w) - m0 - 64 * wm;
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (own == stage_row<ROW>(i, r16)) z[i][j][r] = e.z;
+            }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float own = a.rowc[min(m0 + stage_row<ROW>(4 * wm + i, r16), rows - 1)].z;
+            const int at = __float_as_int(rowl[stage_row<ROW>(4 * wm + i, r16)].y) - 128 * t - 64 * wn - 8 * g;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (at == col(j) + r) z[i][j][r] = own;
+          }
+        }
+      }
+      if (!DW && (t0 + t + 1) * 128 > a.V) {  // tokens past the vocabulary: of zero weights, but not finite perhaps
+        const int n0 = (t0 + t) * 128 + 64 * wn + 8 * g;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (n0 + col(j) + r >= a.V) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) z[i][j][r] = 0.f;
+            }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      // two blocks: the lane's eight consecutive columns, a fragment of the next product
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        bf16x8 b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] = ft.get(j, h, buf * SB);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 u = z[i][2 * h], v = z[i][2 * h + 1];
+          const bf16x8 p = pack8(u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) out[i][j] = mma(b[j], p, out[i][j]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    wait_vm_lgkm<0>();
+  }
+  // the two waves of a row share its columns of the tiles: their sums are added, half of them by each
+  __syncthreads();
+  f32x4* const other = reinterpret_cast<f32x4*>(smem) + wave * 512 + lane;
+  const f32x4* const mine = reinterpret_cast<f32x4*>(smem) + (wave ^ 1) * 512 + lane;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) other[(4 * i + j) * 64] = wn ? out[i][j] : out[2 + i][j];
+  __syncthreads();
+  float* const sums = a.sums + (int64_t)split * a.M * a.N;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int m = m0 + stage_row<ROW>(4 * wm + 2 * wn + i, r16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x4 v = (wn ? out[2 + i][j] : out[i][j]) + mine[(4 * i + j) * 64];
+      const int n = 16 * j + 4 * g;
+      if (m >= rows) continue;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (n + r < a.N) sums[(int64_t)m * a.N + n + r] = v[r];
+    }
+  }
+}
+constexpr int kNarrowLds[2] = {4 * 128 * 128 + 1024, 4 * 128 * 128 + 4 * 4 * 1024};  // dx, dW
+
 struct DxArgs {
   const float* sums;  // [splits][T][D]
   const float4* rowc;
@@ -544,9 +743,35 @@ BwdCut bwd_cut(const Sizes& z) {
   c.dx = cuts[0], c.dw = cuts[1];
   return c;
 }
-int64_t bwd_bytes(const Sizes& z, bool copy) {
+// The narrow kernels' cut: parts of the tiles for each 128 rows kept, so that the last round of workgroups, two on a
+// CU, is nearly full, against the fp32 sums that each part writes and another kernel reads.
+struct NarrowCut {
+  int64_t splits, per;
+};
+NarrowCut narrow_cut(int64_t rows, int64_t tiles, int64_t D) {
+  const int64_t tm = ceil_div(rows, 128);
+  NarrowCut best{1, tiles};
+  double best_us = 1e30;
+  for (int64_t s = 1; s <= std::min<int64_t>(32, tiles); ++s) {
+    const int64_t per = ceil_div(tiles, s);
+    const double us = ceil_div(tm * ceil_div(tiles, per), 512) * (per * 2.5 + 6.0) + ceil_div(tiles, per) * rows * D * 8 / 4e6;
+    if (us < best_us) best_us = us, best = NarrowCut{ceil_div(tiles, per), per};
+  }
+  return best;
+}
+bool narrow(const Sizes& z, int reduction) {
+  return z.dtype == PNFX_BF16 && z.Dp <= 64 && reduction != PNFX_REDUCE_NONE;
+}
+int64_t bwd_bytes(const Sizes& z, int reduction, bool copy) {
   Arena ar{nullptr, 0};
   take_kept(ar, z, copy);
+  if (narrow(z, reduction)) {
+    ar.take<float>(1);
+    ar.take<float4>(z.T);
+    ar.take<float>(narrow_cut(z.T, ceil_div(z.V, 128), z.D).splits * z.T * z.D);
+    ar.take<float>(narrow_cut(z.V, ceil_div(z.T, 128), z.D).splits * z.V * z.D);
+    return ar.used;
+  }
   ar.take<float>(1);
   ar.take<char>(z.T * z.Dp * z.es);  // s x, of a loss per row
   const BwdCut c = bwd_cut(z);
@@ -607,10 +832,34 @@ int xent_bwd(const float* dloss, const void* x, int64_t x_rs, const void* w, int
              bool copy, void* ws, hipStream_t st) {
   Arena ar{static_cast<char*>(ws), 0};
   const Kept k = take_kept(ar, z, copy);
-  const BwdCut c = bwd_cut(z);
   RowsArgs r = {};
   r.lse = lse, r.loss = rows, r.dloss = dloss, r.reduction = reduction;
   r.alpha = ar.take<float>(1);
+  if constexpr (sizeof(T) == 2) {
+    if (narrow(z, reduction)) {
+      r.rowc = ar.take<float4>(z.T);
+      const NarrowCut cx = narrow_cut(z.T, ceil_div(z.V, 128), z.D), cw = narrow_cut(z.V, ceil_div(z.T, 128), z.D);
+      float* sx = ar.take<float>(cx.splits * z.T * z.D);
+      float* sw = ar.take<float>(cw.splits * z.V * z.D);
+      PNFX_TRY(take_w(k, w, w_rs, z, st));
+      PNFX_TRY(keep_rows<T>(k, x, x_rs, target, ignore, z, r, st));
+      if (dx) {
+        const NarrowArgs n{k.xc, w, sx, r.rowc, k.tgt, k.count, z.Dp, w_rs, z.Dp, (int)z.T, (int)z.D, (int)z.V, (int)z.V,
+                           (int)cx.splits, (int)cx.per};
+        PNFX_TRY((launch<xent_narrow_kernel<false>>(ceil_div(z.T, 128) * cx.splits, 256, kNarrowLds[0], n, st, "xent_dx")));
+        const DxArgs x1{sx, r.rowc, k.pos, dx, z.T * z.D, (int)z.D, (int)cx.splits};
+        PNFX_TRY((launch<xent_dx_kernel<T>>(ceil_div(x1.TD, z.D % 4 == 0 ? 1024 : 256), 256, 0, x1, st, "xent_dx")));
+      }
+      if (dw) {
+        const NarrowArgs n{w, k.xc, sw, r.rowc, k.tgt, k.count, w_rs, z.Dp, z.Dp, (int)z.V, (int)z.D, (int)z.T, (int)z.V,
+                           (int)cw.splits, (int)cw.per};
+        PNFX_TRY((launch<xent_narrow_kernel<true>>(ceil_div(z.V, 128) * cw.splits, 256, kNarrowLds[1], n, st, "xent_dw")));
+        PNFX_TRY(sum_splits(sw, (int)cw.splits, z.V, z.D, dw, r.alpha, z.dtype, st));
+      }
+      return PNFX_OK;
+    }
+  }
+  const BwdCut c = bwd_cut(z);
   void* xs = ar.take<char>(z.T * z.Dp * z.es);
   if (reduction == PNFX_REDUCE_NONE) r.xs = xs;
   r.rowc = ar.take<float4>(z.T);
@@ -674,10 +923,10 @@ extern "C" int64_t pnfx_xent_fwd_workspace_size(int64_t T, int64_t D, int64_t V,
   if (check_sizes("xent", T, D, V, PNFX_REDUCE_NONE, dtype) != PNFX_OK) return 0;
   return fwd_bytes(sizes_of(T, D, V, dtype), copies);
 }
-extern "C" int64_t pnfx_xent_bwd_workspace_size(int64_t T, int64_t D, int64_t V, int copies, int dtype) {
+extern "C" int64_t pnfx_xent_bwd_workspace_size(int64_t T, int64_t D, int64_t V, int reduction, int copies, int dtype) {
   using namespace pnfx;
-  if (check_sizes("xent", T, D, V, PNFX_REDUCE_NONE, dtype) != PNFX_OK) return 0;
-  return bwd_bytes(sizes_of(T, D, V, dtype), copies);
+  if (check_sizes("xent", T, D, V, reduction, dtype) != PNFX_OK) return 0;
+  return bwd_bytes(sizes_of(T, D, V, dtype), reduction, copies);
 }
 
 extern "C" int pnfx_xent_fwd(const void* x, int64_t x_rs, const void* w, int64_t w_rs, const int64_t* target,
@@ -712,7 +961,7 @@ extern "C" int pnfx_xent_bwd(const float* dloss, const void* x, int64_t x_rs, co
                "xent_bwd: gradients must be 16-byte aligned");
   const Sizes z = sizes_of(T, D, V, dtype);
   const bool copy = copies_w(w, w_rs, z);
-  const int64_t need = bwd_bytes(z, copy);
+  const int64_t need = bwd_bytes(z, reduction, copy);
   PNFX_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= need,
                "xent_bwd: workspace needs %lld bytes", (long long)need);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);

@@ -119,7 +119,7 @@ def test_c_abi_refuses_bad_arguments_on_the_host():
     for kw in (dict(dloss=None), dict(dx=odd), dict(rs=8), dict(reduction=-1), dict(wsb=64), dict(D=0)):
         assert xent_b(**kw) == -1, kw
     assert lib.pnfx_ffn_fwd_workspace_size(0, 8, 8, 8, 0, 0, 1) == 0
-    assert lib.pnfx_xent_bwd_workspace_size(4, 8, 0, 0, 1) == 0
+    assert lib.pnfx_xent_bwd_workspace_size(4, 8, 0, 2, 0, 1) == 0
 
 
 @pytest.mark.parametrize("T,D,V,dtype", [(16384, 256, 33278, 1), (1, 8, 2, 1), (200000, 64, 32000, 1), (2048, 256, 8191, 0)])
@@ -127,7 +127,7 @@ def test_cross_entropy_workspace_is_bounded_by_a_piece(T, D, V, dtype):
     """The backward's workspace holds 256 MB of logits' gradients at most (or 2048 tokens' worth), never all of them,
     beside x-sized buffers and the fp32 sums of the two gradients."""
     es = 2 if dtype else 4
-    got = _lib.lib().pnfx_xent_bwd_workspace_size(T, D, V, 0, dtype)
+    got = _lib.lib().pnfx_xent_bwd_workspace_size(T, D, V, 2, 0, dtype)
     piece = min(max(256 << 20, 2048 * T * es), T * (V + 7) * es) + 256 * T * es
     assert got <= piece + 2 * T * (D + 8) * es + 40 * T + 80 * T * D * 4 + 80 * (V + 256) * D * 4 + 65536
 
