@@ -561,7 +561,7 @@ void bwd_cuts(const Sizes& z, Shape* s, Cut* cuts) {
   s[0] = Shape{z.T, z.D, 2 * z.Fp, false};
   s[1] = Shape{z.Fp + z.F, z.D, z.T, false};
   s[2] = Shape{z.Do, z.F, z.T, false};
-  cut_group(s, 3, z.dtype, cuts);
+  cut_group(s, 3, z.dtype, true, cuts);
 }
 int64_t bwd_bytes(const Sizes& z, bool copies) {
   Arena ar{nullptr, 0};

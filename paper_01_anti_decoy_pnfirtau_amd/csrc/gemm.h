@@ -486,15 +486,21 @@ struct Thin {
   }
 };
 
-// Workgroup `id` of tm x tn tiles.  Consecutive ids go to the eight XCDs in turn: each XCD takes a range of
-// tiles of its own, column by column over bands of four tile rows, so that its L2 holds what they share.
-// (Where the number of rows is on the device, tm is of those, so that no XCD is left with tiles of none.)
-__device__ __forceinline__ void tile_of(int id, int tm, int tn, int& m, int& n) {
-  const int total = tm * tn, q = total / 8, r = total % 8, x = id % 8, y = id / 8;
-  id = x < r ? x * (q + 1) + y : r * (q + 1) + (x - r) * q + y;
+// Consecutive workgroups go to the eight XCDs in turn: the place of workgroup `id` of `total` in an order of which
+// each XCD has a range of its own, so that its L2 holds what neighbours share.  (Where a number of rows is on the
+// device, the total is of those, so that no XCD is left with workgroups that have nothing to do.)
+__device__ __forceinline__ int xcd_id(int id, int total) {
+  const int q = total / 8, r = total % 8, x = id % 8, y = id / 8;
+  return x < r ? x * (q + 1) + y : r * (q + 1) + (x - r) * q + y;
+}
+// Tile `id` of tm x tn: column by column over bands of four tile rows.
+__device__ __forceinline__ void band_tile(int id, int tm, int tn, int& m, int& n) {
   const int band = id / (4 * tn), first = 4 * band, high = min(tm - first, 4), in = id - band * 4 * tn;
   m = first + in % high;
   n = in / high;
+}
+__device__ __forceinline__ void tile_of(int id, int tm, int tn, int& m, int& n) {
+  band_tile(xcd_id(id, tm * tn), tm, tn, m, n);
 }
 
 // Sizes that the staging's 32-bit byte offsets cover.

@@ -32,15 +32,15 @@ struct Cut {
   int64_t steps;  // steps of a split
   bool big() const { return kind == BIG; }
 };
-// can_split: whether k may be divided, over workgroups or a workgroup's waves; sums: fp32 sums are wanted anyway.
-Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool can_split, bool sums = false);
+// can_split: whether k may be divided, over workgroups or a workgroup's waves.
+Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool can_split);
 
-// The cuts of products that run in one launch.
+// The cuts, of one kind, of up to three products that run in one launch.  sums: fp32 sums are wanted anyway.
 struct Shape {
   int64_t M, N, K;
   bool sums;
 };
-void cut_group(const Shape* shapes, int n, int dtype, Cut* cuts);
+void cut_group(const Shape* shapes, int n, int dtype, bool can_split, Cut* cuts);
 
 // Workspace of a product with a C (not sums) at this cut, in bytes.
 int64_t product_workspace(const Cut& cut, int64_t M, int64_t N);

@@ -1,6 +1,7 @@
 // Plain matrix products, the sum of their splits, and zero-padded copies.  What bounds the products and how they
 // are staged: gemm.h.
 #include <algorithm>
+#include <cmath>
 
 #include "product.h"
 
@@ -16,7 +17,7 @@ struct MmArgs {
   int gap_at, gap;
   const int *m_count, *k_count;
   const float* alpha;
-  bool add, by_xcd;
+  bool add;
 };
 
 // Row of C of product row m, or -1.
@@ -52,15 +53,10 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g, int block, char* sm) {
   const int M = g.m_count ? min(g.M, *g.m_count) : g.M;
   const int tms = (M + C::TM - 1) / C::TM, tiles = tms * g.tn;
   if (block >= tiles * g.splits) return;
-  int split = block / tiles, id = block % tiles;
-  if (g.by_xcd) {
-    // the tiles of a split read the same k: all on one XCD (workgroup id % 8), which so reads it once
-    split = block / 8 / tiles * 8 + block % 8;
-    id = block / 8 % tiles;
-  }
+  // split by split: the tiles of one read the same k, and an XCD's workgroups are of few splits
+  const int place = xcd_id(block, tiles * g.splits), split = place / tiles;
   int tm, tn;
-  if (g.by_xcd) tn = id % g.tn, tm = id / g.tn;
-  else tile_of(id, tms, g.tn, tm, tn);
+  band_tile(place % tiles, tms, g.tn, tm, tn);
   const int m0 = tm * C::TM, n0 = tn * C::TN;
   const int64_t K = g.k_count ? min<int64_t>(g.K, *g.k_count) : g.K;
   const int all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -234,65 +230,67 @@ int mm_kinds(int ka, int kb, const MmArgs& g, hipStream_t st) {
 
 }  // namespace
 
-// The cut that is expected to be done first.  A tile's step takes, with one of its kind on every CU, the time of
-// its products at the rate that gemm.h's figures give, or half a microsecond if the step's loads are not hidden by
-// another workgroup's products; a split adds its fp32 sums' way to memory and back.
-static Cut cut_kind(int64_t M, int64_t N, int64_t K, int dtype, bool can_split, bool sums, int only, double* cost) {
-  const int es = dtype == PNFX_F32 ? 4 : 2;
-  const int64_t steps = ceil_div(K, 128 / es);
-  Cut best{Cut::MID, 1, steps};
-  double best_us = 1e30;
-  for (int kind = 0; kind < 3; ++kind) {
-    if (kind == Cut::BIG && dtype == PNFX_F32) continue;
-    if (kind == Cut::DUO && !can_split) continue;
-    if (only >= 0 && kind != only) continue;
-    const int64_t T = kind == Cut::BIG ? 256 : 128, tiles = ceil_div(M, T) * ceil_div(N, T);
+// What a cut is expected to take.  A tile's step takes, with one of its kind on every CU, the time of its products at
+// the rate that gemm.h's figures give, or half a microsecond if the step's loads are not hidden by another
+// workgroup's products; a split's fp32 sums are written, and read by another kernel.
+struct Cost {
+  double work = 0, longest = 0, last = 0, after = 0;  // us of all workgroups, of one, and behind them
+  bool summed = false;
+  void add(int kind, const Shape& s, int dtype, int64_t splits, int64_t per) {
+    const int es = dtype == PNFX_F32 ? 4 : 2;
+    const int64_t T = kind == Cut::BIG ? 256 : 128, n = ceil_div(s.M, T) * ceil_div(s.N, T) * splits;
     const double rate = dtype == PNFX_F32 ? 120e6 : kind == Cut::BIG ? 1300e6 : 1050e6;  // operations per us, 256 CUs
-    const double step_us = 2.0 * T * T * (128 / es) / (rate / 256);  // of one tile that has the CU to itself
-    for (int64_t s = 1; s <= 64; s *= 2) {
-      if (s > 1 && (!can_split || steps / s < 4 || tiles * s > 2048)) break;
-      const int64_t per = ceil_div(steps, s), work = tiles * s;
-      double us = 3.0;
-      if (kind == Cut::MID) {
-        // pairs on a CU; the last round may have CUs with one, whose step is not hidden
-        const int64_t full = work / 512, rest = work % 512;
-        us += full * (per * 2 * step_us + 1.5);
-        if (rest) us += per * (rest > 256 ? 2 * step_us : std::max(1.75 * step_us, 0.45)) + 1.5;
-      } else if (kind == Cut::DUO) {
-        us += ceil_div(work, 256) * (ceil_div(per, 2) * std::max(2 * step_us, 0.45) + 2.0);
-      } else {
-        us += ceil_div(work, 256) * (per * step_us + 3.0);
-      }
-      us += (s > 1 || sums ? s * M * N * 4 / 4e6 : 0) + (s > 1 && !sums ? 4.0 + s * M * N * 4 / 4e6 : 0);
-      if (us < best_us) {
-        best_us = us;
-        best = Cut{(Cut::Kind)kind, (int)ceil_div(steps, per), per};
-      }
-    }
+    const double step = 2.0 * T * T * (128 / es) / (rate / 256);  // of one tile that has the CU to itself
+    const double one = kind == Cut::MID   ? per * std::max(2 * step, 0.45) + 1.5
+                       : kind == Cut::DUO ? ceil_div(per, 2) * std::max(2 * step, 0.45) + 2.0
+                                          : per * step + 3.0;
+    work += n * one;
+    last = one;
+    longest = std::max(longest, one);
+    const double sums_us = (double)splits * s.M * s.N * 4 / 4e6;
+    if (splits > 1 || s.sums) after += sums_us;
+    if (splits > 1 && !s.sums) after += sums_us, summed = true;
   }
-  if (cost) *cost = best_us;
-  return best;
-}
-Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool can_split, bool sums) {
-  return cut_kind(M, N, K, dtype, can_split, sums, -1, nullptr);
-}
-// One kind of tile for all of a group: that with the least sum of times.
-void cut_group(const Shape* shapes, int n, int dtype, Cut* cuts) {
+  double us(int kind) const {
+    // rounds of the last product's workgroups
+    const int64_t places = kind == Cut::MID ? 512 : 256;
+    const double run = std::ceil(work / (places * last) - 1e-6) * last;
+    return std::max(run, longest) + after + (summed ? 4.0 : 0);
+  }
+};
+
+void cut_group(const Shape* shapes, int n, int dtype, bool can_split, Cut* cuts) {
+  const int ks = 128 / (dtype == PNFX_F32 ? 4 : 2);
+  int64_t most = 1;
+  for (int i = 0; i < n; ++i) most = std::max(most, ceil_div(shapes[i].K, ks));
   double best = 1e30;
   for (int kind = 0; kind < 3; ++kind) {
     if (kind == Cut::BIG && dtype == PNFX_F32) continue;
-    Cut got[kMaxGroup];
-    double total = 0;
-    for (int i = 0; i < n; ++i) {
-      double us;
-      got[i] = cut_kind(shapes[i].M, shapes[i].N, shapes[i].K, dtype, true, shapes[i].sums, kind, &us);
-      total += us;
-    }
-    if (total < best) {
-      best = total;
-      for (int i = 0; i < n; ++i) cuts[i] = got[i];
+    if (kind == Cut::DUO && !can_split) continue;
+    // workgroups of all of k, and of half, a quarter, ... of the longest k, each about as long as the others
+    for (int64_t len = most; len >= 4 || len == most; len = (len + 1) / 2) {
+      Cut got[3];
+      Cost cost;
+      for (int i = 0; i < n; ++i) {
+        const int64_t steps = std::max<int64_t>(1, ceil_div(shapes[i].K, ks));
+        const int64_t splits = std::min<int64_t>(ceil_div(steps, len), 64), per = ceil_div(steps, splits);
+        got[i] = Cut{(Cut::Kind)kind, (int)ceil_div(steps, per), per};
+        cost.add(kind, shapes[i], dtype, got[i].splits, per);
+      }
+      const double us = cost.us(kind);
+      if (us < best) {
+        best = us;
+        for (int i = 0; i < n; ++i) cuts[i] = got[i];
+      }
+      if (!can_split || len == 1) break;
     }
   }
+}
+Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool can_split) {
+  const Shape s{M, N, K, false};
+  Cut c;
+  cut_group(&s, 1, dtype, can_split, &c);
+  return c;
 }
 
 int64_t product_workspace(const Cut& cut, int64_t M, int64_t N) {
@@ -327,7 +325,6 @@ static int mm_args(const ProductArgs& p, const Cut& cut, int es, void* ws, MmArg
   g.k_count = p.k_count;
   g.add = p.add;
   g.alpha = summed ? nullptr : p.alpha;
-  g.by_xcd = cut.splits % 8 == 0;
   return PNFX_OK;
 }
 

@@ -739,7 +739,7 @@ BwdCut bwd_cut(const Sizes& z) {
   c.P = std::min(piece_of(z), round_up(z.V, 8));
   const Shape s[2] = {{z.T, z.D, c.P, true}, {c.P, z.D, z.T, false}};
   Cut cuts[2];
-  cut_group(s, 2, z.dtype, cuts);
+  cut_group(s, 2, z.dtype, true, cuts);
   c.dx = cuts[0], c.dw = cuts[1];
   return c;
 }
