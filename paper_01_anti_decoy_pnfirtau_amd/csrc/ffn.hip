@@ -288,6 +288,9 @@ __global__ __launch_bounds__(threads_of<C>, 2) void glu_bwd_kernel(GluArgs a) {
 }
 
 // ------------------------------------------------------------------------ few rows
+// Up to here ffn_rows_kernel takes them (us of a call, bf16, this kernel / the tiles: 17 rows, D = 1024, F = 4096 10.9 /
+// 21.8; 64 rows 16.3 / 25.5; 64 rows, D = 2048, F = 8192 33.5 / 40.9; D = 4096, F = 11008 73 / 91; beyond, its four
+// blocks of 16 rows would not do).
 constexpr int kFewRows = 64;
 
 struct RowsArgs {

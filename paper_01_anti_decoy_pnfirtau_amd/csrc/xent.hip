@@ -660,6 +660,15 @@ struct Arena {
   }
 };
 
+// Whether logits are formed in tiles of 256.  The exponentials of such a tile are not hidden by a neighbour's products
+// (128-tiles share a CU), so it pays where the products are long (us of the loss, tiles of 128 / 256, 8192 rows
+// by 32768 tokens: D = 384 236 / 231, training 1063 / 1125; D = 512 294 / 273, 1116 / 1078; D = 1024 540 / 467, 2035 /
+// 1866), there are tiles for every CU, and rounding the rows up to it costs little (333 rows by 50257 tokens, D = 1000:
+// 70 / 75; 512 rows by 65536, D = 2048: 156 / 130).
+bool big_tiles(const Sizes& z, int64_t tokens) {
+  return z.dtype == PNFX_BF16 && z.D >= 512 && ceil_div(z.T, 256) * ceil_div(tokens, 256) >= 256 &&
+         round_up(z.T, 256) * 4 <= round_up(z.T, 128) * 5;
+}
 // The forward's cut: tiles of rows by ranges of the vocabulary, two or more workgroups for each place on the chip.
 struct FwdCut {
   bool big;
@@ -673,9 +682,7 @@ int64_t tiles_per(const Sizes& z, int64_t tm, int64_t tn) {
 }
 FwdCut fwd_cut(const Sizes& z) {
   FwdCut c;
-  // The exponentials of a 256-tile are not hidden by a neighbour's products (128-tiles share a CU), so a large
-  // tile pays only where the products take several times as long.
-  c.big = z.dtype == PNFX_BF16 && z.D >= 768 && ceil_div(z.T, 256) * ceil_div(z.V, 256) >= 512;
+  c.big = big_tiles(z, z.V);
   c.tm = ceil_div(z.T, c.big ? 256 : 128);
   c.tn = ceil_div(z.V, c.big ? 256 : 128);
   c.per = tiles_per(z, c.tm, c.tn);
@@ -872,7 +879,7 @@ int xent_bwd(const float* dloss, const void* x, int64_t x_rs, const void* w, int
     const int64_t n = std::min(c.P, z.V - v0);
     const T* wp = static_cast<const T*>(w) + v0 * w_rs;
     GradArgs g{k.xc, wp, d, r.rowc, k.tgt, k.count, z.Dp, w_rs, z.Dp, c.P, (int)v0, (int)n, 0, 0, 0};
-    const bool big = cut_of(z.T, n, z.Dp, z.dtype, false).big() && z.D >= 768;
+    const bool big = big_tiles(z, n);
     const int64_t tm = ceil_div(z.T, big ? 256 : 128);
     g.tn = (int)ceil_div(round_up(n, 8), big ? 256 : 128);
     g.per = (int)tiles_per(z, tm, g.tn);
