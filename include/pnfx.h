@@ -306,8 +306,8 @@ int pnfx_flash_bwd_noalloc(const void* q, int64_t qsb, int64_t qsh, int64_t qsn,
  * are not null: dx [T, D], dw_in [2 F, D], dw_down [Do, F], contiguous, 16-byte aligned.
  * Operands whose columns are not a multiple of 8, or whose base or rows are not 16-byte aligned, are copied
  * into the workspace first.  T < 2^29; D, F, Do <= 2^18.  Workspace: 16-byte aligned, as large as
- * pnfx_ffn_*_workspace_size says, with `copies` not 0 where an operand has to be copied (F not a multiple of 8,
- * too).  Bitwise repeatable.
+ * pnfx_ffn_*_workspace_size says (0 for sizes that are refused), with `copies` not 0 where an operand has to be
+ * copied (F not a multiple of 8, too).  Bitwise repeatable.
  */
 #define PNFX_ACT_SILU 0
 #define PNFX_ACT_GELU 1 /* g Phi(g), the error-function form */

@@ -84,8 +84,9 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     reach no other result.  Another target outside 0 .. V - 1 makes its row's loss and gradients NaN (the
     host is never made to wait for a check).  Logits, maxima and sums are fp32; the gradient of the
     logits is rounded to x's type for the products with weight and x.  The memory beside the gradients is a
-    piece of the vocabulary's logits, 64 MB or 2048 tokens' worth, and an fp32 copy of x's gradient.  Bitwise
-    repeatable; second derivatives are refused.
+    piece of the vocabulary's logits, 256 MB or 2048 tokens' worth (none for bf16 rows of up to 64 columns
+    and one loss value), and fp32 sums of the gradients.  Bitwise repeatable; second derivatives are
+    refused.
     """
     _one_of("reduction", reduction, REDUCTIONS)
     x, weight = _autocast(x, weight)
