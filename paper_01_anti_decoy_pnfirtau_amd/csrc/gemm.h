@@ -516,7 +516,8 @@ inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 template <auto KERNEL, typename Arg>
 int launch(int64_t grid, int threads, int lds, const Arg& a, hipStream_t st, const char* what) {
   if (grid <= 0) return PNFX_OK;
-  PNFX_REQUIRE(grid < (1ll << 31), "%s: %lld workgroups", what, (long long)grid);
+  // HIP counts a launch's threads in 32 bits
+  PNFX_REQUIRE(grid * threads < (1ll << 32), "%s: %lld workgroups of %d", what, (long long)grid, threads);
   if (lds > 65536) {
     static std::atomic<uint64_t> told{0};
     int dev = 0;

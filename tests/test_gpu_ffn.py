@@ -117,6 +117,15 @@ def test_forward_and_gradients(dev, T, D, F, Do, dtype, act):
         close(a, want, name)
 
 
+@pytest.mark.parametrize("dtype,T,D,F,Do", [
+    (BF16, 2100, 520, 2060, 520),   # 256-tiles forward, k shared by two groups of waves backward
+    (BF16, 4100, 2056, 4104, 2056),  # 256-tiles throughout
+    (F32, 700, 300, 500, 300),      # splits of k, summed by another kernel
+])
+def test_larger_tiles_and_splits(dev, dtype, T, D, F, Do):
+    test_forward_and_gradients(dev, T, D, F, Do, dtype, "silu")
+
+
 def e4m3(b):
     return b.view(torch.float8_e4m3fn).double()
 

@@ -145,3 +145,59 @@ def test_opcheck_linear_xent(dev, dtype, reduction):
     loss, rows, lse = torch.ops.pnfx.linear_xent(*a, t, 5, reduction)
     torch.library.opcheck(torch.ops.pnfx.linear_xent_bwd.default,
                           (torch.ones_like(loss), *a, t, rows, lse, 5, reduction, [True, True]))
+
+
+def test_compiled_block_and_loss(dev):
+    """torch.compile traces block and loss as one graph, forward and backward (AOTAutograd's eager backend)."""
+    from paper_01_anti_decoy_pnfirtau_amd.wikilm import GatedFFN
+
+    f = GatedFFN(32, 40, "gelu", checkpoint="e4m3").to(dev).bfloat16()
+    w = seeded((50, 32), 30, torch.bfloat16, dev).requires_grad_()
+    x, target = seeded((3, 20, 32), 31, torch.bfloat16, dev), torch.randint(0, 50, (3, 20)).to(dev)
+
+    def step(x, target):
+        return linear_cross_entropy(x + f(x), w, target)
+
+    compiled = torch.compile(step, backend="aot_eager", fullgraph=True)
+    leaves = [w, *f.parameters()]
+    for _ in range(2):
+        got, ref = compiled(x, target), step(x, target)
+        assert torch.equal(got, ref)
+        for a, b in zip(torch.autograd.grad(got, leaves), torch.autograd.grad(ref, leaves)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("T", [1, 40, 300])
+def test_threads_and_streams_at_once(dev, T):
+    """Four threads with a stream each, inference and training calls mixed: every result is that of a call alone."""
+    import threading
+
+    D, Fd, V = 64, 96, 700
+    w_in, w_down = seeded((2 * Fd, D), 32, torch.bfloat16, dev, 0.1), seeded((D, Fd), 33, torch.bfloat16, dev, 0.1)
+    w = seeded((V, D), 34, torch.bfloat16, dev)
+
+    def run(i):
+        x = seeded((T, D), 40 + i, torch.bfloat16, dev).requires_grad_()
+        target = torch.arange(T, device=dev) * (i + 1) % V
+        with torch.no_grad():
+            y = gated_ffn(x, w_in, w_down)
+        loss = linear_cross_entropy(gated_ffn(x, w_in, w_down), w, target)
+        return [y, loss.detach(), torch.autograd.grad(loss, x)[0]]
+
+    ref = [run(i) for i in range(4)]
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got[i] = run(i)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(got, ref):
+        assert all(torch.equal(u, v) for u, v in zip(a, b))

@@ -100,10 +100,22 @@ def test_loss_and_gradients(dev, T, D, V, dtype, reduction):
         close(a, want, name)
 
 
-def test_several_pieces_of_the_vocabulary(dev, monkeypatch):
-    """More tokens than a piece holds (64 MB of logits' gradients): 17000 rows take pieces of 2048."""
-    print("[xent pieces]", flush=True)
-    T, D, V = 17000, 24, 5000
+@pytest.mark.parametrize("dtype,T,D,V", [
+    (BF16, 2600, 520, 6000), (BF16, 3000, 1032, 9000),                        # 256-tiles of logits
+    (BF16, 2600, 64, 4000), (BF16, 2600, 128, 4000), (BF16, 5200, 192, 3001),  # rows' fragments in registers
+    (BF16, 2600, 256, 4001), (F32, 700, 300, 3000),
+])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_larger_tiles_and_splits(dev, dtype, T, D, V, reduction):
+    test_loss_and_gradients(dev, T, D, V, dtype, reduction)
+
+
+@pytest.mark.parametrize("D", [24, 72])
+def test_several_pieces_of_the_vocabulary(dev, D):
+    """More tokens than a piece holds (256 MB of logits' gradients): 17000 rows take pieces of 7936 of them, and
+    rows of up to 64 columns none at all."""
+    print(f"[xent pieces D={D}]", flush=True)
+    T, V = 17000, 9000
     x, w, target = make(T, D, V, BF16, dev, 0.1, 7)
     leaves = [t.clone().requires_grad_() for t in (x, w)]
     loss = linear_cross_entropy(*leaves, target, reduction="sum")
