@@ -19,9 +19,10 @@
 // fp32 results where it is one value, and for a loss per row dx's rows and the x of dW = d^T (s x).  The target's
 // own element is expm1(-loss_t), which keeps its digits where the softmax is close to one.
 //
-// Exponentials are taken in base 2.  The forward's are exp2(z L - m L) with L = log2 e as one fma per logit; the
-// rounding of m L is the same for a whole row and comes out again as the factor unround(m) = exp2(round(m L) - m L):
-// without it logits around 5e4 would be 4e-3 off.
+// Exponentials are taken in base 2, exp2(z L - m L) with L = log2 e as one fma per logit.  In the forward the rounding
+// of m L is the same for a whole row and comes out again at its end, as the factor unround(m) = exp2(round(m L) - m L):
+// without it logits around 5e4 would be 4e-3 off.  (In the backward m is the log-sum-exp, which is itself rounded
+// to fp32: nothing is gained by it there.)
 #include <algorithm>
 #include <type_traits>
 
@@ -227,18 +228,29 @@ __global__ __launch_bounds__(threads_of<C>, 2) void xent_fwd_kernel(FwdArgs a) {
       for (int j = 0; j < P::NJ; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[i][j][r]);
-      const float ref = m == -INFINITY ? 0.f : m;
-      float s = 0.f;
+      // The reference follows the maximum only once it is 8 behind (the exponentials stay below e^8), which after the
+      // first tiles is hardly ever: 95 against 106 us at T = 16384, D = 64, V = 33278, 1.52 against 1.58 ms at T = 8192,
+      // D = 4096, V = 32000.  With A's four steps in registers there is none left for the branch (16 spilled: 350
+      // against 302 us at T = 16384, D = 256, V = 33278), and it follows at every tile.
+      if (KS == 4 || __any(m > top[i] + 8.f)) {
+#pragma clang fp contract(off)  // both products rounded as below, so that unround() of the last takes all of it out
+        const float next = fmaxf(top[i], m);
+        sum[i] = top[i] == -INFINITY ? 0.f : sum[i] * exp2_fast(top[i] * kLog2e - next * kLog2e);
+        top[i] = next;
+      }
+      const float c = top[i] == -INFINITY ? 0.f : top[i] * kLog2e;
+      float s = sum[i];
 #pragma unroll
       for (int j = 0; j < P::NJ; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s += exp2_fast(__builtin_fmaf(acc[i][j][r], kLog2e, -(ref * kLog2e)));
-      join(top[i], sum[i], m, s * unround(ref));
+        for (int r = 0; r < 4; ++r) s += exp2_fast(__builtin_fmaf(acc[i][j][r], kLog2e, -c));
+      sum[i] = s;
     }
   });
   // over the four lanes of a row
 #pragma unroll
   for (int i = 0; i < P::MI; ++i) {
+    if (top[i] != -INFINITY) sum[i] *= unround(top[i]);
 #pragma unroll
     for (int o = 16; o <= 32; o <<= 1)
       join(top[i], sum[i], __shfl_xor(top[i], o, 64), __shfl_xor(sum[i], o, 64));
@@ -346,12 +358,12 @@ __global__ __launch_bounds__(threads_of<C>, 2) void xent_grad_kernel(GradArgs a)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave / C::WN * P::MI, wn = wave % C::WN * P::NJ;
   const int Pc = (a.P + 7) & ~7;  // columns past the piece, up to a whole chunk, are zero
-  // of each row its log-sum-exp and its target's column in the piece, if it has one there (in LDS: there are
+  // of each row its log-sum-exp times log2 e and its target's column in the piece, if it has one there (in LDS: there are
   // no registers left for them beside A's fragments); published by the loop's first barrier
   __shared__ float2 rows[C::TM];
   for (int r = threadIdx.x; r < C::TM; r += threads_of<C>) {
     const int m = min(m0 + r, M - 1);
-    rows[r] = float2{a.rowc[m].x, __int_as_float(a.tgt[m] - a.v0)};
+    rows[r] = float2{a.rowc[m].x * kLog2e, __int_as_float(a.tgt[m] - a.v0)};
   }
   const auto out = __builtin_amdgcn_make_buffer_rsrc(static_cast<T*>(a.d) + m0 * a.ldd, 0,
                                                      (int)(min(M - m0, C::TM) * a.ldd * sizeof(T)), 0x00027000);
@@ -374,7 +386,7 @@ __global__ __launch_bounds__(threads_of<C>, 2) void xent_grad_kernel(GradArgs a)
       for (int j = 0; j < P::NJ; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          acc[i][j][r] = exp2_fast((acc[i][j][r] - c.x) * kLog2e);
+          acc[i][j][r] = exp2_fast(__builtin_fmaf(acc[i][j][r], kLog2e, -c.x));
       // 16 bytes at a time; the buffer's bounds drop the rows past M, a far offset the columns past the piece
       const unsigned at = row + stage_row<ROW>(i, 0) * ldb + nl * (unsigned)sizeof(T);
 #pragma unroll
@@ -470,11 +482,11 @@ __global__ __launch_bounds__(256, 2) void xent_narrow_kernel(NarrowArgs a) {
     }
     wait_vm_lgkm<0>();
     __builtin_amdgcn_s_barrier();
-    // dx: each row's log-sum-exp and target, as a column of the first tile; published by the loop's first barrier
+    // dx: each row's log-sum-exp times log2 e and target, as a column of the first tile; published by the loop's first barrier
     if constexpr (!DW) {
       if (threadIdx.x < 128) {
         const int m = min(m0 + (int)threadIdx.x, rows - 1);
-        rowl[threadIdx.x] = float2{a.rowc[m].x, __int_as_float(a.tgt[m] - t0 * 128)};
+        rowl[threadIdx.x] = float2{a.rowc[m].x * kLog2e, __int_as_float(a.tgt[m] - t0 * 128)};
       }
       wait_vm_lgkm<0>();
     }
@@ -510,9 +522,9 @@ __global__ __launch_bounds__(256, 2) void xent_narrow_kernel(NarrowArgs a) {
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float l = c[8 * g + col(j) + r].x;
+            const float l = c[8 * g + col(j) + r].x * kLog2e;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) z[i][j][r] = exp2_fast((z[i][j][r] - l) * kLog2e);
+            for (int i = 0; i < 4; ++i) z[i][j][r] = exp2_fast(__builtin_fmaf(z[i][j][r], kLog2e, -l));
           }
         hit = (unsigned)(__float_as_int(c[lane].w) - m0 - 64 * wm) < 64u;
       } else {
@@ -523,7 +535,7 @@ __global__ __launch_bounds__(256, 2) void xent_narrow_kernel(NarrowArgs a) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) z[i][j][r] = exp2_fast((z[i][j][r] - c.x) * kLog2e);
+            for (int r = 0; r < 4; ++r) z[i][j][r] = exp2_fast(__builtin_fmaf(z[i][j][r], kLog2e, -c.x));
           hit = hit || (unsigned)(__float_as_int(c.y) - 128 * t - 64 * wn - 8 * g) < 40u;
         }
       }
