@@ -111,7 +111,7 @@ struct Stage {
   static_assert(SPL == 32 || SPL == 64, "a load fills half a sub-tile or a whole one");
   static constexpr int ES = (int)sizeof(T), KS = k_step<T>;
   const char* base[KIND == PAIR ? 2 : 1];  // element (first row, k0)
-  int64_t K, left;  // k of a tile, and those left of it
+  int K, left;     // k of a tile, and those left of it
   int rows;        // rows from the tile's first on
   unsigned ldb;    // bytes from row to row
   unsigned limit;  // ROW, PAIR: bytes to the last row in reach; COL: bytes of a row in reach
@@ -122,7 +122,7 @@ struct Stage {
   __device__ __forceinline__ void init(const T* p, int64_t ld, int nrows, int64_t k, int tid,
                                        const T* p2 = nullptr) {
     ldb = (unsigned)(ES * ld);
-    K = left = k;
+    K = left = (int)k;
     rows = nrows;
     base[0] = reinterpret_cast<const char*>(p);
     const int slot = tid / 8;
@@ -152,7 +152,8 @@ struct Stage {
   }
   // The next step's tile to LDS byte address lds.
   __device__ __forceinline__ void load(unsigned lds, int wave) {
-    const unsigned ks = (unsigned)max<int64_t>(0, min<int64_t>(left, KS));
+    // (in 32 bits: HIP's min and max of 64-bit integers go through double, 2 % of the large products' time)
+    const unsigned ks = (unsigned)max(0, min(left, KS));
     const unsigned dst = lds + wave * 1024;
     if constexpr (KIND == COL) {
       const u32x4 d = buffer_of(base[0], ks ? (ks - 1) * ldb + limit : 0u);

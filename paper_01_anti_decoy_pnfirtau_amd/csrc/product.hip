@@ -58,16 +58,17 @@ __device__ __forceinline__ void mm_tile(const MmArgs& g, int block, char* sm) {
   int tm, tn;
   band_tile(place % tiles, tms, g.tn, tm, tn);
   const int m0 = tm * C::TM, n0 = tn * C::TN;
-  const int64_t K = g.k_count ? min<int64_t>(g.K, *g.k_count) : g.K;
+  const int K = g.k_count ? min((int)g.K, *g.k_count) : (int)g.K;
   const int all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   constexpr int WAVES = C::WM * C::WN;
   const int group = all / WAVES, wave = all % WAVES;
   int64_t k0 = split * g.steps * k_step<T>;
-  int64_t ks = min<int64_t>(K - k0, g.steps * k_step<T>);
-  int steps = (int)((ks + k_step<T> - 1) / k_step<T>);
+  const int64_t left = K - k0, most = g.steps * k_step<T>;
+  int ks = (int)(left < most ? left : most);
+  int steps = (ks + k_step<T> - 1) / k_step<T>;
   if constexpr (C::KG == 2) {  // as many steps for either group; past the end they read zeros
     steps = (steps + 1) / 2;
-    const int64_t half = (int64_t)steps * k_step<T>;
+    const int half = steps * k_step<T>;
     k0 += group * half;
     ks = group ? ks - half : min(ks, half);
   }
@@ -300,7 +301,7 @@ int64_t product_workspace(const Cut& cut, int64_t M, int64_t N) {
 // The kernel's arguments of a product; `ws`: where its splits' sums go, if it has any.
 static int mm_args(const ProductArgs& p, const Cut& cut, int es, void* ws, MmArgs& g) {
   PNFX_REQUIRE(operand_ok(p.a, p.lda, es) && operand_ok(p.b, p.ldb, es), "product: operand alignment");
-  PNFX_REQUIRE(p.M < (1 << 30) && p.N < (1 << 30) && p.K < (1ll << 31), "product: %lld x %lld over %lld",
+  PNFX_REQUIRE(p.M < (1 << 30) && p.N < (1 << 30) && p.K < (1 << 30), "product: %lld x %lld over %lld",
                (long long)p.M, (long long)p.N, (long long)p.K);
   const bool summed = !p.sums && cut.splits > 1;
   PNFX_REQUIRE(!summed || ws, "product: no workspace");
