@@ -358,12 +358,14 @@ __global__ __launch_bounds__(threads_of<C>, 2) void xent_grad_kernel(GradArgs a)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave / C::WN * P::MI, wn = wave % C::WN * P::NJ;
   const int Pc = (a.P + 7) & ~7;  // columns past the piece, up to a whole chunk, are zero
-  // of each row its log-sum-exp times log2 e and its target's column in the piece, if it has one there (in LDS: there are
-  // no registers left for them beside A's fragments); published by the loop's first barrier
-  __shared__ float2 rows[C::TM];
+  // of each row its log-sum-exp times log2 e, its target's column in the piece, if it has one there, and its target's
+  // element of d (in LDS: there are no registers left for them beside A's fragments, and a read from global memory waits
+  // for every load and store on its way); published by the loop's first barrier
+  __shared__ float4 rows[C::TM];
   for (int r = threadIdx.x; r < C::TM; r += threads_of<C>) {
     const int m = min(m0 + r, M - 1);
-    rows[r] = float2{a.rowc[m].x * kLog2e, __int_as_float(a.tgt[m] - a.v0)};
+    const float4 c = a.rowc[m];
+    rows[r] = float4{c.x * kLog2e, __int_as_float(a.tgt[m] - a.v0), c.z, 0.f};
   }
   const auto out = __builtin_amdgcn_make_buffer_rsrc(static_cast<T*>(a.d) + m0 * a.ldd, 0,
                                                      (int)(min(M - m0, C::TM) * a.ldd * sizeof(T)), 0x00027000);
@@ -381,7 +383,8 @@ __global__ __launch_bounds__(threads_of<C>, 2) void xent_grad_kernel(GradArgs a)
     const bool edge = n0 + C::TN > a.P;
 #pragma unroll
     for (int i = 0; i < P::MI; ++i) {
-      const float2 c = rows[stage_row<ROW>(wm + i, lane & 15)];
+      const float4& row4 = rows[stage_row<ROW>(wm + i, lane & 15)];
+      const float2 c{row4.x, row4.y};
 #pragma unroll
       for (int j = 0; j < P::NJ; ++j)
 #pragma unroll
@@ -411,7 +414,7 @@ __global__ __launch_bounds__(threads_of<C>, 2) void xent_grad_kernel(GradArgs a)
       // seldom: the row's target is among the lane's columns; this store is the same thread's and comes later
       const int own = __float_as_int(c.y) - nl;
       if ((unsigned)own < 16u * P::NJ && (own & 24) == 0) {
-        const T v = from_f32<T>(a.rowc[min(m0 + stage_row<ROW>(wm + i, lane & 15), M - 1)].z);
+        const T v = from_f32<T>(row4.z);
         if constexpr (sizeof(T) == 2)
           __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), out, at + own * 2, 0, 0);
         else
@@ -445,7 +448,7 @@ __global__ __launch_bounds__(256, 2) void xent_narrow_kernel(NarrowArgs a) {
   extern __shared__ __align__(16) char smem[];
   bf16* const sm = reinterpret_cast<bf16*>(smem);
   float4* const cols = reinterpret_cast<float4*>(smem + RING * SB * 2);  // DW: [RING][wave][64] of the tile's rows
-  float2* const rowl = reinterpret_cast<float2*>(smem + RING * SB * 2);  // dx: [128] of the rows kept
+  float4* const rowl = reinterpret_cast<float4*>(smem + RING * SB * 2);  // dx: [128] of the rows kept
   const int count = *a.count;
   const int rows = DW ? a.M : count, nb = DW ? count : a.nb;
   const int tms = (rows + 127) / 128;
@@ -482,11 +485,13 @@ __global__ __launch_bounds__(256, 2) void xent_narrow_kernel(NarrowArgs a) {
     }
     wait_vm_lgkm<0>();
     __builtin_amdgcn_s_barrier();
-    // dx: each row's log-sum-exp times log2 e and target, as a column of the first tile; published by the loop's first barrier
+    // dx: each row's log-sum-exp times log2 e, its target as a column of the first tile, and the target's element;
+    // published by the loop's first barrier
     if constexpr (!DW) {
       if (threadIdx.x < 128) {
         const int m = min(m0 + (int)threadIdx.x, rows - 1);
-        rowl[threadIdx.x] = float2{a.rowc[m].x * kLog2e, __int_as_float(a.tgt[m] - t0 * 128)};
+        const float4 c = a.rowc[m];
+        rowl[threadIdx.x] = float4{c.x * kLog2e, __int_as_float(a.tgt[m] - t0 * 128), c.z, 0.f};
       }
       wait_vm_lgkm<0>();
     }
@@ -515,7 +520,7 @@ __global__ __launch_bounds__(256, 2) void xent_narrow_kernel(NarrowArgs a) {
       }
       const auto col = [](int j) { return stage_row<ROW>(j, 0); };  // block j's first column of the lane's
       const float4* const c = cols + (buf * 4 + wave) * 64;
-      bool hit;
+      // Seldom a target's own element is among the wave's: which of its blocks have one.
       if constexpr (DW) {
         // (the log-sum-exps of the lane's 16 columns)
 #pragma unroll
@@ -526,23 +531,11 @@ __global__ __launch_bounds__(256, 2) void xent_narrow_kernel(NarrowArgs a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) z[i][j][r] = exp2_fast(__builtin_fmaf(z[i][j][r], kLog2e, -l));
           }
-        hit = (unsigned)(__float_as_int(c[lane].w) - m0 - 64 * wm) < 64u;
-      } else {
-        hit = false;
+        const uint64_t hits = __ballot((unsigned)(__float_as_int(c[lane].w) - m0 - 64 * wm) < 64u);
+        if (hits) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 c = rowl[stage_row<ROW>(4 * wm + i, r16)];
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) z[i][j][r] = exp2_fast(__builtin_fmaf(z[i][j][r], kLog2e, -c.x));
-          hit = hit || (unsigned)(__float_as_int(c.y) - 128 * t - 64 * wn - 8 * g) < 40u;
-        }
-      }
-      if (__any(hit)) {  // seldom: a target's own element
-        if constexpr (DW) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
+          for (int j = 0; j < 4; ++j) {
+            if (!(hits >> col(j) & 0x0f0f0f0fu)) continue;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const float4 e = c[8 * g + col(j) + r];
@@ -551,11 +544,20 @@ __global__ __launch_bounds__(256, 2) void xent_narrow_kernel(NarrowArgs a) {
               for (int i = 0; i < 4; ++i)
                 if (own == stage_row<ROW>(i, r16)) z[i][j][r] = e.z;
             }
-        } else {
+          }
+        }
+      } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float own = a.rowc[min(m0 + stage_row<ROW>(4 * wm + i, r16), rows - 1)].z;
-            const int at = __float_as_int(rowl[stage_row<ROW>(4 * wm + i, r16)].y) - 128 * t - 64 * wn - 8 * g;
+        for (int i = 0; i < 4; ++i) {
+          const float4& c = rowl[stage_row<ROW>(4 * wm + i, r16)];
+          const float l = c.x;
+          const int at = __float_as_int(c.y) - 128 * t - 64 * wn - 8 * g;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) z[i][j][r] = exp2_fast(__builtin_fmaf(z[i][j][r], kLog2e, -l));
+          if (__any((unsigned)at < 40u)) {
+            const float own = c.z;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -618,7 +620,7 @@ __global__ __launch_bounds__(256, 2) void xent_narrow_kernel(NarrowArgs a) {
     }
   }
 }
-constexpr int kNarrowLds[2] = {4 * 128 * 128 + 1024, 4 * 128 * 128 + 4 * 4 * 1024};  // dx, dW
+constexpr int kNarrowLds[2] = {4 * 128 * 128 + 128 * 16, 4 * 128 * 128 + 4 * 4 * 1024};  // dx, dW
 
 struct DxArgs {
   const float* sums;  // [splits][T][D]
