@@ -1033,7 +1033,7 @@ class GatedFfnFn : public torch::autograd::Function<GatedFfnFn> {
   }
 };
 
-// Without a gradient to come nothing is kept, whatever `keep` says.
+// A call that records a gradient has to keep something; one that records none keeps what its caller asks for.
 std::tuple<Tensor, Tensor, Tensor> gated_ffn_autograd(const Tensor& x, const Tensor& w_in,
                                                       const Tensor& w_down, int64_t act,
                                                       int64_t keep) {
