@@ -77,11 +77,17 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs a) {
   // kept rows before this workgroup's, and (backward, for the mean) behind them
   int before = 0, total = 0;
   const int to = a.rowc ? a.T : r0;
-#pragma unroll 8
-  for (int r = tid; r < to; r += 256) {
-    const int k = a.target[r] != a.ignore;
-    total += k;
-    before += r < r0 ? k : 0;
+  constexpr int U = 16;  // a thread's loads on their way (8 and single ones at the end: 15.3 against 14 us, T = 16384)
+  for (int b = tid; b < to; b += 256 * U) {
+    int64_t t[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) t[u] = a.target[min(b + 256 * u, to - 1)];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = b + 256 * u, k = r < to && t[u] != a.ignore;
+      total += k;
+      before += r < r0 ? k : 0;
+    }
   }
   const auto block_sum = [&](int v) {
     v = wave_sum_i(v);
