@@ -710,8 +710,8 @@ FwdCut fwd_cut(const Sizes& z) {
   return c;
 }
 // Tokens of a piece: 256 MB of d, the last-level cache's size.  Smaller pieces write and read dx's fp32 sums
-// more often and give the products fewer k or rows (xent_lm 2102 us at 64 MB, 1830 at 128, 1711 at 256, 1739 at 512;
-// xent_narrow 914, 743, 685, 741; xent_large 7018, 6461, 6362, 6246).
+// more often and give the products fewer k or rows, larger ones leave the cache (16384 x 256 x 33278: 1681 us at 128 MB,
+// 1511 at 192, 1246 at 256, 1680 at 320; 8192 x 2048 x 65536: 5825, 5993, 5706, 5708).
 int64_t piece_of(const Sizes& z) {
   const int64_t most = std::min(round_up(std::max<int64_t>((256ll << 20) / (z.T * z.es), 2048), 256), kMaxLd / 2);
   const int64_t n = ceil_div(z.V, most);
