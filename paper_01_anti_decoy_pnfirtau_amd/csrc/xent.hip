@@ -240,8 +240,9 @@ __global__ __launch_bounds__(threads_of<C>, 2) void xent_fwd_kernel(FwdArgs a) {
       // against 302 us at T = 16384, D = 256, V = 33278), and it follows at every tile.
       if (KS == 4 || __any(m > top[i] + 8.f)) {
 #pragma clang fp contract(off)  // both products rounded as below, so that unround() of the last takes all of it out
+        // (while nothing but -infinity and NaN was seen there is nothing to scale; a sum that is NaN by then stays so)
         const float next = fmaxf(top[i], m);
-        sum[i] = top[i] == -INFINITY ? 0.f : sum[i] * exp2_fast(top[i] * kLog2e - next * kLog2e);
+        sum[i] = next == -INFINITY ? sum[i] : sum[i] * exp2_fast(top[i] * kLog2e - next * kLog2e);
         top[i] = next;
       }
       const float c = top[i] == -INFINITY ? 0.f : top[i] * kLog2e;
