@@ -21,8 +21,8 @@
 //
 // Exponentials are taken in base 2, exp2(z L - m L) with L = log2 e as one fma per logit.  In the forward the rounding
 // of m L is the same for a whole row and comes out again at its end, as the factor unround(m) = exp2(round(m L) - m L):
-// without it logits around 5e4 would be 4e-3 off.  (In the backward m is the log-sum-exp, which is itself rounded
-// to fp32: nothing is gained by it there.)
+// without it logits around 5e4 would be 4e-3 off.  Beyond 2^24 logits are subtracted first.  (In the backward m is the
+// log-sum-exp, which is itself rounded to fp32: nothing is gained by it there.)
 #include <algorithm>
 #include <type_traits>
 
@@ -35,6 +35,10 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float unround(float m) { return exp2_fast(-__builtin_fmaf(m, kLog2e, -(m * kLog2e))); }
+// Beyond here the rounding of m L reaches whole units and, from about 2^30 on, more than an exponent holds: infinite or NaN
+// sums for lanes whose logits so far are all the type's lowest value, say.  A workgroup that ends with such a maximum or sum
+// goes through its tiles again and subtracts first.  (Tokens that are masked so cost that where they fill a lane's columns.)
+constexpr float kFarTop = 16777216.f;
 // Joins (top, sum) with (top2, sum2): maxima of logits and sums of exponentials beside them.  While nothing but
 // -infinity was seen there is nothing to scale.
 __device__ __forceinline__ void join(float& top, float& sum, float top2, float sum2) {
@@ -206,58 +210,95 @@ __global__ __launch_bounds__(threads_of<C>, 2) void xent_fwd_kernel(FwdArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave / C::WN * P::MI, wn = wave % C::WN * P::NJ;
   float top[P::MI], sum[P::MI];
-#pragma unroll
-  for (int i = 0; i < P::MI; ++i) top[i] = -INFINITY, sum[i] = 0.f;
   const int t0 = split * a.per, tiles = min(a.tn - t0, a.per);
-  typename P::StageA sa;
-  typename P::StageB sb;
-  sa.init(static_cast<const T*>(a.xc) + m0 * a.ldx, a.ldx, M - m0, a.K, threadIdx.x);
-  sb.init(static_cast<const T*>(a.w) + (int64_t)t0 * C::TN * a.ldw, a.ldw, a.V - t0 * C::TN, a.K, threadIdx.x);
-  f32x4 acc[P::MI][P::NJ] = {};
-  P::go(sa, sb, a.K, tiles, reinterpret_cast<T*>(sm), wave, lane, acc, [&](int t) {
-    const int n0 = (t0 + t) * C::TN;
-    if (n0 + C::TN > a.V) {  // past the vocabulary
+  const auto pass = [&](auto far) {
+    constexpr bool FAR = decltype(far)::value;
+    // the second pass works its addresses out anew: kept over the first one's loop they were 13 spilled registers
+    int tid = threadIdx.x;
+    if (FAR) asm volatile("" : "+v"(tid));
+    const int lane = tid & 63;
 #pragma unroll
-      for (int j = 0; j < P::NJ; ++j) {
-        const int n = n0 + stage_row<ROW>(wn + j, 4 * (lane >> 4));
+    for (int i = 0; i < P::MI; ++i) top[i] = -INFINITY, sum[i] = 0.f;
+    typename P::StageA sa;
+    typename P::StageB sb;
+    sa.init(static_cast<const T*>(a.xc) + m0 * a.ldx, a.ldx, M - m0, a.K, tid);
+    sb.init(static_cast<const T*>(a.w) + (int64_t)t0 * C::TN * a.ldw, a.ldw, a.V - t0 * C::TN, a.K, tid);
+    f32x4 acc[P::MI][P::NJ] = {};
+    P::go(sa, sb, a.K, tiles, reinterpret_cast<T*>(sm), wave, lane, acc, [&](int t) {
+      const int n0 = (t0 + t) * C::TN;
+      if (n0 + C::TN > a.V) {  // past the vocabulary
 #pragma unroll
-        for (int i = 0; i < P::MI; ++i)
+        for (int j = 0; j < P::NJ; ++j) {
+          const int n = n0 + stage_row<ROW>(wn + j, 4 * (lane >> 4));
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (n + r >= a.V) acc[i][j][r] = -INFINITY;
+          for (int i = 0; i < P::MI; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (n + r >= a.V) acc[i][j][r] = -INFINITY;
+        }
       }
-    }
 #pragma unroll
-    for (int i = 0; i < P::MI; ++i) {
-      float m = acc[i][0][0];
+      for (int i = 0; i < P::MI; ++i) {
+        float m = acc[i][0][0];
 #pragma unroll
-      for (int j = 0; j < P::NJ; ++j)
+        for (int j = 0; j < P::NJ; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[i][j][r]);
-      // The reference follows the maximum only once it is 8 behind (the exponentials stay below e^8), which after the
-      // first tiles is hardly ever: 95 against 106 us at T = 16384, D = 64, V = 33278, 1.52 against 1.58 ms at T = 8192,
-      // D = 4096, V = 32000.  With A's four steps in registers there is none left for the branch (16 spilled: 350
-      // against 302 us at T = 16384, D = 256, V = 33278), and it follows at every tile.
-      if (KS == 4 || __any(m > top[i] + 8.f)) {
+          for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[i][j][r]);
+        // While nothing but -infinity and NaN was seen there is nothing to scale; a sum that is NaN by then stays so.
+        if constexpr (FAR) {
+          const float next = fmaxf(top[i], m), ref = next == -INFINITY ? 0.f : next;
+          float s = next == -INFINITY ? sum[i] : sum[i] * exp2_fast((top[i] - next) * kLog2e);
+#pragma unroll
+          for (int j = 0; j < P::NJ; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s += exp2_fast((acc[i][j][r] - ref) * kLog2e);
+          top[i] = next;
+          sum[i] = s;
+          continue;
+        }
+        // The reference follows the maximum only once it is 8 behind (the exponentials stay below e^8), which after the
+        // first tiles is hardly ever: 95 against 106 us at T = 16384, D = 64, V = 33278, 1.52 against 1.58 ms at T = 8192,
+        // D = 4096, V = 32000.  With A's four steps in registers there is none left for the branch (16 spilled: 350
+        // against 302 us at T = 16384, D = 256, V = 33278), and it follows at every tile.
+        if (KS == 4 || __any(m > top[i] + 8.f)) {
 #pragma clang fp contract(off)  // both products rounded as below, so that unround() of the last takes all of it out
-        // (while nothing but -infinity and NaN was seen there is nothing to scale; a sum that is NaN by then stays so)
-        const float next = fmaxf(top[i], m);
-        sum[i] = next == -INFINITY ? sum[i] : sum[i] * exp2_fast(top[i] * kLog2e - next * kLog2e);
-        top[i] = next;
+          const float next = fmaxf(top[i], m);
+          sum[i] = next == -INFINITY ? sum[i] : sum[i] * exp2_fast(top[i] * kLog2e - next * kLog2e);
+          top[i] = next;
+        }
+        const float c = top[i] == -INFINITY ? 0.f : top[i] * kLog2e;
+        float s = sum[i];
+#pragma unroll
+        for (int j = 0; j < P::NJ; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s += exp2_fast(__builtin_fmaf(acc[i][j][r], kLog2e, -c));
+        sum[i] = s;
       }
-      const float c = top[i] == -INFINITY ? 0.f : top[i] * kLog2e;
-      float s = sum[i];
+    });
+  };
+  pass(std::false_type{});
+  bool far = false;
 #pragma unroll
-      for (int j = 0; j < P::NJ; ++j)
+  for (int i = 0; i < P::MI; ++i) far |= !(sum[i] < INFINITY) || (fabsf(top[i]) > kFarTop && top[i] != -INFINITY);
+  // (the loop's last barrier has left the LDS free)
+  int* const votes = reinterpret_cast<int*>(sm);
+  if (lane == 0) votes[wave] = 0;
+  if (far) votes[wave] = 1;
+  __syncthreads();
+  far = false;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s += exp2_fast(__builtin_fmaf(acc[i][j][r], kLog2e, -c));
-      sum[i] = s;
-    }
-  });
+  for (int v = 0; v < C::WM * C::WN; ++v) far |= votes[v] != 0;
+  __syncthreads();
+  if (far) {
+    pass(std::true_type{});
+  } else {
+#pragma unroll
+    for (int i = 0; i < P::MI; ++i)
+      if (top[i] != -INFINITY) sum[i] *= unround(top[i]);
+  }
   // over the four lanes of a row
 #pragma unroll
   for (int i = 0; i < P::MI; ++i) {
-    if (top[i] != -INFINITY) sum[i] *= unround(top[i]);
 #pragma unroll
     for (int o = 16; o <= 32; o <<= 1)
       join(top[i], sum[i], __shfl_xor(top[i], o, 64), __shfl_xor(sum[i], o, 64));
