@@ -21,8 +21,10 @@
 //
 // Exponentials are taken in base 2, exp2(z L - m L) with L = log2 e as one fma per logit.  In the forward the rounding
 // of m L is the same for a whole row and comes out again at its end, as the factor unround(m) = exp2(round(m L) - m L):
-// without it logits around 5e4 would be 4e-3 off.  Beyond 2^24 logits are subtracted first.  (In the backward m is the
-// log-sum-exp, which is itself rounded to fp32: nothing is gained by it there.)
+// without it logits around 5e4 would be 4e-3 off.  Beyond 2^24 logits are subtracted first.  In the backward m is the
+// log-sum-exp, rounded to fp32, and the softmax is off by 2^-23 of it; rows for which that would show (kFarLse) are
+// subtracted first, too, and what the rounding took from the log-sum-exp comes back from the loss: dot(x_t, W_target) +
+// loss_t is the same number in two parts.  That leaves 2^-23 of the loss, or of the log-sum-exp where it is the smaller.
 #include <algorithm>
 #include <type_traits>
 
@@ -39,12 +41,24 @@ __device__ __forceinline__ float unround(float m) { return exp2_fast(-__builtin_
 // sums for lanes whose logits so far are all the type's lowest value, say.  A workgroup that ends with such a maximum or sum
 // goes through its tiles again and subtracts first.  (Tokens that are masked so cost that where they fill a lane's columns.)
 constexpr float kFarTop = 16777216.f;
+// The backward's |log-sum-exp| from which on a row is far: 2^-13 and 2^-18 of an element of the softmax.
+template <typename T>
+constexpr float kFarLse = sizeof(T) == 2 ? 1024.f : 32.f;
 // Joins (top, sum) with (top2, sum2): maxima of logits and sums of exponentials beside them.  While nothing but
 // -infinity was seen there is nothing to scale.
 __device__ __forceinline__ void join(float& top, float& sum, float top2, float sum2) {
   const float next = fmaxf(top, top2), ref = next == -INFINITY ? 0.f : next;
   sum = sum * exp2_fast((top - ref) * kLog2e) + sum2 * exp2_fast((top2 - ref) * kLog2e);
   top = next;
+}
+
+// A lane's part of x . w; U loads on their way, the same bits for any U.
+template <int U, typename T>
+__device__ __forceinline__ float dot_part(const T* x, const T* w, int K, int lane) {
+  float dot = 0.f;
+#pragma unroll U
+  for (int k = lane; k < K; k += 64) dot = __builtin_fmaf(to_f32(x[k]), to_f32(w[k]), dot);
+  return dot;
 }
 
 // -------------------------------------------------------------------------- kept rows
@@ -60,11 +74,16 @@ struct RowsArgs {
   int* count;
   int64_t x_rs, ignore;
   int T, D, Dp, V, per;  // per: rows of a workgroup
-  // backward only: row constants {lse, s_t, expm1(-loss_t), target or -1}; s_t where it is one value; s_t x_t where not
+  // backward only: row constants {lse, the rest of it times log2 e, expm1(-loss_t), target or -1}; s_t; it again where it is
+  // one value; s_t x_t where not
+  const void* w;
+  int64_t ldw;
   const float* lse;
   const float* loss;
   const float* dloss;
   float4* rowc;
+  float* s;
+  int* far;  // of each workgroup: whether a row of its own is far
   float* alpha;
   void* xs;
   int reduction;
@@ -76,6 +95,7 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs a) {
   __shared__ int red[4];
   __shared__ int list[256];
   __shared__ float scale[256];
+  __shared__ float2 stat[256];  // log-sum-exp, loss
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int r0 = blockIdx.x * a.per, r1 = min(r0 + a.per, a.T);
   // kept rows before this workgroup's, and (backward, for the mean) behind them
@@ -108,6 +128,7 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs a) {
                 : total ? a.dloss[0] / (float)total : 0.f;  // no rows: no gradients
     if (blockIdx.x == 0 && tid == 0) *a.alpha = row_scale;
   }
+  bool far = false;
   for (int c0 = r0; c0 < r1; c0 += 256) {
     const int r = c0 + tid;
     const int64_t t = r < r1 ? a.target[r] : a.ignore;
@@ -128,9 +149,12 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs a) {
       if (a.rowc) {
         const float s = a.reduction == PNFX_REDUCE_NONE ? a.dloss[r] : row_scale;
         // a target that is no token: its loss is NaN, and so are its gradients
-        a.rowc[i] = float4{valid ? a.lse[r] : __builtin_nanf(""), s, expm1f(-a.loss[r]),
-                           __int_as_float(valid ? (int)t : -1)};
+        const float lse = valid ? a.lse[r] : __builtin_nanf(""), loss = a.loss[r];
+        a.rowc[i] = float4{lse, 0.f, expm1f(-loss), __int_as_float(valid ? (int)t : -1)};
+        a.s[i] = s;
+        far |= fabsf(lse) > kFarLse<T>;
         scale[at] = s;
+        stat[at] = float2{lse, loss};
       }
     }
     if (r < r1) a.pos[r] = keep ? before + at : -1;
@@ -161,7 +185,20 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs a) {
         }
       }
     }
+    if (a.rowc) {  // seldom: far rows (a target that is no token has a NaN here, and is not far)
+      for (int i = wave; i < n; i += 4) {
+        const float lse = stat[i].x, loss = stat[i].y;
+        if (!(fabsf(lse) > kFarLse<T> && loss < 0.5f * fabsf(lse))) continue;
+        const float dot = wave_sum(dot_part<1>(static_cast<const T*>(a.x) + (int64_t)list[i] * a.x_rs,
+                                               static_cast<const T*>(a.w) + a.target[list[i]] * a.ldw, a.D, lane));
+        if (lane == 0) a.rowc[before + i].y = ((dot - lse) + loss) * kLog2e;
+      }
+    }
     before += n;
+  }
+  if (a.rowc) {
+    far = block_sum(far) != 0;
+    if (tid == 0) a.far[blockIdx.x] = far;
   }
   if (r1 == a.T && tid == 0) *a.count = before;
 }
@@ -213,7 +250,9 @@ __global__ __launch_bounds__(threads_of<C>, 2) void xent_fwd_kernel(FwdArgs a) {
   const int t0 = split * a.per, tiles = min(a.tn - t0, a.per);
   const auto pass = [&](auto far) {
     constexpr bool FAR = decltype(far)::value;
-    // the second pass works its addresses out anew: kept over the first one's loop they were 13 spilled registers
+    // The second pass takes the loop over k (the same sums) and works its addresses out anew: with A's fragments in
+    // registers, or its addresses kept over the first pass's loop, it spilled.
+    typedef Tiles<T, C, FAR ? 0 : KS, 0> P;
     int tid = threadIdx.x;
     if (FAR) asm volatile("" : "+v"(tid));
     const int lane = tid & 63;
@@ -254,6 +293,7 @@ __global__ __launch_bounds__(threads_of<C>, 2) void xent_fwd_kernel(FwdArgs a) {
             for (int r = 0; r < 4; ++r) s += exp2_fast((acc[i][j][r] - ref) * kLog2e);
           top[i] = next;
           sum[i] = s;
+          __builtin_amdgcn_sched_barrier(0);
           continue;
         }
         // The reference follows the maximum only once it is 8 behind (the exponentials stay below e^8), which after the
@@ -273,6 +313,7 @@ __global__ __launch_bounds__(threads_of<C>, 2) void xent_fwd_kernel(FwdArgs a) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) s += exp2_fast(__builtin_fmaf(acc[i][j][r], kLog2e, -c));
         sum[i] = s;
+        if (KS == 4) __builtin_amdgcn_sched_barrier(0);  // one row block at a time (285 against 277 us at the size above)
       }
     });
   };
@@ -282,14 +323,13 @@ __global__ __launch_bounds__(threads_of<C>, 2) void xent_fwd_kernel(FwdArgs a) {
   for (int i = 0; i < P::MI; ++i) far |= !(sum[i] < INFINITY) || (fabsf(top[i]) > kFarTop && top[i] != -INFINITY);
   // (the loop's last barrier has left the LDS free)
   int* const votes = reinterpret_cast<int*>(sm);
-  if (lane == 0) votes[wave] = 0;
-  if (far) votes[wave] = 1;
+  far = __any(far);
+  if (lane == 0) votes[wave] = far;
   __syncthreads();
-  far = false;
 #pragma unroll
   for (int v = 0; v < C::WM * C::WN; ++v) far |= votes[v] != 0;
-  __syncthreads();
   if (far) {
+    __syncthreads();
     pass(std::true_type{});
   } else {
 #pragma unroll
@@ -336,12 +376,8 @@ __global__ __launch_bounds__(256) void xent_loss_kernel(LossArgs a) {
       }
       const int t = a.tgt[i];
       float dot = 0.f;
-      if (t >= 0) {
-        const T* x = static_cast<const T*>(a.xc) + i * a.ldx;
-        const T* w = static_cast<const T*>(a.w) + t * a.ldw;
-#pragma unroll 8
-        for (int k = lane; k < a.K; k += 64) dot = __builtin_fmaf(to_f32(x[k]), to_f32(w[k]), dot);
-      }
+      if (t >= 0)
+        dot = dot_part<8>(static_cast<const T*>(a.xc) + i * a.ldx, static_cast<const T*>(a.w) + t * a.ldw, a.K, lane);
       const float m = wave_max(top), ref = m == -INFINITY ? 0.f : m;
       sum = wave_sum(sum * exp2_fast((top - ref) * kLog2e));
       dot = wave_sum(dot);
@@ -388,6 +424,15 @@ struct GradArgs {
   int v0, P, tn, splits, per;  // the piece's first token, its tokens; column tiles of a workgroup
 };
 
+// Whether one of the wave's N rows from m0 on (of M) is far.
+template <typename T, int N>
+__device__ __forceinline__ bool any_far(const float4* rowc, int m0, int M, int lane) {
+  bool far = false;
+#pragma unroll
+  for (int r = 0; r < N; r += 64) far |= fabsf(rowc[min(m0 + r + lane, M - 1)].x) > kFarLse<T>;
+  return __any(far);
+}
+
 __device__ __forceinline__ void store16(__amdgpu_buffer_rsrc_t d, unsigned at, u32x4 v) {
   __builtin_amdgcn_raw_buffer_store_b128(v, d, at, 0, 0);
 }
@@ -406,15 +451,16 @@ __global__ __launch_bounds__(threads_of<C>, 2) void xent_grad_kernel(GradArgs a)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave / C::WN * P::MI, wn = wave % C::WN * P::NJ;
   const int Pc = (a.P + 7) & ~7;  // columns past the piece, up to a whole chunk, are zero
-  // of each row its log-sum-exp times log2 e, its target's column in the piece, if it has one there, and its target's
-  // element of d (in LDS: there are no registers left for them beside A's fragments, and a read from global memory waits
-  // for every load and store on its way); published by the loop's first barrier
+  // of each row its log-sum-exp, its target's column in the piece, if it has one there, its target's element of d, and the
+  // rest of the log-sum-exp (in LDS: there are no registers left for them beside A's fragments, and a read from global
+  // memory waits for every load and store on its way); published by the loop's first barrier
   __shared__ float4 rows[C::TM];
   for (int r = threadIdx.x; r < C::TM; r += threads_of<C>) {
     const int m = min(m0 + r, M - 1);
     const float4 c = a.rowc[m];
-    rows[r] = float4{c.x * kLog2e, __int_as_float(a.tgt[m] - a.v0), c.z, 0.f};
+    rows[r] = float4{c.x, __int_as_float(a.tgt[m] - a.v0), c.z, c.y};
   }
+  const bool far = any_far<T, C::TM / C::WM>(a.rowc, m0 + 16 * wm, M, lane);
   const auto out = __builtin_amdgcn_make_buffer_rsrc(static_cast<T*>(a.d) + m0 * a.ldd, 0,
                                                      (int)(min(M - m0, C::TM) * a.ldd * sizeof(T)), 0x00027000);
   const unsigned ldb = (unsigned)(a.ldd * sizeof(T)), row = stage_row<ROW>(wm, lane & 15) * ldb;
@@ -433,11 +479,19 @@ __global__ __launch_bounds__(threads_of<C>, 2) void xent_grad_kernel(GradArgs a)
     for (int i = 0; i < P::MI; ++i) {
       const float4& row4 = rows[stage_row<ROW>(wm + i, lane & 15)];
       const float2 c{row4.x, row4.y};
+      float l = c.x * kLog2e;
+      if (far) {
+#pragma unroll
+        for (int j = 0; j < P::NJ; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][j][r] -= c.x;
+        l = row4.w;
+      }
 #pragma unroll
       for (int j = 0; j < P::NJ; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          acc[i][j][r] = exp2_fast(__builtin_fmaf(acc[i][j][r], kLog2e, -c.x));
+          acc[i][j][r] = exp2_fast(__builtin_fmaf(acc[i][j][r], kLog2e, -l));
       // 16 bytes at a time; the buffer's bounds drop the rows past M, a far offset the columns past the piece
       const unsigned at = row + stage_row<ROW>(i, 0) * ldb + nl * (unsigned)sizeof(T);
 #pragma unroll
@@ -484,10 +538,11 @@ struct NarrowArgs {
   const void* b;    // tiles, of ldb
   float* sums;      // [splits][M][N]: of a's rows
   const float4* rowc;
-  const int *tgt, *count;
+  const int *tgt, *count, *far;
   int64_t lda, ldb, K;
   int M, N, nb;     // rows of a and columns of the result (all of the array's); rows of b
   int V, splits, per;
+  int blocks;       // of far
 };
 template <bool DW>
 __global__ __launch_bounds__(256, 2) void xent_narrow_kernel(NarrowArgs a) {
@@ -521,8 +576,16 @@ __global__ __launch_bounds__(256, 2) void xent_narrow_kernel(NarrowArgs a) {
     };
     constexpr int NI = St::NI + (DW ? 1 : 0);
     sa.load(la, wave);
+    // whether any row is far, which takes another loop (a branch in the one for the others cost them up to 4 %)
+    bool far = false;
+    for (int b = threadIdx.x; b < a.blocks; b += 256) far |= a.far[b] != 0;
+    int* const votes = reinterpret_cast<int*>(cols);
+    far = __any(far);
+    if (lane == 0) votes[wave] = far;
     wait_vm_lgkm<0>();
-    __builtin_amdgcn_s_barrier();
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < 4; ++v) far |= votes[v] != 0;
     bf16x8 fa[2][4];
     {
       const Frags<bf16, ROW> f(sm + wm * 64 * 64, lane);
@@ -532,14 +595,14 @@ __global__ __launch_bounds__(256, 2) void xent_narrow_kernel(NarrowArgs a) {
         for (int i = 0; i < 4; ++i) fa[hf][i] = f.get(i, hf, 0);
     }
     wait_vm_lgkm<0>();
-    __builtin_amdgcn_s_barrier();
-    // dx: each row's log-sum-exp times log2 e, its target as a column of the first tile, and the target's element;
-    // published by the loop's first barrier
+    __syncthreads();
+    // dx: each row's log-sum-exp, its target as a column of the first tile, the target's element, and the rest of the
+    // log-sum-exp; published by the loop's first barrier
     if constexpr (!DW) {
       if (threadIdx.x < 128) {
         const int m = min(m0 + (int)threadIdx.x, rows - 1);
         const float4 c = a.rowc[m];
-        rowl[threadIdx.x] = float4{c.x * kLog2e, __int_as_float(a.tgt[m] - t0 * 128), c.z, 0.f};
+        rowl[threadIdx.x] = float4{c.x, __int_as_float(a.tgt[m] - t0 * 128), c.z, c.y};
       }
       wait_vm_lgkm<0>();
     }
@@ -548,100 +611,107 @@ __global__ __launch_bounds__(256, 2) void xent_narrow_kernel(NarrowArgs a) {
     load(0);
     if (tiles > 1) load(1);
     if (tiles > 2) load(2);
-    for (int t = 0; t < tiles; ++t) {
-      const int buf = t % RING;
-      if (t + 2 < tiles) wait_vm_lgkm<2 * NI>();
-      else wait_vm_lgkm<0>();
-      __builtin_amdgcn_s_barrier();
-      if (t + 3 < tiles) load(t + 3);
-      __builtin_amdgcn_sched_barrier(0);
-      f32x4 z[4][4];
+    const auto loop = [&](auto far) {
+      constexpr bool FAR = decltype(far)::value;
+      for (int t = 0; t < tiles; ++t) {
+        const int buf = t % RING;
+        if (t + 2 < tiles) wait_vm_lgkm<2 * NI>();
+        else wait_vm_lgkm<0>();
+        __builtin_amdgcn_s_barrier();
+        if (t + 3 < tiles) load(t + 3);
+        __builtin_amdgcn_sched_barrier(0);
+        f32x4 z[4][4];
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        bf16x8 b[4];
+        for (int hf = 0; hf < 2; ++hf) {
+          bf16x8 b[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) b[j] = fb.get(j, hf, buf * SB);
+          for (int j = 0; j < 4; ++j) b[j] = fb.get(j, hf, buf * SB);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) z[i][j] = mma(b[j], fa[hf][i], hf ? z[i][j] : f32x4{});
-      }
-      const auto col = [](int j) { return stage_row<ROW>(j, 0); };  // block j's first column of the lane's
-      const float4* const c = cols + (buf * 4 + wave) * 64;
-      // Seldom a target's own element is among the wave's: which of its blocks have one.
-      if constexpr (DW) {
-        // (the log-sum-exps of the lane's 16 columns)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float l = c[8 * g + col(j) + r].x * kLog2e;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) z[i][j][r] = exp2_fast(__builtin_fmaf(z[i][j][r], kLog2e, -l));
-          }
-        const uint64_t hits = __ballot((unsigned)(__float_as_int(c[lane].w) - m0 - 64 * wm) < 64u);
-        if (hits) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (!(hits >> col(j) & 0x0f0f0f0fu)) continue;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float4 e = c[8 * g + col(j) + r];
-              const int own = __float_as_int(e.w) - m0 - 64 * wm;
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (own == stage_row<ROW>(i, r16)) z[i][j][r] = e.z;
-            }
-          }
+            for (int j = 0; j < 4; ++j) z[i][j] = mma(b[j], fa[hf][i], hf ? z[i][j] : f32x4{});
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float4& c = rowl[stage_row<ROW>(4 * wm + i, r16)];
-          const float l = c.x;
-          const int at = __float_as_int(c.y) - 128 * t - 64 * wn - 8 * g;
+        const auto col = [](int j) { return stage_row<ROW>(j, 0); };  // block j's first column of the lane's
+        const float4* const c = cols + (buf * 4 + wave) * 64;
+        // Seldom a target's own element is among the wave's: which of its blocks have one.
+        if constexpr (DW) {
+          // (the log-sum-exps of the lane's 16 columns)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) z[i][j][r] = exp2_fast(__builtin_fmaf(z[i][j][r], kLog2e, -l));
-          if (__any((unsigned)at < 40u)) {
-            const float own = c.z;
+            for (int r = 0; r < 4; ++r) {
+              const float4& c4 = c[8 * g + col(j) + r];
+              const float lse = c4.x, l = FAR ? c4.y : lse * kLog2e;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) z[i][j][r] = exp2_fast(__builtin_fmaf(FAR ? z[i][j][r] - lse : z[i][j][r], kLog2e, -l));
+            }
+          const uint64_t hits = __ballot((unsigned)(__float_as_int(c[lane].w) - m0 - 64 * wm) < 64u);
+          if (hits) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (!(hits >> col(j) & 0x0f0f0f0fu)) continue;
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const float4 e = c[8 * g + col(j) + r];
+                const int own = __float_as_int(e.w) - m0 - 64 * wm;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if (own == stage_row<ROW>(i, r16)) z[i][j][r] = e.z;
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4& c = rowl[stage_row<ROW>(4 * wm + i, r16)];
+            const float lse = c.x, l = FAR ? c.w : lse * kLog2e;
+            const int at = __float_as_int(c.y) - 128 * t - 64 * wn - 8 * g;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
               for (int r = 0; r < 4; ++r)
-                if (at == col(j) + r) z[i][j][r] = own;
+                z[i][j][r] = exp2_fast(__builtin_fmaf(FAR ? z[i][j][r] - lse : z[i][j][r], kLog2e, -l));
+            if (__any((unsigned)at < 40u)) {
+              const float own = c.z;
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  if (at == col(j) + r) z[i][j][r] = own;
+            }
           }
         }
-      }
-      if (!DW && (t0 + t + 1) * 128 > a.V) {  // tokens past the vocabulary: of zero weights, but not finite perhaps
-        const int n0 = (t0 + t) * 128 + 64 * wn + 8 * g;
+        if (!DW && (t0 + t + 1) * 128 > a.V) {  // tokens past the vocabulary: of zero weights, but not finite perhaps
+          const int n0 = (t0 + t) * 128 + 64 * wn + 8 * g;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+          for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (n0 + col(j) + r >= a.V) {
+            for (int r = 0; r < 4; ++r)
+              if (n0 + col(j) + r >= a.V) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) z[i][j][r] = 0.f;
-            }
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      // two blocks: the lane's eight consecutive columns, a fragment of the next product
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        bf16x8 b[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) b[j] = ft.get(j, h, buf * SB);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x4 u = z[i][2 * h], v = z[i][2 * h + 1];
-          const bf16x8 p = pack8(u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) out[i][j] = mma(b[j], p, out[i][j]);
+                for (int i = 0; i < 4; ++i) z[i][j][r] = 0.f;
+              }
         }
+        __builtin_amdgcn_sched_barrier(0);
+        // two blocks: the lane's eight consecutive columns, a fragment of the next product
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          bf16x8 b[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) b[j] = ft.get(j, h, buf * SB);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const f32x4 u = z[i][2 * h], v = z[i][2 * h + 1];
+            const bf16x8 p = pack8(u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out[i][j] = mma(b[j], p, out[i][j]);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
-    }
+    };
+    if (far) loop(std::true_type{});
+    else loop(std::false_type{});
     wait_vm_lgkm<0>();
   }
   // the two waves of a row share its columns of the tiles: their sums are added, half of them by each
@@ -672,7 +742,7 @@ constexpr int kNarrowLds[2] = {4 * 128 * 128 + 128 * 16, 4 * 128 * 128 + 4 * 4 *
 
 struct DxArgs {
   const float* sums;  // [splits][T][D]
-  const float4* rowc;
+  const float* s;     // [kept]
   const int* pos;
   void* dx;           // [T][D]
   int64_t TD;
@@ -691,14 +761,14 @@ __global__ __launch_bounds__(256) void xent_dx_kernel(DxArgs a) {
     f32x4 v = {};
     if (i >= 0)
       for (int p = 0; p < a.splits; ++p) v += *reinterpret_cast<const f32x4*>(s + p * a.TD);
-    if (i >= 0) v *= a.rowc[i].y;
+    if (i >= 0) v *= a.s[i];
     if constexpr (sizeof(T) == 2) *reinterpret_cast<bf16x4*>(dx) = bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
     else *reinterpret_cast<f32x4*>(dx) = v;
   } else {
     float v = 0.f;
     if (i >= 0)
       for (int p = 0; p < a.splits; ++p) v += s[p * a.TD];
-    if (i >= 0) v *= a.rowc[i].y;
+    if (i >= 0) v *= a.s[i];
     *dx = from_f32<T>(v);
   }
 }
@@ -836,12 +906,16 @@ int64_t bwd_bytes(const Sizes& z, int reduction, bool copy) {
   take_kept(ar, z, copy);
   if (narrow(z, reduction)) {
     ar.take<float>(1);
+    ar.take<float>(z.T);
+    ar.take<int>(kRowsBlocks);
     ar.take<float4>(z.T);
     ar.take<float>(narrow_cut(z.T, ceil_div(z.V, 128), z.D).splits * z.T * z.D);
     ar.take<float>(narrow_cut(z.V, ceil_div(z.T, 128), z.D).splits * z.V * z.D);
     return ar.used;
   }
   ar.take<float>(1);
+  ar.take<float>(z.T);
+  ar.take<int>(kRowsBlocks);
   ar.take<char>(z.T * z.Dp * z.es);  // s x, of a loss per row
   const BwdCut c = bwd_cut(z);
   ar.take<float4>(z.T);
@@ -851,15 +925,19 @@ int64_t bwd_bytes(const Sizes& z, int reduction, bool copy) {
   return ar.used;
 }
 
+// Workgroups of xent_rows_kernel and their rows.
+int64_t rows_per(const Sizes& z) { return std::max<int64_t>(4, ceil_div(z.T, kRowsBlocks)); }
+int64_t rows_blocks(const Sizes& z) { return ceil_div(z.T, rows_per(z)); }
+
 template <typename T>
 int keep_rows(const Kept& k, const void* x, int64_t x_rs, const int64_t* target, int64_t ignore, const Sizes& z,
               RowsArgs a, hipStream_t st) {
   a.x = x, a.target = target, a.xc = k.xc, a.pos = k.pos, a.src = k.src, a.tgt = k.tgt, a.count = k.count;
   a.x_rs = x_rs, a.ignore = ignore;
   a.T = (int)z.T, a.D = (int)z.D, a.Dp = (int)z.Dp, a.V = (int)z.V;
-  a.per = (int)std::max<int64_t>(4, ceil_div(z.T, kRowsBlocks));
+  a.per = (int)rows_per(z);
   a.vec = z.D == z.Dp && operand_ok(x, x_rs, z.es);
-  return launch<xent_rows_kernel<T>>(ceil_div(z.T, a.per), 256, 0, a, st, "xent rows");
+  return launch<xent_rows_kernel<T>>(rows_blocks(z), 256, 0, a, st, "xent rows");
 }
 // W in place, or its padded copy.
 int take_w(const Kept& k, const void*& w, int64_t& w_rs, const Sizes& z, hipStream_t st) {
@@ -904,6 +982,8 @@ int xent_bwd(const float* dloss, const void* x, int64_t x_rs, const void* w, int
   RowsArgs r = {};
   r.lse = lse, r.loss = rows, r.dloss = dloss, r.reduction = reduction;
   r.alpha = ar.take<float>(1);
+  r.s = ar.take<float>(z.T);
+  r.far = ar.take<int>(kRowsBlocks);
   if constexpr (sizeof(T) == 2) {
     if (narrow(z, reduction)) {
       r.rowc = ar.take<float4>(z.T);
@@ -911,17 +991,18 @@ int xent_bwd(const float* dloss, const void* x, int64_t x_rs, const void* w, int
       float* sx = ar.take<float>(cx.splits * z.T * z.D);
       float* sw = ar.take<float>(cw.splits * z.V * z.D);
       PNFX_TRY(take_w(k, w, w_rs, z, st));
+      r.w = w, r.ldw = w_rs;
       PNFX_TRY(keep_rows<T>(k, x, x_rs, target, ignore, z, r, st));
       if (dx) {
-        const NarrowArgs n{k.xc, w, sx, r.rowc, k.tgt, k.count, z.Dp, w_rs, z.Dp, (int)z.T, (int)z.D, (int)z.V, (int)z.V,
-                           (int)cx.splits, (int)cx.per};
+        const NarrowArgs n{k.xc, w, sx, r.rowc, k.tgt, k.count, r.far, z.Dp, w_rs, z.Dp, (int)z.T, (int)z.D, (int)z.V,
+                           (int)z.V, (int)cx.splits, (int)cx.per, (int)rows_blocks(z)};
         PNFX_TRY((launch<xent_narrow_kernel<false>>(ceil_div(z.T, 128) * cx.splits, 256, kNarrowLds[0], n, st, "xent_dx")));
-        const DxArgs x1{sx, r.rowc, k.pos, dx, z.T * z.D, (int)z.D, (int)cx.splits};
+        const DxArgs x1{sx, r.s, k.pos, dx, z.T * z.D, (int)z.D, (int)cx.splits};
         PNFX_TRY((launch<xent_dx_kernel<T>>(ceil_div(x1.TD, z.D % 4 == 0 ? 1024 : 256), 256, 0, x1, st, "xent_dx")));
       }
       if (dw) {
-        const NarrowArgs n{w, k.xc, sw, r.rowc, k.tgt, k.count, w_rs, z.Dp, z.Dp, (int)z.V, (int)z.D, (int)z.T, (int)z.V,
-                           (int)cw.splits, (int)cw.per};
+        const NarrowArgs n{w, k.xc, sw, r.rowc, k.tgt, k.count, r.far, w_rs, z.Dp, z.Dp, (int)z.V, (int)z.D, (int)z.T,
+                           (int)z.V, (int)cw.splits, (int)cw.per, (int)rows_blocks(z)};
         PNFX_TRY((launch<xent_narrow_kernel<true>>(ceil_div(z.V, 128) * cw.splits, 256, kNarrowLds[1], n, st, "xent_dw")));
         PNFX_TRY(sum_splits(sw, (int)cw.splits, z.V, z.D, dw, r.alpha, z.dtype, st));
       }
@@ -936,6 +1017,7 @@ int xent_bwd(const float* dloss, const void* x, int64_t x_rs, const void* w, int
   float* sums = ar.take<float>(c.dx.splits * z.T * z.D);
   void* dw_ws = ar.take<char>(product_workspace(c.dw, c.P, z.D));
   PNFX_TRY(take_w(k, w, w_rs, z, st));
+  r.w = w, r.ldw = w_rs;
   PNFX_TRY(keep_rows<T>(k, x, x_rs, target, ignore, z, r, st));
   for (int64_t v0 = 0; v0 < z.V; v0 += c.P) {
     const int64_t n = std::min(c.P, z.V - v0);
@@ -970,7 +1052,7 @@ int xent_bwd(const float* dloss, const void* x, int64_t x_rs, const void* w, int
     if (nj) PNFX_TRY(products(jobs, nj, z.dtype, st));
   }
   if (!dx) return PNFX_OK;
-  const DxArgs x1{sums, r.rowc, k.pos, dx, z.T * z.D, (int)z.D, c.dx.splits};
+  const DxArgs x1{sums, r.s, k.pos, dx, z.T * z.D, (int)z.D, c.dx.splits};
   return launch<xent_dx_kernel<T>>(ceil_div(x1.TD, z.D % 4 == 0 ? 1024 : 256), 256, 0, x1, st, "xent_dx");
 }
 
