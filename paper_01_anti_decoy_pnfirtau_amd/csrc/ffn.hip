@@ -121,6 +121,17 @@ __global__ __launch_bounds__(threads_of<C>, 2) void glu_fwd_kernel(GluArgs a) {
   f32x4 acc[P::MI][P::NJ] = {};
   P::run(sa, sb, (int)((a.K + k_step<T> - 1) / k_step<T>), reinterpret_cast<T*>(sm), wave, lane, acc);
   const int wm = wave / C::WN * P::MI, wn = wave % C::WN * P::NJ, ag = lane >> 4;
+  // columns past F are of zero weights: zero for any x, an infinite one too
+  if (f0 + C::TN / 2 > a.F) {
+#pragma unroll
+    for (int j = 0; j < P::NJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (f0 + 32 * ((wn + j) / 4) + 8 * ag + 4 * (j & 1) + r >= a.F) {
+#pragma unroll
+          for (int i = 0; i < P::MI; ++i) acc[i][j][r] = 0.f;
+        }
+  }
 #pragma unroll
   for (int i = 0; i < P::MI; ++i) {
     const int m = m0 + stage_row<ROW>(wm + i, lane & 15);
@@ -144,7 +155,7 @@ __global__ __launch_bounds__(threads_of<C>, 2) void glu_fwd_kernel(GluArgs a) {
           store8(static_cast<float*>(a.gu) + at + a.Fp, u);
         }
       } else {
-        // columns past F are zero and change no maximum
+        // columns past F change no maximum
         const float tg = block_top(g), tu = block_top(u);
         const bool half = a.keep == PNFX_KEEP_FULL;
         const int eg = half ? half_exp(tg) : scale_exp(tg), eu = half ? half_exp(tu) : scale_exp(tu);
@@ -401,7 +412,8 @@ __global__ __launch_bounds__((64 * FewRows<PAIRED, MB>::W), 2) void ffn_rows_ker
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int n = n0 + 4 * g + r;
-      if (n < a.cols) y[n] = from_f32<T>(PAIRED ? act_of<ACT>(acc[0][b][r]) * acc[NM - 1][b][r] : acc[0][b][r]);
+      const float v = PAIRED ? act_of<ACT>(acc[0][b][r]) * acc[NM - 1][b][r] : acc[0][b][r];
+      if (n < a.cols) y[n] = from_f32<T>(n < a.N ? v : 0.f);  // (zero weights past N, but x may be infinite)
     }
   }
 }
