@@ -1,15 +1,16 @@
-"""The gated feed-forward block where padding meets infinities."""
+"""The gated feed-forward block where padding meets infinities, and the tails of its activations in full precision."""
 import math
 
 import pytest
 import torch
 
-from paper_01_anti_decoy_pnfirtau_amd import ops  # noqa: F401  (loads the ops)
+from paper_01_anti_decoy_pnfirtau_amd import gated_ffn, ops  # noqa: F401  (loads the ops)
 from paper_01_anti_decoy_pnfirtau_amd._lib import PNFX_ACT, PNFX_KEEP
 from tests.helpers import seeded
 
 pytestmark = pytest.mark.gpu
 
+E = 2.0 ** -24
 BF16, F32 = torch.bfloat16, torch.float32
 
 
@@ -31,3 +32,21 @@ def test_infinite_rows_over_padded_columns(dev, T, D, F, dtype, keep, act):
     assert torch.equal(y[rest], ref[rest])
     if keep != "none":
         assert not bool((gu[:, :, F:].float() != 0).any())  # (NaN is not zero)
+
+
+def test_gelu_tails_in_full_precision(dev):
+    """g Phi(g) and its slope in fp32 keep their digits far out: 16 roundings, and those of g^2 in the exponent."""
+    g = torch.cat([torch.linspace(-12, 12, 4001), torch.logspace(-6, 1, 200), -torch.logspace(-6, 1, 200)]).to(dev)
+    x = torch.stack([g, torch.ones_like(g)], 1).requires_grad_()
+    w_in, w_down = torch.eye(2, device=dev), torch.ones(1, 1, device=dev)  # gate g, up projection 1
+    y = gated_ffn(x, w_in, w_down, "gelu")
+    dx = torch.autograd.grad(y.sum(), x)[0][:, 0]
+    v = g.double()
+    cdf, rest = torch.special.erfc(-v * 0.5 ** 0.5) / 2, v * torch.exp(-v * v / 2) / math.sqrt(2 * math.pi)
+    rel = E * (16 + 4 * v * v)
+    for got, want, size in ((y[:, 0].detach(), v * cdf, (v * cdf).abs()), (dx, cdf + rest, cdf + rest.abs())):
+        over = (got.double() - want).abs() - rel * size - 2.0 ** -126
+        assert bool((over <= 0).all()), (float(over.max()), float(v[over.argmax()]))
+    with torch.no_grad():  # the kernel of few rows
+        few = gated_ffn(x[1000:1040], w_in, w_down, "gelu")
+    assert bool(((few[:, 0].double() - (v * cdf)[1000:1040]).abs() <= (rel * (v * cdf).abs())[1000:1040] + 2.0 ** -126).all())
