@@ -82,7 +82,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     Returns fp32: one value ("mean" over the rows that are not ignored, "sum") or target's shape ("none").
     Rows whose target is ``ignore_index`` cost nothing, have loss and gradient 0 and, whatever they hold,
     reach no other result.  Another target outside 0 .. V - 1 makes its row's loss and gradients NaN (the
-    host is never made to wait for a check).  Logits, maxima and sums are fp32; the gradient of the
+    host is never made to wait for a check; CPU tensors raise an IndexError).  Logits, maxima and sums are fp32; the gradient of the
     logits is rounded to x's type for the products with weight and x.  Before that its softmax is off by 2^-13
     at most, relative (fp32 operands: 2^-18), or by 2^-23 of a row's loss or log-sum-exp where the smaller of the two is
     larger than 1024 (32).  The memory beside the gradients is a
@@ -94,6 +94,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     x, weight = _autocast(x, weight)
     if not x.is_cuda:
         V = weight.shape[0]
+        x = torch.where((target != ignore_index).unsqueeze(-1), x, 0)  # what ignored rows hold reaches dW otherwise
         loss = F.cross_entropy(F.linear(x, weight).reshape(-1, V).float(), target.reshape(-1),
                                ignore_index=ignore_index, reduction=reduction)
         return loss.view(target.shape) if reduction == "none" else loss
