@@ -69,7 +69,6 @@ struct RowsArgs {
   const int64_t* target;
   void* xc;         // [T][Dp] kept rows, zero-padded
   int* pos;         // [T] place of a row among the kept ones, or -1
-  int* src;         // [kept] row
   int* tgt;         // [kept] target, or -1 where it is no token
   int* count;
   int64_t x_rs, ignore;
@@ -144,7 +143,6 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(RowsArgs a) {
       const int i = before + at;
       const bool valid = t >= 0 && t < a.V;
       list[at] = r;
-      a.src[i] = r;
       a.tgt[i] = valid ? (int)t : -1;
       if (a.rowc) {
         const float s = a.reduction == PNFX_REDUCE_NONE ? a.dloss[r] : row_scale;
@@ -210,7 +208,7 @@ struct FwdArgs {
   float2* part;  // [T][splits * WN] running maximum and sum
   const int* count;
   int64_t ldx, ldw, K;
-  int T, V, tn, splits, per;  // per: vocabulary tiles of a split
+  int V, tn, splits, per;  // per: vocabulary tiles of a split
 };
 
 // The tiles' product: KS > 0: of that many steps of k at most, A's fragments in registers.
@@ -351,7 +349,7 @@ struct LossArgs {
   const void* xc;
   const void* w;
   const float2* part;
-  const int *pos, *tgt, *count;
+  const int *pos, *tgt;
   float *rows, *lse;   // [T] loss and log-sum-exp of every row (ignored: 0)
   float* out;          // reduction none: [T]
   double* sums;        // per workgroup
@@ -845,14 +843,13 @@ int by_width(bool big, const Sizes& z, Fn f) {
 
 struct Kept {
   void* xc;
-  int *pos, *src, *tgt, *count;
+  int *pos, *tgt, *count;
   void* w;  // padded copy, or null
 };
 Kept take_kept(Arena& ar, const Sizes& z, bool copy) {
   Kept k;
   k.xc = ar.take<char>(z.T * z.Dp * z.es);
   k.pos = ar.take<int>(z.T);
-  k.src = ar.take<int>(z.T);
   k.tgt = ar.take<int>(z.T);
   k.count = ar.take<int>(1);
   k.w = copy ? ar.take<char>(z.V * z.Dp * z.es) : nullptr;
@@ -916,7 +913,7 @@ int64_t bwd_bytes(const Sizes& z, int reduction, bool copy) {
   ar.take<float>(1);
   ar.take<float>(z.T);
   ar.take<int>(kRowsBlocks);
-  ar.take<char>(z.T * z.Dp * z.es);  // s x, of a loss per row
+  if (reduction == PNFX_REDUCE_NONE) ar.take<char>(z.T * z.Dp * z.es);  // s x
   const BwdCut c = bwd_cut(z);
   ar.take<float4>(z.T);
   ar.take<char>(z.T * c.P * z.es);
@@ -932,7 +929,7 @@ int64_t rows_blocks(const Sizes& z) { return ceil_div(z.T, rows_per(z)); }
 template <typename T>
 int keep_rows(const Kept& k, const void* x, int64_t x_rs, const int64_t* target, int64_t ignore, const Sizes& z,
               RowsArgs a, hipStream_t st) {
-  a.x = x, a.target = target, a.xc = k.xc, a.pos = k.pos, a.src = k.src, a.tgt = k.tgt, a.count = k.count;
+  a.x = x, a.target = target, a.xc = k.xc, a.pos = k.pos, a.tgt = k.tgt, a.count = k.count;
   a.x_rs = x_rs, a.ignore = ignore;
   a.T = (int)z.T, a.D = (int)z.D, a.Dp = (int)z.Dp, a.V = (int)z.V;
   a.per = (int)rows_per(z);
@@ -958,14 +955,14 @@ int xent_fwd(const void* x, int64_t x_rs, const void* w, int64_t w_rs, const int
   double* sums = ar.take<double>(loss_blocks(z));
   PNFX_TRY(take_w(k, w, w_rs, z, st));
   PNFX_TRY(keep_rows<T>(k, x, x_rs, target, ignore, z, RowsArgs{}, st));
-  FwdArgs f{k.xc, w, part, k.count, z.Dp, w_rs, z.Dp, (int)z.T, (int)z.V, (int)c.tn, (int)c.splits, (int)c.per};
+  FwdArgs f{k.xc, w, part, k.count, z.Dp, w_rs, z.Dp, (int)z.V, (int)c.tn, (int)c.splits, (int)c.per};
   const int wn = c.big ? Big::WN : Mid::WN;
   PNFX_TRY((by_width<T>(c.big, z, [&](auto cfg, auto ks) {
     typedef decltype(cfg) C;
     constexpr int KS = decltype(ks)::value;
     return launch<xent_fwd_kernel<T, C, KS>>(c.tm * c.splits, threads_of<C>, Tiles<T, C, KS, 0>::LDS, f, st, "xent_fwd");
   })));
-  LossArgs l{k.xc, w, part, k.pos, k.tgt, k.count, rows, lse, out, sums, z.Dp, w_rs,
+  LossArgs l{k.xc, w, part, k.pos, k.tgt, rows, lse, out, sums, z.Dp, w_rs,
              (int)z.T, (int)z.D, (int)c.splits * wn, reduction, loss_rows_per(z)};
   PNFX_TRY((launch<xent_loss_kernel<T>>(loss_blocks(z), 256, 0, l, st, "xent_loss")));
   if (reduction == PNFX_REDUCE_NONE) return PNFX_OK;
@@ -1010,8 +1007,7 @@ int xent_bwd(const float* dloss, const void* x, int64_t x_rs, const void* w, int
     }
   }
   const BwdCut c = bwd_cut(z);
-  void* xs = ar.take<char>(z.T * z.Dp * z.es);
-  if (reduction == PNFX_REDUCE_NONE) r.xs = xs;
+  if (reduction == PNFX_REDUCE_NONE) r.xs = ar.take<char>(z.T * z.Dp * z.es);
   r.rowc = ar.take<float4>(z.T);
   T* d = reinterpret_cast<T*>(ar.take<char>(z.T * c.P * z.es));
   float* sums = ar.take<float>(c.dx.splits * z.T * z.D);
@@ -1044,7 +1040,7 @@ int xent_bwd(const float* dloss, const void* x, int64_t x_rs, const void* w, int
     }
     if (dw) {
       ProductArgs p = {};
-      p.a = d, p.b = r.xs ? xs : k.xc, p.c = static_cast<T*>(dw) + v0 * z.D, p.lda = c.P, p.ldb = z.Dp, p.ldc = z.D;
+      p.a = d, p.b = r.xs ? r.xs : k.xc, p.c = static_cast<T*>(dw) + v0 * z.D, p.lda = c.P, p.ldb = z.Dp, p.ldc = z.D;
       p.M = n, p.N = z.D, p.K = z.T, p.k_count = k.count;
       p.alpha = r.xs ? nullptr : r.alpha;
       jobs[nj++] = Job{COL, COL, p, c.dw, dw_ws};

@@ -1,8 +1,10 @@
-"""The feed-forward block and the vocabulary cross entropy without a GPU: rows that are ignored."""
+"""The feed-forward block and the vocabulary cross entropy without a GPU: rows that are ignored, and the workspaces'
+sizes."""
 import pytest
 import torch
 
 import paper_01_anti_decoy_pnfirtau_amd as P
+from paper_01_anti_decoy_pnfirtau_amd import _lib
 
 
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
@@ -25,3 +27,19 @@ def test_ignored_rows_reach_nothing_on_cpu(reduction):
     for a, b in ((loss, ref), (dx[kept], rdx), (dw, rdw)):
         assert torch.allclose(a, b, rtol=1e-6, atol=1e-6)
     assert not bool(dx[~kept].any())
+
+
+@pytest.mark.parametrize("T,D,V,dtype", [(65536, 256, 65536, "bf16"), (16384, 256, 33278, "bf16"), (8192, 2048, 65536, "bf16"),
+                                         (65536, 256, 65536, "f32"), (16384, 512, 40001, "f32")])
+def test_cross_entropy_backward_workspace_is_a_piece_and_little_else(T, D, V, dtype):
+    """A piece of d (256 MB, or 2048 tokens), the kept rows, fp32 sums of the two gradients, of two splits at most at these
+    sizes, and a few words for each row: far from all of d.  A loss per row has the rows times their factors beside."""
+    es, code = (2, _lib.PNFX_BF16) if dtype == "bf16" else (4, _lib.PNFX_F32)
+    piece = max(256 << 20, 2048 * T * es)
+    copies = D % 8 != 0
+    mean, per_row = (_lib.lib().pnfx_xent_bwd_workspace_size(T, D, V, _lib.PNFX_REDUCE[r], copies, code) for r in ("mean", "none"))
+    tokens = piece // (T * es)
+    assert mean <= piece + T * D * es + 2 * T * D * 4 + 2 * tokens * D * 4 + 40 * T + 65536
+    assert mean < T * V * es / 2
+    assert per_row == mean + T * D * es
+    assert _lib.lib().pnfx_xent_bwd_workspace_size(T, D, V, _lib.PNFX_REDUCE["sum"], copies, code) == mean
