@@ -56,12 +56,14 @@ def gated_ffn(x: torch.Tensor, w_in: torch.Tensor, w_down: torch.Tensor, activat
     and h is rounded to x's type for the second product.  Any sizes and row strides; operands whose
     inner size is not a multiple of 8, or that are not 16-byte aligned, are copied first.
 
-    ``checkpoint``: how g and u are kept for the backward pass (nothing is kept when no gradient is
-    recorded).  "full": in fp32 for fp32 operands, else in 16 bits, half precision with a power of two
-    for each block of 32 columns (2^-11 at most beside g and u, relative).  "e4m3" (bf16 only): in 8 bits with
-    such scales, half the memory: 2^-4 at most beside g and u, relative, or 2^-10 of the block's scale.  The
-    gradients are those at the values that the kept ones stand for; y is the same.  The backward
-    is bitwise repeatable; second derivatives are refused.
+    ``checkpoint``: how g and u are kept for the backward pass.  "full": in fp32 for fp32 operands, else in
+    16 bits, half precision with a power of two for each block of 32 columns (2^-11 at most beside g and u, relative, or
+    2^-39 of the block's largest).  "e4m3": in 8 bits with such scales, half the memory: 2^-4 at most beside g and
+    u, relative, or 2^-10 of the block's scale; of bf16 operands, and a call that would have to keep fp32 ones
+    so is refused (ValueError).  Where the kernels keep nothing, as no gradient is recorded or the tensors are on the
+    CPU, both settings are taken and change nothing.  The gradients are those at the values that the kept ones
+    stand for; y is the same.  The backward is bitwise repeatable; second derivatives and tangents (forward mode) are
+    refused.
     """
     _one_of("activation", activation, ACTIVATIONS)
     _one_of("checkpoint", checkpoint, CHECKPOINTS)
@@ -87,8 +89,13 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     at most, relative (fp32 operands: 2^-18), or by 2^-23 of a row's loss or log-sum-exp where the smaller of the two is
     larger than 1024 (32).  The memory beside the gradients is a
     piece of the vocabulary's logits, 256 MB or 2048 tokens' worth (none for bf16 rows of up to 64 columns
-    and one loss value), and fp32 sums of the gradients.  Bitwise repeatable; second derivatives are
-    refused.
+    and one loss value), and fp32 sums of the gradients.  Bitwise repeatable; second derivatives
+    and tangents (forward mode) are refused.
+
+    In bf16 it is also the faster way (2 to 4 times F.linear and F.cross_entropy, training).  In fp32 the logits' second
+    product costs more than their memory traffic where the rows are few or the head is wide: 153 rows, D = 1952, 52097
+    tokens take 1670 us against 920, 4096 x 512 x 33278 4430 against 4000, 333 x 1000 x 50257 1230 against 1390; there
+    it is for logits that should not be in memory.
     """
     _one_of("reduction", reduction, REDUCTIONS)
     x, weight = _autocast(x, weight)

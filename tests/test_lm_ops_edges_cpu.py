@@ -1,5 +1,5 @@
-"""The feed-forward block and the vocabulary cross entropy without a GPU: rows that are ignored, and the workspaces'
-sizes."""
+"""The feed-forward block and the vocabulary cross entropy without a GPU: rows that are ignored, what is kept, the workspaces'
+sizes, and what the C ABI says of strides."""
 import pytest
 import torch
 
@@ -43,3 +43,24 @@ def test_cross_entropy_backward_workspace_is_a_piece_and_little_else(T, D, V, dt
     assert mean < T * V * es / 2
     assert per_row == mean + T * D * es
     assert _lib.lib().pnfx_xent_bwd_workspace_size(T, D, V, _lib.PNFX_REDUCE["sum"], copies, code) == mean
+
+
+def test_cpu_tensors_keep_what_torch_keeps():
+    """The CPU composition takes both checkpoint settings, which are the GPU kernel's, and gives the same gradients."""
+    g = torch.Generator().manual_seed(3)
+    for dtype in (torch.float32, torch.bfloat16):
+        leaves = [torch.randn(s, generator=g).to(dtype).requires_grad_() for s in ((5, 8), (12, 8), (7, 6))]
+        grads = [torch.autograd.grad(P.gated_ffn(*leaves, checkpoint=keep).sum(), leaves) for keep in ("full", "e4m3")]
+        assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_c_abi_names_bad_row_strides():
+    import ctypes
+
+    p, big, lib = ctypes.c_void_p(256), 1 << 40, _lib.lib()
+    assert lib.pnfx_ffn_fwd(p, 15, p, 16, p, 8, p, p, p, 4, 16, 8, 16, 0, 1, 1, p, big, None) == -1
+    assert b"row strides 15, 16, 8" in lib.pnfx_last_error()
+    assert lib.pnfx_ffn_bwd(p, 15, p, 16, p, 16, p, 8, p, p, p, p, p, 4, 16, 8, 16, 0, 1, 1, p, big, None) == -1
+    assert b"row strides 15, 16, 16, 8" in lib.pnfx_last_error()
+    assert lib.pnfx_xent_fwd(p, 8, p, 16, p, -100, p, p, p, 4, 16, 20, 2, 1, p, big, None) == -1
+    assert b"row strides 8, 16" in lib.pnfx_last_error()
