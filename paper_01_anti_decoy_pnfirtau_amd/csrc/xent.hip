@@ -10,14 +10,15 @@
 // running maximum and the sum of exponentials of what each lane has seen; xent_loss_kernel joins them.  The
 // target's logit is a dot product of its own.
 //
-// Backward: z is computed again for a piece of the vocabulary at a time (a piece's d, in the operands' type,
-// stays in the 256 MB last-level cache while both gradients read it) and d is written in place of the
-// logits; then dx += d W over the piece, in fp32, and the piece's rows of dW = d^T x.  bf16 operands: d is
-// rounded to bf16 once, 2^-8 of each of its elements at most, as it is an operand of bf16 products.  It is
-// rounded without s_t: the target's element, close to -1 for most rows, would otherwise be off by the same
-// amount in each of them, and a frequent token's sum with it (0.4 % where 1 / rows rounds badly).  s_t enters the
-// fp32 results where it is one value, and for a loss per row dx's rows and the x of dW = d^T (s x).  The target's
-// own element is expm1(-loss_t), which keeps its digits where the softmax is close to one.
+// Backward: z is computed again for a piece of the vocabulary at a time (whose d, in the operands' type, is 256 MB
+// or 2048 tokens' worth) and d is written in place of the logits; then dx += d W over the piece, in fp32, and
+// the piece's rows of dW = d^T x.  bf16 operands: d is rounded to bf16 once, 2^-8 of each of its elements at
+// most, as it is an operand of bf16 products.  It is rounded without s_t: the target's element, close to -1 for
+// most rows, would otherwise be off by the same amount in each of them, and a frequent token's sum with it (0.4 % where
+// 1 / rows rounds badly).  s_t enters the fp32 results where it is one value.  For a loss per row it enters dx's rows in
+// fp32 and the x of dW = d^T (s x), which is rounded to bf16 with it, 2^-8 once more: the sum over rows leaves no
+// place behind the product, and in d it would round the target's elements as above.  The target's own element is
+// expm1(-loss_t), which keeps its digits where the softmax is close to one.
 //
 // Exponentials are taken in base 2, exp2(z L - m L) with L = log2 e as one fma per logit.  In the forward the rounding
 // of m L is the same for a whole row and comes out again at its end, as the factor unround(m) = exp2(round(m L) - m L):
@@ -819,9 +820,11 @@ FwdCut fwd_cut(const Sizes& z) {
   c.splits = ceil_div(c.tn, c.per);
   return c;
 }
-// Tokens of a piece: 256 MB of d, the last-level cache's size.  Smaller pieces write and read dx's fp32 sums
-// more often and give the products fewer k or rows, larger ones leave the cache (16384 x 256 x 33278: 1681 us at 128 MB,
-// 1511 at 192, 1246 at 256, 1680 at 320; 8192 x 2048 x 65536: 5825, 5993, 5706, 5708).
+// Tokens of a piece: 256 MB of d.  Smaller pieces write and read dx's fp32 sums more often, larger ones take more memory;
+// in between the time goes by how well the piece's two products divide, and not by its size.  Training calls, us, by the
+// most that a piece may hold (MB): 16384 x 256 x 33278 128 1681, 160 1563, 192 1511, 224 1242, 256 1246, 320 1680, 384 1684,
+// where 224 and 256 are the same five pieces and the only ones for which cut_group takes 256-tiles; 8192 x 2048 x 65536, with
+// 256-tiles at each, 128 5825, 192 5993, 224 5855, 256 and 320, the same four pieces, 5706 and 5708, 384 5921.
 int64_t piece_of(const Sizes& z) {
   const int64_t most = std::min(round_up(std::max<int64_t>((256ll << 20) / (z.T * z.es), 2048), 256), kMaxLd / 2);
   const int64_t n = ceil_div(z.V, most);

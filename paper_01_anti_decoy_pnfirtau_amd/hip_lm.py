@@ -8,7 +8,8 @@
 Neither has a counterpart in the reference, whose model takes torch's two-layer FFN and cross entropy
 (experiments/exp4_wikitext2_lm.py:183-247, :334-348).  GPU tensors, bf16 or fp32, run the HIP kernels
 (``pnfx::gated_ffn``, ``pnfx::linear_xent``); CPU tensors the same composition of torch operations.
-Under autocast both compute in the autocast type, as ``nn.Linear`` does.
+Under autocast both compute in the autocast type, as ``nn.Linear`` does: the gradients of fp32 weights are
+rounded to it, too.
 """
 from __future__ import annotations
 
@@ -84,18 +85,18 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     Returns fp32: one value ("mean" over the rows that are not ignored, "sum") or target's shape ("none").
     Rows whose target is ``ignore_index`` cost nothing, have loss and gradient 0 and, whatever they hold,
     reach no other result.  Another target outside 0 .. V - 1 makes its row's loss and gradients NaN (the
-    host is never made to wait for a check; CPU tensors raise an IndexError).  Logits, maxima and sums are fp32; the gradient of the
-    logits is rounded to x's type for the products with weight and x.  Before that its softmax is off by 2^-13
-    at most, relative (fp32 operands: 2^-18), or by 2^-23 of a row's loss or log-sum-exp where the smaller of the two is
-    larger than 1024 (32).  The memory beside the gradients is a
-    piece of the vocabulary's logits, 256 MB or 2048 tokens' worth (none for bf16 rows of up to 64 columns
-    and one loss value), and fp32 sums of the gradients.  Bitwise repeatable; second derivatives
-    and tangents (forward mode) are refused.
+    host is never made to wait for a check; CPU tensors raise an IndexError).  Logits, maxima and sums are fp32;
+    the gradient of the logits is rounded to x's type for the products with weight and x.  Before that its
+    softmax is off by 2^-13 at most, relative (fp32 operands: 2^-18), beside the logits' own roundings, or by 2^-23 of a
+    row's loss or log-sum-exp where the smaller of the two is larger than 1024 (32).  The memory beside the
+    gradients is a piece of the vocabulary's logits, 256 MB or 2048 tokens' worth (none for bf16 rows of up to
+    64 columns and one loss value), and fp32 sums of the gradients.  Bitwise repeatable; second derivatives and
+    tangents (forward mode) are refused.
 
-    In bf16 it is also the faster way (2 to 4 times F.linear and F.cross_entropy, training).  In fp32 the logits' second
-    product costs more than their memory traffic where the rows are few or the head is wide: 153 rows, D = 1952, 52097
-    tokens take 1670 us against 920, 4096 x 512 x 33278 4430 against 4000, 333 x 1000 x 50257 1230 against 1390; there
-    it is for logits that should not be in memory.
+    In bf16 it is also the faster way (training 1.9 to 4.3 times F.linear and F.cross_entropy).  In fp32 the logits' second
+    product mostly costs more than their memory traffic: 153 rows, D = 1952, 52097 tokens take 1670 us against 920, 4096 x
+    512 x 33278 4430 against 4000, 333 x 1000 x 50257 1230 against 1390; there it is for logits that are not to be in
+    memory.
     """
     _one_of("reduction", reduction, REDUCTIONS)
     x, weight = _autocast(x, weight)
