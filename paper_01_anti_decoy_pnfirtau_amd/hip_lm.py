@@ -101,9 +101,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     _one_of("reduction", reduction, REDUCTIONS)
     x, weight = _autocast(x, weight)
     if not x.is_cuda:
-        V = weight.shape[0]
-        x = torch.where((target != ignore_index).unsqueeze(-1), x, 0)  # what ignored rows hold reaches dW otherwise
-        loss = F.cross_entropy(F.linear(x, weight).reshape(-1, V).float(), target.reshape(-1),
-                               ignore_index=ignore_index, reduction=reduction)
+        rows, to = x.reshape(-1, x.shape[-1]), target.reshape(-1)
+        rows = torch.where((to != ignore_index).unsqueeze(1), rows, 0)  # what ignored rows hold reaches dW otherwise
+        loss = F.cross_entropy(F.linear(rows, weight).float(), to, ignore_index=ignore_index, reduction=reduction)
         return loss.view(target.shape) if reduction == "none" else loss
     return _op("linear_xent")(x, weight, target, int(ignore_index), _lib.PNFX_REDUCE[reduction])[0]

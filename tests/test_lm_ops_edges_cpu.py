@@ -29,6 +29,16 @@ def test_ignored_rows_reach_nothing_on_cpu(reduction):
     assert not bool(dx[~kept].any())
 
 
+def test_cpu_tensors_take_flat_targets():
+    """The rows of [B, N, D] against B N targets in a row, as F.cross_entropy takes flattened logits."""
+    g = torch.Generator().manual_seed(4)
+    x, w, target = torch.randn(2, 5, 8, generator=g), torch.randn(11, 8, generator=g), torch.arange(10)
+    target[3] = -100
+    assert torch.equal(P.linear_cross_entropy(x, w, target), P.linear_cross_entropy(x, w, target.view(2, 5)))
+    assert P.linear_cross_entropy(x, w, target, reduction="none").shape == (10,)
+    assert float(P.linear_cross_entropy(x[:0], w, target[:0].view(0, 5), reduction="sum")) == 0.0
+
+
 @pytest.mark.parametrize("T,D,V,dtype", [(65536, 256, 65536, "bf16"), (16384, 256, 33278, "bf16"), (8192, 2048, 65536, "bf16"),
                                          (65536, 256, 65536, "f32"), (16384, 512, 40001, "f32")])
 def test_cross_entropy_backward_workspace_is_a_piece_and_little_else(T, D, V, dtype):
