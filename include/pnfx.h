@@ -354,6 +354,81 @@ int pnfx_xent_bwd(const float* dloss, const void* x, int64_t x_rs, const void* w
                   void* dx, void* dw, int64_t T, int64_t D, int64_t V, int reduction, int dtype,
                   void* workspace, int64_t workspace_bytes, void* stream);
 
+/*
+ * The 8-bit key and value cache, and attention over it.  No counterpart in the reference, which has dense attention
+ * only.
+ *
+ * Tokens come in blocks of 16, blocks in pages of `page` tokens (a power of two from 16 on); row b of `table` names
+ * the pages of sequence b in order.  D: the head size d rounded up to a multiple of 16; columns past d hold zeros.
+ *   k        [pages, H, page, D]           keys behind the FIR, e4m3 bytes (no infinity; NaN: what was not finite)
+ *   v        [pages, H, page / 16, D, 16]  values, the 16 tokens of a block side by side
+ *   k_scale  [pages, H, page / 16]         exponent + 127 of the power of two that a block's bytes are times
+ *   v_scale  likewise
+ *   raw      [B, H, 16, d]                 the last 16 keys before the FIR, position p at p % 16, of the appended
+ *                                          keys' type; may be null where no FIR is used
+ * k and v 16-byte aligned; d <= 256; pages * H * page * D may pass 2^31.
+ *
+ * Every call takes a position for each sequence, `start` int32 [B], or start_all for all where start is null, and
+ * `counts` int32 [B]: how many of the call's N tokens a sequence has (null: all).
+ *
+ * pnfx_cache_append writes tokens start .. start + count - 1 of each sequence from k, v [B, H, N, d] (strides sb, sh,
+ * sn, 1), the keys behind the FIR with `taps` fp32 [taps_rows, K] (as pnfx_fir_fwd, null: none; K <= 16; the keys
+ * before the call come from raw, those before position 0 are zero), summed in 64 bits.  A block's scale is the smallest power
+ * of two 2^E, E >= -100, for which no finite |number| is above 448 * 2^E, at least the block's so far where the call
+ * begins inside it, whose earlier tokens are then rounded again.  A sequence with start < 0 or more tokens than its
+ * pages hold is left as it is, and so are blocks in pages that the table does not name (an entry outside 0 .. pages - 1).
+ * Sequences that are appended to in one call must not share the pages that are written.
+ *
+ * pnfx_cache_read writes positions first .. first + count - 1 as dense contiguous k, v [B, H, count, d]: zeros
+ * outside 0 .. width * page - 1, NaN in pages that the table does not name.
+ *
+ * pnfx_cached_attn: pn_fir_tau attention (p = 10, peak gate) of query tokens start .. start + count - 1, q and o
+ * [B, Hq, N, d] (Hq a multiple of H: query head h reads key head h / (Hq / H)), over the sequence's keys 0 .. start +
+ * count - 1, for causal != 0 those up to the token's own.  Rows past a sequence's count are zeros.  Sequences that
+ * append leaves alone, and rows that see a page which the table does not name, are NaN.  Workspace: 16-byte aligned,
+ * as large as pnfx_cached_attn_workspace_size says.  Bitwise repeatable.
+ */
+#define PNFX_CACHE_MAX_HEAD 256
+typedef struct pnfx_cache {
+  uint8_t *k, *v, *k_scale, *v_scale;
+  void* raw;
+  const int32_t* table;
+  int64_t table_rs;             /* row stride of table */
+  int64_t B, H, d, D, page;
+  int64_t pages, width;         /* pages in all, and of a sequence */
+} pnfx_cache;
+int pnfx_cache_append(const pnfx_cache* cache, const void* k, int64_t ksb, int64_t ksh, int64_t ksn,
+                      const void* v, int64_t vsb, int64_t vsh, int64_t vsn, int64_t N, const int32_t* start,
+                      int64_t start_all, const int32_t* counts, const float* taps, int64_t taps_rows, int K,
+                      int dtype, void* stream);
+int pnfx_cache_read(const pnfx_cache* cache, const int32_t* first, int64_t first_all, int64_t count, void* k,
+                    void* v, int dtype, void* stream);
+int64_t pnfx_cached_attn_workspace_size(const pnfx_cache* cache, int64_t Hq, int64_t N);
+int pnfx_cached_attn(const pnfx_cache* cache, const void* q, int64_t qsb, int64_t qsh, int64_t qsn, void* o,
+                     int64_t osb, int64_t osh, int64_t osn, int64_t Hq, int64_t N, const int32_t* start,
+                     int64_t start_all, const int32_t* counts, const float* tau, float scale, float gamma,
+                     int has_gamma, int causal, int dtype, void* workspace, int64_t workspace_bytes,
+                     void* stream);
+
+/*
+ * One token of each row of logits [B, V] (row stride rs), from random numbers u in [0, 1).  No counterpart in the
+ * reference.  Weights w_i = exp((z_i - max z) / temperature), in the order of z, the lower index first among equals:
+ * top_k keeps the first k (0 or less: all), top_p the fewest first ones of these that have its share of their weight
+ * (1: all), min_p those whose weight is at least min_p times the largest; the first is always kept.  tokens[b] is the
+ * first, by index, at which the running weight of the kept ones is above u times their whole weight.  temperature <= 0:
+ * the first of the order.  Settings of one row each (`*_each`, on the device) take the place of the others where they are
+ * not null.  -infinity is never drawn; a row with a NaN, or of nothing else, gets -1.  Weights are taken in 64 bits and
+ * summed in 64-bit fixed point, so that results do not depend on any order.  V <= 2^20.
+ */
+typedef struct pnfx_sampling {
+  double temperature, top_p, min_p;
+  int64_t top_k;
+  const float *temperature_each, *top_p_each, *min_p_each;
+  const int32_t* top_k_each;
+} pnfx_sampling;
+int pnfx_sample(const void* logits, int64_t rs, int64_t B, int64_t V, const float* u,
+                const pnfx_sampling* settings, int64_t* tokens, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

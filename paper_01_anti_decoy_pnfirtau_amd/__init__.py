@@ -30,6 +30,9 @@ __all__ = [
     "triton_pn_fir_tau_scores",
     "gated_ffn",
     "linear_cross_entropy",
+    "KVCache",
+    "cached_attention",
+    "sample_tokens",
 ]
 
 
@@ -44,5 +47,10 @@ def __getattr__(name):
         from . import hip_lm
 
         globals()[name] = getattr(hip_lm, name)  # found directly from now on
+        return globals()[name]
+    if name in ("KVCache", "cached_attention", "sample_tokens"):
+        from . import hip_cache
+
+        globals()[name] = getattr(hip_cache, name)
         return globals()[name]
     raise AttributeError(name)

@@ -23,6 +23,21 @@ PNFX_NOALLOC_SCRATCH_BYTES = 128 << 20
 _lib = None
 
 
+class PnfxCache(ctypes.Structure):
+    """pnfx_cache: the 8-bit key and value cache."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "raw", "table")] + [
+        (n, ctypes.c_int64) for n in ("table_rs", "B", "H", "d", "D", "page", "pages", "width")]
+
+
+class PnfxSampling(ctypes.Structure):
+    """pnfx_sampling: the settings of a draw."""
+
+    _fields_ = [("temperature", ctypes.c_double), ("top_p", ctypes.c_double), ("min_p", ctypes.c_double),
+                ("top_k", ctypes.c_int64)] + [
+        (n, ctypes.c_void_p) for n in ("temperature_each", "top_p_each", "min_p_each", "top_k_each")]
+
+
 class PnfxError(RuntimeError):
     """A libpnfx.so entry point returned a non-zero status."""
 
@@ -78,6 +93,13 @@ def _declare(lib: ctypes.CDLL) -> None:
                             + [vp, i64, vp], i32)
     sig["pnfx_xent_bwd"] = ([vp] + [vp, i64] * 2 + [vp, i64, vp, vp, vp, vp] + [i64] * 3 + [i32] * 2
                             + [vp, i64, vp], i32)
+    cache = ctypes.POINTER(PnfxCache)
+    sig["pnfx_cache_append"] = ([cache] + [vp, i64, i64, i64] * 2 + [i64, vp, i64, vp, vp, i64, i32, i32, vp], i32)
+    sig["pnfx_cache_read"] = ([cache, vp, i64, i64, vp, vp, i32, vp], i32)
+    sig["pnfx_cached_attn_workspace_size"] = ([cache, i64, i64], i64)
+    sig["pnfx_cached_attn"] = ([cache] + [vp, i64, i64, i64] * 2
+                               + [i64, i64, vp, i64, vp, vp, f32, f32, i32, i32, i32, vp, i64, vp], i32)
+    sig["pnfx_sample"] = ([vp, i64, i64, i64, vp, ctypes.POINTER(PnfxSampling), vp, i32, vp], i32)
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
         fn.argtypes = args
@@ -119,4 +141,6 @@ def exported_symbols() -> list[str]:
         "pnfx_ffn_fwd_workspace_size", "pnfx_ffn_fwd", "pnfx_ffn_bwd_workspace_size", "pnfx_ffn_bwd",
         "pnfx_xent_fwd_workspace_size", "pnfx_xent_fwd", "pnfx_xent_bwd_workspace_size",
         "pnfx_xent_bwd",
+        "pnfx_cache_append", "pnfx_cache_read", "pnfx_cached_attn_workspace_size", "pnfx_cached_attn",
+        "pnfx_sample",
     ]

@@ -16,6 +16,9 @@
 // pnfx::linear / _wgrad     (none: x W^T with its weight gradient's fp32 sums)
 // pnfx::gated_ffn / _bwd    (none: the gated feed-forward block, both projections in one kernel)
 // pnfx::linear_xent / _bwd  (none: cross entropy over the vocabulary without the logits)
+// pnfx::cache_append / _read (none: the 8-bit key and value cache, written and read back)
+// pnfx::cached_attn         (none: pn_fir_tau attention over that cache)
+// pnfx::sample_tokens       (none: one token of each row of logits)
 // pnfx::sum_f64             the fp64 sum of tau's row gradients  :784
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
@@ -420,6 +423,153 @@ std::tuple<Tensor, Tensor> linear_xent_bwd_cuda(const Tensor& dloss_in, const Te
                          ws.data_ptr(), wsb, stream_of(x_in)),
            "pnfx_xent_bwd");
   return {dx, dw};
+}
+
+// ------------------------------------------------------------------------ cache, sampling
+using OptTensor = std::optional<Tensor>;
+
+// The cache's tensors as the C ABI takes them (raw: may be undefined where a call does not use it).
+pnfx_cache cache_of(const char* what, const Tensor& k, const Tensor& v, const Tensor& k_scale, const Tensor& v_scale,
+                    const Tensor& table, int64_t d) {
+  TORCH_CHECK_VALUE(k.dim() == 4 && v.dim() == 5 && k_scale.dim() == 3 && table.dim() == 2 && k.size(2) >= 16 &&
+                        v.sizes() == at::IntArrayRef({k.size(0), k.size(1), k.size(2) / 16, k.size(3), 16}) &&
+                        k_scale.sizes() == at::IntArrayRef({k.size(0), k.size(1), k.size(2) / 16}) &&
+                        v_scale.sizes() == k_scale.sizes(),
+                    what, ": a cache of k ", k.sizes(), ", v ", v.sizes(), ", k_scale ", k_scale.sizes(),
+                    ", v_scale ", v_scale.sizes(), ", table ", table.sizes());
+  for (const Tensor* t : {&k, &v, &k_scale, &v_scale, &table}) {
+    TORCH_CHECK_TYPE(t->scalar_type() == (t == &table ? at::kInt : at::kByte), what, ": a cache tensor is ",
+                     t->scalar_type());
+    TORCH_CHECK_VALUE(t->is_contiguous() && t->device() == k.device(), what,
+                      ": the cache's tensors must be contiguous, on one device");
+  }
+  pnfx_cache c = {};
+  c.k = k.data_ptr<uint8_t>(), c.v = v.data_ptr<uint8_t>();
+  c.k_scale = k_scale.data_ptr<uint8_t>(), c.v_scale = v_scale.data_ptr<uint8_t>();
+  c.table = table.data_ptr<int32_t>(), c.table_rs = table.size(1);
+  c.B = table.size(0), c.H = k.size(1), c.d = d, c.D = k.size(3), c.page = k.size(2);
+  c.pages = k.size(0), c.width = table.size(1);
+  return c;
+}
+
+// One int32 (or fp32) for each row, contiguous on the operands' device; null where there is none.
+template <typename T>
+const T* each_of(const char* what, const char* name, const OptTensor& t, at::ScalarType st, int64_t n,
+                 const Tensor& like, Tensor& hold) {
+  if (!t.has_value()) return nullptr;
+  TORCH_CHECK_TYPE(t->scalar_type() == st, what, ": ", name, " is ", t->scalar_type());
+  TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == n && t->device() == like.device(), what, ": ", name, " ",
+                    t->sizes(), " on ", t->device(), " for ", n, " rows on ", like.device());
+  hold = t->contiguous();
+  return hold.data_ptr<T>();
+}
+
+Tensor unit_inner(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+
+void cache_append_cuda(const Tensor& k_in, const Tensor& v_in, Tensor& ck, Tensor& cv, Tensor& k_scale,
+                       Tensor& v_scale, Tensor& raw, const Tensor& table, const OptTensor& start, int64_t start_all,
+                       const OptTensor& counts, const OptTensor& taps) {
+  const char* what = "cache_append";
+  TORCH_CHECK_VALUE(raw.dim() == 4 && raw.size(2) == 16 && raw.is_contiguous() && raw.device() == ck.device(), what,
+                    ": raw ", raw.sizes());
+  pnfx_cache c = cache_of(what, ck, cv, k_scale, v_scale, table, raw.size(3));
+  TORCH_CHECK_VALUE(k_in.dim() == 4 && v_in.sizes() == k_in.sizes() && k_in.size(0) == c.B && k_in.size(1) == c.H &&
+                        k_in.size(3) == c.d && raw.size(0) == c.B && raw.size(1) == c.H,
+                    what, ": k ", k_in.sizes(), " and v ", v_in.sizes(), " to a cache of raw ", raw.sizes(),
+                    " and table ", table.sizes());
+  TORCH_CHECK_TYPE(k_in.scalar_type() == raw.scalar_type() && v_in.scalar_type() == raw.scalar_type(), what, ": k is ",
+                   k_in.scalar_type(), ", v is ", v_in.scalar_type(), ", the cache is for ", raw.scalar_type());
+  TORCH_CHECK_VALUE(k_in.device() == ck.device() && v_in.device() == ck.device(), what, ": k on ", k_in.device(),
+                    ", v on ", v_in.device(), ", the cache on ", ck.device());
+  const int code = dtype_code(k_in, what);
+  if (k_in.size(2) == 0 || c.B * c.H == 0) return;
+  const c10::DeviceGuard guard(ck.device());
+  const Tensor k = unit_inner(k_in), v = unit_inner(v_in);
+  c.raw = raw.data_ptr();
+  Tensor t32, hold[2];
+  if (taps.has_value()) {
+    TORCH_CHECK_VALUE(taps->dim() == 1 || taps->dim() == 2, what, ": taps ", taps->sizes());
+    t32 = taps->reshape({-1, taps->size(-1)});
+    if (t32.scalar_type() != at::kFloat || !t32.is_contiguous() || t32.device() != ck.device())
+      t32 = t32.to(ck.device(), at::kFloat).contiguous();
+  }
+  const int32_t* s = each_of<int32_t>(what, "start", start, at::kInt, c.B, ck, hold[0]);
+  const int32_t* n = each_of<int32_t>(what, "counts", counts, at::kInt, c.B, ck, hold[1]);
+  check_rc(pnfx_cache_append(&c, k.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.data_ptr(), v.stride(0),
+                             v.stride(1), v.stride(2), k.size(2), s, start_all, n,
+                             t32.defined() ? t32.data_ptr<float>() : nullptr, t32.defined() ? t32.size(0) : 0,
+                             t32.defined() ? (int)t32.size(1) : 0, code, stream_of(ck)),
+           "pnfx_cache_append");
+}
+
+std::tuple<Tensor, Tensor> cache_read_cuda(const Tensor& ck, const Tensor& cv, const Tensor& k_scale,
+                                           const Tensor& v_scale, const Tensor& table, const OptTensor& first,
+                                           int64_t first_all, int64_t count, int64_t d, at::ScalarType dtype) {
+  const char* what = "cache_read";
+  const pnfx_cache c = cache_of(what, ck, cv, k_scale, v_scale, table, d);
+  TORCH_CHECK_VALUE(count >= 0, what, ": count ", count);
+  const auto opts = ck.options().dtype(dtype);
+  Tensor k = at::empty({c.B, c.H, count, d}, opts), v = at::empty({c.B, c.H, count, d}, opts);
+  const int code = dtype_code(k, what);
+  if (k.numel() == 0) return {k, v};
+  const c10::DeviceGuard guard(ck.device());
+  Tensor hold;
+  const int32_t* f = each_of<int32_t>(what, "first", first, at::kInt, c.B, ck, hold);
+  check_rc(pnfx_cache_read(&c, f, first_all, count, k.data_ptr(), v.data_ptr(), code, stream_of(ck)),
+           "pnfx_cache_read");
+  return {k, v};
+}
+
+Tensor cached_attn_cuda(const Tensor& q_in, const Tensor& ck, const Tensor& cv, const Tensor& k_scale,
+                        const Tensor& v_scale, const Tensor& table, const OptTensor& start, int64_t start_all,
+                        const OptTensor& counts, const Tensor& tau, double scale, double gamma, bool has_gamma,
+                        bool causal) {
+  const char* what = "cached_attn";
+  TORCH_CHECK_VALUE(q_in.dim() == 4, what, ": q ", q_in.sizes());
+  const pnfx_cache c = cache_of(what, ck, cv, k_scale, v_scale, table, q_in.size(3));
+  TORCH_CHECK_VALUE(q_in.size(0) == c.B && c.H > 0 && q_in.size(1) % c.H == 0 && (c.d + 15) / 16 * 16 == c.D, what,
+                    ": q ", q_in.sizes(), " over a cache of k ", ck.sizes(), " and table ", table.sizes());
+  TORCH_CHECK_VALUE(q_in.device() == ck.device(), what, ": q on ", q_in.device(), ", the cache on ", ck.device());
+  const int code = dtype_code(q_in, what);
+  const int64_t Hq = q_in.size(1), N = q_in.size(2);
+  Tensor o = at::empty({c.B, N, Hq, c.d}, q_in.options()).permute({0, 2, 1, 3});
+  if (o.numel() == 0) return o;
+  const c10::DeviceGuard guard(ck.device());
+  const Tensor q = unit_inner(q_in), t32 = tau32(tau, ck);
+  Tensor hold[2], ws;
+  const int32_t* s = each_of<int32_t>(what, "start", start, at::kInt, c.B, ck, hold[0]);
+  const int32_t* n = each_of<int32_t>(what, "counts", counts, at::kInt, c.B, ck, hold[1]);
+  const int64_t wsb = pnfx_cached_attn_workspace_size(&c, Hq, N);
+  if (wsb) ws = at::empty({wsb}, ck.options());
+  check_rc(pnfx_cached_attn(&c, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), o.data_ptr(), o.stride(0),
+                            o.stride(1), o.stride(2), Hq, N, s, start_all, n, t32.data_ptr<float>(), (float)scale,
+                            (float)gamma, has_gamma, causal, code, wsb ? ws.data_ptr() : nullptr, wsb, stream_of(ck)),
+           "pnfx_cached_attn");
+  return o;
+}
+
+Tensor sample_tokens_cuda(const Tensor& z_in, const Tensor& u_in, double temperature, int64_t top_k, double top_p,
+                          double min_p, const OptTensor& temperature_each, const OptTensor& top_k_each,
+                          const OptTensor& top_p_each, const OptTensor& min_p_each) {
+  const char* what = "sample_tokens";
+  TORCH_CHECK_VALUE(z_in.dim() == 2 && z_in.size(1) >= 1, what, ": logits ", z_in.sizes());
+  const int code = dtype_code(z_in, what);
+  const int64_t B = z_in.size(0), V = z_in.size(1);
+  Tensor tokens = at::empty({B}, z_in.options().dtype(at::kLong));
+  Tensor hold[5];
+  const c10::DeviceGuard guard(z_in.device());
+  const float* u = each_of<float>(what, "u", u_in, at::kFloat, B, z_in, hold[0]);
+  pnfx_sampling set = {};
+  set.temperature = temperature, set.top_k = top_k, set.top_p = top_p, set.min_p = min_p;
+  set.temperature_each = each_of<float>(what, "temperature", temperature_each, at::kFloat, B, z_in, hold[1]);
+  set.top_k_each = each_of<int32_t>(what, "top_k", top_k_each, at::kInt, B, z_in, hold[2]);
+  set.top_p_each = each_of<float>(what, "top_p", top_p_each, at::kFloat, B, z_in, hold[3]);
+  set.min_p_each = each_of<float>(what, "min_p", min_p_each, at::kFloat, B, z_in, hold[4]);
+  if (B == 0) return tokens;
+  const Tensor z = z_in.stride(1) == 1 && z_in.stride(0) >= V ? z_in : z_in.contiguous();
+  check_rc(pnfx_sample(z.data_ptr(), z.stride(0), B, V, u, &set, tokens.data_ptr<int64_t>(), code, stream_of(z)),
+           "pnfx_sample");
+  return tokens;
 }
 
 // ------------------------------------------------------------------------------ flash
@@ -1131,6 +1281,16 @@ TORCH_LIBRARY(pnfx, m) {
   m.def("flash_fwd_fir(Tensor q, Tensor k_raw, Tensor v, Tensor tau, Tensor taps, float scale, "
         "float gamma, bool has_gamma, bool causal, bool o_bnhd=False) -> "
         "(Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("cache_append(Tensor k, Tensor v, Tensor(a!) ck, Tensor(b!) cv, Tensor(c!) k_scale, "
+        "Tensor(d!) v_scale, Tensor(e!) raw, Tensor table, Tensor? start, int start_all, Tensor? counts, "
+        "Tensor? taps) -> ()");
+  m.def("cache_read(Tensor ck, Tensor cv, Tensor k_scale, Tensor v_scale, Tensor table, Tensor? first, "
+        "int first_all, int count, int d, ScalarType dtype) -> (Tensor, Tensor)");
+  m.def("cached_attn(Tensor q, Tensor ck, Tensor cv, Tensor k_scale, Tensor v_scale, Tensor table, "
+        "Tensor? start, int start_all, Tensor? counts, Tensor tau, float scale, float gamma, "
+        "bool has_gamma, bool causal) -> Tensor");
+  m.def("sample_tokens(Tensor logits, Tensor u, float temperature, int top_k, float top_p, float min_p, "
+        "Tensor? temperature_each, Tensor? top_k_each, Tensor? top_p_each, Tensor? min_p_each) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(pnfx, CUDA, m) {
@@ -1150,6 +1310,10 @@ TORCH_LIBRARY_IMPL(pnfx, CUDA, m) {
   m.impl("attn_rows", attn_rows_cuda);
   m.impl("attn_rows_bwd", attn_rows_bwd_cuda);
   m.impl("flash_fwd_fir", flash_fwd_fir_cuda);
+  m.impl("cache_append", cache_append_cuda);
+  m.impl("cache_read", cache_read_cuda);
+  m.impl("cached_attn", cached_attn_cuda);
+  m.impl("sample_tokens", sample_tokens_cuda);
 }
 
 TORCH_LIBRARY_IMPL(pnfx, Autograd, m) {

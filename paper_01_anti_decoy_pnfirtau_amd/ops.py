@@ -18,6 +18,9 @@ pnfx::linear           (none: x W^T whose weight gradient is linear_wgrad)
 pnfx::linear_wgrad     (none: dY^T X of bf16 rows, fp32 sums)
 pnfx::gated_ffn/_bwd   (none: the gated feed-forward block, both projections in one kernel)
 pnfx::linear_xent/_bwd (none: cross entropy over the vocabulary without the logits)
+pnfx::cache_append/_read (none: the 8-bit key and value cache, written and read back)
+pnfx::cached_attn      (none: pn_fir_tau attention over that cache)
+pnfx::sample_tokens    (none: one token of each row of logits)
 pnfx::sum_f64          the fp64 sum of tau's row gradients  :784
 """
 from __future__ import annotations
@@ -222,3 +225,25 @@ def _(x, w, target, ignore_index, reduction):
 @torch.library.register_fake("pnfx::linear_xent_bwd")
 def _(dloss, x, w, target, rows, lse, ignore_index, reduction, mask):
     return tuple(x.new_empty(t.shape if m else (0,)) for t, m in zip((x, w), mask))
+
+
+@torch.library.register_fake("pnfx::cache_append")
+def _(k, v, ck, cv, k_scale, v_scale, raw, table, start, start_all, counts, taps):
+    return None
+
+
+@torch.library.register_fake("pnfx::cache_read")
+def _(ck, cv, k_scale, v_scale, table, first, first_all, count, d, dtype):
+    shape = (table.shape[0], ck.shape[1], count, d)
+    return ck.new_empty(shape, dtype=dtype), ck.new_empty(shape, dtype=dtype)
+
+
+@torch.library.register_fake("pnfx::cached_attn")
+def _(q, ck, cv, k_scale, v_scale, table, start, start_all, counts, tau, scale, gamma, has_gamma, causal):
+    B, H, N, d = q.shape
+    return q.new_empty((B, N, H, d)).permute(0, 2, 1, 3)
+
+
+@torch.library.register_fake("pnfx::sample_tokens")
+def _(logits, u, temperature, top_k, top_p, min_p, temperature_each, top_k_each, top_p_each, min_p_each):
+    return logits.new_empty(logits.shape[0], dtype=torch.int64)
