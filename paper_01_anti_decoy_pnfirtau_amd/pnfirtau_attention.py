@@ -159,6 +159,34 @@ class PnFirTauMHA(nn.Module):
         out = self.out(torch.matmul(w, v).transpose(1, 2).reshape(B, N, D))
         return (out, w) if return_weights else out
 
+    def new_cache(self, batch: int, max_len: int, **kwargs):
+        """An empty cache of this layer for sequences of up to max_len tokens (hip_cache.KVCache.new)."""
+        from .hip_cache import KVCache
+
+        kwargs = {"device": self.qkv.weight.device, "dtype": self.qkv.weight.dtype, **kwargs}
+        return KVCache.new(batch, self.n_heads, self.head_dim, max_len, **kwargs)
+
+    def forward_cached(self, x: torch.Tensor, cache, start, counts: torch.Tensor | None = None):
+        """The layer's output for the next tokens x [B, N, D] of sequences whose earlier ones are in ``cache``, which
+        these join: positions ``start`` .. start + N - 1, of which a sequence has ``counts`` (hip_cache.KVCache).  Keys
+        and values are those of the cache, 8 bits; no dropout, no gradients.  Causal layers whose scores are the
+        kernels': p = 10 and the peak gate, where the layer's forward goes by its configuration."""
+        from .hip_cache import cached_attention
+
+        cfg = self.cfg
+        if not cfg.causal_mask:
+            raise ValueError("forward_cached: a layer that sees later tokens has no use for a cache")
+        if self._by_config and (cfg.p != 10.0 or (cfg.silence_gamma and cfg.silence_mode != "peak")):
+            raise ValueError(f"forward_cached: p={cfg.p}, silence_mode={cfg.silence_mode}: p = 10 and the peak gate")
+        B, N, D = x.shape
+        q, k, v = (self._split_heads(t) for t in self.qkv(x).split(D, dim=-1))
+        cache.append(k, v, start, taps=self.fir_taps if cfg.fir_k > 1 else None, counts=counts)
+        o = cached_attention(q, cache, start, self.score_tau, 1.0 / math.sqrt(self.head_dim), cfg.silence_gamma,
+                             counts=counts)
+        return self.out(o.transpose(1, 2).reshape(B, N, D))
+
+    _by_config = True  # whether p and silence_mode are consulted
+
 
 class PnFirTauTritonMHA(PnFirTauMHA):
     """Materialised-score variant: HIP FIR + HIP row-fused score kernel (src/pnfirtau_attention.py:250-282).
@@ -192,6 +220,8 @@ class PnFirTauFlashMHA(PnFirTauMHA):
     The flash output is produced in [B, N, H, hd] memory order, so the merge of
     heads before the output projection is a view.
     """
+
+    _by_config = False
 
     def forward(self, x: torch.Tensor, return_weights: bool = False):
         if return_weights:

@@ -11,7 +11,8 @@ Mirrors the reference's WikiText-2 model and step (``experiments/exp4_wikitext2_
 
 Beside the reference's model, ``WikiLMConfig`` offers two choices that it does not have: a gated
 feed-forward block (``ffn="swiglu"`` or ``"geglu"``: ``GatedFFN``, whose activations may be kept in
-8 bits) and the loss without materialised logits (``fused_loss``).
+8 bits) and the loss without materialised logits (``fused_loss``); and a model can answer, which the
+reference's does not: ``generate`` continues prompts token by token over 8-bit caches, ``Decoder`` is its engine.
 
 ``GraphedStep`` captures that whole step (including the optimizer update) in one HIP graph,
 as the reference's ``experiments/exp4c_cuda_graphs.py:81-108`` does for the attention stack:
@@ -25,6 +26,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .hip_cache import KVCache, sample_tokens
 from .hip_lm import gated_ffn, linear_cross_entropy
 from .pnfirtau_attention import PnFirConfig, PnFirTauFlashMHA, PnFirTauMHA, PnFirTauTritonMHA
 
@@ -105,6 +107,10 @@ class Block(nn.Module):
         x = x + self.drop(self.attn(self.ln1(x)))
         return x + self.ffn(self.ln2(x))
 
+    def forward_cached(self, x: torch.Tensor, cache: KVCache, start, counts=None) -> torch.Tensor:
+        x = x + self.attn.forward_cached(self.ln1(x), cache, start, counts)
+        return x + self.ffn(self.ln2(x))
+
 
 class WikiLM(nn.Module):
     """Decoder-only LM with pn_fir_tau attention (experiments/exp4_wikitext2_lm.py:203-247).
@@ -148,6 +154,24 @@ class WikiLM(nn.Module):
 
     def forward(self, idx: torch.Tensor) -> torch.Tensor:
         return self.head(self.hidden(idx))
+
+    def new_caches(self, batch: int, max_len: int | None = None, **kwargs) -> list[KVCache]:
+        """One empty cache for each layer, for sequences of up to max_len tokens, with one table."""
+        caches: list[KVCache] = []
+        for blk in self.blocks:
+            shared = {"table": caches[0].table, "pages": caches[0].k.shape[0]} if caches else {}
+            caches.append(blk.attn.new_cache(batch, max_len or self.cfg.max_seq, **{**kwargs, **shared}))
+        return caches
+
+    def hidden_cached(self, idx: torch.Tensor, caches: list[KVCache], start: int | torch.Tensor,
+                      counts: torch.Tensor | None = None) -> torch.Tensor:
+        """As ``hidden``, of the tokens idx [B, N] that follow those in the caches (which they join): positions start ..
+        start + N - 1, of which a sequence has ``counts``.  In evaluation mode, under torch.no_grad()."""
+        pos = torch.arange(idx.shape[1], device=idx.device) + (start[:, None] if torch.is_tensor(start) else start)
+        h = self.embed(idx) + self.pos(pos.clamp(max=self.cfg.max_seq - 1))
+        for blk, cache in zip(self.blocks, caches):
+            h = blk.forward_cached(h, cache, start, counts)
+        return self.ln_f(h)
 
 
 def zipf_tokens(batch: int, seq: int, vocab: int, seed: int, s: float = 1.1) -> torch.Tensor:
@@ -249,3 +273,94 @@ class GraphedStep:
     def replay(self) -> torch.Tensor:
         self.graph.replay()
         return self.loss
+
+
+class Decoder:
+    """Continues sequences of one model, a token of each at a time, over 8-bit caches.
+
+    ``prefill`` takes the prompts, ``step`` draws the next token of every sequence and takes it in; where the sequences
+    are stands on the device, so that with ``graph`` a step is one captured HIP graph.  ``settings``: sample_tokens'
+    (values, or tensors [B] whose contents may change between steps).  The model must be in evaluation mode.
+    ``amp``: bf16 autocast."""
+
+    def __init__(self, model: WikiLM, batch: int, max_len: int | None = None, amp: bool = False, graph: bool = False,
+                 **settings):
+        if model.training:
+            raise ValueError("Decoder: the model is in training mode")
+        self.model, self.amp, self.graph, self.settings = model, amp, graph, settings
+        self.max_len = model.cfg.max_seq if max_len is None else max_len
+        if self.max_len > model.cfg.max_seq:
+            raise ValueError(f"Decoder: {self.max_len} tokens of a model of {model.cfg.max_seq}")
+        dev, dtype = model.embed.weight.device, model.embed.weight.dtype
+        self.caches = model.new_caches(batch, self.max_len, dtype=torch.bfloat16 if amp else dtype)
+        self.start = torch.zeros(batch, dtype=torch.int32, device=dev)
+        self.rows = torch.zeros(batch, model.cfg.d_model, dtype=dtype, device=dev)  # before the head, of the last tokens
+        self.u = torch.zeros(batch, device=dev)
+        self.token = torch.zeros(batch, dtype=torch.int64, device=dev)
+        self.most = 0  # tokens of the longest sequence
+        self._captured = None
+
+    def _run(self, idx, start, counts=None):
+        with torch.no_grad(), torch.autocast(idx.device.type, torch.bfloat16, enabled=self.amp):
+            return self.model.hidden_cached(idx, self.caches, start, counts)
+
+    def prefill(self, prompt: torch.Tensor, lengths: torch.Tensor | None = None) -> None:
+        """Begins anew with the prompts [B, N], of which sequence b has lengths[b] tokens (at least one; null: N)."""
+        B, N = prompt.shape
+        if not 0 < N <= self.max_len or B != len(self.start):
+            raise ValueError(f"Decoder: prompts {tuple(prompt.shape)} for {len(self.start)} sequences of {self.max_len}")
+        counts = torch.full_like(self.start, N) if lengths is None else lengths.to(self.start).clamp(1, N)
+        h = self._run(prompt, 0, None if lengths is None else counts)
+        self.rows.copy_(h.gather(1, (counts.long() - 1)[:, None, None].expand(B, 1, h.shape[2]))[:, 0])
+        self.start.copy_(counts)
+        self.most = N
+
+    def _step(self) -> None:
+        with torch.no_grad(), torch.autocast(self.rows.device.type, torch.bfloat16, enabled=self.amp):
+            token = sample_tokens(self.model.head(self.rows), self.u, **self.settings)
+        h = self._run(token.clamp(min=0)[:, None], self.start)  # -1: a row of NaN has no token
+        self.rows.copy_(h[:, 0])
+        self.start += 1
+        self.token.copy_(token)
+
+    def step(self, u: torch.Tensor) -> torch.Tensor:
+        """The next token of each sequence, drawn by u [B] in [0, 1); overwritten by the next call."""
+        if self.most + 1 > self.max_len:
+            raise ValueError(f"Decoder: sequences of {self.max_len} tokens are full")
+        self.most += 1
+        self.u.copy_(u)
+        if not (self.graph and self.u.is_cuda):
+            self._step()
+            return self.token
+        if self._captured is None:
+            # the warm-up runs on what a step overwrites: the caches' next token, written again by the replay, and state
+            # that is put back
+            saved = self.rows.clone(), self.start.clone()
+            side = torch.cuda.Stream(self.u.device)
+            side.wait_stream(torch.cuda.current_stream(self.u.device))
+            with torch.cuda.stream(side):
+                self._step()
+                self.rows.copy_(saved[0]), self.start.copy_(saved[1])
+            torch.cuda.current_stream(self.u.device).wait_stream(side)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                self._step()
+            self._captured = graph
+        self._captured.replay()
+        return self.token
+
+
+def generate(model: WikiLM, prompt: torch.Tensor, max_new: int, lengths: torch.Tensor | None = None,
+             u: torch.Tensor | None = None, generator: torch.Generator | None = None, amp: bool = False,
+             graph: bool = False, **settings) -> torch.Tensor:
+    """max_new tokens [B, max_new] that follow the prompts [B, N] (sequence b has lengths[b] of the N), drawn by u
+    [B, max_new] (by default from ``generator``) with sample_tokens' ``settings``."""
+    B, N = prompt.shape
+    if u is None:
+        dev = prompt.device if generator is None else generator.device
+        u = torch.rand(B, max_new, generator=generator, device=dev).to(prompt.device)
+    if u.shape != (B, max_new):
+        raise ValueError(f"generate: u has shape {tuple(u.shape)}, not {(B, max_new)}")
+    dec = Decoder(model, B, N + max_new, amp=amp, graph=graph, **settings)
+    dec.prefill(prompt, lengths)
+    return torch.stack([dec.step(u[:, i]).clone() for i in range(max_new)], 1) if max_new else prompt.new_empty(B, 0)

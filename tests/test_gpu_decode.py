@@ -1,0 +1,73 @@
+"""Layers and the language model over the 8-bit cache on the GPU: a run of its operators as they are used together."""
+import pytest
+import torch
+
+from paper_01_anti_decoy_pnfirtau_amd import PnFirConfig, PnFirTauFlashMHA
+from paper_01_anti_decoy_pnfirtau_amd.wikilm import Decoder, WikiLM, WikiLMConfig, generate
+
+pytestmark = pytest.mark.gpu
+
+
+def model(dev, **kw):
+    torch.manual_seed(0)
+    cfg = WikiLMConfig(d_model=128, n_heads=2, n_layers=3, d_ff=256, max_seq=128, dropout=0.0, **kw)
+    return WikiLM(997, cfg, "pn_fir_tau_flash").eval().to(dev)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_layer_over_the_cache_is_the_dense_layer_up_to_8_bits(dev, dtype):
+    torch.manual_seed(1)
+    layer = PnFirTauFlashMHA(PnFirConfig(d_model=128, n_heads=2)).eval().to(dev, dtype)
+    x = torch.randn(2, 200, 128, device=dev, dtype=dtype)
+    with torch.no_grad():
+        want = layer(x).float()
+        cache = layer.new_cache(2, 200, page=32)
+        got = torch.cat([layer.forward_cached(x[:, a:b], cache, a) for a, b in ((0, 117), (117, 118), (118, 200))], 1)
+    assert (got.float() - want).norm() < 0.15 * want.norm()
+
+
+@pytest.mark.parametrize("amp", [False, True])
+def test_generate_same_as_the_cpu_one_and_captured(dev, amp):
+    m = model(dev)
+    g = torch.Generator().manual_seed(2)
+    prompt = torch.randint(0, 997, (3, 20), generator=g)
+    lengths, u = torch.tensor([20, 7, 1]), torch.rand(3, 30, generator=g)
+    run = lambda **kw: generate(m, prompt.to(dev), 30, lengths.to(dev), u.to(dev), amp=amp, temperature=0.8,  # noqa: E731
+                                top_k=100, top_p=0.95, **kw)
+    eager = run()
+    assert torch.equal(eager, run(graph=True))
+    assert torch.equal(eager, run())
+    assert 0 <= int(eager.min()) and int(eager.max()) < 997
+    if not amp:
+        with torch.no_grad():  # the logits of the prompts' last rows, on the GPU and the CPU
+            on = m.head(m.hidden_cached(prompt.to(dev), m.new_caches(3), 0)).cpu()
+            cpu = m.cpu()
+            off = cpu.head(cpu.hidden_cached(prompt, cpu.new_caches(3), 0))
+        assert (on - off).abs().max() < 1e-2 * off.abs().max()  # fp32 sums move some 8-bit roundings
+
+
+def test_decoders_side_by_side(dev):
+    """Two captured decoders, their replays and eager steps mixed, on two streams, and prompts taken anew."""
+    m = model(dev)
+    g = torch.Generator().manual_seed(4)
+    prompts = [torch.randint(0, 997, (2, 15), generator=g).to(dev) for _ in range(2)]
+    u = torch.rand(2, 24, 2, generator=g).to(dev)
+    want = []
+    for i in range(2):
+        dec = Decoder(m, 2, temperature=0.9)
+        dec.prefill(prompts[i])
+        want.append(torch.stack([dec.step(u[i, t]).clone() for t in range(24)]))
+    decs = [Decoder(m, 2, graph=True, temperature=0.9) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(2):
+        got = [[], []]
+        for i in range(2):
+            decs[i].prefill(prompts[i])
+        torch.cuda.synchronize()
+        for t in range(24):
+            for i in range(2):
+                with torch.cuda.stream(streams[i]):
+                    got[i].append(decs[i].step(u[i, t]).clone())
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(torch.stack(got[i]), want[i])
