@@ -10,7 +10,6 @@
 #include "pnfx_common.h"
 
 namespace pnfx {
-namespace {
 
 constexpr int BLOCK = 16;      // tokens that share a scale
 constexpr int RAW = 16;        // keys before the FIR that are kept of each sequence and head
@@ -45,7 +44,7 @@ __device__ __forceinline__ float two_to(int e) {  // -126 <= e <= 127
 }
 
 // The caller's description, checked.
-int cache_of(const pnfx_cache* c, const char* what, Cache* out) {
+inline int cache_of(const pnfx_cache* c, const char* what, Cache* out) {
   PNFX_REQUIRE(c && c->k && c->v && c->k_scale && c->v_scale && c->table, "%s: null pointer in the cache", what);
   PNFX_REQUIRE(c->B >= 1 && c->H >= 1 && c->pages >= 1 && c->width >= 1 && c->B < (1 << 24) && c->H < (1 << 20) &&
                    c->pages < (1ll << 31) && c->width < (1ll << 31),
@@ -61,9 +60,10 @@ int cache_of(const pnfx_cache* c, const char* what, Cache* out) {
   *out = Cache{c->k, c->v, c->k_scale, c->v_scale, c->raw, c->table, c->table_rs,
                (int)c->B, (int)c->H, (int)c->d, (int)c->D, (int)c->page, __builtin_ctz((unsigned)c->page),
                (int)c->pages, (int)c->width};
+  PNFX_REQUIRE(c->pages * c->H * (c->page / BLOCK) < (1ll << 31), "%s: %lld pages of %lld tokens and %lld heads", what,
+               (long long)c->pages, (long long)c->page, (long long)c->H);
   PNFX_REQUIRE(out->capacity() <= (1ll << 30), "%s: %lld tokens a sequence", what, (long long)out->capacity());
   return PNFX_OK;
 }
 
-}  // namespace
 }  // namespace pnfx

@@ -1,0 +1,648 @@
+// pn_fir_tau attention over the 8-bit cache.
+//
+//   u_j = relu(scale q.k_j - tau), P_j = u_j^10, M = max_j u_j
+//   O   = M / (M + gamma) * sum_j P_j v_j / (sum_j P_j + 1e-12)       over the keys j that the row sees
+//
+// A wave takes 64 keys at a time: four blocks of 16 tokens.  With the keys as rows of the first product and the
+// queries as its columns, and key 16 g + 4 t + i as row 4 g + i of product t, lane group g gets all 16 scores of block
+// g for its query, which is what the second product wants from it (the weights as columns, V^T as rows): scores go
+// from one product to the other in registers, without LDS or exchange.  Key rows and value rows come straight from
+// memory in 16-byte loads, the next tile's while this one is worked on.  Scales are powers of two, so e4m3 times scale
+// is exact in bf16, and a block's key scale is one factor on its lane group's scores.
+//
+// The waves of a workgroup take every fourth tile of the same rows, so that a key is read once by the workgroup
+// whatever its number of rows (16 NT: query heads that share the key head, times query tokens), and add up through
+// LDS.  The work of a call, 256 keys of one unit (sequence, key head, row tile) a step, is cut into equal shares for
+// a fixed number of workgroups, whatever the lengths, which only the device knows; a unit that several workgroups
+// have pieces of is joined by a second kernel.
+//
+// The powers are taken of u 2^-e with one e a row, raised (and the sums scaled, exactly) only when a score passes
+// 2^8 2^e: a power of ten of the tenth lies within fp32 for scores 2^8 above and 2^12 below.  bf16 queries: the
+// weights are rounded to bf16 for the product and the same rounded values are summed, as the dense kernels do.  fp32
+// queries: queries and weights as three bf16 parts each (24 bits), keys and values are exact in one.
+#pragma once
+
+#include "cache.h"
+#include "tiles_bf16.h"
+
+#include <cmath>
+
+namespace pnfx {
+
+struct Header {  // of a piece of a unit, for the join
+  int b, h, rt, first, last;  // the workgroups that have its pieces; first -1: none
+};
+
+struct AttnArgs {
+  Cache c;
+  Span span;
+  const void* q;
+  void* o;
+  int64_t qsb, qsh, qsn, osb, osh, osn;
+  const float* tau;
+  float scale, gamma;
+  int has_gamma, causal;
+  int Hq, G, R;       // query heads, those of a key head, row tiles
+  int shares;         // workgroups that share the call's steps; 0: one workgroup a unit
+  // Pieces, two for each share: the unit it goes on with, and the one that it begins and does not end
+  Header* headers;
+  float *acc, *stats;  // [2 shares][rows][D], and [2 shares][3][rows]: sum, peak, exponent
+};
+
+// How a call is cut: row tiles of 16 NT rows, R for each sequence and key head; shares: workgroups that share the
+// call's steps (0: one workgroup a unit); bytes of workspace.
+struct AttnPlan {
+  int NT, R, shares;
+  int64_t units, header_bytes, acc_bytes, stat_bytes;
+  int64_t bytes() const { return header_bytes + acc_bytes + stat_bytes; }
+};
+
+// The kernels, by the type of the queries and the head size in the cache.
+int attn_bf16_64(const AttnArgs& a, const AttnPlan& p, hipStream_t st);    // up to 64
+int attn_bf16_128(const AttnArgs& a, const AttnPlan& p, hipStream_t st);   // up to 128
+int attn_bf16_256(const AttnArgs& a, const AttnPlan& p, hipStream_t st);
+int attn_f32_64(const AttnArgs& a, const AttnPlan& p, hipStream_t st);
+int attn_f32_128(const AttnArgs& a, const AttnPlan& p, hipStream_t st);
+int attn_f32_256(const AttnArgs& a, const AttnPlan& p, hipStream_t st);
+
+namespace {
+
+typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+constexpr int THREADS = 256, WAVES = 4, TILE = 64, STEP = WAVES * TILE;
+constexpr int E_FIRST = -60;  // of a row without scores: 2^60 u is finite for u up to 2^67, and larger ones raise it again
+constexpr int E_LAST = 120;   // 2^-120 u is within TOP for every fp32 u
+constexpr float TOP = 256.0f;
+
+// Keys that a row tile's last row sees, from which its steps follow.
+template <int NT>
+__device__ __forceinline__ int seen_by(const AttnArgs& a, int64_t start, int n, int rt) {
+  if (start < 0 || start + n > a.c.capacity()) return 0;  // such sequences get NaN
+  const int i0 = rt * 16 * NT / a.G, i1 = min((rt * 16 * NT + 16 * NT - 1) / a.G, n - 1);
+  if (i0 >= n) return 0;
+  return (int)(start + (a.causal ? i1 + 1 : n));
+}
+__device__ __forceinline__ int steps_of(int seen) { return max(1, (seen + STEP - 1) / STEP); }
+
+template <int DT>
+struct Parts {  // how a head's columns fall on loads: whole 64, then 32, then 16, a quarter of each a lane group
+  static constexpr int N64 = DT / 64, N32 = DT % 64 / 32, N16 = DT % 32 / 16;
+  static constexpr int FRAGS = 2 * N64 + N32 + N16;
+  // First of the 8 (N16: 4) columns of lane group g in fragment f.
+  static __device__ __forceinline__ int col(int f, int g) {
+    return f < 2 * N64 ? 64 * (f / 2) + 16 * g + 8 * (f % 2) : N32 && f == 2 * N64 ? 64 * N64 + 8 * g : 64 * N64 + 32 * N32 + 4 * g;
+  }
+};
+
+template <int DT>
+struct Raw {  // a tile of 64 keys and values as it lies in memory
+  using P = Parts<DT>;
+  uint4 k64[4][P::N64 ? P::N64 : 1];
+  uint2 k32[4];
+  unsigned k16[4];
+  uint4 v[DT / 16];
+  float ks, vs;  // scales of block g; NaN where there is no such page
+};
+
+__device__ __forceinline__ bf16x8 eight(unsigned lo, unsigned hi, float s) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, s, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, s, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, s, false);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, s, true);
+  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// The high bits of those of four e4m3 numbers that are not finite: 0x7f of either sign, and under the largest scale,
+// 2^120, from 0x78 (256) on.
+__device__ __forceinline__ unsigned not_finite(unsigned w, float scale) {
+  return ((w & 0x7f7f7f7fu) + (scale < two_to(120) ? 0x01010101u : 0x08080808u)) & 0x80808080u;
+}
+
+template <typename T, int DT, int NT>
+struct Unit {
+  static constexpr int FRAGS = Parts<DT>::FRAGS, ND = DT / 16, TERMS = sizeof(T) == 4 ? 3 : 1;
+  const AttnArgs& a;
+  int lane, wave, g, r16, b, h, rt, n;
+  int64_t start;
+  bf16x8 q[NT][FRAGS][TERMS];
+  f32x4 acc[NT][ND];
+  f32x4 z[NT];  // the weights' sum, the same four times
+  float m[NT], unit[NT], off[NT];  // peak (of u 2^-e), scale 2^-e, -tau 2^-e
+  bf16x8 ones;
+  int e[NT], lim[NT];
+  int min_lim;
+
+  __device__ __forceinline__ Unit(const AttnArgs& args) : a(args) {
+    lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r16 = lane & 15;
+    for (int x = 0; x < 8; ++x) ones[x] = (bf16)1.0f;
+  }
+  __device__ __forceinline__ int row(int nt) const { return (rt * NT + nt) * 16 + r16; }
+  // The lane number and the head size anew, so that what a unit's begin and end compute from them is not held in
+  // registers (or spilled) over the tiles between.
+  __device__ __forceinline__ int anew() {
+    int d = a.c.d;
+    asm volatile("" : "+v"(lane), "+s"(d));
+    g = lane >> 4, r16 = lane & 15;
+    return d;
+  }
+
+  __device__ __forceinline__ void begin(int b_, int h_, int rt_) {
+    b = b_, h = h_, rt = rt_;
+    const int d = anew();
+    start = a.span.first(b), n = a.span.count(b);
+    const int i0 = rt * 16 * NT / a.G;
+    min_lim = a.causal ? (int)min(start + i0 + 1, (int64_t)(1 << 30)) : seen_by<NT>(a, start, n, rt);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = row(nt), i = r / a.G;
+      // rows without a query token see what others see: what they get is not stored
+      lim[nt] = a.causal && i < n ? (int)(start + i + 1) : (int)min(start + n, (int64_t)1 << 30);
+      const T* src = static_cast<const T*>(a.q) + b * a.qsb + (h * a.G + r % a.G) * a.qsh + i * a.qsn;
+#pragma unroll
+      for (int f = 0; f < FRAGS; ++f) {
+        const int col = Parts<DT>::col(f, g);
+        const int width = Parts<DT>::N16 && f == FRAGS - 1 ? 4 : 8;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          float v = 0;
+          if (i < n && x < width && col + x < d) v = to_f32(src[col + x]);
+#pragma unroll
+          for (int t = 0; t < TERMS; ++t) {
+            q[nt][f][t][x] = (bf16)v;
+            v -= (float)(bf16)v;
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < ND; ++j) acc[nt][j] = f32x4{0, 0, 0, 0};
+      z[nt] = f32x4{0, 0, 0, 0}, m[nt] = 0, e[nt] = E_FIRST;
+      rescale(nt);
+    }
+  }
+  __device__ __forceinline__ void rescale(int nt) {
+    const float s = two_to(-e[nt]);
+    unit[nt] = a.scale * s, off[nt] = -a.tau[0] * s;
+  }
+
+  // Where a tile's blocks lie: that of the lane's key rows, and block g.  The table's numbers are asked for a tile
+  // ahead of the rows that they name, before other loads, as loads come back in order.
+  struct Pages {
+    int k, v;
+  };
+  struct At {
+    int k, v;
+    bool there;
+  };
+  __device__ __forceinline__ Pages look(int key0) const {
+    const int* t = a.c.table + b * a.c.table_rs;
+    return Pages{t[min((key0 + 16 * (r16 >> 2)) >> a.c.page_shift, a.c.width - 1)],
+                 t[min((key0 + 16 * g) >> a.c.page_shift, a.c.width - 1)]};
+  }
+  __device__ __forceinline__ int block(int id, int key) const {
+    return (((unsigned)id < (unsigned)a.c.pages ? id : 0) * a.c.H + h) * (a.c.page >> 4) +
+           ((key & (a.c.page - 1)) >> 4);
+  }
+  __device__ __forceinline__ At find(const Pages& p, int key0) const {
+    return At{block(p.k, key0 + 16 * (r16 >> 2)), block(p.v, key0 + 16 * g), (unsigned)p.v < (unsigned)a.c.pages};
+  }
+  __device__ __forceinline__ void load_keys(const At& at, Raw<DT>& raw) const {
+    using P = Parts<DT>;
+    raw.ks = at.there ? two_to((int)a.c.k_scale[at.v] - 127) : __builtin_nanf("");
+    const uint8_t* kb = a.c.k + (int64_t)at.k * (BLOCK * DT) + (r16 & 3) * DT;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const uint8_t* p = kb + 4 * t * DT;
+#pragma unroll
+      for (int i = 0; i < P::N64; ++i) raw.k64[t][i] = *reinterpret_cast<const uint4*>(p + 64 * i + 16 * g);
+      if (P::N32) raw.k32[t] = *reinterpret_cast<const uint2*>(p + 64 * P::N64 + 8 * g);
+      if (P::N16) raw.k16[t] = *reinterpret_cast<const unsigned*>(p + 64 * P::N64 + 32 * P::N32 + 4 * g);
+    }
+  }
+  __device__ __forceinline__ void load_values(const At& at, Raw<DT>& raw) const {
+    raw.vs = two_to(min((int)a.c.v_scale[at.v], 247) - 127);  // never written ones may be anything
+    const uint8_t* vb = a.c.v + (int64_t)at.v * (BLOCK * DT) + r16 * 16;
+#pragma unroll
+    for (int j = 0; j < ND; ++j) raw.v[j] = *reinterpret_cast<const uint4*>(vb + 256 * j);
+  }
+  __device__ __forceinline__ bf16x8 key_frag(const Raw<DT>& raw, int t, int f) const {
+    using P = Parts<DT>;
+    if (f < 2 * P::N64) {
+      const uint4& w = raw.k64[t][f / 2];
+      return f % 2 ? eight(w.z, w.w, 1.0f) : eight(w.x, w.y, 1.0f);
+    }
+    if (P::N32 && f == 2 * P::N64) return eight(raw.k32[t].x, raw.k32[t].y, 1.0f);
+    return eight(raw.k16[t], 0, 1.0f);
+  }
+
+  // Scores of a tile's 16 keys for each of the lane's queries, as u 2^-e; EDGE: keys that a row does not see are 0.
+  template <bool EDGE>
+  __device__ __forceinline__ float scores(const f32x4 (&s)[4], const Raw<DT>& raw, int key0, int nt, float (&u)[16]) const {
+    const float c1 = raw.ks * unit[nt];
+    float top = m[nt];
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      u[x] = __builtin_elementwise_maximum(fmaf(s[x / 4][x % 4], c1, off[nt]), 0.0f);  // NaN stays
+      if (EDGE) u[x] = key0 + 16 * g + x < lim[nt] ? u[x] : 0.0f;
+      top = fmaxf(top, u[x]);
+    }
+    return top;
+  }
+  // A row whose score passes 2^8 2^e: the same e for its four lane groups, from the largest.
+  __device__ __forceinline__ void raise(float top, int nt) {
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    if (!(top > TOP) || e[nt] >= E_LAST) return;
+    int up = 100;  // of an infinite one, too
+    if (top < two_to(100)) frexpf(top, &up);
+    up = min(up, E_LAST - e[nt]);
+    const float f = ldexpf(1.0f, -10 * up);
+    z[nt] *= f, m[nt] = ldexpf(m[nt], -up), e[nt] += up;
+#pragma unroll
+    for (int j = 0; j < ND; ++j) acc[nt][j] *= f;
+    rescale(nt);
+  }
+
+  // One tile.  Its keys' and values' registers take the next tile's as soon as they have been used (`more`), so that
+  // those loads are on their way over half of the work each.
+  template <bool EDGE>
+  __device__ __forceinline__ void tile(Raw<DT>& raw, int key0, bool more, Pages& next) {
+    At at;
+    f32x4 s[NT][4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[nt][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int f = 0; f < FRAGS; ++f) {
+        const bf16x8 kf = key_frag(raw, t, f);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < TERMS; ++i) s[nt][t] = mfma16x16x32(kf, q[nt][f][i], s[nt][t]);
+      }
+    }
+    bf16x8 p[NT][2][TERMS];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float u[16];
+      float top = scores<EDGE>(s[nt], raw, key0, nt, u);
+      while (__builtin_expect(__any(top > TOP && e[nt] < E_LAST), 0)) {
+        raise(top, nt);
+        top = scores<EDGE>(s[nt], raw, key0, nt, u);
+      }
+      m[nt] = top;
+      if (nt == NT - 1 && more) {
+        at = find(next, key0 + STEP);
+        next = look(key0 + 2 * STEP);
+        load_keys(at, raw);
+      }
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const float x2 = u[x] * u[x], x4 = x2 * x2;
+        float w = x4 * x4 * x2;
+#pragma unroll
+        for (int k = 0; k < TERMS; ++k) {
+          const bf16 r = (bf16)w;
+          p[nt][x / 8][k][x % 8] = r;
+          w -= (float)r;
+        }
+      }
+      // the weights' sum, over all lane groups: a product with ones
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int k = 0; k < TERMS; ++k) z[nt] = mfma16x16x32(ones, p[nt][hf][k], z[nt]);
+    }
+    if (EDGE) values_edge(raw, key0);
+#pragma unroll
+    for (int j = 0; j < ND; ++j)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const bf16x8 v = value_frag(raw, j, hf);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < TERMS; ++i) acc[nt][j] = mfma16x16x32(v, p[nt][hf][i], acc[nt][j]);
+      }
+    if (more) load_values(at, raw);
+  }
+  __device__ __forceinline__ bf16x8 value_frag(const Raw<DT>& raw, int j, int hf) const {
+    return hf ? eight(raw.v[j].z, raw.v[j].w, raw.vs) : eight(raw.v[j].x, raw.v[j].y, raw.vs);
+  }
+  // In a tile that some row does not see whole, values that are not finite count as zeros, and a row that sees one gets
+  // NaN there: a weight of zero would make NaN of them.
+  __device__ __forceinline__ void values_edge(Raw<DT>& raw, int key0) {
+    unsigned any = 0;
+#pragma unroll
+    for (int j = 0; j < ND; ++j)
+      any |= not_finite(raw.v[j].x, raw.vs) | not_finite(raw.v[j].y, raw.vs) | not_finite(raw.v[j].z, raw.vs) |
+             not_finite(raw.v[j].w, raw.vs);
+    if (__builtin_expect(!__any(any != 0), 1)) return;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      bf16x8 sees[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < 8; ++x) sees[nt][x] = (bf16)(key0 + 16 * g + 8 * hf + x < lim[nt] ? 1.0f : 0.0f);
+#pragma unroll
+      for (int j = 0; j < ND; ++j) {
+        unsigned& lo = hf ? raw.v[j].z : raw.v[j].x;
+        unsigned& hi = hf ? raw.v[j].w : raw.v[j].y;
+        const unsigned bl = not_finite(lo, raw.vs) >> 7, bh = not_finite(hi, raw.vs) >> 7;
+        lo &= ~(bl * 0xff), hi &= ~(bh * 0xff);
+        const bf16x8 bad = eight(bl * 0x38, bh * 0x38, 1.0f);  // 0x38: one
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const f32x4 hit = mfma16x16x32(bad, sees[nt], f32x4{0, 0, 0, 0});
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (hit[i] > 0) acc[nt][j][i] = __builtin_nanf("");
+        }
+      }
+    }
+  }
+
+  // The steps [s0, s1) of the unit, of which the wave has one tile each.
+  __device__ __forceinline__ void run(int s0, int s1) {
+    const int seen = seen_by<NT>(a, start, n, rt);
+    const int keys = min(seen, s1 * STEP);
+    int key0 = s0 * STEP + wave * TILE;
+    if (key0 >= keys) return;
+    Raw<DT> raw;
+    Pages next = look(key0);
+    const At at = find(next, key0);
+    next = look(key0 + STEP);
+    load_keys(at, raw), load_values(at, raw);
+    for (; key0 + TILE <= min_lim; key0 += STEP) {  // tiles that every row sees whole come first
+      const bool more = key0 + STEP < keys;
+      tile<false>(raw, key0, more, next);
+      if (!more) return;
+    }
+    for (; key0 < keys; key0 += STEP) tile<true>(raw, key0, key0 + STEP < keys, next);
+  }
+
+  // Adds up the four waves' sums in wave 0, in a fixed order.
+  struct Lds {
+    float z[WAVES][16 * NT], m[WAVES][16 * NT];
+    int e[WAVES][16 * NT];
+    float slab[2][NT * ND * 4 * 64];
+  };
+  __device__ __forceinline__ void join(Lds& s) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int o = 16; o <= 32; o *= 2) m[nt] = fmaxf(m[nt], __shfl_xor(m[nt], o, 64));
+      if (g == 0) s.z[wave][16 * nt + r16] = z[nt][0], s.m[wave][16 * nt + r16] = m[nt], s.e[wave][16 * nt + r16] = e[nt];
+    }
+    __syncthreads();
+    const bool used = row(0) < a.G * n;  // of the first row tile's columns: one query token needs few of 16
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      int top = E_FIRST;
+      for (int w = 0; w < WAVES; ++w) top = max(top, s.e[w][16 * nt + r16]);
+      const float f = ldexpf(1.0f, 10 * (e[nt] - top));
+#pragma unroll
+      for (int j = 0; j < ND; ++j) acc[nt][j] *= f;
+      float zs = 0, ms = 0;
+      for (int w = 0; w < WAVES; ++w) {
+        const int up = s.e[w][16 * nt + r16] - top;
+        zs += s.z[w][16 * nt + r16] * ldexpf(1.0f, 10 * up);
+        ms = fmaxf(ms, ldexpf(s.m[w][16 * nt + r16], up));
+      }
+      z[nt][0] = zs, m[nt] = ms, e[nt] = top;
+    }
+    if (wave >= 2) put(s.slab[wave - 2], used);
+    __syncthreads();
+    if (wave < 2) add(s.slab[wave], used);
+    __syncthreads();
+    if (wave == 1) put(s.slab[0], used);
+    __syncthreads();
+    if (wave == 0) add(s.slab[0], used);
+    __syncthreads();
+  }
+  __device__ __forceinline__ void put(float* slab, bool used) const {
+    if (!used) return;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < ND; ++j)
+        *reinterpret_cast<f32x4*>(slab + ((nt * ND + j) * 64 + lane) * 4) = acc[nt][j];
+  }
+  __device__ __forceinline__ void add(const float* slab, bool used) {
+    if (!used) return;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < ND; ++j)
+        acc[nt][j] += *reinterpret_cast<const f32x4*>(slab + ((nt * ND + j) * 64 + lane) * 4);
+  }
+
+  __device__ __forceinline__ bool refused() const { return start < 0 || start + n > a.c.capacity(); }
+  __device__ __forceinline__ void store() {  // wave 0, the whole unit
+    const int d = anew();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = row(nt), i = r / a.G;
+      if (i >= a.span.N) continue;
+      const float f = factor(a, z[nt][0], m[nt], e[nt]);
+      T* to = static_cast<T*>(a.o) + b * a.osb + (h * a.G + r % a.G) * a.osh + i * a.osn;
+#pragma unroll
+      for (int j = 0; j < ND; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int col = 16 * j + 4 * g + x;
+          float v = acc[nt][j][x] * f;
+          if (refused()) v = __builtin_nanf("");
+          if (i >= n) v = 0;  // no query token
+          if (col < d) to[col] = from_f32<T>(v);
+        }
+    }
+  }
+  __device__ __forceinline__ void keep(int slot) {  // wave 0, a piece of the unit
+    anew();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = 16 * nt + r16;
+      if (row(nt) >= a.G * n) continue;
+      float* st = a.stats + (int64_t)slot * 3 * 16 * NT + r;
+      if (g == 0) st[0] = z[nt][0], st[16 * NT] = m[nt], st[2 * 16 * NT] = (float)e[nt];
+      float* to = a.acc + ((int64_t)slot * 16 * NT + r) * DT + 4 * g;
+#pragma unroll
+      for (int j = 0; j < ND; ++j) *reinterpret_cast<f32x4*>(to + 16 * j) = acc[nt][j];
+    }
+  }
+  // What the weighted sum of a row is multiplied by: gate / (sum + 1e-12), both sums in units of 2^(10 e).
+  static __device__ __forceinline__ float factor(const AttnArgs& a, float z, float m, int e) {
+    const float peak = ldexpf(m, e);
+    const float gate = a.has_gamma ? peak / (peak + a.gamma) : 1.0f;
+    return gate / (z + ldexpf(1e-12f, -10 * e));
+  }
+};
+
+// Consecutive shares on one XCD (workgroups go to the eight in turn), where neighbouring row tiles find each other's
+// keys in its L2.
+__device__ __forceinline__ int64_t place(int64_t wg, int64_t n) {
+  const int64_t each = n / 8, more = n % 8, x = wg % 8;
+  return x * each + min(x, more) + wg / 8;
+}
+
+template <typename T, int DT, int NT>
+__global__ __launch_bounds__(THREADS, DT * NT <= 128 ? 2 : 1) void attn_kernel(AttnArgs a) {
+  __shared__ typename Unit<T, DT, NT>::Lds lds;
+  __shared__ int64_t before[THREADS + 1];  // the steps of all sequences before each of 256 groups of them
+  __shared__ int64_t wave_sum[WAVES];
+  Unit<T, DT, NT> u(a);
+  const int w = (int)place(blockIdx.x, gridDim.x);
+  const auto steps_at = [&](int b, int rt) { return steps_of(seen_by<NT>(a, a.span.first(b), a.span.count(b), rt)); };
+  int b, h, rt;
+  int64_t at = 0, end, share = 0, skip = 0;  // steps [at, end) of the call, from step `skip` of unit (b, h, rt) on
+  if (a.shares) {
+    const auto steps_of_sequence = [&](int b) {
+      int64_t t = 0;
+      for (int rt = 0; rt < a.R; ++rt) t += steps_at(b, rt);
+      return t * a.c.H;
+    };
+    const int per = (a.c.B + THREADS - 1) / THREADS;
+    int64_t mine = 0;
+    for (int i = 0; i < per; ++i) {
+      const int x = threadIdx.x * per + i;
+      if (x < a.c.B) mine += steps_of_sequence(x);
+    }
+    int64_t sum = mine;
+    for (int o = 1; o < 64; o *= 2) {
+      const int64_t x = __shfl_up(sum, o, 64);
+      if (u.lane >= o) sum += x;
+    }
+    if (u.lane == 63) wave_sum[u.wave] = sum;
+    __syncthreads();
+    for (int i = 0; i < u.wave; ++i) sum += wave_sum[i];
+    before[threadIdx.x + 1] = sum;
+    if (threadIdx.x == 0) before[0] = 0;
+    __syncthreads();
+    const int64_t all = before[THREADS];
+    share = (all + a.shares - 1) / a.shares;
+    at = w * share, end = min(all, at + share);
+    if (threadIdx.x < 2) a.headers[2 * w + threadIdx.x].first = -1;
+    if (at >= end) return;
+    int lo = 0, hi = THREADS;  // before[lo] <= at < before[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (before[mid] <= at) lo = mid;
+      else hi = mid;
+    }
+    skip = at - before[lo], b = lo * per;
+    for (;;) {
+      const int64_t t = steps_of_sequence(b);
+      if (skip < t) break;
+      skip -= t, ++b;
+    }
+    const int64_t head = steps_of_sequence(b) / a.c.H;
+    h = (int)(skip / head), rt = 0, skip %= head;
+    for (;;) {
+      const int t = steps_at(b, rt);
+      if (skip < t) break;
+      skip -= t, ++rt;
+    }
+  } else {
+    rt = a.R - 1 - w % a.R;  // the longest first
+    b = w / a.R / a.c.H, h = w / a.R % a.c.H;
+    end = steps_at(b, rt);
+  }
+  while (at < end) {
+    u.begin(b, h, rt);
+    const int t = steps_at(b, rt);
+    const int s0 = (int)skip, s1 = (int)min((int64_t)t, s0 + end - at);
+    u.run(s0, s1);
+    u.join(lds);
+    if (u.wave == 0) {
+      if (s0 == 0 && s1 == t) {
+        u.store();
+      } else {
+        const int slot = 2 * w + (s0 == 0);
+        u.keep(slot);
+        if (threadIdx.x == 0)
+          a.headers[slot] = Header{b, h, rt, (int)((at - s0) / share), (int)((at - s0 + t - 1) / share)};
+      }
+    }
+    at += s1 - s0, skip = 0;
+    if (++rt == a.R) {
+      rt = 0;
+      if (++h == a.c.H) h = 0, ++b;
+    }
+  }
+}
+
+// Joins the units that were cut.  Each workgroup that has a piece of a unit joins an equal part of its results: a
+// unit of few rows over a long cache has hundreds of pieces, and one workgroup for each unit took 103 us where this
+// takes 9 (2 sequences of 131072 tokens, 32 heads of 128 on 8).
+template <typename T, int DT, int NT>
+__global__ __launch_bounds__(THREADS) void join_kernel(AttnArgs a) {
+  constexpr int ROWS = 16 * NT;
+  __shared__ float sums[THREADS], row_z[ROWS], row_m[ROWS], row_top[ROWS];
+  const Header u = a.headers[blockIdx.x];
+  if (u.first < 0) return;
+  const int n = u.last - u.first + 1, me = (int)blockIdx.x / 2 - u.first;
+  const auto slot = [&](int i) { return 2ll * (u.first + i) + (i == 0); };
+  const int count = a.span.count(u.b);
+  const int rows = min(ROWS, a.G * a.span.N - u.rt * ROWS), live = min(rows, a.G * count - u.rt * ROWS);
+  const int64_t start = a.span.first(u.b);
+  const bool refused = start < 0 || start + count > a.c.capacity();
+  const int all = rows * a.c.d, x0 = (int)((int64_t)all * me / n), x1 = (int)((int64_t)all * (me + 1) / n);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int r = x0 / a.c.d + wave; r < live && r * a.c.d < x1; r += WAVES) {  // a wave a row
+    float top = E_FIRST, z = 0, m = 0;
+    for (int i = lane; i < n; i += 64) top = fmaxf(top, a.stats[slot(i) * 3 * ROWS + 2 * ROWS + r]);
+    top = wave_max(top);
+    for (int i = lane; i < n; i += 64) {
+      const float* st = a.stats + slot(i) * 3 * ROWS + r;
+      const int up = (int)(st[2 * ROWS] - top);
+      z += st[0] * ldexpf(1.0f, 10 * up), m = fmaxf(m, ldexpf(st[ROWS], up));
+    }
+    z = wave_sum(z), m = wave_max(m);
+    if (lane == 0) row_z[r] = z, row_m[r] = m, row_top[r] = top;
+  }
+  __syncthreads();
+  int width = 1;  // results at a time; the other threads take other pieces
+  while (width < THREADS && width < x1 - x0) width *= 2;
+  const int each = THREADS / width, part = threadIdx.x / width;
+  for (int base = x0; base < x1; base += width) {
+    const int x = base + threadIdx.x % width, r = x / a.c.d, col = x % a.c.d;
+    float v = 0;
+    if (x < x1 && r < live)
+      for (int i = part; i < n; i += each) {
+        const int up = (int)(a.stats[slot(i) * 3 * ROWS + 2 * ROWS + r] - row_top[r]);
+        v += a.acc[(slot(i) * ROWS + r) * DT + col] * ldexpf(1.0f, 10 * up);
+      }
+    sums[threadIdx.x] = v;
+    __syncthreads();
+    if (part == 0 && x < x1) {
+      for (int i = 1; i < each; ++i) v += sums[i * width + threadIdx.x];
+      if (r < live) v *= Unit<T, DT, NT>::factor(a, row_z[r], row_m[r], (int)row_top[r]);
+      if (refused && r < live) v = __builtin_nanf("");
+      const int row = u.rt * ROWS + r;
+      static_cast<T*>(a.o)[u.b * a.osb + (u.h * a.G + row % a.G) * a.osh + row / a.G * a.osn + col] = from_f32<T>(v);
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T, int DT, int NT>
+int run(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
+  attn_kernel<T, DT, NT><<<dim3((unsigned)(p.shares ? p.shares : p.units)), dim3(THREADS), 0, st>>>(a);
+  if (int rc = launch_status("cached_attn")) return rc;
+  if (!p.shares) return PNFX_OK;
+  join_kernel<T, DT, NT><<<dim3((unsigned)(2 * p.shares)), dim3(THREADS), 0, st>>>(a);
+  return launch_status("cached_attn");
+}
+
+template <typename T, int DT>
+int run_rows(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
+  if constexpr (DT <= 128) {
+    if (p.NT == 2) return run<T, DT, 2>(a, p, st);
+  }
+  return run<T, DT, 1>(a, p, st);
+}
+
+}  // namespace
+}  // namespace pnfx

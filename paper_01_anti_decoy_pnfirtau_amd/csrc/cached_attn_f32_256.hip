@@ -1,0 +1,17 @@
+// Attention over the 8-bit cache: fp32 queries, head sizes 144 to 256.
+#include "cached_attn.h"
+
+int pnfx::attn_f32_256(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
+  switch (a.c.D) {
+    case 144: return run_rows<float, 144>(a, p, st);
+    case 160: return run_rows<float, 160>(a, p, st);
+    case 176: return run_rows<float, 176>(a, p, st);
+    case 192: return run_rows<float, 192>(a, p, st);
+    case 208: return run_rows<float, 208>(a, p, st);
+    case 224: return run_rows<float, 224>(a, p, st);
+    case 240: return run_rows<float, 240>(a, p, st);
+    case 256: return run_rows<float, 256>(a, p, st);
+  }
+  set_error("cached_attn: head size %d", a.c.D);
+  return PNFX_EUNSUPPORTED;
+}
