@@ -403,7 +403,7 @@ int pnfx_cache_append(const pnfx_cache* cache, const void* k, int64_t ksb, int64
                       int dtype, void* stream);
 int pnfx_cache_read(const pnfx_cache* cache, const int32_t* first, int64_t first_all, int64_t count, void* k,
                     void* v, int dtype, void* stream);
-int64_t pnfx_cached_attn_workspace_size(const pnfx_cache* cache, int64_t Hq, int64_t N);
+int64_t pnfx_cached_attn_workspace_size(const pnfx_cache* cache, int64_t Hq, int64_t N, int dtype);
 int pnfx_cached_attn(const pnfx_cache* cache, const void* q, int64_t qsb, int64_t qsh, int64_t qsn, void* o,
                      int64_t osb, int64_t osh, int64_t osn, int64_t Hq, int64_t N, const int32_t* start,
                      int64_t start_all, const int32_t* counts, const float* tau, float scale, float gamma,

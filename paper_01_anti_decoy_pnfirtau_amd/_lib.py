@@ -96,7 +96,7 @@ def _declare(lib: ctypes.CDLL) -> None:
     cache = ctypes.POINTER(PnfxCache)
     sig["pnfx_cache_append"] = ([cache] + [vp, i64, i64, i64] * 2 + [i64, vp, i64, vp, vp, i64, i32, i32, vp], i32)
     sig["pnfx_cache_read"] = ([cache, vp, i64, i64, vp, vp, i32, vp], i32)
-    sig["pnfx_cached_attn_workspace_size"] = ([cache, i64, i64], i64)
+    sig["pnfx_cached_attn_workspace_size"] = ([cache, i64, i64, i32], i64)
     sig["pnfx_cached_attn"] = ([cache] + [vp, i64, i64, i64] * 2
                                + [i64, i64, vp, i64, vp, vp, f32, f32, i32, i32, i32, vp, i64, vp], i32)
     sig["pnfx_sample"] = ([vp, i64, i64, i64, vp, ctypes.POINTER(PnfxSampling), vp, i32, vp], i32)

@@ -16,8 +16,9 @@
 // a fixed number of workgroups, whatever the lengths, which only the device knows; a unit that several workgroups
 // have pieces of is joined by a second kernel.
 //
-// The powers are taken of u 2^-e with one e a row, raised (and the sums scaled, exactly) only when a score passes
-// 2^8 2^e: a power of ten of the tenth lies within fp32 for scores 2^8 above and 2^12 below.  bf16 queries: the
+// The powers are taken of u 2^-e with one e a row: 0 or, where a row's first scores are below 2^-8, less; raised (and
+// the sums scaled, exactly) when a score passes 2^8 2^e.  Up to there the power is 2^80, which leaves room for 2^40
+// keys, and it is within fp32 down to 2^-12 2^e, 2^-120 of one at the border.  bf16 queries: the
 // weights are rounded to bf16 for the product and the same rounded values are summed, as the dense kernels do.  fp32
 // queries: queries and weights as three bf16 parts each (24 bits), keys and values are exact in one.
 #pragma once
@@ -57,6 +58,11 @@ struct AttnPlan {
   int64_t bytes() const { return header_bytes + acc_bytes + stat_bytes; }
 };
 
+// Workgroups of a kernel that a CU holds, by its registers: no fewer and no more shares than they all have slots.
+constexpr int resident(int bytes, int D, int NT) {
+  return bytes == 2 && D * NT <= 64 ? 3 : D * NT <= 128 ? 2 : 1;
+}
+
 // The kernels, by the type of the queries and the head size in the cache.
 int attn_bf16_64(const AttnArgs& a, const AttnPlan& p, hipStream_t st);    // up to 64
 int attn_bf16_128(const AttnArgs& a, const AttnPlan& p, hipStream_t st);   // up to 128
@@ -70,9 +76,9 @@ namespace {
 typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int THREADS = 256, WAVES = 4, TILE = 64, STEP = WAVES * TILE;
-constexpr int E_FIRST = -60;  // of a row without scores: 2^60 u is finite for u up to 2^67, and larger ones raise it again
-constexpr int E_LAST = 120;   // 2^-120 u is within TOP for every fp32 u
-constexpr float TOP = 256.0f;
+constexpr int E_LAST = 120;  // 2^-120 u is within TOP for every fp32 u
+constexpr int E_LEAST = -60, E_NONE = -100;  // of a row without scores, once it is joined
+constexpr float TOP = 256.0f, LOW = 1 / 256.0f;
 
 // Keys that a row tile's last row sees, from which its steps follow.
 template <int NT>
@@ -118,6 +124,12 @@ __device__ __forceinline__ unsigned not_finite(unsigned w, float scale) {
   return ((w & 0x7f7f7f7fu) + (scale < two_to(120) ? 0x01010101u : 0x08080808u)) & 0x80808080u;
 }
 
+// What all lanes hold the same, as a scalar.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  return (int64_t)((uint64_t)(unsigned)uniform((int)(x >> 32)) << 32 | (unsigned)uniform((int)x));
+}
+
 template <typename T, int DT, int NT>
 struct Unit {
   static constexpr int FRAGS = Parts<DT>::FRAGS, ND = DT / 16, TERMS = sizeof(T) == 4 ? 3 : 1;
@@ -133,7 +145,7 @@ struct Unit {
   int min_lim;
 
   __device__ __forceinline__ Unit(const AttnArgs& args) : a(args) {
-    lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r16 = lane & 15;
+    lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), g = lane >> 4, r16 = lane & 15;
     for (int x = 0; x < 8; ++x) ones[x] = (bf16)1.0f;
   }
   __device__ __forceinline__ int row(int nt) const { return (rt * NT + nt) * 16 + r16; }
@@ -175,7 +187,7 @@ struct Unit {
       }
 #pragma unroll
       for (int j = 0; j < ND; ++j) acc[nt][j] = f32x4{0, 0, 0, 0};
-      z[nt] = f32x4{0, 0, 0, 0}, m[nt] = 0, e[nt] = E_FIRST;
+      z[nt] = f32x4{0, 0, 0, 0}, m[nt] = 0, e[nt] = 0;
       rescale(nt);
     }
   }
@@ -234,31 +246,25 @@ struct Unit {
     return eight(raw.k16[t], 0, 1.0f);
   }
 
-  // Scores of a tile's 16 keys for each of the lane's queries, as u 2^-e; EDGE: keys that a row does not see are 0.
-  template <bool EDGE>
-  __device__ __forceinline__ float scores(const f32x4 (&s)[4], const Raw<DT>& raw, int key0, int nt, float (&u)[16]) const {
-    const float c1 = raw.ks * unit[nt];
-    float top = m[nt];
-#pragma unroll
-    for (int x = 0; x < 16; ++x) {
-      u[x] = __builtin_elementwise_maximum(fmaf(s[x / 4][x % 4], c1, off[nt]), 0.0f);  // NaN stays
-      if (EDGE) u[x] = key0 + 16 * g + x < lim[nt] ? u[x] : 0.0f;
-      top = fmaxf(top, u[x]);
-    }
-    return top;
-  }
-  // A row whose score passes 2^8 2^e: the same e for its four lane groups, from the largest.
-  __device__ __forceinline__ void raise(float top, int nt) {
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    if (!(top > TOP) || e[nt] >= E_LAST) return;
-    int up = 100;  // of an infinite one, too
-    if (top < two_to(100)) frexpf(top, &up);
-    up = min(up, E_LAST - e[nt]);
-    const float f = ldexpf(1.0f, -10 * up);
+  // A row whose scores pass 2^8 2^e, or whose first ones are all below 2^-8: another e, the same for its four lane
+  // groups, from the largest.
+  __device__ __forceinline__ void another_e(float (&u)[16], float before, int nt) {
+    const auto of_row = [](float x) {
+      x = fmaxf(x, __shfl_xor(x, 16, 64));
+      return fmaxf(x, __shfl_xor(x, 32, 64));
+    };
+    const float top = of_row(m[nt]), was = of_row(before);
+    int up = E_LAST;  // of an infinite one
+    if (top < __builtin_inff()) frexpf(top, &up);
+    if (top > TOP) up = min(up, E_LAST - e[nt]);
+    else if (was == 0 && top > 0 && top < LOW) up = max(up, E_LEAST);
+    else return;
+    const float f = was == 0 ? 1.0f : ldexpf(1.0f, -10 * up);
     z[nt] *= f, m[nt] = ldexpf(m[nt], -up), e[nt] += up;
 #pragma unroll
     for (int j = 0; j < ND; ++j) acc[nt][j] *= f;
+#pragma unroll
+    for (int x = 0; x < 16; ++x) u[x] = ldexpf(u[x], -up);
     rescale(nt);
   }
 
@@ -267,38 +273,47 @@ struct Unit {
   template <bool EDGE>
   __device__ __forceinline__ void tile(Raw<DT>& raw, int key0, bool more, Pages& next) {
     At at;
-    f32x4 s[NT][4];
+    float u[NT][16], before[NT];  // u 2^-e of the lane's 16 keys; m
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) before[nt] = m[nt];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
+      f32x4 s[NT];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[nt][t] = f32x4{0, 0, 0, 0};
+      for (int nt = 0; nt < NT; ++nt) s[nt] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int f = 0; f < FRAGS; ++f) {
         const bf16x8 kf = key_frag(raw, t, f);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int i = 0; i < TERMS; ++i) s[nt][t] = mfma16x16x32(kf, q[nt][f][i], s[nt][t]);
+          for (int i = 0; i < TERMS; ++i) s[nt] = mfma16x16x32(kf, q[nt][f][i], s[nt]);
       }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float c1 = raw.ks * unit[nt];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x = __builtin_elementwise_maximum(fmaf(s[nt][i], c1, off[nt]), 0.0f);  // NaN stays
+          if (EDGE) x = key0 + 16 * g + 4 * t + i < lim[nt] ? x : 0.0f;
+          m[nt] = fmaxf(m[nt], x);
+          u[nt][4 * t + i] = x;
+        }
+      }
+    }
+    if (more) {
+      at = find(next, key0 + STEP);
+      next = look(key0 + 2 * STEP);
+      load_keys(at, raw);
     }
     bf16x8 p[NT][2][TERMS];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float u[16];
-      float top = scores<EDGE>(s[nt], raw, key0, nt, u);
-      while (__builtin_expect(__any(top > TOP && e[nt] < E_LAST), 0)) {
-        raise(top, nt);
-        top = scores<EDGE>(s[nt], raw, key0, nt, u);
-      }
-      m[nt] = top;
-      if (nt == NT - 1 && more) {
-        at = find(next, key0 + STEP);
-        next = look(key0 + 2 * STEP);
-        load_keys(at, raw);
-      }
+      const bool high = m[nt] > TOP && e[nt] < E_LAST, low = before[nt] == 0 && m[nt] > 0 && m[nt] < LOW;
+      if (__builtin_expect(__any(high || low), 0)) another_e(u[nt], before[nt], nt);
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
-        const float x2 = u[x] * u[x], x4 = x2 * x2;
+        const float x2 = u[nt][x] * u[nt][x], x4 = x2 * x2;
         float w = x4 * x4 * x2;
 #pragma unroll
         for (int k = 0; k < TERMS; ++k) {
@@ -393,13 +408,14 @@ struct Unit {
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int o = 16; o <= 32; o *= 2) m[nt] = fmaxf(m[nt], __shfl_xor(m[nt], o, 64));
+      if (m[nt] == 0) e[nt] = E_NONE;
       if (g == 0) s.z[wave][16 * nt + r16] = z[nt][0], s.m[wave][16 * nt + r16] = m[nt], s.e[wave][16 * nt + r16] = e[nt];
     }
     __syncthreads();
     const bool used = row(0) < a.G * n;  // of the first row tile's columns: one query token needs few of 16
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      int top = E_FIRST;
+      int top = E_NONE;
       for (int w = 0; w < WAVES; ++w) top = max(top, s.e[w][16 * nt + r16]);
       const float f = ldexpf(1.0f, 10 * (e[nt] - top));
 #pragma unroll
@@ -488,7 +504,7 @@ __device__ __forceinline__ int64_t place(int64_t wg, int64_t n) {
 }
 
 template <typename T, int DT, int NT>
-__global__ __launch_bounds__(THREADS, DT * NT <= 128 ? 2 : 1) void attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(THREADS, resident(sizeof(T), DT, NT)) void attn_kernel(AttnArgs a) {
   __shared__ typename Unit<T, DT, NT>::Lds lds;
   __shared__ int64_t before[THREADS + 1];  // the steps of all sequences before each of 256 groups of them
   __shared__ int64_t wave_sum[WAVES];
@@ -520,7 +536,7 @@ __global__ __launch_bounds__(THREADS, DT * NT <= 128 ? 2 : 1) void attn_kernel(A
     before[threadIdx.x + 1] = sum;
     if (threadIdx.x == 0) before[0] = 0;
     __syncthreads();
-    const int64_t all = before[THREADS];
+    const int64_t all = uniform(before[THREADS]);
     share = (all + a.shares - 1) / a.shares;
     at = w * share, end = min(all, at + share);
     if (threadIdx.x < 2) a.headers[2 * w + threadIdx.x].first = -1;
@@ -528,10 +544,10 @@ __global__ __launch_bounds__(THREADS, DT * NT <= 128 ? 2 : 1) void attn_kernel(A
     int lo = 0, hi = THREADS;  // before[lo] <= at < before[hi]
     while (hi - lo > 1) {
       const int mid = (lo + hi) / 2;
-      if (before[mid] <= at) lo = mid;
+      if (uniform(before[mid]) <= at) lo = mid;
       else hi = mid;
     }
-    skip = at - before[lo], b = lo * per;
+    skip = at - uniform(before[lo]), b = lo * per;
     for (;;) {
       const int64_t t = steps_of_sequence(b);
       if (skip < t) break;
@@ -591,7 +607,7 @@ __global__ __launch_bounds__(THREADS) void join_kernel(AttnArgs a) {
   const int all = rows * a.c.d, x0 = (int)((int64_t)all * me / n), x1 = (int)((int64_t)all * (me + 1) / n);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int r = x0 / a.c.d + wave; r < live && r * a.c.d < x1; r += WAVES) {  // a wave a row
-    float top = E_FIRST, z = 0, m = 0;
+    float top = E_NONE, z = 0, m = 0;
     for (int i = lane; i < n; i += 64) top = fmaxf(top, a.stats[slot(i) * 3 * ROWS + 2 * ROWS + r]);
     top = wave_max(top);
     for (int i = lane; i < n; i += 64) {

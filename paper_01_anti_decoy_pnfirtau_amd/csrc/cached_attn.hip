@@ -5,7 +5,7 @@
 namespace pnfx {
 namespace {
 
-AttnPlan plan_of(int64_t B, int64_t H, int64_t G, int64_t N, int D, int64_t capacity) {
+AttnPlan plan_of(int64_t B, int64_t H, int64_t G, int64_t N, int D, int64_t capacity, int bytes) {
   AttnPlan p = {};
   const int64_t rows = G * N;
   p.NT = rows <= 16 || D > 128 ? 1 : 2;
@@ -15,7 +15,7 @@ AttnPlan plan_of(int64_t B, int64_t H, int64_t G, int64_t N, int D, int64_t capa
   // One workgroup a unit where no cut can gain: short caches, whose few steps cost less than the join's launch, and
   // enough row tiles for the card to even out by itself.
   if (steps <= 2 || (p.R > 1 && p.units >= 2048)) return p;
-  p.shares = (int)std::min<int64_t>(p.units * steps, 1024);
+  p.shares = (int)std::min<int64_t>(p.units * steps, 256 * resident(bytes, D, p.NT));
   const auto round = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
   p.header_bytes = round(2ll * p.shares * (int64_t)sizeof(Header));
   p.acc_bytes = round(2ll * p.shares * 16 * p.NT * D * 4);
@@ -32,11 +32,11 @@ int run_any(const AttnArgs& a, const AttnPlan& p, int dtype, hipStream_t st) {
 }  // namespace
 }  // namespace pnfx
 
-extern "C" int64_t pnfx_cached_attn_workspace_size(const pnfx_cache* cache, int64_t Hq, int64_t N) {
+extern "C" int64_t pnfx_cached_attn_workspace_size(const pnfx_cache* cache, int64_t Hq, int64_t N, int dtype) {
   using namespace pnfx;
   Cache c;
   if (cache_of(cache, "cached_attn", &c) || N < 1 || Hq < c.H || Hq % c.H) return 0;
-  return plan_of(c.B, c.H, Hq / c.H, N, c.D, c.capacity()).bytes();
+  return plan_of(c.B, c.H, Hq / c.H, N, c.D, c.capacity(), dtype == PNFX_F32 ? 4 : 2).bytes();
 }
 
 extern "C" int pnfx_cached_attn(const pnfx_cache* cache, const void* q, int64_t qsb, int64_t qsh, int64_t qsn, void* o,
@@ -53,7 +53,7 @@ extern "C" int pnfx_cached_attn(const pnfx_cache* cache, const void* q, int64_t 
                (long long)Hq, a.c.H);
   PNFX_REQUIRE(N >= 1 && Hq / a.c.H * N < (1ll << 31) - 64, "cached_attn: N=%lld", (long long)N);
   PNFX_REQUIRE(start || (start_all >= 0 && start_all < (1ll << 31)), "cached_attn: start %lld", (long long)start_all);
-  const AttnPlan p = plan_of(a.c.B, a.c.H, Hq / a.c.H, N, a.c.D, a.c.capacity());
+  const AttnPlan p = plan_of(a.c.B, a.c.H, Hq / a.c.H, N, a.c.D, a.c.capacity(), dtype == PNFX_F32 ? 4 : 2);
   PNFX_REQUIRE(p.units * THREADS < (1ll << 32), "cached_attn: %lld row tiles in one call", (long long)p.units);
   PNFX_REQUIRE(!p.bytes() || (workspace && workspace_bytes >= p.bytes() &&
                               (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),

@@ -539,7 +539,7 @@ Tensor cached_attn_cuda(const Tensor& q_in, const Tensor& ck, const Tensor& cv, 
   Tensor hold[2], ws;
   const int32_t* s = each_of<int32_t>(what, "start", start, at::kInt, c.B, ck, hold[0]);
   const int32_t* n = each_of<int32_t>(what, "counts", counts, at::kInt, c.B, ck, hold[1]);
-  const int64_t wsb = pnfx_cached_attn_workspace_size(&c, Hq, N);
+  const int64_t wsb = pnfx_cached_attn_workspace_size(&c, Hq, N, code);
   if (wsb) ws = at::empty({wsb}, ck.options());
   check_rc(pnfx_cached_attn(&c, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), o.data_ptr(), o.stride(0),
                             o.stride(1), o.stride(2), Hq, N, s, start_all, n, t32.data_ptr<float>(), (float)scale,
