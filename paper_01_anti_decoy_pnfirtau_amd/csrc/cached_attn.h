@@ -10,11 +10,11 @@
 // memory in 16-byte loads, the next tile's while this one is worked on.  Scales are powers of two, so e4m3 times scale
 // is exact in bf16, and a block's key scale is one factor on its lane group's scores.
 //
-// The waves of a workgroup take every fourth tile of the same rows, so that a key is read once by the workgroup
-// whatever its number of rows (16 NT: query heads that share the key head, times query tokens), and add up through
-// LDS.  The work of a call, 256 keys of one unit (sequence, key head, row tile) a step, is cut into equal shares for
-// a fixed number of workgroups, whatever the lengths, which only the device knows; a unit that several workgroups
-// have pieces of is joined by a second kernel.
+// A unit of work is a sequence, a key head and 16 NT rows (the query heads that share the key head, times query
+// tokens).  The tiles of all units are one line that is cut into equal shares, one for each wave that the card has
+// room for, whatever the lengths, which only the device knows; a unit that several waves have pieces of is joined by
+// a second kernel.  Short caches, and calls with enough row tiles to fill the card evenly, do without: a workgroup of
+// four waves has a unit, takes its tiles in turn and adds up through LDS.
 //
 // The powers are taken of u 2^-e with one e a row: 0 or, where a row's first scores are below 2^-8, less; raised (and
 // the sums scaled, exactly) when a score passes 2^8 2^e.  Up to there the power is 2^80, which leaves room for 2^40
@@ -31,7 +31,7 @@
 namespace pnfx {
 
 struct Header {  // of a piece of a unit, for the join
-  int b, h, rt, first, last;  // the workgroups that have its pieces; first -1: none
+  int b, h, rt, first, last;  // the shares that have its pieces; first -1: none
 };
 
 struct AttnArgs {
@@ -44,21 +44,21 @@ struct AttnArgs {
   float scale, gamma;
   int has_gamma, causal;
   int Hq, G, R;       // query heads, those of a key head, row tiles
-  int shares;         // workgroups that share the call's steps; 0: one workgroup a unit
+  int shares;         // waves that share the call's tiles; 0: one workgroup a unit
   // Pieces, two for each share: the unit it goes on with, and the one that it begins and does not end
   Header* headers;
   float *acc, *stats;  // [2 shares][rows][D], and [2 shares][3][rows]: sum, peak, exponent
 };
 
-// How a call is cut: row tiles of 16 NT rows, R for each sequence and key head; shares: workgroups that share the
-// call's steps (0: one workgroup a unit); bytes of workspace.
+// How a call is cut: row tiles of 16 NT rows, R for each sequence and key head; shares: waves that share the call's
+// tiles (0: one workgroup a unit); bytes of workspace.
 struct AttnPlan {
   int NT, R, shares;
   int64_t units, header_bytes, acc_bytes, stat_bytes;
   int64_t bytes() const { return header_bytes + acc_bytes + stat_bytes; }
 };
 
-// Workgroups of a kernel that a CU holds, by its registers: no fewer and no more shares than they all have slots.
+// Waves of a kernel that a SIMD holds, by its registers: as many shares as the card has slots, no fewer and no more.
 constexpr int resident(int bytes, int D, int NT) {
   return bytes == 2 && D * NT <= 64 ? 3 : D * NT <= 128 ? 2 : 1;
 }
@@ -75,12 +75,12 @@ namespace {
 
 typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
-constexpr int THREADS = 256, WAVES = 4, TILE = 64, STEP = WAVES * TILE;
+constexpr int TILE = 64;  // keys that a wave takes at a time
 constexpr int E_LAST = 120;  // 2^-120 u is within TOP for every fp32 u
 constexpr int E_LEAST = -60, E_NONE = -100;  // of a row without scores, once it is joined
 constexpr float TOP = 256.0f, LOW = 1 / 256.0f;
 
-// Keys that a row tile's last row sees, from which its steps follow.
+// Keys that a row tile's last row sees, from which its tiles follow.
 template <int NT>
 __device__ __forceinline__ int seen_by(const AttnArgs& a, int64_t start, int n, int rt) {
   if (start < 0 || start + n > a.c.capacity()) return 0;  // such sequences get NaN
@@ -88,7 +88,7 @@ __device__ __forceinline__ int seen_by(const AttnArgs& a, int64_t start, int n, 
   if (i0 >= n) return 0;
   return (int)(start + (a.causal ? i1 + 1 : n));
 }
-__device__ __forceinline__ int steps_of(int seen) { return max(1, (seen + STEP - 1) / STEP); }
+__device__ __forceinline__ int tiles_of(int seen) { return max(1, (seen + TILE - 1) / TILE); }
 
 template <int DT>
 struct Parts {  // how a head's columns fall on loads: whole 64, then 32, then 16, a quarter of each a lane group
@@ -124,14 +124,23 @@ __device__ __forceinline__ unsigned not_finite(unsigned w, float scale) {
   return ((w & 0x7f7f7f7fu) + (scale < two_to(120) ? 0x01010101u : 0x08080808u)) & 0x80808080u;
 }
 
+// What the weighted sum of a row is multiplied by: gate / (sum + 1e-12), both sums in units of 2^(10 e).
+__device__ __forceinline__ float factor(const AttnArgs& a, float z, float m, int e) {
+  const float peak = ldexpf(m, e);
+  const float gate = a.has_gamma ? peak / (peak + a.gamma) : 1.0f;
+  return gate / (z + ldexpf(1e-12f, -10 * e));
+}
+
 // What all lanes hold the same, as a scalar.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ int64_t uniform(int64_t x) {
   return (int64_t)((uint64_t)(unsigned)uniform((int)(x >> 32)) << 32 | (unsigned)uniform((int)x));
 }
 
-template <typename T, int DT, int NT>
+// WAVES waves with the same rows, each with every WAVES-th tile.
+template <typename T, int DT, int NT, int WAVES>
 struct Unit {
+  static constexpr int STEP = WAVES * TILE;
   static constexpr int FRAGS = Parts<DT>::FRAGS, ND = DT / 16, TERMS = sizeof(T) == 4 ? 3 : 1;
   const AttnArgs& a;
   int lane, wave, g, r16, b, h, rt, n;
@@ -378,11 +387,10 @@ struct Unit {
     }
   }
 
-  // The steps [s0, s1) of the unit, of which the wave has one tile each.
-  __device__ __forceinline__ void run(int s0, int s1) {
-    const int seen = seen_by<NT>(a, start, n, rt);
-    const int keys = min(seen, s1 * STEP);
-    int key0 = s0 * STEP + wave * TILE;
+  // The tiles [t0, t1) of the unit.
+  __device__ __forceinline__ void run(int t0, int t1) {
+    const int keys = min(seen_by<NT>(a, start, n, rt), t1 * TILE);
+    int key0 = (t0 + wave) * TILE;
     if (key0 >= keys) return;
     Raw<DT> raw;
     Pages next = look(key0);
@@ -397,20 +405,24 @@ struct Unit {
     for (; key0 < keys; key0 += STEP) tile<true>(raw, key0, key0 + STEP < keys, next);
   }
 
-  // Adds up the four waves' sums in wave 0, in a fixed order.
+  // Adds up four waves' sums in wave 0, in a fixed order.
   struct Lds {
     float z[WAVES][16 * NT], m[WAVES][16 * NT];
     int e[WAVES][16 * NT];
     float slab[2][NT * ND * 4 * 64];
   };
-  __device__ __forceinline__ void join(Lds& s) {
+  __device__ __forceinline__ void row_peaks() {  // of the four lane groups
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int o = 16; o <= 32; o *= 2) m[nt] = fmaxf(m[nt], __shfl_xor(m[nt], o, 64));
+      m[nt] = fmaxf(m[nt], __shfl_xor(m[nt], 16, 64));
+      m[nt] = fmaxf(m[nt], __shfl_xor(m[nt], 32, 64));
       if (m[nt] == 0) e[nt] = E_NONE;
-      if (g == 0) s.z[wave][16 * nt + r16] = z[nt][0], s.m[wave][16 * nt + r16] = m[nt], s.e[wave][16 * nt + r16] = e[nt];
     }
+  }
+  __device__ __forceinline__ void join(Lds& s) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+      if (g == 0) s.z[wave][16 * nt + r16] = z[nt][0], s.m[wave][16 * nt + r16] = m[nt], s.e[wave][16 * nt + r16] = e[nt];
     __syncthreads();
     const bool used = row(0) < a.G * n;  // of the first row tile's columns: one query token needs few of 16
 #pragma unroll
@@ -435,7 +447,6 @@ struct Unit {
     if (wave == 1) put(s.slab[0], used);
     __syncthreads();
     if (wave == 0) add(s.slab[0], used);
-    __syncthreads();
   }
   __device__ __forceinline__ void put(float* slab, bool used) const {
     if (!used) return;
@@ -455,7 +466,7 @@ struct Unit {
   }
 
   __device__ __forceinline__ bool refused() const { return start < 0 || start + n > a.c.capacity(); }
-  __device__ __forceinline__ void store() {  // wave 0, the whole unit
+  __device__ __forceinline__ void store() {  // one wave, the whole unit
     const int d = anew();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -475,7 +486,7 @@ struct Unit {
         }
     }
   }
-  __device__ __forceinline__ void keep(int slot) {  // wave 0, a piece of the unit
+  __device__ __forceinline__ void keep(int slot) {  // a piece of the unit
     anew();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -488,12 +499,6 @@ struct Unit {
       for (int j = 0; j < ND; ++j) *reinterpret_cast<f32x4*>(to + 16 * j) = acc[nt][j];
     }
   }
-  // What the weighted sum of a row is multiplied by: gate / (sum + 1e-12), both sums in units of 2^(10 e).
-  static __device__ __forceinline__ float factor(const AttnArgs& a, float z, float m, int e) {
-    const float peak = ldexpf(m, e);
-    const float gate = a.has_gamma ? peak / (peak + a.gamma) : 1.0f;
-    return gate / (z + ldexpf(1e-12f, -10 * e));
-  }
 };
 
 // Consecutive shares on one XCD (workgroups go to the eight in turn), where neighbouring row tiles find each other's
@@ -503,85 +508,79 @@ __device__ __forceinline__ int64_t place(int64_t wg, int64_t n) {
   return x * each + min(x, more) + wg / 8;
 }
 
+// One workgroup of four waves a unit.
 template <typename T, int DT, int NT>
-__global__ __launch_bounds__(THREADS, resident(sizeof(T), DT, NT)) void attn_kernel(AttnArgs a) {
-  __shared__ typename Unit<T, DT, NT>::Lds lds;
-  __shared__ int64_t before[THREADS + 1];  // the steps of all sequences before each of 256 groups of them
-  __shared__ int64_t wave_sum[WAVES];
-  Unit<T, DT, NT> u(a);
+__global__ __launch_bounds__(256, resident(sizeof(T), DT, NT)) void unit_kernel(AttnArgs a) {
+  using U = Unit<T, DT, NT, 4>;
+  __shared__ typename U::Lds lds;
+  U u(a);
+  const int w = (int)place(blockIdx.x, gridDim.x), bh = w / a.R;
+  u.begin(bh / a.c.H, bh % a.c.H, a.R - 1 - w % a.R);  // the longest first
+  u.run(0, tiles_of(seen_by<NT>(a, u.start, u.n, u.rt)));
+  u.row_peaks();
+  u.join(lds);
+  if (u.wave == 0) u.store();
+}
+
+// An equal share of the call's tiles for each wave.
+template <typename T, int DT, int NT>
+__global__ __launch_bounds__(64, resident(sizeof(T), DT, NT)) void share_kernel(AttnArgs a) {
+  Unit<T, DT, NT, 1> u(a);
   const int w = (int)place(blockIdx.x, gridDim.x);
-  const auto steps_at = [&](int b, int rt) { return steps_of(seen_by<NT>(a, a.span.first(b), a.span.count(b), rt)); };
-  int b, h, rt;
-  int64_t at = 0, end, share = 0, skip = 0;  // steps [at, end) of the call, from step `skip` of unit (b, h, rt) on
-  if (a.shares) {
-    const auto steps_of_sequence = [&](int b) {
-      int64_t t = 0;
-      for (int rt = 0; rt < a.R; ++rt) t += steps_at(b, rt);
-      return t * a.c.H;
-    };
-    const int per = (a.c.B + THREADS - 1) / THREADS;
-    int64_t mine = 0;
-    for (int i = 0; i < per; ++i) {
-      const int x = threadIdx.x * per + i;
-      if (x < a.c.B) mine += steps_of_sequence(x);
-    }
-    int64_t sum = mine;
-    for (int o = 1; o < 64; o *= 2) {
-      const int64_t x = __shfl_up(sum, o, 64);
-      if (u.lane >= o) sum += x;
-    }
-    if (u.lane == 63) wave_sum[u.wave] = sum;
-    __syncthreads();
-    for (int i = 0; i < u.wave; ++i) sum += wave_sum[i];
-    before[threadIdx.x + 1] = sum;
-    if (threadIdx.x == 0) before[0] = 0;
-    __syncthreads();
-    const int64_t all = uniform(before[THREADS]);
-    share = (all + a.shares - 1) / a.shares;
-    at = w * share, end = min(all, at + share);
-    if (threadIdx.x < 2) a.headers[2 * w + threadIdx.x].first = -1;
-    if (at >= end) return;
-    int lo = 0, hi = THREADS;  // before[lo] <= at < before[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (uniform(before[mid]) <= at) lo = mid;
-      else hi = mid;
-    }
-    skip = at - uniform(before[lo]), b = lo * per;
-    for (;;) {
-      const int64_t t = steps_of_sequence(b);
-      if (skip < t) break;
-      skip -= t, ++b;
-    }
-    const int64_t head = steps_of_sequence(b) / a.c.H;
-    h = (int)(skip / head), rt = 0, skip %= head;
-    for (;;) {
-      const int t = steps_at(b, rt);
-      if (skip < t) break;
-      skip -= t, ++rt;
-    }
-  } else {
-    rt = a.R - 1 - w % a.R;  // the longest first
-    b = w / a.R / a.c.H, h = w / a.R % a.c.H;
-    end = steps_at(b, rt);
+  const auto tiles_at = [&](int b, int rt) { return tiles_of(seen_by<NT>(a, a.span.first(b), a.span.count(b), rt)); };
+  const auto tiles_of_sequence = [&](int b) {
+    int64_t t = 0;
+    for (int rt = 0; rt < a.R; ++rt) t += tiles_at(b, rt);
+    return t * a.c.H;
+  };
+  // the tiles of all sequences up to the end of each of 64 groups of them
+  const int per = (a.c.B + 63) / 64;
+  int64_t sum = 0;
+  for (int i = 0; i < per; ++i) {
+    const int x = u.lane * per + i;
+    if (x < a.c.B) sum += tiles_of_sequence(x);
+  }
+  for (int o = 1; o < 64; o *= 2) {
+    const int64_t x = __shfl_up(sum, o, 64);
+    if (u.lane >= o) sum += x;
+  }
+  const int64_t all = uniform(__shfl(sum, 63, 64)), share = (all + a.shares - 1) / a.shares;
+  int64_t at = w * share;
+  const int64_t end = min(all, at + share);
+  if (u.lane == 0) a.headers[2 * w].first = -1, a.headers[2 * w + 1].first = -1;
+  if (at >= end) return;
+  // the unit (b, h, rt) that the share begins in, `skip` tiles behind its first
+  const int group = __builtin_ctzll(__ballot(sum > at));
+  int64_t skip = at - (group ? uniform(__shfl(sum, group - 1, 64)) : 0);
+  int b = group * per;
+  for (;;) {
+    const int64_t t = tiles_of_sequence(b);
+    if (skip < t) break;
+    skip -= t, ++b;
+  }
+  const int64_t head = tiles_of_sequence(b) / a.c.H;
+  int h = (int)(skip / head), rt = 0;
+  skip %= head;
+  for (;;) {
+    const int t = tiles_at(b, rt);
+    if (skip < t) break;
+    skip -= t, ++rt;
   }
   while (at < end) {
     u.begin(b, h, rt);
-    const int t = steps_at(b, rt);
-    const int s0 = (int)skip, s1 = (int)min((int64_t)t, s0 + end - at);
-    u.run(s0, s1);
-    u.join(lds);
-    if (u.wave == 0) {
-      if (s0 == 0 && s1 == t) {
-        u.store();
-      } else {
-        const int slot = 2 * w + (s0 == 0);
-        u.keep(slot);
-        if (threadIdx.x == 0)
-          a.headers[slot] = Header{b, h, rt, (int)((at - s0) / share), (int)((at - s0 + t - 1) / share)};
-      }
+    const int t = tiles_at(b, rt);
+    const int t0 = (int)skip, t1 = (int)min((int64_t)t, t0 + end - at);
+    u.run(t0, t1);
+    u.row_peaks();
+    if (t0 == 0 && t1 == t) {
+      u.store();
+    } else {
+      const int slot = 2 * w + (t0 == 0);
+      u.keep(slot);
+      if (u.lane == 0)
+        a.headers[slot] = Header{b, h, rt, (int)((at - t0) / share), (int)((at - t0 + t - 1) / share)};
     }
-    at += s1 - s0, skip = 0;
+    at += t1 - t0, skip = 0;
     if (++rt == a.R) {
       rt = 0;
       if (++h == a.c.H) h = 0, ++b;
@@ -589,69 +588,65 @@ __global__ __launch_bounds__(THREADS, resident(sizeof(T), DT, NT)) void attn_ker
   }
 }
 
-// Joins the units that were cut.  Each workgroup that has a piece of a unit joins an equal part of its results: a
-// unit of few rows over a long cache has hundreds of pieces, and one workgroup for each unit took 103 us where this
-// takes 9 (2 sequences of 131072 tokens, 32 heads of 128 on 8).
+// Joins the units that were cut: each share that has a piece of one joins an equal part of its results, one wave each.
 template <typename T, int DT, int NT>
-__global__ __launch_bounds__(THREADS) void join_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
   constexpr int ROWS = 16 * NT;
-  __shared__ float sums[THREADS], row_z[ROWS], row_m[ROWS], row_top[ROWS];
-  const Header u = a.headers[blockIdx.x];
+  const int piece = blockIdx.x * 4 + uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (piece >= 2 * a.shares) return;
+  const Header u = a.headers[piece];
   if (u.first < 0) return;
-  const int n = u.last - u.first + 1, me = (int)blockIdx.x / 2 - u.first;
+  const int n = u.last - u.first + 1, me = piece / 2 - u.first;
   const auto slot = [&](int i) { return 2ll * (u.first + i) + (i == 0); };
   const int count = a.span.count(u.b);
   const int rows = min(ROWS, a.G * a.span.N - u.rt * ROWS), live = min(rows, a.G * count - u.rt * ROWS);
   const int64_t start = a.span.first(u.b);
   const bool refused = start < 0 || start + count > a.c.capacity();
   const int all = rows * a.c.d, x0 = (int)((int64_t)all * me / n), x1 = (int)((int64_t)all * (me + 1) / n);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int r = x0 / a.c.d + wave; r < live && r * a.c.d < x1; r += WAVES) {  // a wave a row
+  for (int r = x0 / a.c.d; r * a.c.d < x1; ++r) {
+    const int c0 = max(x0 - r * a.c.d, 0), c1 = min(x1 - r * a.c.d, a.c.d), row = u.rt * ROWS + r;
+    T* to = static_cast<T*>(a.o) + u.b * a.osb + (u.h * a.G + row % a.G) * a.osh + row / a.G * a.osn;
+    if (r >= live) {  // no query token
+      for (int c = c0 + lane; c < c1; c += 64) to[c] = from_f32<T>(0.0f);
+      continue;
+    }
+    const float* st = a.stats + r;
     float top = E_NONE, z = 0, m = 0;
-    for (int i = lane; i < n; i += 64) top = fmaxf(top, a.stats[slot(i) * 3 * ROWS + 2 * ROWS + r]);
+    for (int i = lane; i < n; i += 64) top = fmaxf(top, st[(slot(i) * 3 + 2) * ROWS]);
     top = wave_max(top);
     for (int i = lane; i < n; i += 64) {
-      const float* st = a.stats + slot(i) * 3 * ROWS + r;
-      const int up = (int)(st[2 * ROWS] - top);
-      z += st[0] * ldexpf(1.0f, 10 * up), m = fmaxf(m, ldexpf(st[ROWS], up));
+      const int64_t s = slot(i) * 3 * ROWS;
+      const int up = (int)(st[s + 2 * ROWS] - top);
+      z += st[s] * ldexpf(1.0f, 10 * up), m = fmaxf(m, ldexpf(st[s + ROWS], up));
     }
-    z = wave_sum(z), m = wave_max(m);
-    if (lane == 0) row_z[r] = z, row_m[r] = m, row_top[r] = top;
-  }
-  __syncthreads();
-  int width = 1;  // results at a time; the other threads take other pieces
-  while (width < THREADS && width < x1 - x0) width *= 2;
-  const int each = THREADS / width, part = threadIdx.x / width;
-  for (int base = x0; base < x1; base += width) {
-    const int x = base + threadIdx.x % width, r = x / a.c.d, col = x % a.c.d;
-    float v = 0;
-    if (x < x1 && r < live)
-      for (int i = part; i < n; i += each) {
-        const int up = (int)(a.stats[slot(i) * 3 * ROWS + 2 * ROWS + r] - row_top[r]);
-        v += a.acc[(slot(i) * ROWS + r) * DT + col] * ldexpf(1.0f, 10 * up);
-      }
-    sums[threadIdx.x] = v;
-    __syncthreads();
-    if (part == 0 && x < x1) {
-      for (int i = 1; i < each; ++i) v += sums[i * width + threadIdx.x];
-      if (r < live) v *= Unit<T, DT, NT>::factor(a, row_z[r], row_m[r], (int)row_top[r]);
-      if (refused && r < live) v = __builtin_nanf("");
-      const int row = u.rt * ROWS + r;
-      static_cast<T*>(a.o)[u.b * a.osb + (u.h * a.G + row % a.G) * a.osh + row / a.G * a.osn + col] = from_f32<T>(v);
+    const float f = factor(a, wave_sum(z), wave_max(m), (int)top);
+    int width = 1;  // results at a time; the other lanes take other pieces
+    while (width < 64 && width < c1 - c0) width *= 2;
+    for (int base = c0; base < c1; base += width) {
+      const int c = base + (lane & (width - 1));
+      float v = 0;
+      if (c < c1)
+        for (int i = lane / width; i < n; i += 64 / width) {
+          const int up = (int)(st[(slot(i) * 3 + 2) * ROWS] - top);
+          v += a.acc[(slot(i) * ROWS + r) * DT + c] * ldexpf(1.0f, 10 * up);
+        }
+      for (int o = width; o < 64; o *= 2) v += __shfl_xor(v, o, 64);
+      if (lane < width && c < c1) to[c] = from_f32<T>(refused ? __builtin_nanf("") : v * f);
     }
-    __syncthreads();
   }
 }
 
 template <typename T, int DT, int NT>
 int run(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
-  attn_kernel<T, DT, NT><<<dim3((unsigned)(p.shares ? p.shares : p.units)), dim3(THREADS), 0, st>>>(a);
+  if (!p.shares) {
+    unit_kernel<T, DT, NT><<<dim3((unsigned)p.units), dim3(256), 0, st>>>(a);
+    return launch_status("cached_attn");
+  }
+  share_kernel<T, DT, NT><<<dim3((unsigned)p.shares), dim3(64), 0, st>>>(a);
   if (int rc = launch_status("cached_attn")) return rc;
-  if (!p.shares) return PNFX_OK;
-  join_kernel<T, DT, NT><<<dim3((unsigned)(2 * p.shares)), dim3(THREADS), 0, st>>>(a);
+  join_kernel<T, DT, NT><<<dim3((unsigned)((2 * p.shares + 3) / 4)), dim3(256), 0, st>>>(a);
   return launch_status("cached_attn");
 }
-
 template <typename T, int DT>
 int run_rows(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
   if constexpr (DT <= 128) {

@@ -11,11 +11,11 @@ AttnPlan plan_of(int64_t B, int64_t H, int64_t G, int64_t N, int D, int64_t capa
   p.NT = rows <= 16 || D > 128 ? 1 : 2;
   p.R = (int)((rows + 16 * p.NT - 1) / (16 * p.NT));
   p.units = B * H * p.R;
-  const int64_t steps = (capacity + STEP - 1) / STEP;
-  // One workgroup a unit where no cut can gain: short caches, whose few steps cost less than the join's launch, and
+  const int64_t tiles = (capacity + TILE - 1) / TILE;
+  // One workgroup a unit where no cut can gain: short caches, whose few tiles cost less than the join's launch, and
   // enough row tiles for the card to even out by itself.
-  if (steps <= 2 || (p.R > 1 && p.units >= 2048)) return p;
-  p.shares = (int)std::min<int64_t>(p.units * steps, 256 * resident(bytes, D, p.NT));
+  if (tiles <= 8 || (p.R > 1 && p.units >= 2048)) return p;
+  p.shares = (int)std::min<int64_t>(p.units * tiles, 1024 * resident(bytes, D, p.NT));
   const auto round = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
   p.header_bytes = round(2ll * p.shares * (int64_t)sizeof(Header));
   p.acc_bytes = round(2ll * p.shares * 16 * p.NT * D * 4);
@@ -54,7 +54,7 @@ extern "C" int pnfx_cached_attn(const pnfx_cache* cache, const void* q, int64_t 
   PNFX_REQUIRE(N >= 1 && Hq / a.c.H * N < (1ll << 31) - 64, "cached_attn: N=%lld", (long long)N);
   PNFX_REQUIRE(start || (start_all >= 0 && start_all < (1ll << 31)), "cached_attn: start %lld", (long long)start_all);
   const AttnPlan p = plan_of(a.c.B, a.c.H, Hq / a.c.H, N, a.c.D, a.c.capacity(), dtype == PNFX_F32 ? 4 : 2);
-  PNFX_REQUIRE(p.units * THREADS < (1ll << 32), "cached_attn: %lld row tiles in one call", (long long)p.units);
+  PNFX_REQUIRE(p.units * 256 < (1ll << 32), "cached_attn: %lld row tiles in one call", (long long)p.units);
   PNFX_REQUIRE(!p.bytes() || (workspace && workspace_bytes >= p.bytes() &&
                               (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
                "cached_attn: workspace needs %lld bytes, 16-byte aligned", (long long)p.bytes());
