@@ -11,10 +11,9 @@
 // is exact in bf16, and a block's key scale is one factor on its lane group's scores.
 //
 // A unit of work is a sequence, a key head and 16 NT rows (the query heads that share the key head, times query
-// tokens).  The tiles of all units are one line that is cut into equal shares, one for each wave that the card has
-// room for, whatever the lengths, which only the device knows; a unit that several waves have pieces of is joined by
-// a second kernel.  Short caches, and calls with enough row tiles to fill the card evenly, do without: a workgroup of
-// four waves has a unit, takes its tiles in turn and adds up through LDS.
+// tokens).  A wave has a piece of one, which it finds by itself, as only the device knows the lengths; a second kernel
+// joins the pieces.  Short caches, and calls with enough units to fill the card evenly, do without: a workgroup of four
+// waves has a unit, takes its tiles in turn and adds up through LDS.
 //
 // The powers are taken of u 2^-e with one e a row: 0 or, where a row's first scores are below 2^-8, less; raised (and
 // the sums scaled, exactly) when a score passes 2^8 2^e.  Up to there the power is 2^80, which leaves room for 2^40
@@ -30,8 +29,8 @@
 
 namespace pnfx {
 
-struct Header {  // of a piece of a unit, for the join
-  int b, h, rt, first, last;  // the shares that have its pieces; first -1: none
+struct Header {  // of a piece, for the join: its unit, which of how many it is
+  int b, h, rt, piece, n;
 };
 
 struct AttnArgs {
@@ -44,21 +43,24 @@ struct AttnArgs {
   float scale, gamma;
   int has_gamma, causal;
   int Hq, G, R;       // query heads, those of a key head, row tiles
-  int shares;         // waves that share the call's tiles; 0: one workgroup a unit
-  // Pieces, two for each share: the unit it goes on with, and the one that it begins and does not end
+  int slots;          // waves that the card has room for
+  // Of the pieces: how many there are, headers, [items][slot_rows][D] sums and [items][3][slot_rows]: the weights' sum,
+  // peak, exponent
+  int* items;
   Header* headers;
-  float *acc, *stats;  // [2 shares][rows][D], and [2 shares][3][rows]: sum, peak, exponent
+  float *acc, *stats;
+  int slot_rows, most_items, join_waves;
 };
 
-// How a call is cut: row tiles of 16 NT rows, R for each sequence and key head; shares: waves that share the call's
-// tiles (0: one workgroup a unit); bytes of workspace.
+// How a call is cut: row tiles of 16 NT rows, R for each sequence and key head; items: the most pieces that units are
+// cut into (0: one workgroup a unit); join_waves: that join a piece's part; bytes of workspace.
 struct AttnPlan {
-  int NT, R, shares;
-  int64_t units, header_bytes, acc_bytes, stat_bytes;
+  int NT, R, slots, slot_rows, join_waves;
+  int64_t units, items, header_bytes, acc_bytes, stat_bytes;
   int64_t bytes() const { return header_bytes + acc_bytes + stat_bytes; }
 };
 
-// Waves of a kernel that a SIMD holds, by its registers: as many shares as the card has slots, no fewer and no more.
+// Waves of a kernel that a SIMD holds, by its registers: the card has 1024 times as many slots.
 constexpr int resident(int bytes, int D, int NT) {
   return bytes == 2 && D * NT <= 64 ? 3 : D * NT <= 128 ? 2 : 1;
 }
@@ -141,6 +143,7 @@ __device__ __forceinline__ int64_t uniform(int64_t x) {
 template <typename T, int DT, int NT, int WAVES>
 struct Unit {
   static constexpr int STEP = WAVES * TILE;
+  static constexpr bool ONCE = NT == 1 && DT <= 128;  // a call of up to 16 rows: one row tile
   static constexpr int FRAGS = Parts<DT>::FRAGS, ND = DT / 16, TERMS = sizeof(T) == 4 ? 3 : 1;
   const AttnArgs& a;
   int lane, wave, g, r16, b, h, rt, n;
@@ -226,6 +229,13 @@ struct Unit {
   __device__ __forceinline__ At find(const Pages& p, int key0) const {
     return At{block(p.k, key0 + 16 * (r16 >> 2)), block(p.v, key0 + 16 * g), (unsigned)p.v < (unsigned)a.c.pages};
   }
+  // Sixteen bytes of the cache.  What one row tile alone reads is not to be kept by the L2: 97.6 us against 110.6 for
+  // the loads alone of 64 sequences of 4096 tokens, 16 heads of 64 (5.5 TB/s).
+  static __device__ __forceinline__ uint4 chunk(const uint8_t* p) {
+    if (!ONCE) return *reinterpret_cast<const uint4*>(p);
+    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+    return uint4{v[0], v[1], v[2], v[3]};
+  }
   __device__ __forceinline__ void load_keys(const At& at, Raw<DT>& raw) const {
     using P = Parts<DT>;
     raw.ks = at.there ? two_to((int)a.c.k_scale[at.v] - 127) : __builtin_nanf("");
@@ -234,7 +244,7 @@ struct Unit {
     for (int t = 0; t < 4; ++t) {
       const uint8_t* p = kb + 4 * t * DT;
 #pragma unroll
-      for (int i = 0; i < P::N64; ++i) raw.k64[t][i] = *reinterpret_cast<const uint4*>(p + 64 * i + 16 * g);
+      for (int i = 0; i < P::N64; ++i) raw.k64[t][i] = chunk(p + 64 * i + 16 * g);
       if (P::N32) raw.k32[t] = *reinterpret_cast<const uint2*>(p + 64 * P::N64 + 8 * g);
       if (P::N16) raw.k16[t] = *reinterpret_cast<const unsigned*>(p + 64 * P::N64 + 32 * P::N32 + 4 * g);
     }
@@ -243,7 +253,7 @@ struct Unit {
     raw.vs = two_to(min((int)a.c.v_scale[at.v], 247) - 127);  // never written ones may be anything
     const uint8_t* vb = a.c.v + (int64_t)at.v * (BLOCK * DT) + r16 * 16;
 #pragma unroll
-    for (int j = 0; j < ND; ++j) raw.v[j] = *reinterpret_cast<const uint4*>(vb + 256 * j);
+    for (int j = 0; j < ND; ++j) raw.v[j] = chunk(vb + 256 * j);
   }
   __device__ __forceinline__ bf16x8 key_frag(const Raw<DT>& raw, int t, int f) const {
     using P = Parts<DT>;
@@ -492,9 +502,9 @@ struct Unit {
     for (int nt = 0; nt < NT; ++nt) {
       const int r = 16 * nt + r16;
       if (row(nt) >= a.G * n) continue;
-      float* st = a.stats + (int64_t)slot * 3 * 16 * NT + r;
-      if (g == 0) st[0] = z[nt][0], st[16 * NT] = m[nt], st[2 * 16 * NT] = (float)e[nt];
-      float* to = a.acc + ((int64_t)slot * 16 * NT + r) * DT + 4 * g;
+      float* st = a.stats + (int64_t)slot * 3 * a.slot_rows + r;
+      if (g == 0) st[0] = z[nt][0], st[a.slot_rows] = m[nt], st[2 * a.slot_rows] = (float)e[nt];
+      float* to = a.acc + ((int64_t)slot * a.slot_rows + r) * DT + 4 * g;
 #pragma unroll
       for (int j = 0; j < ND; ++j) *reinterpret_cast<f32x4*>(to + 16 * j) = acc[nt][j];
     }
@@ -522,129 +532,109 @@ __global__ __launch_bounds__(256, resident(sizeof(T), DT, NT)) void unit_kernel(
   if (u.wave == 0) u.store();
 }
 
-// An equal share of the call's tiles for each wave.
+// Pieces of units, one for each wave.  A sequence's tiles are cut alike for all its heads and row tiles, into as many
+// equal pieces as give every wave that the card has room for its share; neighbouring waves then have the same tokens
+// of neighbouring heads, which lie side by side in the pages: 64 sequences of up to 8192 tokens of random length,
+// 16 heads of 64, take PIECES_US, with shares cut through the line of all units 127.
 template <typename T, int DT, int NT>
-__global__ __launch_bounds__(64, resident(sizeof(T), DT, NT)) void share_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64, resident(sizeof(T), DT, NT)) void piece_kernel(AttnArgs a) {
   Unit<T, DT, NT, 1> u(a);
-  const int w = (int)place(blockIdx.x, gridDim.x);
-  const auto tiles_at = [&](int b, int rt) { return tiles_of(seen_by<NT>(a, a.span.first(b), a.span.count(b), rt)); };
   const auto tiles_of_sequence = [&](int b) {
-    int64_t t = 0;
-    for (int rt = 0; rt < a.R; ++rt) t += tiles_at(b, rt);
-    return t * a.c.H;
+    const int64_t start = a.span.first(b);
+    const int n = a.span.count(b);
+    return tiles_of(start < 0 || start + n > a.c.capacity() || n == 0 ? 0 : (int)(start + n));
   };
-  // the tiles of all sequences up to the end of each of 64 groups of them
-  const int per = (a.c.B + 63) / 64;
-  int64_t sum = 0;
-  for (int i = 0; i < per; ++i) {
-    const int x = u.lane * per + i;
-    if (x < a.c.B) sum += tiles_of_sequence(x);
-  }
+  const int per = (a.c.B + 63) / 64, b0 = u.lane * per, b1 = min(b0 + per, a.c.B);
+  int64_t all = 0;
+  for (int b = b0; b < b1; ++b) all += tiles_of_sequence(b);
+  for (int o = 1; o < 64; o *= 2) all += __shfl_xor(all, o, 64);
+  // With s tiles a piece there are at most all / s + B pieces, and half of B less as a rule.
+  const int each = a.c.H * a.R;  // waves a piece
+  const float slots = (float)a.slots / each, room = fmaxf(slots - 0.5f * a.c.B, 0.6f * slots);
+  const int64_t s = max((int64_t)1, uniform((int64_t)ceilf((float)all / room)));
+  const auto pieces_of = [&](int tiles) { return (int)((tiles + s - 1) / s); };
+  int sum = 0;  // pieces of the sequences up to the end of each lane's
+  for (int b = b0; b < b1; ++b) sum += pieces_of(tiles_of_sequence(b));
   for (int o = 1; o < 64; o *= 2) {
-    const int64_t x = __shfl_up(sum, o, 64);
+    const int x = __shfl_up(sum, o, 64);
     if (u.lane >= o) sum += x;
   }
-  const int64_t all = uniform(__shfl(sum, 63, 64)), share = (all + a.shares - 1) / a.shares;
-  int64_t at = w * share;
-  const int64_t end = min(all, at + share);
-  if (u.lane == 0) a.headers[2 * w].first = -1, a.headers[2 * w + 1].first = -1;
-  if (at >= end) return;
-  // the unit (b, h, rt) that the share begins in, `skip` tiles behind its first
-  const int group = __builtin_ctzll(__ballot(sum > at));
-  int64_t skip = at - (group ? uniform(__shfl(sum, group - 1, 64)) : 0);
-  int b = group * per;
+  const int items = uniform(__shfl(sum, 63, 64)) * each;
+  // consecutive items on one XCD (workgroups go to the eight in turn)
+  const int eighth = (items + 7) / 8, item = (int)blockIdx.x % 8 * eighth + (int)blockIdx.x / 8;
+  if ((int)blockIdx.x / 8 >= eighth || item >= items) return;
+  const int line = item / each, group = __builtin_ctzll(__ballot(sum > line));
+  int piece = line - (group ? uniform(__shfl(sum, group - 1, 64)) : 0), b = group * per, tiles, n;
   for (;;) {
-    const int64_t t = tiles_of_sequence(b);
-    if (skip < t) break;
-    skip -= t, ++b;
+    tiles = tiles_of_sequence(b), n = pieces_of(tiles);
+    if (piece < n) break;
+    piece -= n, ++b;
   }
-  const int64_t head = tiles_of_sequence(b) / a.c.H;
-  int h = (int)(skip / head), rt = 0;
-  skip %= head;
-  for (;;) {
-    const int t = tiles_at(b, rt);
-    if (skip < t) break;
-    skip -= t, ++rt;
-  }
-  while (at < end) {
-    u.begin(b, h, rt);
-    const int t = tiles_at(b, rt);
-    const int t0 = (int)skip, t1 = (int)min((int64_t)t, t0 + end - at);
-    u.run(t0, t1);
-    u.row_peaks();
-    if (t0 == 0 && t1 == t) {
-      u.store();
-    } else {
-      const int slot = 2 * w + (t0 == 0);
-      u.keep(slot);
-      if (u.lane == 0)
-        a.headers[slot] = Header{b, h, rt, (int)((at - t0) / share), (int)((at - t0 + t - 1) / share)};
-    }
-    at += t1 - t0, skip = 0;
-    if (++rt == a.R) {
-      rt = 0;
-      if (++h == a.c.H) h = 0, ++b;
-    }
-  }
+  u.begin(b, item % each / a.R, item % a.R);
+  u.run((int)((int64_t)tiles * piece / n), (int)((int64_t)tiles * (piece + 1) / n));
+  u.row_peaks();
+  if (n == 1) u.store();
+  else u.keep(item);
+  if (u.lane == 0) a.headers[item] = Header{b, item % each / a.R, item % a.R, piece, n};
+  // those that no item has, for the join
+  if (u.lane == 0 && item == items - 1) *a.items = items;
 }
 
-// Joins the units that were cut: each share that has a piece of one joins an equal part of its results, one wave each.
+// Joins the units that were cut: the waves of a unit's n pieces, a.join_waves for each, have equal parts of its results.
+// A lane has a result and, where there are fewer results than lanes, every so many of the pieces; it goes over them once,
+// the sums in units of the largest e so far, so that no load waits for another.
 template <typename T, int DT, int NT>
 __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
   constexpr int ROWS = 16 * NT;
-  const int piece = blockIdx.x * 4 + uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (piece >= 2 * a.shares) return;
-  const Header u = a.headers[piece];
-  if (u.first < 0) return;
-  const int n = u.last - u.first + 1, me = piece / 2 - u.first;
-  const auto slot = [&](int i) { return 2ll * (u.first + i) + (i == 0); };
+  const int wave = blockIdx.x * 4 + uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int item = wave / a.join_waves, items = *a.items;
+  const Header u = a.headers[min(item, a.most_items - 1)];
+  if (item >= items || u.n == 1) return;
+  const int each = a.c.H * a.R, parts = u.n * a.join_waves, me = u.piece * a.join_waves + wave % a.join_waves;
   const int count = a.span.count(u.b);
   const int rows = min(ROWS, a.G * a.span.N - u.rt * ROWS), live = min(rows, a.G * count - u.rt * ROWS);
   const int64_t start = a.span.first(u.b);
   const bool refused = start < 0 || start + count > a.c.capacity();
-  const int all = rows * a.c.d, x0 = (int)((int64_t)all * me / n), x1 = (int)((int64_t)all * (me + 1) / n);
-  for (int r = x0 / a.c.d; r * a.c.d < x1; ++r) {
-    const int c0 = max(x0 - r * a.c.d, 0), c1 = min(x1 - r * a.c.d, a.c.d), row = u.rt * ROWS + r;
-    T* to = static_cast<T*>(a.o) + u.b * a.osb + (u.h * a.G + row % a.G) * a.osh + row / a.G * a.osn;
-    if (r >= live) {  // no query token
-      for (int c = c0 + lane; c < c1; c += 64) to[c] = from_f32<T>(0.0f);
-      continue;
+  const int all = rows * a.c.d, x0 = (int)((int64_t)all * me / parts), x1 = (int)((int64_t)all * (me + 1) / parts);
+  int width = 1;  // results at a time
+  while (width < 64 && width < x1 - x0) width *= 2;
+  for (int base = x0; base < x1; base += width) {
+    const int x = base + (lane & (width - 1)), r = x / a.c.d, c = x % a.c.d;
+    float top = E_NONE, z = 0, m = 0, v = 0;
+    const auto add = [&](float e, float z1, float m1, float v1) {
+      const float to = fmaxf(top, e);
+      const int was = (int)(top - to), is = (int)(e - to);
+      const float fw = ldexpf(1.0f, 10 * was), fi = ldexpf(1.0f, 10 * is);
+      z = z * fw + z1 * fi, v = v * fw + v1 * fi, m = fmaxf(ldexpf(m, was), ldexpf(m1, is)), top = to;
+    };
+    if (x < x1 && r < live) {
+#pragma unroll 4
+      for (int i = lane / width; i < u.n; i += 64 / width) {
+        const int64_t slot = item + (i - u.piece) * each;
+        const float* st = a.stats + slot * 3 * a.slot_rows + r;
+        add(st[2 * a.slot_rows], st[0], st[a.slot_rows], a.acc[(slot * a.slot_rows + r) * DT + c]);
+      }
     }
-    const float* st = a.stats + r;
-    float top = E_NONE, z = 0, m = 0;
-    for (int i = lane; i < n; i += 64) top = fmaxf(top, st[(slot(i) * 3 + 2) * ROWS]);
-    top = wave_max(top);
-    for (int i = lane; i < n; i += 64) {
-      const int64_t s = slot(i) * 3 * ROWS;
-      const int up = (int)(st[s + 2 * ROWS] - top);
-      z += st[s] * ldexpf(1.0f, 10 * up), m = fmaxf(m, ldexpf(st[s + ROWS], up));
-    }
-    const float f = factor(a, wave_sum(z), wave_max(m), (int)top);
-    int width = 1;  // results at a time; the other lanes take other pieces
-    while (width < 64 && width < c1 - c0) width *= 2;
-    for (int base = c0; base < c1; base += width) {
-      const int c = base + (lane & (width - 1));
-      float v = 0;
-      if (c < c1)
-        for (int i = lane / width; i < n; i += 64 / width) {
-          const int up = (int)(st[(slot(i) * 3 + 2) * ROWS] - top);
-          v += a.acc[(slot(i) * ROWS + r) * DT + c] * ldexpf(1.0f, 10 * up);
-        }
-      for (int o = width; o < 64; o *= 2) v += __shfl_xor(v, o, 64);
-      if (lane < width && c < c1) to[c] = from_f32<T>(refused ? __builtin_nanf("") : v * f);
+    for (int o = width; o < 64; o *= 2)
+      add(__shfl_xor(top, o, 64), __shfl_xor(z, o, 64), __shfl_xor(m, o, 64), __shfl_xor(v, o, 64));
+    if (lane < width && x < x1) {
+      v = r < live ? v * factor(a, z, m, (int)top) : 0.0f;  // no query token: zero
+      if (refused && r < live) v = __builtin_nanf("");
+      const int row = u.rt * ROWS + r;
+      static_cast<T*>(a.o)[u.b * a.osb + (u.h * a.G + row % a.G) * a.osh + row / a.G * a.osn + c] = from_f32<T>(v);
     }
   }
 }
 
 template <typename T, int DT, int NT>
 int run(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
-  if (!p.shares) {
+  if (!p.items) {
     unit_kernel<T, DT, NT><<<dim3((unsigned)p.units), dim3(256), 0, st>>>(a);
     return launch_status("cached_attn");
   }
-  share_kernel<T, DT, NT><<<dim3((unsigned)p.shares), dim3(64), 0, st>>>(a);
+  piece_kernel<T, DT, NT><<<dim3((unsigned)p.items), dim3(64), 0, st>>>(a);
   if (int rc = launch_status("cached_attn")) return rc;
-  join_kernel<T, DT, NT><<<dim3((unsigned)((2 * p.shares + 3) / 4)), dim3(256), 0, st>>>(a);
+  join_kernel<T, DT, NT><<<dim3((unsigned)((p.items * p.join_waves + 3) / 4)), dim3(256), 0, st>>>(a);
   return launch_status("cached_attn");
 }
 template <typename T, int DT>

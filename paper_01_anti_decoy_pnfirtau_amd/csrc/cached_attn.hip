@@ -12,14 +12,17 @@ AttnPlan plan_of(int64_t B, int64_t H, int64_t G, int64_t N, int D, int64_t capa
   p.R = (int)((rows + 16 * p.NT - 1) / (16 * p.NT));
   p.units = B * H * p.R;
   const int64_t tiles = (capacity + TILE - 1) / TILE;
+  p.slots = 1024 * resident(bytes, D, p.NT);
+  p.slot_rows = (int)std::min<int64_t>(rows, 16 * p.NT);
   // One workgroup a unit where no cut can gain: short caches, whose few tiles cost less than the join's launch, and
-  // enough row tiles for the card to even out by itself.
-  if (tiles <= 8 || (p.R > 1 && p.units >= 2048)) return p;
-  p.shares = (int)std::min<int64_t>(p.units * tiles, 1024 * resident(bytes, D, p.NT));
+  // enough units for the card to even out by itself.
+  if (tiles <= 8 || (p.R > 1 && p.units >= 2048) || p.units >= 4 * p.slots) return p;
+  p.items = (std::min(p.units * tiles, p.units + p.slots) + 7) / 8 * 8;
   const auto round = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
-  p.header_bytes = round(2ll * p.shares * (int64_t)sizeof(Header));
-  p.acc_bytes = round(2ll * p.shares * 16 * p.NT * D * 4);
-  p.stat_bytes = round(2ll * p.shares * 3 * 16 * p.NT * 4);
+  p.join_waves = std::min(8, (p.slot_rows * D + 255) / 256);  // of results, a unit has at least two pieces
+  p.header_bytes = 256 + round(p.items * (int64_t)sizeof(Header));
+  p.acc_bytes = round(p.items * p.slot_rows * D * 4);
+  p.stat_bytes = round(p.items * 3 * p.slot_rows * 4);
   return p;
 }
 
@@ -61,9 +64,11 @@ extern "C" int pnfx_cached_attn(const pnfx_cache* cache, const void* q, int64_t 
   a.span = Span{start, counts, (int)start_all, (int)N};
   a.q = q, a.o = o, a.qsb = qsb, a.qsh = qsh, a.qsn = qsn, a.osb = osb, a.osh = osh, a.osn = osn;
   a.tau = tau, a.scale = scale, a.gamma = gamma, a.has_gamma = has_gamma, a.causal = causal;
-  a.Hq = (int)Hq, a.G = (int)Hq / a.c.H, a.R = p.R, a.shares = p.shares;
+  a.Hq = (int)Hq, a.G = (int)Hq / a.c.H, a.R = p.R, a.slots = p.slots, a.slot_rows = p.slot_rows;
+  a.most_items = (int)p.items, a.join_waves = p.join_waves;
   char* ws = static_cast<char*>(workspace);
-  a.headers = reinterpret_cast<Header*>(ws);
+  a.items = reinterpret_cast<int*>(ws);
+  a.headers = reinterpret_cast<Header*>(ws + 256);
   a.acc = reinterpret_cast<float*>(ws + p.header_bytes);
   a.stats = reinterpret_cast<float*>(ws + p.header_bytes + p.acc_bytes);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
