@@ -76,6 +76,7 @@ int attn_f32_256(const AttnArgs& a, const AttnPlan& p, hipStream_t st);
 namespace {
 
 typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int TILE = 64;  // keys that a wave takes at a time
 constexpr int E_LAST = 120;  // 2^-120 u is within TOP for every fp32 u
@@ -105,10 +106,10 @@ struct Parts {  // how a head's columns fall on loads: whole 64, then 32, then 1
 template <int DT>
 struct Raw {  // a tile of 64 keys and values as it lies in memory
   using P = Parts<DT>;
-  uint4 k64[4][P::N64 ? P::N64 : 1];
-  uint2 k32[4];
+  u32x4 k64[4][P::N64 ? P::N64 : 1];  // vectors, so that a loop holds the loads' own registers, not copies of them
+  u32x2 k32[4];
   unsigned k16[4];
-  uint4 v[DT / 16];
+  u32x4 v[DT / 16];
   float ks, vs;  // scales of block g; NaN where there is no such page
 };
 
@@ -231,10 +232,9 @@ struct Unit {
   }
   // Sixteen bytes of the cache.  What one row tile alone reads is not to be kept by the L2: 97.6 us against 110.6 for
   // the loads alone of 64 sequences of 4096 tokens, 16 heads of 64 (5.5 TB/s).
-  static __device__ __forceinline__ uint4 chunk(const uint8_t* p) {
-    if (!ONCE) return *reinterpret_cast<const uint4*>(p);
-    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
-    return uint4{v[0], v[1], v[2], v[3]};
+  static __device__ __forceinline__ u32x4 chunk(const uint8_t* p) {
+    const u32x4* at = reinterpret_cast<const u32x4*>(p);
+    return ONCE ? __builtin_nontemporal_load(at) : *at;
   }
   __device__ __forceinline__ void load_keys(const At& at, Raw<DT>& raw) const {
     using P = Parts<DT>;
@@ -245,7 +245,7 @@ struct Unit {
       const uint8_t* p = kb + 4 * t * DT;
 #pragma unroll
       for (int i = 0; i < P::N64; ++i) raw.k64[t][i] = chunk(p + 64 * i + 16 * g);
-      if (P::N32) raw.k32[t] = *reinterpret_cast<const uint2*>(p + 64 * P::N64 + 8 * g);
+      if (P::N32) raw.k32[t] = *reinterpret_cast<const u32x2*>(p + 64 * P::N64 + 8 * g);
       if (P::N16) raw.k16[t] = *reinterpret_cast<const unsigned*>(p + 64 * P::N64 + 32 * P::N32 + 4 * g);
     }
   }
@@ -258,10 +258,10 @@ struct Unit {
   __device__ __forceinline__ bf16x8 key_frag(const Raw<DT>& raw, int t, int f) const {
     using P = Parts<DT>;
     if (f < 2 * P::N64) {
-      const uint4& w = raw.k64[t][f / 2];
-      return f % 2 ? eight(w.z, w.w, 1.0f) : eight(w.x, w.y, 1.0f);
+      const u32x4 w = raw.k64[t][f / 2];
+      return f % 2 ? eight(w[2], w[3], 1.0f) : eight(w[0], w[1], 1.0f);
     }
-    if (P::N32 && f == 2 * P::N64) return eight(raw.k32[t].x, raw.k32[t].y, 1.0f);
+    if (P::N32 && f == 2 * P::N64) return eight(raw.k32[t][0], raw.k32[t][1], 1.0f);
     return eight(raw.k16[t], 0, 1.0f);
   }
 
@@ -361,7 +361,7 @@ struct Unit {
     if (more) load_values(at, raw);
   }
   __device__ __forceinline__ bf16x8 value_frag(const Raw<DT>& raw, int j, int hf) const {
-    return hf ? eight(raw.v[j].z, raw.v[j].w, raw.vs) : eight(raw.v[j].x, raw.v[j].y, raw.vs);
+    return eight(raw.v[j][2 * hf], raw.v[j][2 * hf + 1], raw.vs);
   }
   // In a tile that some row does not see whole, values that are not finite count as zeros, and a row that sees one gets
   // NaN there: a weight of zero would make NaN of them.
@@ -369,8 +369,8 @@ struct Unit {
     unsigned any = 0;
 #pragma unroll
     for (int j = 0; j < ND; ++j)
-      any |= not_finite(raw.v[j].x, raw.vs) | not_finite(raw.v[j].y, raw.vs) | not_finite(raw.v[j].z, raw.vs) |
-             not_finite(raw.v[j].w, raw.vs);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) any |= not_finite(raw.v[j][i], raw.vs);
     if (__builtin_expect(!__any(any != 0), 1)) return;
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
@@ -381,10 +381,8 @@ struct Unit {
         for (int x = 0; x < 8; ++x) sees[nt][x] = (bf16)(key0 + 16 * g + 8 * hf + x < lim[nt] ? 1.0f : 0.0f);
 #pragma unroll
       for (int j = 0; j < ND; ++j) {
-        unsigned& lo = hf ? raw.v[j].z : raw.v[j].x;
-        unsigned& hi = hf ? raw.v[j].w : raw.v[j].y;
-        const unsigned bl = not_finite(lo, raw.vs) >> 7, bh = not_finite(hi, raw.vs) >> 7;
-        lo &= ~(bl * 0xff), hi &= ~(bh * 0xff);
+        const unsigned bl = not_finite(raw.v[j][2 * hf], raw.vs) >> 7, bh = not_finite(raw.v[j][2 * hf + 1], raw.vs) >> 7;
+        raw.v[j][2 * hf] &= ~(bl * 0xff), raw.v[j][2 * hf + 1] &= ~(bh * 0xff);
         const bf16x8 bad = eight(bl * 0x38, bh * 0x38, 1.0f);  // 0x38: one
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -407,11 +405,8 @@ struct Unit {
     const At at = find(next, key0);
     next = look(key0 + STEP);
     load_keys(at, raw), load_values(at, raw);
-    for (; key0 + TILE <= min_lim; key0 += STEP) {  // tiles that every row sees whole come first
-      const bool more = key0 + STEP < keys;
-      tile<false>(raw, key0, more, next);
-      if (!more) return;
-    }
+    // tiles that every row sees whole, and others behind them, come first
+    for (; key0 + TILE <= min_lim && key0 + STEP < keys; key0 += STEP) tile<false>(raw, key0, true, next);
     for (; key0 < keys; key0 += STEP) tile<true>(raw, key0, key0 + STEP < keys, next);
   }
 
@@ -535,7 +530,7 @@ __global__ __launch_bounds__(256, resident(sizeof(T), DT, NT)) void unit_kernel(
 // Pieces of units, one for each wave.  A sequence's tiles are cut alike for all its heads and row tiles, into as many
 // equal pieces as give every wave that the card has room for its share; neighbouring waves then have the same tokens
 // of neighbouring heads, which lie side by side in the pages: 64 sequences of up to 8192 tokens of random length,
-// 16 heads of 64, take PIECES_US, with shares cut through the line of all units 127.
+// 16 heads of 64, take 106, with shares cut through the line of all units 127.
 template <typename T, int DT, int NT>
 __global__ __launch_bounds__(64, resident(sizeof(T), DT, NT)) void piece_kernel(AttnArgs a) {
   Unit<T, DT, NT, 1> u(a);
@@ -590,12 +585,15 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
   const int item = wave / a.join_waves, items = *a.items;
   const Header u = a.headers[min(item, a.most_items - 1)];
   if (item >= items || u.n == 1) return;
-  const int each = a.c.H * a.R, parts = u.n * a.join_waves, me = u.piece * a.join_waves + wave % a.join_waves;
+  const int each = a.c.H * a.R, me = u.piece * a.join_waves + wave % a.join_waves;
   const int count = a.span.count(u.b);
   const int rows = min(ROWS, a.G * a.span.N - u.rt * ROWS), live = min(rows, a.G * count - u.rt * ROWS);
   const int64_t start = a.span.first(u.b);
   const bool refused = start < 0 || start + count > a.c.capacity();
-  const int all = rows * a.c.d, x0 = (int)((int64_t)all * me / parts), x1 = (int)((int64_t)all * (me + 1) / parts);
+  // no part of less than 16 results: pieces come in lines of the cache
+  const int all = rows * a.c.d, parts = min(u.n * a.join_waves, max(1, all / 16));
+  if (me >= parts) return;
+  const int x0 = (int)((int64_t)all * me / parts), x1 = (int)((int64_t)all * (me + 1) / parts);
   int width = 1;  // results at a time
   while (width < 64 && width < x1 - x0) width *= 2;
   for (int base = x0; base < x1; base += width) {
@@ -608,7 +606,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
       z = z * fw + z1 * fi, v = v * fw + v1 * fi, m = fmaxf(ldexpf(m, was), ldexpf(m1, is)), top = to;
     };
     if (x < x1 && r < live) {
-#pragma unroll 4
+#pragma unroll 8
       for (int i = lane / width; i < u.n; i += 64 / width) {
         const int64_t slot = item + (i - u.piece) * each;
         const float* st = a.stats + slot * 3 * a.slot_rows + r;
