@@ -14,7 +14,6 @@ namespace pnfx {
 constexpr int BLOCK = 16;      // tokens that share a scale
 constexpr int RAW = 16;        // keys before the FIR that are kept of each sequence and head
 constexpr int E_LOWEST = -100; // smallest scale: 2^E_LOWEST
-constexpr unsigned char E4M3_NAN = 0x7f;
 
 struct Cache {
   uint8_t *k, *v, *k_scale, *v_scale;

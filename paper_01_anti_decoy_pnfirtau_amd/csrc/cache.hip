@@ -1,8 +1,9 @@
 // Writing the 8-bit key and value cache, and reading it back.
 //
-// Append.  One group of threads has a block of 16 tokens of one sequence and head, one thread a column of the head:
-// it holds the column's 16 tokens, so the FIR slides through registers, the largest |number| is a maximum over
-// registers and then over the group, and the value block's row is one 16-byte store.
+// Append.  One group of threads has the keys, or the values, of a block of 16 tokens of one sequence and head, one thread
+// a column of the head: it holds the column's 16 tokens, so the FIR slides through registers, the largest |number| is a
+// maximum over registers and then over the group, and the value block's row is one 16-byte store; the key block, whose
+// rows are tokens, is turned through LDS and stored likewise.
 //   k~_t = sum_j taps[j] k_{t-K+1+j}     in 64 bits: an fp32 sum would land on the other side of a rounding border
 //                                        every few hundred thousand numbers, a 64-bit one practically never does
 //   E    = the smallest for which no finite |number| is above 448 2^E, at least the block's so far if it is begun
@@ -29,7 +30,7 @@ struct AppendArgs {
   int64_t ksb, ksh, ksn, vsb, vsh, vsn;
   const float* taps;
   int taps_rows, K;
-  int group, groups;  // threads a block, groups a sequence and head
+  int groups;  // of a sequence and head, for keys as for values
   int64_t items;
 };
 
@@ -47,8 +48,9 @@ __device__ __forceinline__ float cut(double x) {
   const uint64_t hi = (b & 0xffffffff00000000ull) | ((uint64_t)((unsigned)b != 0) << 32);
   return (float)__builtin_bit_cast(double, hi);
 }
-__device__ __forceinline__ unsigned e4m3(float x) {  // |x| <= 448, or NaN
-  return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false) & 0xff;
+__device__ __forceinline__ unsigned e4m3x4(const float (&x)[4]) {  // |x| <= 448, or NaN
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+  return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], lo, true);
 }
 __device__ __forceinline__ float value(unsigned byte) { return __builtin_amdgcn_cvt_f32_fp8((int)byte, 0); }
 
@@ -57,124 +59,201 @@ __device__ __forceinline__ unsigned byte_of(const uint4& w, int t) {
   return u[t >> 2] >> (8 * (t & 3)) & 0xff;
 }
 
-// Maximum over the threads of a group (a power of two of them).
-__device__ __forceinline__ int group_max(int x, int group, int* lds) {
-  for (int o = min(group, 64) >> 1; o >= 1; o >>= 1) x = max(x, __shfl_xor(x, o, 64));
-  if (group > 64) {  // the same for the whole workgroup
-    const int wave = threadIdx.x >> 6, first = wave & ~(group / 64 - 1);
+// The threads of a group (GROUP, a power of two) wait for each other's LDS accesses; one wave's are in order.
+template <int GROUP>
+__device__ __forceinline__ void group_sync() {
+  if (GROUP > 64) {
+    __syncthreads();
+  } else {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+template <int GROUP>
+__device__ __forceinline__ int group_max(int x, int* lds) {
+#pragma unroll
+  for (int o = (GROUP < 64 ? GROUP : 64) / 2; o >= 1; o /= 2) x = max(x, __shfl_xor(x, o, 64));
+  if (GROUP > 64) {
+    const int wave = threadIdx.x >> 6, first = wave & ~(GROUP / 64 - 1);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) lds[wave] = x;
     __syncthreads();
-    for (int i = 0; i < group / 64; ++i) x = max(x, lds[first + i]);
+#pragma unroll
+    for (int i = 0; i < GROUP / 64; ++i) x = max(x, lds[first + i]);
   }
   return x;
 }
 
-// KT: the window that the FIR's taps are at the end of; 0: no FIR.
-template <typename T, int KT>
+// A column's 16 bytes with those of tokens t0 .. t1 - 1 from x (in units of 1), the kept ones before them over `again`.
+template <typename X>
+__device__ __forceinline__ uint4 column(const X (&x)[BLOCK], X inv, uint4 old, int t0, int t1, float again) {
+  unsigned out[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float y[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const X scaled = x[4 * i + u] * inv;
+      y[u] = sizeof(X) == 8 ? cut((double)scaled) : (float)scaled;
+      if (!(fabsf(y[u]) < __builtin_inff())) y[u] = __builtin_nanf("");
+    }
+    out[i] = e4m3x4(y);
+  }
+  if (t0 > 0 || t1 < BLOCK) {
+    const unsigned was[4] = {old.x, old.y, old.z, old.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float y[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) y[u] = value(was[i] >> (8 * u) & 0xff) * again;
+      const unsigned kept = e4m3x4(y);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const unsigned mask = 0xffu << (8 * u);
+        const int t = 4 * i + u;
+        out[i] = (out[i] & ~mask) | ((t < t0 ? kept : t < t1 ? out[i] : was[i]) & mask);
+      }
+    }
+  }
+  return uint4{out[0], out[1], out[2], out[3]};
+}
+
+// The largest finite |x| of tokens t0 .. t1 - 1.
+template <typename X>
+__device__ __forceinline__ double largest(const X (&x)[BLOCK], int t0, int t1) {
+  X top = 0;
+#pragma unroll
+  for (int t = 0; t < BLOCK; ++t) {
+    const X a = fabs(x[t]);  // NaN loses in the maximum
+    if (t >= t0 && t < t1 && a < (X)__builtin_inf()) top = fmax(top, a);
+  }
+  return (double)top;
+}
+
+// KT: the window that the FIR's taps are at the end of; 0: no FIR.  GROUP: threads of a block, at least its columns.
+template <typename T, int KT, int GROUP>
 __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
-  __shared__ int lds[4];
-  constexpr int HIST = KT ? KT - 1 : 0;
+  __shared__ int peaks[THREADS / 64];
+  __shared__ uint4 turn[THREADS];  // a key block, 16 bytes a thread
+  constexpr int HIST = KT ? KT - 1 : 0, PER = THREADS / GROUP;
   const Cache& c = a.c;
-  const int per = THREADS / a.group;
-  int64_t item = (int64_t)blockIdx.x * per + threadIdx.x / a.group;
+  int within = threadIdx.x / GROUP;
+  if (GROUP >= 64) within = __builtin_amdgcn_readfirstlane(within);  // the same for a wave: rows by scalar addresses
+  int64_t item = (int64_t)blockIdx.x * PER + within;
   const bool exists = item < a.items;
   if (!exists) item = 0;
+  const bool keys = item % 2 == 0;
+  item /= 2;
   const int j = (int)(item % a.groups);
-  const int h = (int)(item / a.groups % c.H), b = (int)(item / a.groups / c.H);
-  const int col = threadIdx.x & (a.group - 1);
-  const bool mine = exists && col < c.d;  // a column of the head; the others up to D hold zeros
+  const int bh = (int)(item / a.groups), b = bh / c.H, h = bh % c.H;
+  const int col = threadIdx.x & (GROUP - 1);
+  const bool mine = col < c.d;  // a column of the head; the others up to D hold zeros
   const int64_t s = a.span.first(b);
   const int n = a.span.count(b);
-  const bool fits = exists && s >= 0 && s + n <= c.capacity();
-  const T* k = static_cast<const T*>(a.k) + b * a.ksb + h * a.ksh + (mine ? col : 0);
-  const T* v = static_cast<const T*>(a.v) + b * a.vsb + h * a.vsh + (mine ? col : 0);
-  T* raw = static_cast<T*>(c.raw) + ((int64_t)b * c.H + h) * RAW * c.d + col;
+  const bool fits = exists && n > 0 && s >= 0 && s + n <= c.capacity();
+  const T* src = keys ? static_cast<const T*>(a.k) + b * a.ksb + h * a.ksh
+                      : static_cast<const T*>(a.v) + b * a.vsb + h * a.vsh;
+  const int64_t sn = keys ? a.ksn : a.vsn;
+  const int at_col = mine ? col : 0;
+  T* raw = static_cast<T*>(c.raw) + (int64_t)bh * RAW * c.d + at_col;
   const int skip = KT == 7 ? 0 : KT - a.K;  // a shorter filter's taps are the window's last
-  double taps[KT ? KT : 1];
-#pragma unroll
-  for (int i = 0; i < KT; ++i)
-    taps[i] = i >= skip ? (double)a.taps[(a.taps_rows > 1 ? (int64_t)h * a.K : 0) + i - skip] : 0.0;
-  // Group 0 has two blocks.  Groups of several waves meet at barriers, so there the others take a second, empty round.
-  const int from = j == 0 ? 0 : j + 1, rounds = j == 0 || a.group > 64 ? 2 : 1;
+  // Group 0 has two blocks, if the call's tokens may reach a second one.
+  const int from = j == 0 ? 0 : j + 1, rounds = j == 0 ? 2 : 1;
   for (int r = 0; r < rounds; ++r) {
     const int i = from + r;
     const int64_t pos0 = (s & ~(int64_t)(BLOCK - 1)) + (int64_t)i * BLOCK;
     const int t0 = (int)max((int64_t)0, s - pos0);
-    const int64_t left = s + n - pos0;
-    const int t1 = (int)min((int64_t)BLOCK, left);
-    bool live = fits && t1 > t0 && (r == 0 || j == 0);
-    int64_t block = -1;
-    if (live) block = c.block_at(b, h, pos0);
-    live = live && block >= 0;
-    double x[BLOCK];
-    float y[BLOCK];
-    double top_k = 0, top_v = 0;
-    if (live && mine) {
-      double w[HIST + BLOCK];
-#pragma unroll
-      for (int t = 0; t < HIST + BLOCK; ++t) {
-        const int64_t at = pos0 - HIST + t - s;  // of the call's tokens
-        w[t] = (double)to_f32(k[min(max(at, (int64_t)0), (int64_t)n - 1) * a.ksn]);
-      }
-      if (HIST && pos0 - HIST < s) {
-#pragma unroll
-        for (int t = 0; t < HIST + BLOCK - 1; ++t) {
-          const int64_t pos = pos0 - HIST + t;
-          if (pos < s) w[t] = pos >= 0 && s - pos < a.K ? (double)to_f32(raw[(pos & (RAW - 1)) * c.d]) : 0.0;
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < BLOCK; ++t) {
-        double acc = KT ? 0.0 : w[t];
-#pragma unroll
-        for (int u = 0; u < KT; ++u)
-          if (KT == 7 || u >= skip) acc = fma(taps[u], w[t + u], acc);
-        x[t] = acc;
-        y[t] = to_f32(v[min(max(pos0 + t - s, (int64_t)0), (int64_t)n - 1) * a.vsn]);
-        if (t >= t0 && t < t1) {
-          if (fabs(acc) < __builtin_inf()) top_k = fmax(top_k, fabs(acc));
-          if (fabsf(y[t]) < __builtin_inff()) top_v = fmax(top_v, (double)fabsf(y[t]));
-        }
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < BLOCK; ++t) x[t] = 0, y[t] = 0;
-    }
-    int ek = group_max(need(top_k), a.group, lds), ev = group_max(need(top_v), a.group, lds);
-    if (!live) continue;
-    const int was_k = min((int)c.k_scale[block], 247) - 127, was_v = min((int)c.v_scale[block], 247) - 127;
-    if (t0 > 0) ek = max(ek, was_k), ev = max(ev, was_v);
-    if (col >= c.D) continue;
-    const double ik = __builtin_bit_cast(double, (uint64_t)(1023 - ek) << 52);
-    const float iv = two_to(-ev);
-    uint8_t* kb = c.k + block * BLOCK * c.D + col;
-    uint8_t* vb = c.v + block * BLOCK * c.D + col * BLOCK;
-    uint4 old = {0, 0, 0, 0};
+    const int t1 = (int)min((int64_t)BLOCK, s + n - pos0);
+    const int64_t block = fits && t1 > t0 ? c.block_at(b, h, pos0) : -1;
+    const bool live = block >= 0;
+    const int i0 = (int)(pos0 - s);  // of the block's first place among the call's tokens
     const bool part = t0 > 0 || t1 < BLOCK;
-    if (part) old = *reinterpret_cast<const uint4*>(vb);
-    const float again_k = ldexpf(1.0f, was_k - ek), again_v = ldexpf(1.0f, was_v - ev);
-    unsigned out[4] = {0, 0, 0, 0};
+    uint8_t* bytes = (keys ? c.k : c.v) + block * BLOCK * c.D;
+    uint8_t* scale = (keys ? c.k_scale : c.v_scale) + block;
+    const auto token = [&](int i) { return to_f32(src[min(max(i, 0), n - 1) * sn + at_col]); };
+    uint4 out = {0, 0, 0, 0}, old = {0, 0, 0, 0};
+    int was = 0, e = E_LOWEST;
+    // the block's bytes so far and its scale: a value column's own, or 16 bytes of the key block to be turned
+    if (live && part && col < c.D) old = *reinterpret_cast<const uint4*>(bytes + col * BLOCK);
+    if (live && t0 > 0) was = min((int)*scale, 247) - 127;
+    if (keys) {
+      double x[BLOCK];
+      if (live) {
+        float w[HIST + BLOCK];
 #pragma unroll
-    for (int t = 0; t < BLOCK; ++t) {
-      unsigned byte;
-      if (t < t0) {
-        if (ek != was_k) kb[t * c.D] = (uint8_t)e4m3(value(kb[t * c.D]) * again_k);
-        byte = e4m3(value(byte_of(old, t)) * again_v);
-      } else if (t < t1) {
-        const bool fk = fabs(x[t]) < __builtin_inf(), fv = fabsf(y[t]) < __builtin_inff();
-        kb[t * c.D] = fk ? (uint8_t)e4m3(cut(x[t] * ik)) : E4M3_NAN;
-        byte = fv ? e4m3(y[t] * iv) : E4M3_NAN;
-      } else {
-        byte = byte_of(old, t);
+        for (int t = 0; t < HIST + BLOCK; ++t) w[t] = token(i0 - HIST + t);
+        if (HIST && i0 < HIST) {
+#pragma unroll
+          for (int t = 0; t < HIST + BLOCK - 1; ++t) {
+            const int64_t pos = pos0 - HIST + t;
+            if (pos < s) w[t] = pos >= 0 && s - pos < a.K ? to_f32(raw[(pos & (RAW - 1)) * c.d]) : 0.0f;
+          }
+        }
+        if (KT) {
+          const float* taps = a.taps + (a.taps_rows > 1 ? (int64_t)h * a.K : 0) - skip;
+          double tap[KT ? KT : 1], win[KT ? KT : 1];
+#pragma unroll
+          for (int u = 0; u < KT; ++u) tap[u] = u >= skip ? (double)taps[u] : 0.0;
+#pragma unroll
+          for (int u = 0; u < HIST; ++u) win[u] = (double)w[u];
+#pragma unroll
+          for (int t = 0; t < BLOCK; ++t) {
+            win[(HIST + t) % (KT ? KT : 1)] = (double)w[HIST + t];
+            double acc = 0;
+#pragma unroll
+            for (int u = 0; u < KT; ++u)
+              if (KT == 7 || u >= skip) acc = fma(tap[u], win[(t + u) % (KT ? KT : 1)], acc);
+            x[t] = mine ? acc : 0.0;
+          }
+        } else {
+#pragma unroll
+          for (int t = 0; t < BLOCK; ++t) x[t] = mine ? (double)w[t] : 0.0;
+        }
+        e = need(largest(x, t0, t1));
       }
-      out[t >> 2] |= byte << (8 * (t & 3));
+      e = group_max<GROUP>(e, peaks);
+      if (t0 > 0) e = max(e, was);
+      uint8_t* lds = reinterpret_cast<uint8_t*>(turn + (threadIdx.x & ~(GROUP - 1)));
+      if (part) {  // the column's old bytes
+        group_sync<GROUP>();
+        if (live && col < c.D) turn[threadIdx.x] = old;
+        group_sync<GROUP>();
+        unsigned q[4] = {0, 0, 0, 0};
+        if (live && col < c.D)
+#pragma unroll
+          for (int t = 0; t < BLOCK; ++t) q[t >> 2] |= (unsigned)lds[t * c.D + col] << (8 * (t & 3));
+        old = uint4{q[0], q[1], q[2], q[3]};
+      }
+      if (live) {
+        const double inv = __builtin_bit_cast(double, (uint64_t)(1023 - e) << 52);
+        out = column(x, inv, old, t0, t1, ldexpf(1.0f, was - e));
+      }
+      group_sync<GROUP>();
+      if (live && col < c.D)
+#pragma unroll
+        for (int t = 0; t < BLOCK; ++t) lds[t * c.D + col] = (uint8_t)byte_of(out, t);
+      group_sync<GROUP>();
+      out = turn[threadIdx.x];
+    } else {
+      float y[BLOCK];
+      if (live) {
+#pragma unroll
+        for (int t = 0; t < BLOCK; ++t) y[t] = mine ? token(i0 + t) : 0.0f;
+        e = need(largest(y, t0, t1));
+      }
+      e = group_max<GROUP>(e, peaks);
+      if (GROUP > 64) {  // the barriers that the workgroup's key group waits at
+        if (part) group_sync<GROUP>(), group_sync<GROUP>();
+        group_sync<GROUP>(), group_sync<GROUP>();
+      }
+      if (t0 > 0) e = max(e, was);
+      if (live) out = column(y, two_to(-e), old, t0, t1, ldexpf(1.0f, was - e));
     }
-    *reinterpret_cast<uint4*>(vb) = uint4{out[0], out[1], out[2], out[3]};
-    if (col == 0) c.k_scale[block] = (uint8_t)(ek + 127), c.v_scale[block] = (uint8_t)(ev + 127);
+    if (live && col < c.D) *reinterpret_cast<uint4*>(bytes + col * BLOCK) = out;
+    if (live && col == 0) *scale = (uint8_t)(e + 127);
   }
-  if (c.raw && j == 0 && fits && mine)
-    for (int t = max(0, n - RAW); t < n; ++t) raw[((s + t) & (RAW - 1)) * c.d] = k[t * a.ksn];
+  if (keys && c.raw && j == 0 && fits && mine)
+    for (int t = max(0, n - RAW); t < n; ++t) raw[((s + t) & (RAW - 1)) * c.d] = src[t * sn + at_col];
 }
 
 struct ReadArgs {
@@ -260,12 +339,22 @@ int grid_of(int64_t items, int group, const char* what, int64_t* grid) {
   return PNFX_OK;
 }
 
-template <typename T>
-void append_any(const AppendArgs& a, int64_t grid, hipStream_t st) {
+template <typename T, int KT>
+void append_group(const AppendArgs& a, int group, int64_t grid, hipStream_t st) {
   const auto go = [&](auto kernel) { kernel<<<dim3((unsigned)grid), dim3(THREADS), 0, st>>>(a); };
-  if (!a.taps) go(append_kernel<T, 0>);
-  else if (a.K == 7) go(append_kernel<T, 7>);  // the framework's filters
-  else go(append_kernel<T, 16>);
+  switch (group) {
+    case 16: return go(append_kernel<T, KT, 16>);
+    case 32: return go(append_kernel<T, KT, 32>);
+    case 64: return go(append_kernel<T, KT, 64>);
+    case 128: return go(append_kernel<T, KT, 128>);
+    default: return go(append_kernel<T, KT, 256>);
+  }
+}
+template <typename T>
+void append_any(const AppendArgs& a, int group, int64_t grid, hipStream_t st) {
+  if (!a.taps) append_group<T, 0>(a, group, grid, st);
+  else if (a.K == 7) append_group<T, 7>(a, group, grid, st);  // the framework's filters
+  else append_group<T, 16>(a, group, grid, st);
 }
 
 }  // namespace
@@ -288,15 +377,15 @@ extern "C" int pnfx_cache_append(const pnfx_cache* cache, const void* k, int64_t
   a.span = Span{start, counts, (int)start_all, (int)N};
   a.k = k, a.v = v, a.ksb = ksb, a.ksh = ksh, a.ksn = ksn, a.vsb = vsb, a.vsh = vsh, a.vsn = vsn;
   a.taps = taps, a.taps_rows = (int)taps_rows, a.K = taps ? K : 1;
-  a.group = group_of(a.c.D);
+  const int group = group_of(a.c.D);
   const int64_t blocks = (N + 2 * BLOCK - 2) / BLOCK;  // a call may begin at a block's last token
   a.groups = (int)(blocks > 1 ? blocks - 1 : 1);
-  a.items = (int64_t)a.c.B * a.c.H * a.groups;
+  a.items = 2ll * a.c.B * a.c.H * a.groups;
   int64_t grid;
-  if (int rc = grid_of(a.items, a.group, "cache_append", &grid)) return rc;
+  if (int rc = grid_of(a.items, group, "cache_append", &grid)) return rc;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (dtype == PNFX_F32) append_any<float>(a, grid, st);
-  else append_any<bf16>(a, grid, st);
+  if (dtype == PNFX_F32) append_any<float>(a, group, grid, st);
+  else append_any<bf16>(a, group, grid, st);
   return launch_status("cache_append");
 }
 

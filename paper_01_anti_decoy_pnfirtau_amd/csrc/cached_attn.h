@@ -62,7 +62,7 @@ struct AttnPlan {
 
 // Waves of a kernel that a SIMD holds, by its registers: the card has 1024 times as many slots.
 constexpr int resident(int bytes, int D, int NT) {
-  return bytes == 2 && D * NT <= 64 ? 3 : D * NT <= 128 ? 2 : 1;
+  return D * NT <= 32 ? 4 : bytes == 2 && D * NT <= 64 ? 3 : D * NT <= 128 ? 2 : 1;
 }
 
 // The kernels, by the type of the queries and the head size in the cache.
