@@ -139,13 +139,12 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
   const Cache& c = a.c;
   int within = threadIdx.x / GROUP;
   if (GROUP >= 64) within = __builtin_amdgcn_readfirstlane(within);  // the same for a wave: rows by scalar addresses
-  int64_t item = (int64_t)blockIdx.x * PER + within;
-  const bool exists = item < a.items;
+  unsigned item = blockIdx.x * PER + within;
+  const bool exists = item < (unsigned)a.items;
   if (!exists) item = 0;
   const bool keys = item % 2 == 0;
-  item /= 2;
-  const int j = (int)(item % a.groups);
-  const int bh = (int)(item / a.groups), b = bh / c.H, h = bh % c.H;
+  const int j = (int)(item / 2 % (unsigned)a.groups);
+  const int bh = (int)(item / 2 / (unsigned)a.groups), b = bh / c.H, h = bh % c.H;
   const int col = threadIdx.x & (GROUP - 1);
   const bool mine = col < c.d;  // a column of the head; the others up to D hold zeros
   const int64_t s = a.span.first(b);
@@ -155,6 +154,7 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
                       : static_cast<const T*>(a.v) + b * a.vsb + h * a.vsh;
   const int64_t sn = keys ? a.ksn : a.vsn;
   const int at_col = mine ? col : 0;
+  const unsigned mask = mine ? ~0u : 0u;
   T* raw = static_cast<T*>(c.raw) + (int64_t)bh * RAW * c.d + at_col;
   const int skip = KT == 7 ? 0 : KT - a.K;  // a shorter filter's taps are the window's last
   // Group 0 has two blocks, if the call's tokens may reach a second one.
@@ -170,7 +170,10 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
     const bool part = t0 > 0 || t1 < BLOCK;
     uint8_t* bytes = (keys ? c.k : c.v) + block * BLOCK * c.D;
     uint8_t* scale = (keys ? c.k_scale : c.v_scale) + block;
-    const auto token = [&](int i) { return to_f32(src[min(max(i, 0), n - 1) * sn + at_col]); };
+    // (a mask, as the compiler turns a choice of a load or zero into a branch for each, which waits for its load)
+    const auto token = [&](int i) {
+      return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, to_f32(src[min(max(i, 0), n - 1) * sn + at_col])) & mask);
+    };
     uint4 out = {0, 0, 0, 0}, old = {0, 0, 0, 0};
     int was = 0, e = E_LOWEST;
     // the block's bytes so far and its scale: a value column's own, or 16 bytes of the key block to be turned
@@ -186,7 +189,7 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
 #pragma unroll
           for (int t = 0; t < HIST + BLOCK - 1; ++t) {
             const int64_t pos = pos0 - HIST + t;
-            if (pos < s) w[t] = pos >= 0 && s - pos < a.K ? to_f32(raw[(pos & (RAW - 1)) * c.d]) : 0.0f;
+            if (pos < s) w[t] = pos >= 0 && s - pos < a.K && mine ? to_f32(raw[(pos & (RAW - 1)) * c.d]) : 0.0f;
           }
         }
         if (KT) {
@@ -203,11 +206,11 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
 #pragma unroll
             for (int u = 0; u < KT; ++u)
               if (KT == 7 || u >= skip) acc = fma(tap[u], win[(t + u) % (KT ? KT : 1)], acc);
-            x[t] = mine ? acc : 0.0;
+            x[t] = acc;
           }
         } else {
 #pragma unroll
-          for (int t = 0; t < BLOCK; ++t) x[t] = mine ? (double)w[t] : 0.0;
+          for (int t = 0; t < BLOCK; ++t) x[t] = (double)w[t];
         }
         e = need(largest(x, t0, t1));
       }
@@ -238,7 +241,7 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
       float y[BLOCK];
       if (live) {
 #pragma unroll
-        for (int t = 0; t < BLOCK; ++t) y[t] = mine ? token(i0 + t) : 0.0f;
+        for (int t = 0; t < BLOCK; ++t) y[t] = token(i0 + t);
         e = need(largest(y, t0, t1));
       }
       e = group_max<GROUP>(e, peaks);
@@ -270,13 +273,13 @@ template <typename T>
 __global__ __launch_bounds__(THREADS) void read_kernel(ReadArgs a) {
   const Cache& c = a.c;
   const int per = THREADS / a.group;
-  const int64_t item = (int64_t)blockIdx.x * per + threadIdx.x / a.group;
+  const unsigned item = blockIdx.x * per + threadIdx.x / a.group;
   const int col = threadIdx.x & (a.group - 1);
-  if (item >= a.items || col >= c.D) return;
-  const int64_t bh = item / a.groups;
-  const int b = (int)(bh / c.H), h = (int)(bh % c.H);
+  if (item >= (unsigned)a.items || col >= c.D) return;
+  const int64_t bh = item / (unsigned)a.groups;
+  const int b = (int)bh / c.H, h = (int)bh % c.H;
   const int64_t first = a.first ? a.first[b] : a.first_all;
-  const int64_t pos0 = (first & ~(int64_t)(BLOCK - 1)) + item % a.groups * BLOCK;
+  const int64_t pos0 = (first & ~(int64_t)(BLOCK - 1)) + (int64_t)(item % (unsigned)a.groups) * BLOCK;
   const bool there = pos0 >= 0 && pos0 < c.capacity();
   const int64_t block = there ? c.block_at(b, h, pos0) : -1;
   constexpr int VEC = 16 / sizeof(T);
