@@ -48,7 +48,8 @@ __device__ __forceinline__ float cut(double x) {
   const uint64_t hi = (b & 0xffffffff00000000ull) | ((uint64_t)((unsigned)b != 0) << 32);
   return (float)__builtin_bit_cast(double, hi);
 }
-__device__ __forceinline__ unsigned e4m3x4(const float (&x)[4]) {  // |x| <= 448, or NaN
+// |x| <= 448, infinite or NaN: e4m3 has no infinity, both become NaN.
+__device__ __forceinline__ unsigned e4m3x4(const float (&x)[4]) {
   const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
   return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], lo, true);
 }
@@ -95,7 +96,6 @@ __device__ __forceinline__ uint4 column(const X (&x)[BLOCK], X inv, uint4 old, i
     for (int u = 0; u < 4; ++u) {
       const X scaled = x[4 * i + u] * inv;
       y[u] = sizeof(X) == 8 ? cut((double)scaled) : (float)scaled;
-      if (!(fabsf(y[u]) < __builtin_inff())) y[u] = __builtin_nanf("");
     }
     out[i] = e4m3x4(y);
   }
@@ -122,9 +122,15 @@ __device__ __forceinline__ uint4 column(const X (&x)[BLOCK], X inv, uint4 old, i
 template <typename X>
 __device__ __forceinline__ double largest(const X (&x)[BLOCK], int t0, int t1) {
   X top = 0;
+  if (t0 == 0 && t1 == BLOCK) {
+#pragma unroll
+    for (int t = 0; t < BLOCK; ++t) top = fmax(top, fabs(x[t]));  // NaN loses in the maximum
+    if (__builtin_expect(__all(top < (X)__builtin_inf()), 1)) return (double)top;
+    top = 0;
+  }
 #pragma unroll
   for (int t = 0; t < BLOCK; ++t) {
-    const X a = fabs(x[t]);  // NaN loses in the maximum
+    const X a = fabs(x[t]);
     if (t >= t0 && t < t1 && a < (X)__builtin_inf()) top = fmax(top, a);
   }
   return (double)top;
@@ -171,9 +177,12 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
     uint8_t* bytes = (keys ? c.k : c.v) + block * BLOCK * c.D;
     uint8_t* scale = (keys ? c.k_scale : c.v_scale) + block;
     // (a mask, as the compiler turns a choice of a load or zero into a branch for each, which waits for its load)
-    const auto token = [&](int i) {
-      return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, to_f32(src[min(max(i, 0), n - 1) * sn + at_col])) & mask);
+    const bool inner = i0 >= HIST && i0 + BLOCK <= n;  // no token beside the call's: rows by one step
+    const T* at = src + (i0 - HIST) * sn + at_col;
+    const auto masked = [&](T x) {
+      return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, to_f32(x)) & mask);
     };
+    const auto token = [&](int i) { return masked(src[min(max(i, 0), n - 1) * sn + at_col]); };
     uint4 out = {0, 0, 0, 0}, old = {0, 0, 0, 0};
     int was = 0, e = E_LOWEST;
     // the block's bytes so far and its scale: a value column's own, or 16 bytes of the key block to be turned
@@ -183,8 +192,13 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
       double x[BLOCK];
       if (live) {
         float w[HIST + BLOCK];
+        if (inner) {
 #pragma unroll
-        for (int t = 0; t < HIST + BLOCK; ++t) w[t] = token(i0 - HIST + t);
+          for (int t = 0; t < HIST + BLOCK; ++t) w[t] = masked(at[t * sn]);
+        } else {
+#pragma unroll
+          for (int t = 0; t < HIST + BLOCK; ++t) w[t] = token(i0 - HIST + t);
+        }
         if (HIST && i0 < HIST) {
 #pragma unroll
           for (int t = 0; t < HIST + BLOCK - 1; ++t) {
@@ -240,8 +254,13 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
     } else {
       float y[BLOCK];
       if (live) {
+        if (inner) {
 #pragma unroll
-        for (int t = 0; t < BLOCK; ++t) y[t] = token(i0 + t);
+          for (int t = 0; t < BLOCK; ++t) y[t] = masked(at[(HIST + t) * sn]);
+        } else {
+#pragma unroll
+          for (int t = 0; t < BLOCK; ++t) y[t] = token(i0 + t);
+        }
         e = need(largest(y, t0, t1));
       }
       e = group_max<GROUP>(e, peaks);

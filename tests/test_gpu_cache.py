@@ -119,6 +119,26 @@ def test_values_that_are_not_finite_stay_where_they_are_seen(dev):
         assert o[0, 0, 0].isnan().sum() == 1 and o[0, 0, 1].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("K", [None, 7])
+def test_append_of_what_is_not_finite(dev, dtype, K):
+    taps = None if K is None else causal_gaussian_taps(K)
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(1, 2, 50, 24, generator=g).to(dtype) for _ in range(2))
+    for t in (k, v):
+        t[0, 0, 20, 3], t[0, 1, 21, 5], t[0, 0, 40, :], t[0, 1, 7, 1] = torch.inf, -torch.inf, torch.nan, torch.nan
+    k[0, 1, 33, 2] = torch.finfo(dtype).max
+    cache, want = KVCache.new(1, 2, 24, 50, page=16, dtype=dtype, device=dev), O.Cache(1, 2, 24, 64)
+    for a, b in ((0, 37), (37, 38), (38, 50)):
+        cache.append(k[:, :, a:b].to(dev), v[:, :, a:b].to(dev), a, taps=None if K is None else taps.to(dev))
+        with np.errstate(invalid="ignore"):
+            want.append(F64(k[:, :, a:b]), F64(v[:, :, a:b]), [a], None if K is None else F64(taps))
+    with np.errstate(over="ignore"):  # fp32's largest rounds up to 2^128 in e4m3, infinity as fp32
+        want = [x.astype(np.float32) for x in want.dense()]
+    for got, exact in zip(cache.read(0, 50, F32), want):
+        assert np.array_equal(got[0].cpu().numpy(), exact[0, :, :50], equal_nan=True)
+
+
 def test_what_does_not_fit_is_left_alone(dev):
     cache, want = filled(2, 2, 20, CALLS[1], causal_gaussian_taps(7), F32, device=dev)
     before = [t.clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale, cache.raw)]
