@@ -35,19 +35,21 @@ struct AppendArgs {
 };
 
 // The exponent of the smallest scale for numbers up to top >= 0: 448 = 1.75 * 2^8.
-__device__ __forceinline__ int need(double top) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, top);
-  const int e = (int)(b >> 52) - 1023 - 8 + ((b & 0xfffffffffffffull) > 0xc000000000000ull);
+__device__ __forceinline__ int need(float top) {
+  const unsigned b = __builtin_bit_cast(unsigned, top);
+  const int e = (int)(b >> 23) - 127 - 8 + ((b & 0x7fffff) > 0x600000);
   return max(e, E_LOWEST);  // zero and what is below the normal numbers: far below
 }
 
-// x as e4m3: the number is first cut to 20 fraction bits, the lowest set if any bit behind it was, from which fp32 is
-// exact and the conversion's rounding that of x itself.
+// x cut to 20 fraction bits, the lowest set if any bit behind it was: fp32 holds that exactly (what is below its normal
+// numbers is below every scale), times powers of two as well, and its rounding to e4m3 is that of x itself, as is its
+// place beside 1.75 * 2^n.  From 2^128 on: infinite.
 __device__ __forceinline__ float cut(double x) {
   const uint64_t b = __builtin_bit_cast(uint64_t, x);
   const uint64_t hi = (b & 0xffffffff00000000ull) | ((uint64_t)((unsigned)b != 0) << 32);
   return (float)__builtin_bit_cast(double, hi);
 }
+
 // |x| <= 448, infinite or NaN: e4m3 has no infinity, both become NaN.
 __device__ __forceinline__ unsigned e4m3x4(const float (&x)[4]) {
   const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
@@ -85,18 +87,14 @@ __device__ __forceinline__ int group_max(int x, int* lds) {
   return x;
 }
 
-// A column's 16 bytes with those of tokens t0 .. t1 - 1 from x (in units of 1), the kept ones before them over `again`.
-template <typename X>
-__device__ __forceinline__ uint4 column(const X (&x)[BLOCK], X inv, uint4 old, int t0, int t1, float again) {
+// A column's 16 bytes with those of tokens t0 .. t1 - 1 from x inv, the kept ones before them over `again`.
+__device__ __forceinline__ uint4 column(const float (&x)[BLOCK], float inv, uint4 old, int t0, int t1, float again) {
   unsigned out[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float y[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const X scaled = x[4 * i + u] * inv;
-      y[u] = sizeof(X) == 8 ? cut((double)scaled) : (float)scaled;
-    }
+    for (int u = 0; u < 4; ++u) y[u] = x[4 * i + u] * inv;
     out[i] = e4m3x4(y);
   }
   if (t0 > 0 || t1 < BLOCK) {
@@ -119,21 +117,20 @@ __device__ __forceinline__ uint4 column(const X (&x)[BLOCK], X inv, uint4 old, i
 }
 
 // The largest finite |x| of tokens t0 .. t1 - 1.
-template <typename X>
-__device__ __forceinline__ double largest(const X (&x)[BLOCK], int t0, int t1) {
-  X top = 0;
+__device__ __forceinline__ float largest(const float (&x)[BLOCK], int t0, int t1) {
+  float top = 0;
   if (t0 == 0 && t1 == BLOCK) {
 #pragma unroll
-    for (int t = 0; t < BLOCK; ++t) top = fmax(top, fabs(x[t]));  // NaN loses in the maximum
-    if (__builtin_expect(__all(top < (X)__builtin_inf()), 1)) return (double)top;
+    for (int t = 0; t < BLOCK; ++t) top = fmaxf(top, fabsf(x[t]));  // NaN loses in the maximum
+    if (__builtin_expect(__all(top < __builtin_inff()), 1)) return top;
     top = 0;
   }
 #pragma unroll
   for (int t = 0; t < BLOCK; ++t) {
-    const X a = fabs(x[t]);
-    if (t >= t0 && t < t1 && a < (X)__builtin_inf()) top = fmax(top, a);
+    const float a = fabsf(x[t]);
+    if (t >= t0 && t < t1 && a < __builtin_inff()) top = fmaxf(top, a);
   }
-  return (double)top;
+  return top;
 }
 
 // KT: the window that the FIR's taps are at the end of; 0: no FIR.  GROUP: threads of a block, at least its columns.
@@ -189,7 +186,7 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
     if (live && part && col < c.D) old = *reinterpret_cast<const uint4*>(bytes + col * BLOCK);
     if (live && t0 > 0) was = min((int)*scale, 247) - 127;
     if (keys) {
-      double x[BLOCK];
+      float x[BLOCK];
       if (live) {
         float w[HIST + BLOCK];
         if (inner) {
@@ -220,11 +217,11 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
 #pragma unroll
             for (int u = 0; u < KT; ++u)
               if (KT == 7 || u >= skip) acc = fma(tap[u], win[(t + u) % (KT ? KT : 1)], acc);
-            x[t] = acc;
+            x[t] = cut(acc);
           }
         } else {
 #pragma unroll
-          for (int t = 0; t < BLOCK; ++t) x[t] = (double)w[t];
+          for (int t = 0; t < BLOCK; ++t) x[t] = w[t];
         }
         e = need(largest(x, t0, t1));
       }
@@ -242,8 +239,7 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
         old = uint4{q[0], q[1], q[2], q[3]};
       }
       if (live) {
-        const double inv = __builtin_bit_cast(double, (uint64_t)(1023 - e) << 52);
-        out = column(x, inv, old, t0, t1, ldexpf(1.0f, was - e));
+        out = column(x, two_to(-e), old, t0, t1, ldexpf(1.0f, was - e));
       }
       group_sync<GROUP>();
       if (live && col < c.D)

@@ -297,6 +297,7 @@ def _append(cache: KVCache, k, v, start, taps, counts) -> None:
         hist = cache.raw.double().gather(2, (old % RAW)[:, None, :, None].expand(B, H, -1, d))
         hist = torch.where((old >= 0)[:, None, :, None], hist, 0.0)
         x = (torch.cat([hist, x], 2).unfold(2, K, 1) * taps[:, None, None]).sum(-1)
+        x = torch.where(x.abs() < 2.0 ** 128, x, x * torch.inf)  # beyond fp32: not finite
     D = cache.k.shape[3]
     for b in range(B):
         s, end = int(start[b]), int(start[b] + n[b])
