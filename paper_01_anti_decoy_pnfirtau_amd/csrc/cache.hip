@@ -11,9 +11,12 @@
 // The tokens a begun block already has are rounded again when its scale grows: exact except below 2^-6 2^E, as a
 // power of two leaves the significant bits alone.
 //
+// A group has several blocks in a row and asks for the next one's tokens before it works on this one's; the FIR's window
+// stays in registers.
+//
 // The keys before the FIR that the next call needs are in `raw`, position p at p % 16.  Whoever reads them (the first
-// and the second block of a sequence's tokens) must have done so before they are overwritten: one group has both
-// blocks, each thread reads and writes its own column only, and writes last.
+// and, for want of tokens before it, the second block of a call) must have done so before they are overwritten: one
+// group has both blocks, each thread reads and writes its own column only, and writes last.
 #include "cache.h"
 
 #include <cmath>
@@ -22,6 +25,7 @@ namespace pnfx {
 namespace {
 
 constexpr int THREADS = 256;
+constexpr int EACH = 2;  // blocks of a group, at least 2; 4 x 16 heads x 8192 tokens of 64: 87 us, with 4 also, with 8 95
 
 struct AppendArgs {
   Cache c;
@@ -160,73 +164,79 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
   const unsigned mask = mine ? ~0u : 0u;
   T* raw = static_cast<T*>(c.raw) + (int64_t)bh * RAW * c.d + at_col;
   const int skip = KT == 7 ? 0 : KT - a.K;  // a shorter filter's taps are the window's last
-  // Group 0 has two blocks, if the call's tokens may reach a second one.
-  const int from = j == 0 ? 0 : j + 1, rounds = j == 0 ? 2 : 1;
-  for (int r = 0; r < rounds; ++r) {
-    const int i = from + r;
-    const int64_t pos0 = (s & ~(int64_t)(BLOCK - 1)) + (int64_t)i * BLOCK;
+  // (a mask, as the compiler turns a choice of a load or zero into a branch for each, which waits for its load)
+  const auto masked = [&](T x) {
+    return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, to_f32(x)) & mask);
+  };
+  // The call's tokens i0 .. i0 + count - 1 of the column; what is beside them is some token of it.
+  const auto load = [&](auto& x, int off, int i0, auto count) {
+    if (i0 >= 0 && i0 + count() <= n) {  // rows by one step
+      const T* at = src + i0 * sn + at_col;
+#pragma unroll
+      for (int t = 0; t < count(); ++t) x[off + t] = masked(at[t * sn]);
+    } else {
+#pragma unroll
+      for (int t = 0; t < count(); ++t) x[off + t] = masked(src[min(max(i0 + t, 0), n - 1) * sn + at_col]);
+    }
+  };
+  struct Whole { constexpr int operator()() const { return HIST + BLOCK; } };
+  struct Next { constexpr int operator()() const { return BLOCK; } };
+  // w: the column's numbers, for keys those before the block, too; the next block's are on their way meanwhile
+  float w[HIST + BLOCK];
+  int64_t pos0 = (s & ~(int64_t)(BLOCK - 1)) + (int64_t)j * EACH * BLOCK;
+  if (fits && pos0 < s + n) {
+    load(w, 0, (int)(pos0 - s) - HIST, Whole{});
+    if (HIST && keys && pos0 - HIST < s) {  // the first block
+#pragma unroll
+      for (int t = 0; t < HIST + BLOCK - 1; ++t) {
+        const int64_t pos = pos0 - HIST + t;
+        if (pos < s) w[t] = pos >= 0 && s - pos < a.K && mine ? to_f32(raw[(pos & (RAW - 1)) * c.d]) : 0.0f;
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < EACH; ++r, pos0 += BLOCK) {
+    if (GROUP >= 64 && pos0 >= s + n) break;  // the same for all that meet at a barrier
     const int t0 = (int)max((int64_t)0, s - pos0);
     const int t1 = (int)min((int64_t)BLOCK, s + n - pos0);
     const int64_t block = fits && t1 > t0 ? c.block_at(b, h, pos0) : -1;
     const bool live = block >= 0;
-    const int i0 = (int)(pos0 - s);  // of the block's first place among the call's tokens
     const bool part = t0 > 0 || t1 < BLOCK;
     uint8_t* bytes = (keys ? c.k : c.v) + block * BLOCK * c.D;
     uint8_t* scale = (keys ? c.k_scale : c.v_scale) + block;
-    // (a mask, as the compiler turns a choice of a load or zero into a branch for each, which waits for its load)
-    const bool inner = i0 >= HIST && i0 + BLOCK <= n;  // no token beside the call's: rows by one step
-    const T* at = src + (i0 - HIST) * sn + at_col;
-    const auto masked = [&](T x) {
-      return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, to_f32(x)) & mask);
-    };
-    const auto token = [&](int i) { return masked(src[min(max(i, 0), n - 1) * sn + at_col]); };
     uint4 out = {0, 0, 0, 0}, old = {0, 0, 0, 0};
     int was = 0, e = E_LOWEST;
     // the block's bytes so far and its scale: a value column's own, or 16 bytes of the key block to be turned
     if (live && part && col < c.D) old = *reinterpret_cast<const uint4*>(bytes + col * BLOCK);
     if (live && t0 > 0) was = min((int)*scale, 247) - 127;
-    if (keys) {
-      float x[BLOCK];
-      if (live) {
-        float w[HIST + BLOCK];
-        if (inner) {
+    float next[BLOCK], x[BLOCK];
+    if (r + 1 < EACH && fits && pos0 + BLOCK < s + n) load(next, 0, (int)(pos0 + BLOCK - s), Next{});
+    if (live) {
+      if (KT && keys) {
+        const float* taps = a.taps + (a.taps_rows > 1 ? (int64_t)h * a.K : 0) - skip;
+        double tap[KT ? KT : 1], win[KT ? KT : 1];
 #pragma unroll
-          for (int t = 0; t < HIST + BLOCK; ++t) w[t] = masked(at[t * sn]);
-        } else {
+        for (int u = 0; u < KT; ++u) tap[u] = u >= skip ? (double)taps[u] : 0.0;
 #pragma unroll
-          for (int t = 0; t < HIST + BLOCK; ++t) w[t] = token(i0 - HIST + t);
+        for (int u = 0; u < HIST; ++u) win[u] = (double)w[u];
+#pragma unroll
+        for (int t = 0; t < BLOCK; ++t) {
+          win[(HIST + t) % (KT ? KT : 1)] = (double)w[HIST + t];
+          double acc = 0;
+#pragma unroll
+          for (int u = 0; u < KT; ++u)
+            if (KT == 7 || u >= skip) acc = fma(tap[u], win[(t + u) % (KT ? KT : 1)], acc);
+          x[t] = cut(acc);
         }
-        if (HIST && i0 < HIST) {
+      } else {
 #pragma unroll
-          for (int t = 0; t < HIST + BLOCK - 1; ++t) {
-            const int64_t pos = pos0 - HIST + t;
-            if (pos < s) w[t] = pos >= 0 && s - pos < a.K && mine ? to_f32(raw[(pos & (RAW - 1)) * c.d]) : 0.0f;
-          }
-        }
-        if (KT) {
-          const float* taps = a.taps + (a.taps_rows > 1 ? (int64_t)h * a.K : 0) - skip;
-          double tap[KT ? KT : 1], win[KT ? KT : 1];
-#pragma unroll
-          for (int u = 0; u < KT; ++u) tap[u] = u >= skip ? (double)taps[u] : 0.0;
-#pragma unroll
-          for (int u = 0; u < HIST; ++u) win[u] = (double)w[u];
-#pragma unroll
-          for (int t = 0; t < BLOCK; ++t) {
-            win[(HIST + t) % (KT ? KT : 1)] = (double)w[HIST + t];
-            double acc = 0;
-#pragma unroll
-            for (int u = 0; u < KT; ++u)
-              if (KT == 7 || u >= skip) acc = fma(tap[u], win[(t + u) % (KT ? KT : 1)], acc);
-            x[t] = cut(acc);
-          }
-        } else {
-#pragma unroll
-          for (int t = 0; t < BLOCK; ++t) x[t] = w[t];
-        }
-        e = need(largest(x, t0, t1));
+        for (int t = 0; t < BLOCK; ++t) x[t] = w[HIST + t];
       }
-      e = group_max<GROUP>(e, peaks);
-      if (t0 > 0) e = max(e, was);
+      e = need(largest(x, t0, t1));
+    }
+    e = group_max<GROUP>(e, peaks);
+    if (t0 > 0) e = max(e, was);
+    if (keys) {
       uint8_t* lds = reinterpret_cast<uint8_t*>(turn + (threadIdx.x & ~(GROUP - 1)));
       if (part) {  // the column's old bytes
         group_sync<GROUP>();
@@ -238,9 +248,7 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
           for (int t = 0; t < BLOCK; ++t) q[t >> 2] |= (unsigned)lds[t * c.D + col] << (8 * (t & 3));
         old = uint4{q[0], q[1], q[2], q[3]};
       }
-      if (live) {
-        out = column(x, two_to(-e), old, t0, t1, ldexpf(1.0f, was - e));
-      }
+      if (live) out = column(x, two_to(-e), old, t0, t1, ldexpf(1.0f, was - e));
       group_sync<GROUP>();
       if (live && col < c.D)
 #pragma unroll
@@ -248,27 +256,18 @@ __global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
       group_sync<GROUP>();
       out = turn[threadIdx.x];
     } else {
-      float y[BLOCK];
-      if (live) {
-        if (inner) {
-#pragma unroll
-          for (int t = 0; t < BLOCK; ++t) y[t] = masked(at[(HIST + t) * sn]);
-        } else {
-#pragma unroll
-          for (int t = 0; t < BLOCK; ++t) y[t] = token(i0 + t);
-        }
-        e = need(largest(y, t0, t1));
-      }
-      e = group_max<GROUP>(e, peaks);
       if (GROUP > 64) {  // the barriers that the workgroup's key group waits at
         if (part) group_sync<GROUP>(), group_sync<GROUP>();
         group_sync<GROUP>(), group_sync<GROUP>();
       }
-      if (t0 > 0) e = max(e, was);
-      if (live) out = column(y, two_to(-e), old, t0, t1, ldexpf(1.0f, was - e));
+      if (live) out = column(x, two_to(-e), old, t0, t1, ldexpf(1.0f, was - e));
     }
     if (live && col < c.D) *reinterpret_cast<uint4*>(bytes + col * BLOCK) = out;
     if (live && col == 0) *scale = (uint8_t)(e + 127);
+#pragma unroll
+    for (int t = 0; t < HIST; ++t) w[t] = w[BLOCK + t];
+#pragma unroll
+    for (int t = 0; t < BLOCK; ++t) w[HIST + t] = next[t];
   }
   if (keys && c.raw && j == 0 && fits && mine)
     for (int t = max(0, n - RAW); t < n; ++t) raw[((s + t) & (RAW - 1)) * c.d] = src[t * sn + at_col];
@@ -397,7 +396,7 @@ extern "C" int pnfx_cache_append(const pnfx_cache* cache, const void* k, int64_t
   a.taps = taps, a.taps_rows = (int)taps_rows, a.K = taps ? K : 1;
   const int group = group_of(a.c.D);
   const int64_t blocks = (N + 2 * BLOCK - 2) / BLOCK;  // a call may begin at a block's last token
-  a.groups = (int)(blocks > 1 ? blocks - 1 : 1);
+  a.groups = (int)((blocks + EACH - 1) / EACH);
   a.items = 2ll * a.c.B * a.c.H * a.groups;
   int64_t grid;
   if (int rc = grid_of(a.items, group, "cache_append", &grid)) return rc;
