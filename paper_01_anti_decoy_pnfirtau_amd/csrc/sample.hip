@@ -5,10 +5,14 @@
 // threshold logit, and of the tokens that equal it those up to an index.  The token is the first by index at which
 // the kept ones' running weight passes u times their whole weight.
 //
-// One workgroup of 16 waves has a row, in registers where it fits them, and goes over it several times: the maximum;
-// for top-k, the threshold by a histogram of max z - z, then of the logits' bits within its bin; for top-p, the same
-// with the weights' sums; then the sum of each wave's 64 chunks, in the order of the row, the chunks in which u falls,
-// and the token in them.
+// One workgroup of 16 waves has a row and goes over it several times, the next chunks on their way (a row held in
+// registers gained nothing: 37 us either way for 33278 bf16 logits): the maximum; for top-k, the threshold by a
+// histogram of max z - z, then of the logits' bits within its bin; for top-p, the same with the weights' sums; then the
+// sum of each wave's 64 chunks, in the order of the row, the chunks in which u falls, and the token in them.
+//
+// Long bf16 rows have few different logits: with the magnitudes from 2^-32 to 2^16, 12289 of them.  Their weights are a
+// table in LDS, one exponential for each in place of one for each token, and one histogram of them settles both
+// thresholds.  TABLE_FIGURES
 //
 // Integers decide: weights are 64-bit fixed point, 2^S for the largest, so that sums are exact and the same in any
 // order (the histogram's atomics among them), and a token differs from the real numbers' only where u falls within about
@@ -25,7 +29,7 @@ constexpr int THREADS = 1024, WAVES = THREADS / 64;
 constexpr int DIGIT = 11, BINS = 1 << DIGIT;
 constexpr int STEPS = 256;        // of the exponential's table, an octave
 constexpr float SPAN = 64;        // of the first histogram, at most: what lies further below shares its last bin
-constexpr int MAX_PARTS = 256;    // chunks of a thread in the longest rows: 2^20 fp32, four a chunk
+constexpr int MAX_PARTS = 257;    // chunks of a thread in the longest rows: 2^20 fp32, four a chunk, at any alignment
 constexpr double LOG2E = 1.4426950408889634, LN2 = 0.6931471805599453;
 
 struct SampleArgs {
@@ -44,23 +48,17 @@ __device__ __forceinline__ unsigned key_of(float z) {
 }
 
 // A row, cut into 16-byte chunks, chunk c for thread c % THREADS: part j of all threads holds the logits right before
-// part j + 1, and wave by wave in order.  PARTS: those that a thread has in registers, 0: read again each time.  Places
-// beside the row hold -infinity, whose weight is 0.
-template <typename T, int PARTS>
+// part j + 1, and wave by wave in order.  Places beside the row hold -infinity, whose weight is 0.
+template <typename T>
 struct Row {
   static constexpr int E = 16 / sizeof(T);  // elements of a chunk
-  static constexpr int KEEP = PARTS ? PARTS : 1;
   typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
   const T* base;  // aligned: the row begins `off` elements behind it
-  int off, V, chunks, parts;
-  u32x4 kept[KEEP];
+  int off, V, parts;
   __device__ __forceinline__ Row(const T* p, int V_) : V(V_) {
     off = (int)(reinterpret_cast<uintptr_t>(p) % 16 / sizeof(T));
     base = p - off;
-    chunks = (off + V + E - 1) / E;
-    parts = PARTS ? PARTS : (chunks + THREADS - 1) / THREADS;
-#pragma unroll
-    for (int j = 0; j < PARTS; ++j) kept[j] = read(j);
+    parts = ((off + V + E - 1) / E + THREADS - 1) / THREADS;
   }
   __device__ __forceinline__ u32x4 read(int j) const {
     const int c = j * THREADS + threadIdx.x;
@@ -83,44 +81,57 @@ struct Row {
   // f(part, its chunk), parts in order
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-    if (PARTS) {
+    constexpr int AHEAD = 4;
+    u32x4 w[AHEAD];
 #pragma unroll
-      for (int j = 0; j < PARTS; ++j) {
-        u32x4 w = kept[j];
-        asm volatile("" : "+v"(w));  // what a pass makes of the chunks is not held for the next one
-        f(j, w);
-      }
-    } else {
-      constexpr int AHEAD = 4;
-      for (int j0 = 0; j0 < parts; j0 += AHEAD) {
-        u32x4 w[AHEAD];
+    for (int k = 0; k < AHEAD; ++k)
+      if (k < parts) w[k] = read(k);
+    for (int j0 = 0; j0 < parts; j0 += AHEAD) {
+      u32x4 next[AHEAD];
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k)
-          if (j0 + k < parts) w[k] = read(j0 + k);
+      for (int k = 0; k < AHEAD; ++k)
+        if (j0 + AHEAD + k < parts) next[k] = read(j0 + AHEAD + k);
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k)
-          if (j0 + k < parts) f(j0 + k, w[k]);
+      for (int k = 0; k < AHEAD; ++k) {
+        if (j0 + k < parts) f(j0 + k, w[k]);
+        w[k] = next[k];
       }
     }
   }
-  __device__ __forceinline__ u32x4 part(int j) const {
-    if (!PARTS) return read(j);
-    u32x4 w = kept[0];
-#pragma unroll
-    for (int k = 1; k < PARTS; ++k)
-      if (k == j) w = kept[k];
-    return w;
-  }
 };
 
-struct Lds {
+// Sums over a wave in registers: rows of 16 lanes, then from row to row (lanes without a source add 0).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long moved(unsigned long long x) {
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)x, CTRL, ROWS, 0xf, false);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(x >> 32), CTRL, ROWS, 0xf, false);
+  return (unsigned long long)hi << 32 | lo;
+}
+__device__ __forceinline__ unsigned long long wave_running(unsigned long long x) {
+  x += moved<0x111, 0xf>(x);  // row_shr:1, 2, 4, 8
+  x += moved<0x112, 0xf>(x);
+  x += moved<0x114, 0xf>(x);
+  x += moved<0x118, 0xf>(x);
+  x += moved<0x142, 0xa>(x);  // row_bcast:15 into rows 1 and 3
+  x += moved<0x143, 0xc>(x);  // row_bcast:31 into rows 2 and 3
+  return x;
+}
+__device__ __forceinline__ unsigned long long lane_of(unsigned long long x, int lane) {
+  return (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 |
+         (unsigned)__builtin_amdgcn_readlane((int)(unsigned)x, lane);
+}
+__device__ __forceinline__ unsigned long long wave_total(unsigned long long x) { return lane_of(wave_running(x), 63); }
+
+struct Common {
   double table[STEPS];
-  unsigned long long sums[MAX_PARTS * WAVES];  // of each part and wave; the histogram's bins
-  unsigned count[BINS];
   unsigned long long wave[WAVES];
   float top[WAVES], low[WAVES];
   unsigned long long before;
   int digit, found;
+};
+struct Lds : Common {
+  unsigned long long sums[MAX_PARTS * WAVES];  // of each part and wave; the histogram's bins
+  unsigned count[BINS];
 };
 static_assert(BINS <= MAX_PARTS * WAVES, "");
 
@@ -148,28 +159,14 @@ struct Weights {
   __device__ __forceinline__ unsigned long long operator()(float z) const { return of_steps(steps(z)); }
 };
 
-__device__ __forceinline__ unsigned long long wave_total(unsigned long long x) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
-  return x;
-}
-__device__ __forceinline__ unsigned long long wave_running(unsigned long long x, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const unsigned long long y = __shfl_up(x, o, 64);
-    if (lane >= o) x += y;
-  }
-  return x;
-}
-
 struct Cut {  // what is kept: logits of keys above, and those equal up to an index
   unsigned key;
   int index;
 };
 
-template <typename T, int PARTS>
+template <typename T>
 struct Sampler {
-  using R = Row<T, PARTS>;
+  using R = Row<T>;
   static constexpr int E = R::E;
   R row;
   Lds& s;
@@ -183,41 +180,44 @@ struct Sampler {
     return k > cut.key || (k == cut.key && row.index(j, i) <= cut.index);
   }
 
-  // First index at which the running sum of f(logit, part, place) passes target(sum of all).
+  // First index at which the running sum of f(logit's bits, part, place) passes target(sum of all).
   template <typename F, typename G>
-  __device__ __forceinline__ int first(F f, G target) const {
+  __device__ __forceinline__ int first_of(unsigned long long* sums, F f, G target) const {
+    const auto at_place = [&](const auto& w, int j, int i) {
+      return f(sizeof(T) == 4 ? w[i] : w[i / 2] >> (i % 2 * 16), j, i);
+    };
     __syncthreads();
     row.each([&](int j, const auto& w) {
       unsigned long long sum = 0;
 #pragma unroll
-      for (int i = 0; i < E; ++i) sum += f(R::element(w, i), j, i);
+      for (int i = 0; i < E; ++i) sum += at_place(w, j, i);
       sum = __any(sum != 0) ? wave_total(sum) : 0;
-      if (lane == 0) s.sums[j * WAVES + wave] = sum;
+      if (lane == 0) sums[j * WAVES + wave] = sum;
     });
     __syncthreads();
     // each wave finds the part and wave in which it is, 64 sums at a time
     unsigned long long all = 0, left = 0;
     const int n = row.parts * WAVES;
-    for (int i = lane; i < n; i += 64) all += s.sums[i];
+    for (int i = lane; i < n; i += 64) all += sums[i];
     left = target(wave_total(all));
     int at = n - 1;
     for (int i0 = 0; i0 < n; i0 += 64) {
-      const unsigned long long mine = i0 + lane < n ? s.sums[i0 + lane] : 0, run = wave_running(mine, lane);
+      const unsigned long long mine = i0 + lane < n ? sums[i0 + lane] : 0, run = wave_running(mine);
       const unsigned long long hit = __ballot(run > left);
       if (hit) {
         const int l = __builtin_ctzll(hit);
-        at = i0 + l, left -= __shfl(run - mine, l, 64);
+        at = i0 + l, left -= lane_of(run - mine, l);
         break;
       }
-      left -= __shfl(run, 63, 64);
+      left -= lane_of(run, 63);
     }
     if (wave == at % WAVES) {
       const int j = at / WAVES;
-      const auto w = row.part(j);
+      const auto w = row.read(j);
       unsigned long long mine[E], sum = 0;
 #pragma unroll
-      for (int i = 0; i < E; ++i) mine[i] = f(R::element(w, i), j, i), sum += mine[i];
-      unsigned long long past = wave_running(sum, lane) - sum;
+      for (int i = 0; i < E; ++i) mine[i] = at_place(w, j, i), sum += mine[i];
+      unsigned long long past = wave_running(sum) - sum;
       int found = -1;
 #pragma unroll
       for (int i = 0; i < E; ++i) {
@@ -225,11 +225,21 @@ struct Sampler {
         past += mine[i];
       }
       const unsigned long long hit = __ballot(found >= 0);
-      if (lane == 0) s.found = -1;
-      if (found >= 0 && lane == __builtin_ctzll(hit)) s.found = found;
+      if (hit ? lane == __builtin_ctzll(hit) : lane == 0) s.found = found;
     }
     __syncthreads();
     return s.found;
+  }
+  // The same of the logits themselves.
+  template <typename F, typename G>
+  __device__ __forceinline__ int first(F f, G target) const {
+    return first_of(
+        s.sums,
+        [&](unsigned bits, int j, int i) -> unsigned long long {
+          const unsigned b = sizeof(T) == 4 ? bits : bits << 16;
+          return f(__builtin_bit_cast(float, b) + 0.0f, j, i);
+        },
+        target);
   }
 
   __device__ __forceinline__ int bin(float z) const { return (int)fminf((top - z) * scale, (float)(BINS - 1)); }
@@ -240,7 +250,7 @@ struct Sampler {
   __device__ __forceinline__ int fall(unsigned long long& target, bool down) const {
     const int bin = down ? BINS - 1 - 2 * tid : 2 * tid, next = down ? bin - 1 : bin + 1;
     const unsigned long long v0 = MASS ? s.sums[bin] : s.count[bin], v1 = MASS ? s.sums[next] : s.count[next];
-    const unsigned long long run = wave_running(v0 + v1, lane);
+    const unsigned long long run = wave_running(v0 + v1);
     if (lane == 63) s.wave[wave] = run;
     __syncthreads();
     unsigned long long past = run - v0 - v1;
@@ -317,9 +327,131 @@ struct Sampler {
   }
 };
 
-template <typename T, int PARTS>
+// The table of long bf16 rows: place 6144 for zero, those above it for the positive numbers from 2^-32 to 2^16, those
+// below for the negative ones; what is beyond -2^16 shares the first, as its weight is 0.
+constexpr int TINY = (127 - 32) << 7, HALF = 48 << 7, PLACES = 2 * HALF + 1;  // TINY: the bits of 2^-32
+constexpr int MINE = HALF * 2 / THREADS;                                      // places of a thread, and place 0
+struct Table {
+  unsigned long long weight[PLACES + 1];
+  union {
+    unsigned count[PLACES];
+    unsigned long long sums[(MAX_PARTS + 1) / 2 * WAVES];
+  };
+};
+__device__ __forceinline__ int place_of(unsigned bits) {  // of bf16 bits
+  const int d = min(max((int)(bits & 0x7fff), TINY - 1), TINY - 1 + HALF) - (TINY - 1);
+  return HALF + (bits & 0x8000 ? -d : d);
+}
+__device__ __forceinline__ float number_at(int place) {
+  const int d = place - HALF, b = d ? TINY - 1 + abs(d) : 0;
+  return __builtin_bit_cast(float, (unsigned)(b | (d < 0 ? 0x8000 : 0)) << 16);
+}
+
+struct Settings {
+  double top_p, u;
+  int64_t top_k;
+};
+
+// A row whose logits the table holds: nothing between 0 and 2^-32, the largest below 2^16, no weight at -2^16.
+__device__ __forceinline__ int from_table(const Sampler<bf16>& me, Table& t, const Weights& w, const Settings& set) {
+  const int tid = me.tid, lane = me.lane, wave = me.wave;
+  const bool cut = (set.top_k > 0 && set.top_k < me.row.V) || set.top_p < 1;
+  // The thread's places, from the top, and place 0
+  const auto place = [&](int i) { return i < MINE ? PLACES - 1 - (tid * MINE + i) : 0; };
+  const int n = tid == THREADS - 1 ? MINE + 1 : MINE;
+  if (cut)
+    for (int i = tid; i < PLACES; i += THREADS) t.count[i] = 0;
+  for (int i = 0; i < n; ++i) {
+    const float z = number_at(place(i));
+    t.weight[place(i)] = z > me.top ? 0 : w(z);
+  }
+  __syncthreads();
+  int at = -1, take = 0;  // the last place that is kept, and how many of its tokens
+  bool some = false;      // not all
+  if (cut) {
+    me.row.each([&](int, const auto& x) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) atomicAdd(&t.count[place_of(x[i / 2] >> (i % 2 * 16))], 1u);
+    });
+    __syncthreads();
+    // The place in which the target falls, going down by f(place, its tokens)
+    const auto fall = [&](auto f, auto target_of) {
+      unsigned long long sum = 0;
+      for (int i = 0; i < n; ++i) sum += f(place(i), t.count[place(i)]);
+      const unsigned long long run = wave_running(sum);
+      if (lane == 63) me.s.wave[wave] = run;
+      __syncthreads();
+      unsigned long long past = run - sum, all = 0;
+      for (int i = 0; i < WAVES; ++i) past += i < wave ? me.s.wave[i] : 0, all += me.s.wave[i];
+      const unsigned long long target = target_of(all);
+      if (past < target && target <= past + sum)
+        for (int i = 0; i < n; ++i) {
+          const unsigned long long v = f(place(i), t.count[place(i)]);
+          if (past < target && target <= past + v) me.s.digit = place(i), me.s.before = target - past;
+          past += v;
+        }
+      __syncthreads();
+    };
+    if (set.top_k > 0 && set.top_k < me.row.V) {
+      fall([](int, unsigned c) -> unsigned long long { return c; },
+           [&](unsigned long long) { return (unsigned long long)set.top_k; });
+      at = me.s.digit, take = (int)me.s.before;
+      __syncthreads();
+    }
+    if (set.top_p < 1) {
+      const auto kept = [&](int p, unsigned c) -> unsigned { return p > at ? c : p == at ? (unsigned)take : 0; };
+      fall([&](int p, unsigned c) { return t.weight[p] * kept(p, c); },
+           [&](unsigned long long all) {
+             const double part = ceil(fmax(set.top_p, 0.0) * (double)all);
+             return min(max((unsigned long long)part, 1ull), all);
+           });
+      const unsigned long long each = t.weight[me.s.digit];
+      const int to = me.s.digit;
+      take = (int)min((me.s.before + each - 1) / each, (unsigned long long)kept(to, t.count[to])), at = to;
+      __syncthreads();
+    }
+    some = (unsigned)take < t.count[at];
+    __syncthreads();
+  }
+  // What is not kept has no weight from here on
+  for (int i = 0; i < n; ++i)
+    if (place(i) < at || w.steps(number_at(place(i))) < w.low) t.weight[place(i)] = 0;
+  const auto look = [&](unsigned bits) { return t.weight[place_of(bits)]; };
+  int last = me.row.V;  // of the tokens at the last place
+  if (some)
+    last = me.first_of(t.sums, [&](unsigned bits, int, int) -> unsigned long long { return place_of(bits) == at; },
+                       [&](unsigned long long) { return (unsigned long long)take - 1; });
+  const auto target = [&](unsigned long long all) { return min((unsigned long long)(set.u * (double)all), all - 1); };
+  if (some)
+    return me.first_of(
+        t.sums,
+        [&](unsigned bits, int j, int i) -> unsigned long long {
+          const int p = place_of(bits);
+          return p == at && me.row.index(j, i) > last ? 0 : t.weight[p];
+        },
+        target);
+  return me.first_of(t.sums, [&](unsigned bits, int, int) { return look(bits); }, target);
+}
+
+template <bool TABLE>
+union Shared {
+  Lds s;
+  __device__ Shared() {}
+};
+template <>
+union Shared<true> {
+  Lds s;
+  struct {
+    Common common;
+    Table table;
+  } t;
+  __device__ Shared() {}
+};
+
+template <typename T, bool TABLE>
 __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
-  __shared__ Lds s;
+  __shared__ Shared<TABLE> shared;
+  Lds& s = shared.s;
   const int64_t b = blockIdx.x;
   const pnfx_sampling& set = a.set;
   const double temperature = set.temperature_each ? (double)set.temperature_each[b] : set.temperature;
@@ -327,26 +459,32 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
   const double top_p = set.top_p_each ? (double)set.top_p_each[b] : set.top_p;
   const double min_p = set.min_p_each ? (double)set.min_p_each[b] : set.min_p;
   const double u = fmin(fmax((double)a.u[b], 0.0), 1.0);
-  Sampler<T, PARTS> me(static_cast<const T*>(a.z) + b * a.rs, a.V, s);
-  using R = Row<T, PARTS>;
+  Sampler<T> me(static_cast<const T*>(a.z) + b * a.rs, a.V, s);
+  using R = Row<T>;
   if (me.tid < STEPS) s.table[me.tid] = ldexp(exp2(me.tid * (1.0 / STEPS)), a.S);
-  float top = -__builtin_inff(), low = __builtin_inff();
+  float top = -__builtin_inff(), low = __builtin_inff(), tiny = __builtin_inff();
   me.row.each([&](int, const auto& w) {
 #pragma unroll
     for (int i = 0; i < R::E; ++i) {
       const float z = R::element(w, i);
       top = __builtin_elementwise_maximum(top, z);  // a NaN stays
-      low = fminf(low, fabsf(z) < __builtin_inff() ? z : low);
+      if (!TABLE) low = fminf(low, fabsf(z) < __builtin_inff() ? z : low);
+      else tiny = fminf(tiny, z != 0 ? fabsf(z) : tiny);
     }
   });
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) {
     top = __builtin_elementwise_maximum(top, __shfl_xor(top, o, 64));
     low = fminf(low, __shfl_xor(low, o, 64));
+    if (TABLE) tiny = fminf(tiny, __shfl_xor(tiny, o, 64));
   }
-  if (me.lane == 0) s.top[me.wave] = top, s.low[me.wave] = low;
+  if (me.lane == 0) s.top[me.wave] = top, s.low[me.wave] = TABLE ? tiny : low;
   __syncthreads();
-  for (int w = 0; w < WAVES; ++w) top = __builtin_elementwise_maximum(top, s.top[w]), low = fminf(low, s.low[w]);
+  for (int w = 0; w < WAVES; ++w) {
+    top = __builtin_elementwise_maximum(top, s.top[w]);
+    if (TABLE) tiny = fminf(tiny, s.low[w]);
+    else low = fminf(low, s.low[w]);
+  }
   int token = -1;
   if (top > -__builtin_inff()) {  // neither NaN nor nothing
     if (!(temperature > 0) || top_k == 1) {
@@ -357,8 +495,16 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
       w.table = s.table, w.infinite = top == __builtin_inff();
       w.c = fmin(STEPS * LOG2E / temperature, 1e300), w.top = top;
       w.low = min_p > 0 ? STEPS * log2(fmin(min_p, 1.0)) : -__builtin_inf();
-      // of an infinite maximum, the finite logits are all in the last bin
       me.top = top;
+      if constexpr (TABLE) {
+        if (tiny >= 0x1p-32f && top < 65536.0f && w.steps(-65280.0f) < -60.0 * STEPS) {
+          token = from_table(me, shared.t.table, w, Settings{top_p, u, top_k});
+          if (me.tid == 0) a.tokens[b] = token;
+          return;
+        }
+        low = top - SPAN;
+      }
+      // of an infinite maximum, the finite logits are all in the last bin
       me.scale = w.infinite ? 1.0f : (BINS - 1) / fmaxf(fminf(top - low, SPAN), 1e-30f);
       Cut cut{0, a.V};
       if (top_k > 0 && top_k < a.V)
@@ -382,12 +528,10 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
 
 template <typename T>
 void sample_any(const SampleArgs& a, int64_t B, hipStream_t st) {
-  const auto go = [&](auto kernel) { kernel<<<dim3((unsigned)B), dim3(THREADS), 0, st>>>(a); };
-  const int parts = (a.V + 2 * (16 / (int)sizeof(T)) - 2) / (16 / (int)sizeof(T) * THREADS) + 1;  // at any alignment
-  if (parts <= 2) go(sample_kernel<T, 2>);
-  else if (parts <= 5) go(sample_kernel<T, 5>);
-  else if (parts <= 9) go(sample_kernel<T, 9>);
-  else go(sample_kernel<T, 0>);
+  const dim3 grid((unsigned)B), block(THREADS);
+  // a table pays where a thread has more logits than places of it
+  if (sizeof(T) == 2 && a.V > PLACES) sample_kernel<T, sizeof(T) == 2><<<grid, block, 0, st>>>(a);
+  else sample_kernel<T, false><<<grid, block, 0, st>>>(a);
 }
 
 }  // namespace
