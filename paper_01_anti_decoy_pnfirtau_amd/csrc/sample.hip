@@ -330,12 +330,19 @@ struct Sampler {
 // The table of long bf16 rows: place 6144 for zero, those above it for the positive numbers from 2^-32 to 2^16, those
 // below for the negative ones; what is beyond -2^16 shares the first, as its weight is 0.
 constexpr int TINY = (127 - 32) << 7, HALF = 48 << 7, PLACES = 2 * HALF + 1;  // TINY: the bits of 2^-32
-constexpr int MINE = HALF * 2 / THREADS;                                      // places of a thread, and place 0
+constexpr int MINE = 2 * HALF / THREADS;  // places of a thread; place 0 is nobody's, and nothing is counted there
+constexpr int COPIES = 3;                 // of the histogram, for every third lane: neighbours meet in it often
 struct Table {
-  unsigned long long weight[PLACES + 1];
+  union {
+    unsigned long long weight[PLACES];
+    unsigned more[COPIES - 1][PLACES];
+  };
   union {
     unsigned count[PLACES];
-    unsigned long long sums[(MAX_PARTS + 1) / 2 * WAVES];
+    struct {
+      unsigned long long sums[(MAX_PARTS + 1) / 2 * WAVES];
+      int ties[(MAX_PARTS + 1) / 2 * WAVES];
+    };
   };
 };
 __device__ __forceinline__ int place_of(unsigned bits) {  // of bf16 bits
@@ -353,85 +360,198 @@ struct Settings {
 };
 
 // A row whose logits the table holds: nothing between 0 and 2^-32, the largest below 2^16, no weight at -2^16.
-__device__ __forceinline__ int from_table(const Sampler<bf16>& me, Table& t, const Weights& w, const Settings& set) {
-  const int tid = me.tid, lane = me.lane, wave = me.wave;
-  const bool cut = (set.top_k > 0 && set.top_k < me.row.V) || set.top_p < 1;
-  // The thread's places, from the top, and place 0
-  const auto place = [&](int i) { return i < MINE ? PLACES - 1 - (tid * MINE + i) : 0; };
-  const int n = tid == THREADS - 1 ? MINE + 1 : MINE;
-  if (cut)
-    for (int i = tid; i < PLACES; i += THREADS) t.count[i] = 0;
-  for (int i = 0; i < n; ++i) {
-    const float z = number_at(place(i));
-    t.weight[place(i)] = z > me.top ? 0 : w(z);
-  }
-  __syncthreads();
-  int at = -1, take = 0;  // the last place that is kept, and how many of its tokens
-  bool some = false;      // not all
-  if (cut) {
+struct FromTable {
+  const Sampler<bf16>& me;
+  Table& t;
+  const Weights& w;
+  int last, take;  // the last place that is kept, and how many of its tokens, the first ones
+
+  __device__ __forceinline__ void histogram() const {
+    const int tid = me.tid;
+    unsigned* const copy = tid % COPIES ? t.more[tid % COPIES - 1] : t.count;
+    for (int i = tid; i < PLACES; i += THREADS) {
+      t.count[i] = 0;
+#pragma unroll
+      for (int c = 0; c < COPIES - 1; ++c) t.more[c][i] = 0;
+    }
+    __syncthreads();
     me.row.each([&](int, const auto& x) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) atomicAdd(&t.count[place_of(x[i / 2] >> (i % 2 * 16))], 1u);
+      for (int i = 0; i < 8; ++i) {
+        const int p = place_of(x[i / 2] >> (i % 2 * 16));
+        if (p) atomicAdd(&copy[p], 1u);
+      }
     });
     __syncthreads();
-    // The place in which the target falls, going down by f(place, its tokens)
-    const auto fall = [&](auto f, auto target_of) {
-      unsigned long long sum = 0;
-      for (int i = 0; i < n; ++i) sum += f(place(i), t.count[place(i)]);
-      const unsigned long long run = wave_running(sum);
-      if (lane == 63) me.s.wave[wave] = run;
-      __syncthreads();
-      unsigned long long past = run - sum, all = 0;
-      for (int i = 0; i < WAVES; ++i) past += i < wave ? me.s.wave[i] : 0, all += me.s.wave[i];
-      const unsigned long long target = target_of(all);
-      if (past < target && target <= past + sum)
-        for (int i = 0; i < n; ++i) {
-          const unsigned long long v = f(place(i), t.count[place(i)]);
-          if (past < target && target <= past + v) me.s.digit = place(i), me.s.before = target - past;
-          past += v;
-        }
-      __syncthreads();
-    };
-    if (set.top_k > 0 && set.top_k < me.row.V) {
-      fall([](int, unsigned c) -> unsigned long long { return c; },
-           [&](unsigned long long) { return (unsigned long long)set.top_k; });
-      at = me.s.digit, take = (int)me.s.before;
-      __syncthreads();
+    unsigned sum[MINE];
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      const int p = 1 + i * THREADS + tid;
+      sum[i] = t.count[p];
+#pragma unroll
+      for (int c = 0; c < COPIES - 1; ++c) sum[i] += t.more[c][p];
     }
-    if (set.top_p < 1) {
-      const auto kept = [&](int p, unsigned c) -> unsigned { return p > at ? c : p == at ? (unsigned)take : 0; };
-      fall([&](int p, unsigned c) { return t.weight[p] * kept(p, c); },
-           [&](unsigned long long all) {
-             const double part = ceil(fmax(set.top_p, 0.0) * (double)all);
-             return min(max((unsigned long long)part, 1ull), all);
-           });
-      const unsigned long long each = t.weight[me.s.digit];
-      const int to = me.s.digit;
-      take = (int)min((me.s.before + each - 1) / each, (unsigned long long)kept(to, t.count[to])), at = to;
-      __syncthreads();
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) t.count[1 + i * THREADS + tid] = sum[i];
+    for (int i = 0; i < MINE; ++i) {
+      const int p = 1 + i * THREADS + tid;
+      if (sum[i]) t.weight[p] = w(number_at(p));
     }
-    some = (unsigned)take < t.count[at];
     __syncthreads();
   }
-  // What is not kept has no weight from here on
-  for (int i = 0; i < n; ++i)
-    if (place(i) < at || w.steps(number_at(place(i))) < w.low) t.weight[place(i)] = 0;
-  const auto look = [&](unsigned bits) { return t.weight[place_of(bits)]; };
-  int last = me.row.V;  // of the tokens at the last place
-  if (some)
-    last = me.first_of(t.sums, [&](unsigned bits, int, int) -> unsigned long long { return place_of(bits) == at; },
-                       [&](unsigned long long) { return (unsigned long long)take - 1; });
-  const auto target = [&](unsigned long long all) { return min((unsigned long long)(set.u * (double)all), all - 1); };
-  if (some)
-    return me.first_of(
-        t.sums,
-        [&](unsigned bits, int j, int i) -> unsigned long long {
-          const int p = place_of(bits);
-          return p == at && me.row.index(j, i) > last ? 0 : t.weight[p];
-        },
-        target);
-  return me.first_of(t.sums, [&](unsigned bits, int, int) { return look(bits); }, target);
-}
+  __device__ __forceinline__ void all_weights() const {
+    for (int p = 1 + me.tid; p < PLACES; p += THREADS) {
+      const float z = number_at(p);
+      if (z <= me.top) t.weight[p] = w(z);
+    }
+  }
+
+  // The place in which the target falls, going down by f(place, its tokens), and what of the target is left there.
+  template <typename F, typename G>
+  __device__ __forceinline__ int fall(F f, G target_of, unsigned long long* left) const {
+    Lds& s = me.s;
+    const int p0 = PLACES - 1 - me.tid * MINE;
+    unsigned long long v[MINE], sum = 0;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) v[i] = f(p0 - i, t.count[p0 - i]), sum += v[i];
+    const unsigned long long run = wave_running(sum);
+    if (me.lane == 63) s.wave[me.wave] = run;
+    if (me.tid == 0) s.digit = 0, s.before = ~0ull;  // beyond all that is counted: nothing is cut
+    __syncthreads();
+    unsigned long long past = run - sum, all = 0;
+    for (int i = 0; i < WAVES; ++i) past += i < me.wave ? s.wave[i] : 0, all += s.wave[i];
+    const unsigned long long target = target_of(all);
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      if (past < target && target <= past + v[i]) s.digit = p0 - i, s.before = target - past;
+      past += v[i];
+    }
+    __syncthreads();
+    const int digit = s.digit;
+    *left = s.before;
+    __syncthreads();
+    return digit;
+  }
+
+  // The first token at which the kept ones' running weight passes u times their whole weight.
+  __device__ __forceinline__ int token(double u, bool ties) const {
+    Lds& s = me.s;
+    const int lane = me.lane, wave = me.wave;
+    const unsigned long long tie = last > 0 ? t.weight[last] : 0;
+    __syncthreads();
+    me.row.each([&](int j, const auto& x) {
+      unsigned long long sum = 0;
+      int equal = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int p = place_of(x[i / 2] >> (i % 2 * 16));
+        if (p > last) sum += t.weight[p];
+        if (ties) equal += __popcll(__ballot(p == last));
+      }
+      sum = __any(sum != 0) ? wave_total(sum) : 0;
+      if (lane == 0) t.sums[j * WAVES + wave] = sum, t.ties[j * WAVES + wave] = equal;
+    });
+    __syncthreads();
+    const int n = me.row.parts * WAVES;
+    // `before`: the equal ones in what lies before; of a sum's own, so many as are still kept count
+    const auto whole = [&](int i, unsigned long long& before) {
+      unsigned long long sum = i < n ? t.sums[i] : 0;
+      if (ties) {
+        const int mine = i < n ? t.ties[i] : 0;
+        const unsigned long long run = wave_running((unsigned long long)mine);
+        sum += tie * (unsigned)min(mine, max(0, take - (int)(before + run) + mine));
+        before += lane_of(run, 63);
+      }
+      return sum;
+    };
+    unsigned long long all = 0, before = 0;
+    for (int i0 = 0; i0 < n; i0 += 64) all += whole(i0 + lane, before);
+    all = wave_total(all);
+    unsigned long long left = min((unsigned long long)(u * (double)all), all - 1);
+    before = 0;
+    int at = n - 1, equal = 0;
+    for (int i0 = 0; i0 < n; i0 += 64) {
+      const unsigned long long was = before, mine = whole(i0 + lane, before), run = wave_running(mine);
+      const unsigned long long hit = __ballot(run > left);
+      if (hit) {
+        const int l = __builtin_ctzll(hit);
+        at = i0 + l, left -= lane_of(run - mine, l);
+        if (ties) {
+          const unsigned long long c = lane < l ? t.ties[i0 + lane] : 0;
+          equal = (int)(was + wave_total(c));
+        }
+        break;
+      }
+      left -= lane_of(run, 63);
+    }
+    if (wave == at % WAVES) {
+      const int j = at / WAVES;
+      const auto x = me.row.read(j);
+      int p[8], mine = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = place_of(x[i / 2] >> (i % 2 * 16)), mine += p[i] == last;
+      equal += (int)wave_running((unsigned long long)mine) - mine;
+      unsigned long long v[8], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = p[i] > last ? t.weight[p[i]] : ties && p[i] == last && equal < take ? tie : 0;
+        equal += p[i] == last;
+        sum += v[i];
+      }
+      unsigned long long past = wave_running(sum) - sum;
+      int found = -1;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (past <= left && left < past + v[i]) found = me.row.index(j, i);
+        past += v[i];
+      }
+      const unsigned long long hit = __ballot(found >= 0);
+      if (hit ? lane == __builtin_ctzll(hit) : lane == 0) s.found = found;
+    }
+    __syncthreads();
+    return s.found;
+  }
+
+  __device__ __forceinline__ int run(const Settings& set) {
+    const bool by_k = set.top_k > 0 && set.top_k < me.row.V, by_p = set.top_p < 1;
+    last = 0, take = 0;
+    bool ties = false;
+    if (by_k || by_p) {
+      histogram();
+      unsigned long long left;
+      if (by_k) {
+        last = fall([](int, unsigned c) -> unsigned long long { return c; },
+                    [&](unsigned long long) { return (unsigned long long)set.top_k; }, &left);
+        take = (int)min(left, (unsigned long long)(1 << 30));
+      }
+      if (by_p) {
+        const auto kept = [&](int p, unsigned c) { return p > last ? c : p == last && by_k ? min(c, (unsigned)take) : !by_k ? c : 0; };
+        const int to = fall([&](int p, unsigned c) { return c ? t.weight[p] * kept(p, c) : 0; },
+                            [&](unsigned long long all) {
+                              const double part = ceil(fmax(set.top_p, 0.0) * (double)all);
+                              return min(max((unsigned long long)part, 1ull), all);
+                            }, &left);
+        const unsigned long long each = t.weight[to], most = kept(to, t.count[to]);
+        take = (int)min((left + each - 1) / each, most), last = to;
+      }
+      ties = last > 0 && (unsigned)take < t.count[last];
+      if (last > 0 && !ties) last -= 1;  // all of its tokens: what is above the place below it
+    } else {
+      all_weights();
+    }
+    if (w.low > -__builtin_inf()) {  // the last place that min_p drops
+      int lo = 0, hi = PLACES - 1;
+      while (hi > lo) {
+        const int mid = (lo + hi + 1) / 2;
+        if (w.steps(number_at(mid)) < w.low) lo = mid;
+        else hi = mid - 1;
+      }
+      if (lo > last || (lo == last && ties)) last = lo, ties = false;
+    }
+    return token(set.u, ties);
+  }
+};
 
 template <bool TABLE>
 union Shared {
@@ -498,7 +618,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
       me.top = top;
       if constexpr (TABLE) {
         if (tiny >= 0x1p-32f && top < 65536.0f && w.steps(-65280.0f) < -60.0 * STEPS) {
-          token = from_table(me, shared.t.table, w, Settings{top_p, u, top_k});
+          token = FromTable{me, shared.t.table, w, 0, 0}.run(Settings{top_p, u, top_k});
           if (me.tid == 0) a.tokens[b] = token;
           return;
         }
