@@ -27,7 +27,6 @@ namespace {
 
 constexpr int THREADS = 1024, WAVES = THREADS / 64;
 constexpr int DIGIT = 11, BINS = 1 << DIGIT;
-constexpr int STEPS = 256;        // of the exponential's table, an octave
 constexpr float SPAN = 64;        // of the first histogram, at most: what lies further below shares its last bin
 constexpr int MAX_PARTS = 257;    // chunks of a thread in the longest rows: 2^20 fp32, four a chunk, at any alignment
 constexpr double LOG2E = 1.4426950408889634, LN2 = 0.6931471805599453;
@@ -81,7 +80,7 @@ struct Row {
   // f(part, its chunk), parts in order
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-    constexpr int AHEAD = 4;
+    constexpr int AHEAD = 2;
     u32x4 w[AHEAD];
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
@@ -122,6 +121,7 @@ __device__ __forceinline__ unsigned long long lane_of(unsigned long long x, int 
 }
 __device__ __forceinline__ unsigned long long wave_total(unsigned long long x) { return lane_of(wave_running(x), 63); }
 
+template <int STEPS>
 struct Common {
   double table[STEPS];
   unsigned long long wave[WAVES];
@@ -129,34 +129,48 @@ struct Common {
   unsigned long long before;
   int digit, found;
 };
-struct Lds : Common {
+template <int STEPS>
+struct Lds : Common<STEPS> {
   unsigned long long sums[MAX_PARTS * WAVES];  // of each part and wave; the histogram's bins
   unsigned count[BINS];
 };
 static_assert(BINS <= MAX_PARTS * WAVES, "");
 
+// STEPS: of the table, an octave.  With 256 a cubic is 1.4e-13 off at most, relative, with 4096 a square 1.0e-13.
+template <int STEPS>
 struct Weights {
   const double* table;  // 2^S times the steps of an octave
   double c, top;        // steps of the table a unit of logit; the maximum
   double low;           // min_p's border, in steps
-  bool infinite;        // the maximum is: it alone has a weight
-  __device__ __forceinline__ double steps(float z) const {
-    if (infinite) return z == __builtin_inff() ? 0.0 : -__builtin_inf();
-    return ((double)z - top) * c;
+  float least;          // a logit of no weight in fixed point: about 2^-60 of the largest
+  bool wide;            // there is none: the maximum is infinite, or temperatures are too low for fp32's steps there
+  __device__ __forceinline__ void set(const double* t, float top_, double temperature, double min_p) {
+    table = t, top = top_;
+    c = fmin(STEPS * LOG2E / temperature, 1e300);
+    low = min_p > 0 ? STEPS * log2(fmin(min_p, 1.0)) : -__builtin_inf();
+    least = (float)fmax(top - 60.0 * STEPS / c, -3.4028234663852886e38);
+    const double to = (least - top) * c;
+    wide = !(to < -58.0 * STEPS && to > -61.0 * STEPS);
   }
-  __device__ __forceinline__ unsigned long long of_steps(double y) const {
+  __device__ __forceinline__ double steps(float z) const {
+    return wide && z == top ? 0.0 : ((double)z - top) * c;  // an infinite maximum: all others -infinity
+  }
+  __device__ __forceinline__ unsigned long long of_steps(double y) const {  // y >= -61 STEPS
     const double round = 6755399441055744.0;  // 1.5 * 2^52
     constexpr double A = LN2 / STEPS;
-    y = fmax(y, -60.0 * STEPS);  // 2^-60: 0 in fixed point
     const double t = y + round;
     const int n = (int)__builtin_bit_cast(uint64_t, t);
     const double r = y - (t - round);
-    const double p = fma(r, fma(r, fma(r, A * A * A / 6, A * A / 2), A), 1.0);
-    const uint64_t s = __builtin_bit_cast(uint64_t, table[n & (STEPS - 1)]) + ((uint64_t)(uint32_t)(n >> 8 << 20) << 32);
-    return __builtin_bit_cast(uint64_t, fma(__builtin_bit_cast(double, s), p, 4503599627370496.0)) -
-           0x4330000000000000ull;  // the bits of 2^52
+    const double p = fma(r, STEPS == 256 ? fma(r, fma(r, A * A * A / 6, A * A / 2), A) : fma(r, A * A / 2, A), 1.0);
+    constexpr int SHIFT = STEPS == 256 ? 8 : 12;
+    const uint64_t e = (uint64_t)(uint32_t)(n >> SHIFT << 20) << 32;
+    const double s = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, table[n & (STEPS - 1)]) + e);
+    return __builtin_bit_cast(uint64_t, fma(s, p, 4503599627370496.0)) - 0x4330000000000000ull;  // the bits of 2^52
   }
-  __device__ __forceinline__ unsigned long long operator()(float z) const { return of_steps(steps(z)); }
+  __device__ __forceinline__ unsigned long long operator()(float z) const {
+    if (wide) return of_steps(fmax(steps(z), -60.0 * STEPS));
+    return of_steps(((double)fmaxf(z, least) - top) * c);
+  }
 };
 
 struct Cut {  // what is kept: logits of keys above, and those equal up to an index
@@ -164,15 +178,16 @@ struct Cut {  // what is kept: logits of keys above, and those equal up to an in
   int index;
 };
 
-template <typename T>
+template <typename T, int STEPS>
 struct Sampler {
   using R = Row<T>;
+  using W = Weights<STEPS>;
   static constexpr int E = R::E;
   R row;
-  Lds& s;
+  Lds<STEPS>& s;
   int tid, lane, wave;
   float top, scale;  // the largest logit, and bins of the first histogram a unit below it
-  __device__ __forceinline__ Sampler(const T* p, int V, Lds& lds) : row(p, V), s(lds) {
+  __device__ __forceinline__ Sampler(const T* p, int V, Lds<STEPS>& lds) : row(p, V), s(lds) {
     tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   }
   __device__ __forceinline__ bool keeps(const Cut& cut, float z, int j, int i) const {
@@ -272,7 +287,7 @@ struct Sampler {
   // The threshold of the first tokens, in order, that have `target` (at least 1, at most all) in sum: of the kept
   // ones' weights, or of the kept ones themselves.
   template <bool MASS, typename G>
-  __device__ __forceinline__ Cut threshold(const Cut& kept, const Weights& weight, G target_of) const {
+  __device__ __forceinline__ Cut threshold(const Cut& kept, const W& weight, G target_of) const {
     clear();
     row.each([&](int j, const auto& w) {
 #pragma unroll
@@ -361,9 +376,9 @@ struct Settings {
 
 // A row whose logits the table holds: nothing between 0 and 2^-32, the largest below 2^16, no weight at -2^16.
 struct FromTable {
-  const Sampler<bf16>& me;
+  const Sampler<bf16, 256>& me;
   Table& t;
-  const Weights& w;
+  const Weights<256>& w;
   int last, take;  // the last place that is kept, and how many of its tokens, the first ones
 
   __device__ __forceinline__ void histogram() const {
@@ -410,7 +425,7 @@ struct FromTable {
   // The place in which the target falls, going down by f(place, its tokens), and what of the target is left there.
   template <typename F, typename G>
   __device__ __forceinline__ int fall(F f, G target_of, unsigned long long* left) const {
-    Lds& s = me.s;
+    Lds<256>& s = me.s;
     const int p0 = PLACES - 1 - me.tid * MINE;
     unsigned long long v[MINE], sum = 0;
 #pragma unroll
@@ -436,7 +451,7 @@ struct FromTable {
 
   // The first token at which the kept ones' running weight passes u times their whole weight.
   __device__ __forceinline__ int token(double u, bool ties) const {
-    Lds& s = me.s;
+    Lds<256>& s = me.s;
     const int lane = me.lane, wave = me.wave;
     const unsigned long long tie = last > 0 ? t.weight[last] : 0;
     __syncthreads();
@@ -555,14 +570,14 @@ struct FromTable {
 
 template <bool TABLE>
 union Shared {
-  Lds s;
+  Lds<4096> s;
   __device__ Shared() {}
 };
 template <>
 union Shared<true> {
-  Lds s;
+  Lds<256> s;
   struct {
-    Common common;
+    Common<256> common;
     Table table;
   } t;
   __device__ Shared() {}
@@ -571,7 +586,8 @@ union Shared<true> {
 template <typename T, bool TABLE>
 __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
   __shared__ Shared<TABLE> shared;
-  Lds& s = shared.s;
+  constexpr int STEPS = TABLE ? 256 : 4096;
+  Lds<STEPS>& s = shared.s;
   const int64_t b = blockIdx.x;
   const pnfx_sampling& set = a.set;
   const double temperature = set.temperature_each ? (double)set.temperature_each[b] : set.temperature;
@@ -579,9 +595,9 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
   const double top_p = set.top_p_each ? (double)set.top_p_each[b] : set.top_p;
   const double min_p = set.min_p_each ? (double)set.min_p_each[b] : set.min_p;
   const double u = fmin(fmax((double)a.u[b], 0.0), 1.0);
-  Sampler<T> me(static_cast<const T*>(a.z) + b * a.rs, a.V, s);
+  Sampler<T, STEPS> me(static_cast<const T*>(a.z) + b * a.rs, a.V, s);
   using R = Row<T>;
-  if (me.tid < STEPS) s.table[me.tid] = ldexp(exp2(me.tid * (1.0 / STEPS)), a.S);
+  if (me.tid < 256) s.table[STEPS / 256 * me.tid] = ldexp(exp2(me.tid * (1.0 / 256)), a.S);
   float top = -__builtin_inff(), low = __builtin_inff(), tiny = __builtin_inff();
   me.row.each([&](int, const auto& w) {
 #pragma unroll
@@ -598,6 +614,15 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
     low = fminf(low, __shfl_xor(low, o, 64));
     if (TABLE) tiny = fminf(tiny, __shfl_xor(tiny, o, 64));
   }
+  if (!TABLE) {  // the steps between
+    __syncthreads();
+    double between = 1, step = 1 + LN2 / STEPS + LN2 / STEPS * (LN2 / STEPS) / 2 + LN2 / STEPS * (LN2 / STEPS) * (LN2 / STEPS) / 6;
+    const int part = me.tid & 255, from = me.tid >> 8;
+    for (int i = 1; i < STEPS / 256; ++i) {
+      between *= step;
+      if (i % 4 == from) s.table[STEPS / 256 * part + i] = s.table[STEPS / 256 * part] * between;
+    }
+  }
   if (me.lane == 0) s.top[me.wave] = top, s.low[me.wave] = TABLE ? tiny : low;
   __syncthreads();
   for (int w = 0; w < WAVES; ++w) {
@@ -611,13 +636,11 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
       token = me.first([&](float z, int, int) -> unsigned long long { return z == top; },
                        [](unsigned long long) { return 0ull; });
     } else {
-      Weights w;
-      w.table = s.table, w.infinite = top == __builtin_inff();
-      w.c = fmin(STEPS * LOG2E / temperature, 1e300), w.top = top;
-      w.low = min_p > 0 ? STEPS * log2(fmin(min_p, 1.0)) : -__builtin_inf();
+      Weights<STEPS> w;
+      w.set(s.table, top, temperature, min_p);
       me.top = top;
       if constexpr (TABLE) {
-        if (tiny >= 0x1p-32f && top < 65536.0f && w.steps(-65280.0f) < -60.0 * STEPS) {
+        if (tiny >= 0x1p-32f && top < 65536.0f && !w.wide && w.least > -65280.0f) {
           token = FromTable{me, shared.t.table, w, 0, 0}.run(Settings{top_p, u, top_k});
           if (me.tid == 0) a.tokens[b] = token;
           return;
@@ -625,7 +648,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
         low = top - SPAN;
       }
       // of an infinite maximum, the finite logits are all in the last bin
-      me.scale = w.infinite ? 1.0f : (BINS - 1) / fmaxf(fminf(top - low, SPAN), 1e-30f);
+      me.scale = top == __builtin_inff() ? 1.0f : (BINS - 1) / fmaxf(fminf(top - low, SPAN), 1e-30f);
       Cut cut{0, a.V};
       if (top_k > 0 && top_k < a.V)
         cut = me.template threshold<false>(cut, w, [&](unsigned long long) { return (unsigned long long)top_k; });
@@ -634,13 +657,15 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
           const double part = ceil(fmax(top_p, 0.0) * (double)all);
           return min(max((unsigned long long)part, 1ull), all);
         });
-      token = me.first(
-          [&](float z, int j, int i) -> unsigned long long {
-            if (!me.keeps(cut, z, j, i)) return 0;
-            const double y = w.steps(z);
-            return y >= w.low ? w.of_steps(y) : 0;
-          },
-          [&](unsigned long long all) { return min((unsigned long long)(u * (double)all), all - 1); });
+      const auto target = [&](unsigned long long all) { return min((unsigned long long)(u * (double)all), all - 1); };
+      if (cut.key == 0 && !(min_p > 0))
+        token = me.first([&](float z, int, int) { return w(z); }, target);
+      else
+        token = me.first(
+            [&](float z, int j, int i) -> unsigned long long {
+              return me.keeps(cut, z, j, i) && w.steps(z) >= w.low ? w(z) : 0;
+            },
+            target);
     }
   }
   if (me.tid == 0) a.tokens[b] = token;
