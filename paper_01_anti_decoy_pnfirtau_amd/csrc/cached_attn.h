@@ -15,9 +15,11 @@
 // joins the pieces.  Short caches, and calls with enough units to fill the card evenly, do without: a workgroup of four
 // waves has a unit, takes its tiles in turn and adds up through LDS.
 //
-// The powers are taken of u 2^-e with one e a row: 0 or, where a row's first scores are below 2^-8, less; raised (and
-// the sums scaled, exactly) when a score passes 2^8 2^e.  Up to there the power is 2^80, which leaves room for 2^40
-// keys, and it is within fp32 down to 2^-12 2^e, 2^-120 of one at the border.  bf16 queries: the
+// The powers are taken of u 2^-e with one e a row: 0 or, where a row's first scores are below 1/4, less; raised (and the
+// sums scaled, exactly) when a score passes 2 2^e.  So weights stay below 2^10, and those down to 2^-100 of the
+// largest are within fp32; values are summed with them as they are, so that 2^117 over the number of keys is the largest
+// that cannot overflow.  With 2^8 in place of 2 it would be 2^47, and no faster.
+// bf16 queries: the
 // weights are rounded to bf16 for the product and the same rounded values are summed, as the dense kernels do.  fp32
 // queries: queries and weights as three bf16 parts each (24 bits), keys and values are exact in one.
 #pragma once
@@ -79,9 +81,9 @@ typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int TILE = 64;  // keys that a wave takes at a time
-constexpr int E_LAST = 120;  // 2^-120 u is within TOP for every fp32 u
+constexpr int E_LAST = 120;  // 2^-120 u is below 2^8 for every fp32 u
 constexpr int E_LEAST = -60, E_NONE = -100;  // of a row without scores, once it is joined
-constexpr float TOP = 256.0f, LOW = 1 / 256.0f;
+constexpr float TOP = 2.0f, LOW = 0.25f;
 
 // Keys that a row tile's last row sees, from which its tiles follow.
 template <int NT>
@@ -265,7 +267,7 @@ struct Unit {
     return eight(raw.k16[t], 0, 1.0f);
   }
 
-  // A row whose scores pass 2^8 2^e, or whose first ones are all below 2^-8: another e, the same for its four lane
+  // A row whose scores pass 2 2^e, or whose first ones are all below 1/4: another e, the same for its four lane
   // groups, from the largest.
   __device__ __forceinline__ void another_e(float (&u)[16], float before, int nt) {
     const auto of_row = [](float x) {
@@ -546,15 +548,19 @@ __global__ __launch_bounds__(64, resident(sizeof(T), DT, NT)) void piece_kernel(
   // With s tiles a piece there are at most all / s + B pieces, and half of B less as a rule.
   const int each = a.c.H * a.R;  // waves a piece
   const float slots = (float)a.slots / each, room = fmaxf(slots - 0.5f * a.c.B, 0.6f * slots);
-  const int64_t s = max((int64_t)1, uniform((int64_t)ceilf((float)all / room)));
+  int64_t s = max((int64_t)1, uniform((int64_t)ceilf((float)all / room)));
   const auto pieces_of = [&](int tiles) { return (int)((tiles + s - 1) / s); };
-  int sum = 0;  // pieces of the sequences up to the end of each lane's
-  for (int b = b0; b < b1; ++b) sum += pieces_of(tiles_of_sequence(b));
-  for (int o = 1; o < 64; o *= 2) {
-    const int x = __shfl_up(sum, o, 64);
-    if (u.lane >= o) sum += x;
+  int sum, items;  // pieces of the sequences up to the end of each lane's; waves of all of them
+  for (;; ++s) {   // (again only if fp32's rounding gave a piece more than there is room for)
+    sum = 0;
+    for (int b = b0; b < b1; ++b) sum += pieces_of(tiles_of_sequence(b));
+    for (int o = 1; o < 64; o *= 2) {
+      const int x = __shfl_up(sum, o, 64);
+      if (u.lane >= o) sum += x;
+    }
+    items = uniform(__shfl(sum, 63, 64)) * each;
+    if (items <= a.most_items) break;
   }
-  const int items = uniform(__shfl(sum, 63, 64)) * each;
   // consecutive items on one XCD (workgroups go to the eight in turn)
   const int eighth = (items + 7) / 8, item = (int)blockIdx.x % 8 * eighth + (int)blockIdx.x / 8;
   if ((int)blockIdx.x / 8 >= eighth || item >= items) return;

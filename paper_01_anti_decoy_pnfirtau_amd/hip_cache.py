@@ -156,7 +156,7 @@ class KVCache:
         it among the last 16 that were appended."""
         _no_gradient("KVCache.append", k, v)
         start, at, counts = self._span("append", start, counts, k.shape[2] if k.dim() == 4 else 0)
-        if k.is_cuda:
+        if self.k.is_cuda:
             _op("cache_append")(k, v, self.k, self.v, self.k_scale, self.v_scale, self.raw, self.table, start, at, counts,
                                 taps)
         else:
@@ -187,13 +187,14 @@ def cached_attention(q: torch.Tensor, cache: KVCache, start: int | torch.Tensor,
 
     Keys and values are what their bytes stand for, exactly; scores and sums are fp32.  bf16 queries: the weights are
     rounded to bf16 (2^-9 at most, relative) for their product with the values and normalised by the sum of the rounded
-    ones; fp32 queries: 24 bits throughout.  Bitwise repeatable for one shape of call."""
+    ones; fp32 queries: 24 bits throughout.  They are normalised last: values beyond 2^117 over the number of keys may
+    overflow.  Bitwise repeatable for one shape of call."""
     _no_gradient("cached_attention", q, score_tau)
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     has_gamma = gamma is not None and gamma > 0.0
     start, at, counts = cache._span("cached_attention", start, counts, q.shape[2] if q.dim() == 4 else 0)
-    if q.is_cuda:
+    if cache.k.is_cuda:
         return _op("cached_attn")(q, cache.k, cache.v, cache.k_scale, cache.v_scale, cache.table, start, at, counts,
                                   score_tau, float(scale), float(gamma) if has_gamma else 0.0, has_gamma,
                                   bool(causal_mask))
@@ -254,6 +255,8 @@ def _checked(cache: KVCache, what: str, x: torch.Tensor, start, counts) -> tuple
     B, H, d = cache.table.shape[0], cache.raw.shape[1], cache.raw.shape[3]
     if x.dim() != 4 or x.shape[0] != B or x.shape[3] != d or x.shape[1] % H or not x.shape[2]:
         raise ValueError(f"{what}: {tuple(x.shape)} for a cache of B={B} H={H} head size {d}")
+    if x.device != cache.k.device:
+        raise ValueError(f"{what}: a tensor on {x.device}, the cache on {cache.k.device}")
     start = torch.as_tensor(start).long().expand(B)
     n = torch.full((B,), x.shape[2]) if counts is None else counts.long().clamp(0, x.shape[2])
     if (start < 0).any() or (start + n > cache.capacity).any():
