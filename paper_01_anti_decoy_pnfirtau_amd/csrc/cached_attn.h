@@ -19,9 +19,9 @@
 // sums scaled, exactly) when a score passes 2 2^e.  So weights stay below 2^10, and those down to 2^-100 of the
 // largest are within fp32; values are summed with them as they are, so that 2^117 over the number of keys is the largest
 // that cannot overflow.  With 2^8 in place of 2 it would be 2^47, and no faster.
-// bf16 queries: the
-// weights are rounded to bf16 for the product and the same rounded values are summed, as the dense kernels do.  fp32
-// queries: queries and weights as three bf16 parts each (24 bits), keys and values are exact in one.
+//
+// bf16 queries: the weights are rounded to bf16 for the product and the same rounded values are summed, as the dense
+// kernels do.  fp32 queries: queries and weights as three bf16 parts each (24 bits), keys and values are exact in one.
 #pragma once
 
 #include "cache.h"
@@ -532,7 +532,7 @@ __global__ __launch_bounds__(256, resident(sizeof(T), DT, NT)) void unit_kernel(
 // Pieces of units, one for each wave.  A sequence's tiles are cut alike for all its heads and row tiles, into as many
 // equal pieces as give every wave that the card has room for its share; neighbouring waves then have the same tokens
 // of neighbouring heads, which lie side by side in the pages: 64 sequences of up to 8192 tokens of random length,
-// 16 heads of 64, take 106, with shares cut through the line of all units 127.
+// 16 heads of 64, take 106 us, with shares cut through the line of all units 127.
 template <typename T, int DT, int NT>
 __global__ __launch_bounds__(64, resident(sizeof(T), DT, NT)) void piece_kernel(AttnArgs a) {
   Unit<T, DT, NT, 1> u(a);

@@ -190,10 +190,12 @@ def cached_attention(q: torch.Tensor, cache: KVCache, start: int | torch.Tensor,
     ones; fp32 queries: 24 bits throughout.  They are normalised last: values beyond 2^117 over the number of keys may
     overflow.  Bitwise repeatable for one shape of call."""
     _no_gradient("cached_attention", q, score_tau)
+    if q.dim() != 4 or q.shape[3] != cache.raw.shape[3]:
+        raise ValueError(f"cached_attention: q {tuple(q.shape)}, the cache's head size is {cache.raw.shape[3]}")
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     has_gamma = gamma is not None and gamma > 0.0
-    start, at, counts = cache._span("cached_attention", start, counts, q.shape[2] if q.dim() == 4 else 0)
+    start, at, counts = cache._span("cached_attention", start, counts, q.shape[2])
     if cache.k.is_cuda:
         return _op("cached_attn")(q, cache.k, cache.v, cache.k_scale, cache.v_scale, cache.table, start, at, counts,
                                   score_tau, float(scale), float(gamma) if has_gamma else 0.0, has_gamma,
@@ -253,7 +255,7 @@ def _two_to(e: torch.Tensor) -> torch.Tensor:
 def _checked(cache: KVCache, what: str, x: torch.Tensor, start, counts) -> tuple[torch.Tensor, torch.Tensor]:
     """start and counts as int64 [B]; what the kernels leave alone raises here."""
     B, H, d = cache.table.shape[0], cache.raw.shape[1], cache.raw.shape[3]
-    if x.dim() != 4 or x.shape[0] != B or x.shape[3] != d or x.shape[1] % H or not x.shape[2]:
+    if x.dim() != 4 or x.shape[0] != B or x.shape[3] != d or x.shape[1] % H:
         raise ValueError(f"{what}: {tuple(x.shape)} for a cache of B={B} H={H} head size {d}")
     if x.device != cache.k.device:
         raise ValueError(f"{what}: a tensor on {x.device}, the cache on {cache.k.device}")
@@ -288,6 +290,8 @@ def _append(cache: KVCache, k, v, start, taps, counts) -> None:
     if k.shape != v.shape or k.dtype != cache.raw.dtype or v.dtype != k.dtype or k.shape[1] != H:
         raise ValueError(f"append: k {k.dtype} {tuple(k.shape)}, v {v.dtype} {tuple(v.shape)} to a cache of "
                          f"{cache.raw.dtype} {tuple(cache.raw.shape)}")
+    if not k.numel():
+        return
     start, n = _checked(cache, "append", k, start, counts)
     N = k.shape[2]
     x = k.double()
@@ -327,7 +331,7 @@ def _append(cache: KVCache, k, v, start, taps, counts) -> None:
 
 
 def _read(cache: KVCache, first, count: int, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
-    if count < 1 or dtype not in (torch.float32, torch.bfloat16):
+    if count < 0 or dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"read: {count} positions as {dtype}")
     B, H, _, d = cache.raw.shape
     pos = torch.as_tensor(first).long().expand(B)[:, None] + torch.arange(count)
@@ -347,12 +351,12 @@ def _read(cache: KVCache, first, count: int, dtype: torch.dtype) -> tuple[torch.
 
 
 def _attend(q, cache: KVCache, start, tau, scale, gamma, causal, counts) -> torch.Tensor:
-    B, Hq, N, d = q.shape if q.dim() == 4 else (0, 0, 0, 0)
+    B, Hq, N, d = q.shape
     start, n = _checked(cache, "cached_attention", q, start, counts)
-    H, L = cache.raw.shape[1], int((start + n).max())
     o = q.new_zeros(B, N, Hq, d).transpose(1, 2)
-    if not L:
+    if not q.numel():
         return o
+    H, L = cache.raw.shape[1], int((start + n).max())
     k, v = (t.repeat_interleave(Hq // H, 1) for t in _read(cache, 0, L, torch.float32))
     end = start[:, None] + (torch.arange(N) + 1 if causal else n[:, None])  # [B, N]
     sees = (torch.arange(L) < end.expand(B, N)[..., None]) & (torch.arange(N) < n[:, None])[..., None]

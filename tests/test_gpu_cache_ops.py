@@ -320,3 +320,24 @@ def test_sampling_of_odd_rows(dev, dtype):
     assert each.shape == (3, 4) and each.flatten().tolist() == want
     beyond = torch.tensor([-0.5, 1.0, 7.0, float("nan")] * 3)
     assert ((sample_tokens(z.to(dev), beyond.to(dev), top_k=3) >= 0).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("off", [0, 1])
+def test_sampling_of_the_longest_rows(dev, dtype, off):
+    g = torch.Generator().manual_seed(off)
+    V = 1 << 20
+    wide = (torch.randn(3, V + 8, generator=g) * 2).to(dtype)
+    z, u = wide.to(dev)[:, off:off + V], torch.rand(3, generator=g)
+    for setting in (dict(), dict(top_k=1000, top_p=0.9)):
+        want = [O.sample(F64(wide[i, off:off + V]), float(u[i]), **setting) for i in range(3)]
+        got = sample_tokens(z, u.to(dev), **setting).tolist()
+        assert all(a == b or near < V * 2.0 ** -42 for a, (b, near) in zip(got, want)), (got, want)
+    z = torch.zeros(2, V, device=dev, dtype=dtype)  # all weights the largest
+    assert sample_tokens(z, torch.tensor([0.25, 1 - 2.0 ** -24], device=dev)).tolist() == [V // 4, V - 1]
+
+
+def test_other_head_sizes_of_the_same_rows_are_refused(dev):
+    cache = random_cache(2, 2, 20, [50, 50], 16, dev, 9)
+    with pytest.raises(ValueError, match="head size"):
+        cached_attention(torch.zeros(2, 2, 1, 25, device=dev), cache, 40, tau(dev))
