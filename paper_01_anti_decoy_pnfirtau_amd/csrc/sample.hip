@@ -381,7 +381,9 @@ struct FromTable {
   const Weights<256>& w;
   int last, take;  // the last place that is kept, and how many of its tokens, the first ones
 
-  __device__ __forceinline__ void histogram() const {
+  // Counts the row's logits by places; the largest logit, or -infinity if the table does not hold the row.
+  static __device__ __forceinline__ float histogram(const Sampler<bf16, 256>& me, Table& t) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
     const int tid = me.tid;
     unsigned* const copy = tid % COPIES ? t.more[tid % COPIES - 1] : t.count;
     for (int i = tid; i < PLACES; i += THREADS) {
@@ -390,7 +392,15 @@ struct FromTable {
       for (int c = 0; c < COPIES - 1; ++c) t.more[c][i] = 0;
     }
     __syncthreads();
+    u16x2 least = 0xffff, most = 0;  // magnitudes: the least but zero, less one; the largest
     me.row.each([&](int, const auto& x) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned pair = x[i];
+        const u16x2 a = __builtin_bit_cast(u16x2, pair & 0x7fff7fffu);
+        least = __builtin_elementwise_min(least, (u16x2)(a - (unsigned short)1));
+        most = __builtin_elementwise_max(most, a);
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int p = place_of(x[i / 2] >> (i % 2 * 16));
@@ -399,19 +409,29 @@ struct FromTable {
     });
     __syncthreads();
     unsigned sum[MINE];
+    int top = 0;
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
       const int p = 1 + i * THREADS + tid;
       sum[i] = t.count[p];
 #pragma unroll
       for (int c = 0; c < COPIES - 1; ++c) sum[i] += t.more[c][p];
+      if (sum[i]) top = p;
     }
+    if (min(least.x, least.y) < TINY - 1 || max(most.x, most.y) > 0x7f80) top = PLACES;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
+    if (me.lane == 0) me.s.top[me.wave] = (float)top;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < MINE; ++i) t.count[1 + i * THREADS + tid] = sum[i];
+    for (int i = 0; i < WAVES; ++i) top = max(top, (int)me.s.top[i]);
+    return top == 0 || top >= PLACES - 1 ? -__builtin_inff() : number_at(top);
+  }
+  __device__ __forceinline__ void weights() const {  // of those that were counted
     for (int i = 0; i < MINE; ++i) {
-      const int p = 1 + i * THREADS + tid;
-      if (sum[i]) t.weight[p] = w(number_at(p));
+      const int p = 1 + i * THREADS + me.tid;
+      if (t.count[p]) t.weight[p] = w(number_at(p));
     }
     __syncthreads();
   }
@@ -533,7 +553,7 @@ struct FromTable {
     last = 0, take = 0;
     bool ties = false;
     if (by_k || by_p) {
-      histogram();
+      weights();
       unsigned long long left;
       if (by_k) {
         last = fall([](int, unsigned c) -> unsigned long long { return c; },
@@ -597,7 +617,24 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
   const double u = fmin(fmax((double)a.u[b], 0.0), 1.0);
   Sampler<T, STEPS> me(static_cast<const T*>(a.z) + b * a.rs, a.V, s);
   using R = Row<T>;
+  const bool cut_off = (top_k > 0 && top_k < a.V) || top_p < 1;
   if (me.tid < 256) s.table[STEPS / 256 * me.tid] = ldexp(exp2(me.tid * (1.0 / 256)), a.S);
+  const Settings settings{top_p, u, top_k};
+  bool counted = false;
+  if constexpr (TABLE) {
+    counted = cut_off && temperature > 0 && top_k != 1;
+    if (counted) {  // the maximum comes from the counts, with one reading of the row less
+      me.top = FromTable::histogram(me, shared.t.table);
+      Weights<STEPS> w;
+      w.set(s.table, me.top, temperature, min_p);
+      if (me.top > -__builtin_inff() && !w.wide && w.least > -65280.0f) {
+        const int token = FromTable{me, shared.t.table, w, 0, 0}.run(settings);
+        if (me.tid == 0) a.tokens[b] = token;
+        return;
+      }
+      __syncthreads();  // s.top
+    }
+  }
   float top = -__builtin_inff(), low = __builtin_inff(), tiny = __builtin_inff();
   me.row.each([&](int, const auto& w) {
 #pragma unroll
@@ -640,8 +677,8 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
       w.set(s.table, top, temperature, min_p);
       me.top = top;
       if constexpr (TABLE) {
-        if (tiny >= 0x1p-32f && top < 65536.0f && !w.wide && w.least > -65280.0f) {
-          token = FromTable{me, shared.t.table, w, 0, 0}.run(Settings{top_p, u, top_k});
+        if (!counted && tiny >= 0x1p-32f && top < 65536.0f && !w.wide && w.least > -65280.0f) {
+          token = FromTable{me, shared.t.table, w, 0, 0}.run(settings);
           if (me.tid == 0) a.tokens[b] = token;
           return;
         }
