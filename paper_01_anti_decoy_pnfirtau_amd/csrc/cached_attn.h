@@ -43,7 +43,7 @@ struct AttnArgs {
   int64_t qsb, qsh, qsn, osb, osh, osn;
   const float* tau;
   float scale, gamma;
-  int has_gamma, causal;
+  int has_gamma, causal, vec;  // vec: query rows of whole 8-byte parts, heads of whole 8 elements
   int Hq, G, R;       // query heads, those of a key head, row tiles
   int slots;          // waves that the card has room for
   // Of the pieces: how many there are, headers, [items][slot_rows][D] sums and [items][3][slot_rows]: the weights' sum,
@@ -184,26 +184,52 @@ struct Unit {
       const int r = row(nt), i = r / a.G;
       // rows without a query token see what others see: what they get is not stored
       lim[nt] = a.causal && i < n ? (int)(start + i + 1) : (int)min(start + n, (int64_t)1 << 30);
-      const T* src = static_cast<const T*>(a.q) + b * a.qsb + (h * a.G + r % a.G) * a.qsh + i * a.qsn;
+      const int there = max(min(i, n - 1), 0);
+      const T* src = static_cast<const T*>(a.q) + b * a.qsb + (h * a.G + r % a.G) * a.qsh + there * a.qsn;
 #pragma unroll
       for (int f = 0; f < FRAGS; ++f) {
-        const int col = Parts<DT>::col(f, g);
         const int width = Parts<DT>::N16 && f == FRAGS - 1 ? 4 : 8;
+        float v[8] = {};
+        query(v, src, Parts<DT>::col(f, g), width, d);
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          float v = 0;
-          if (i < n && x < width && col + x < d) v = to_f32(src[col + x]);
+        for (int x = 0; x < 8; ++x)
 #pragma unroll
           for (int t = 0; t < TERMS; ++t) {
-            q[nt][f][t][x] = (bf16)v;
-            v -= (float)(bf16)v;
+            q[nt][f][t][x] = (bf16)v[x];
+            v[x] -= (float)(bf16)v[x];
           }
-        }
       }
 #pragma unroll
       for (int j = 0; j < ND; ++j) acc[nt][j] = f32x4{0, 0, 0, 0};
       z[nt] = f32x4{0, 0, 0, 0}, m[nt] = 0, e[nt] = 0;
       rescale(nt);
+    }
+  }
+  // Elements col .. col + width - 1 of a query row of d, zeros past its end.  (Loads within the row and masks: of a choice
+  // between a load and zero the compiler makes a branch for each element, which took most of the time of calls with few
+  // tiles.)
+  __device__ __forceinline__ void query(float (&v)[8], const T* row, int col, int width, int d) const {
+    if (a.vec) {  // whole 16 bytes, and no row ends inside 8 elements
+      constexpr int EACH = 8 / sizeof(T);  // elements of 8 bytes
+      const unsigned mask = col < d ? ~0u : 0u;
+      const T* p = row + (col < d ? col : 0);
+#pragma unroll
+      for (int x = 0; x < 8; x += EACH) {
+        if (x >= width) break;
+        u32x2 w = *reinterpret_cast<const u32x2*>(p + x);
+        w &= mask;
+#pragma unroll
+        for (int y = 0; y < EACH; ++y) {
+          const unsigned u = w[sizeof(T) == 4 ? y : y / 2], bits = sizeof(T) == 4 ? u : y % 2 ? u & 0xffff0000u : u << 16;
+          v[x + y] = __builtin_bit_cast(float, bits);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < width; ++x) {
+        const unsigned bits = __builtin_bit_cast(unsigned, to_f32(row[min(col + x, d - 1)]));
+        v[x] = __builtin_bit_cast(float, col + x < d ? bits : 0u);
+      }
     }
   }
   __device__ __forceinline__ void rescale(int nt) {
@@ -226,7 +252,7 @@ struct Unit {
                  t[min((key0 + 16 * g) >> a.c.page_shift, a.c.width - 1)]};
   }
   __device__ __forceinline__ int block(int id, int key) const {
-    return (((unsigned)id < (unsigned)a.c.pages ? id : 0) * a.c.H + h) * (a.c.page >> 4) +
+    return ((((unsigned)id < (unsigned)a.c.pages ? id : 0) * a.c.H + h) << (a.c.page_shift - 4)) +
            ((key & (a.c.page - 1)) >> 4);
   }
   __device__ __forceinline__ At find(const Pages& p, int key0) const {

@@ -63,6 +63,9 @@ extern "C" int pnfx_cached_attn(const pnfx_cache* cache, const void* q, int64_t 
                "cached_attn: workspace needs %lld bytes, 16-byte aligned", (long long)p.bytes());
   a.span = Span{start, counts, (int)start_all, (int)N};
   a.q = q, a.o = o, a.qsb = qsb, a.qsh = qsh, a.qsn = qsn, a.osb = osb, a.osh = osh, a.osn = osn;
+  const int64_t parts = dtype == PNFX_F32 ? 2 : 4;  // elements of 8 bytes
+  a.vec = a.c.d % 8 == 0 && qsb % parts == 0 && qsh % parts == 0 && qsn % parts == 0 &&
+          (reinterpret_cast<uintptr_t>(q) & 7) == 0;
   a.tau = tau, a.scale = scale, a.gamma = gamma, a.has_gamma = has_gamma, a.causal = causal;
   a.Hq = (int)Hq, a.G = (int)Hq / a.c.H, a.R = p.R, a.slots = p.slots, a.slot_rows = p.slot_rows;
   a.most_items = (int)p.items, a.join_waves = p.join_waves;
