@@ -57,6 +57,7 @@ struct AttnArgs {
 // How a call is cut: row tiles of 16 NT rows, R for each sequence and key head; items: the most pieces that units are
 // cut into (0: one workgroup a unit); join_waves: that join a piece's part; bytes of workspace.
 struct AttnPlan {
+  bool shared;  // workgroups of four waves share their keys through LDS, in units of four row tiles
   int NT, R, slots, slot_rows, join_waves;
   int64_t units, items, header_bytes, acc_bytes, stat_bytes;
   int64_t bytes() const { return header_bytes + acc_bytes + stat_bytes; }
@@ -66,6 +67,8 @@ struct AttnPlan {
 constexpr int resident(int bytes, int D, int NT) {
   return D * NT <= 32 ? 4 : bytes == 2 && D * NT <= 64 ? 3 : D * NT <= 128 ? 2 : 1;
 }
+// The same of the kernel whose waves share their keys: 256 times as many workgroups.
+constexpr int RESIDENT_SHARED = 2;
 
 // The kernels, by the type of the queries and the head size in the cache.
 int attn_bf16_64(const AttnArgs& a, const AttnPlan& p, hipStream_t st);    // up to 64
@@ -315,6 +318,39 @@ struct Unit {
     rescale(nt);
   }
 
+  // u 2^-e of four of the lane's keys, from the product s.
+  template <bool EDGE>
+  __device__ __forceinline__ void scores(const f32x4& s, int nt, int t, float ks, int key0, float (&u)[16]) {
+    const float c1 = ks * unit[nt];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x = __builtin_elementwise_maximum(fmaf(s[i], c1, off[nt]), 0.0f);  // NaN stays
+      if (EDGE) x = key0 + 16 * g + 4 * t + i < lim[nt] ? x : 0.0f;
+      m[nt] = fmaxf(m[nt], x);
+      u[4 * t + i] = x;
+    }
+  }
+  // The weights of the lane's 16 keys, and their sum over all lane groups: a product with ones.
+  __device__ __forceinline__ void weights(float (&u)[16], float before, int nt, bf16x8 (&p)[2][TERMS]) {
+    const bool high = m[nt] > TOP && e[nt] < E_LAST, low = before == 0 && m[nt] > 0 && m[nt] < LOW;
+    if (__builtin_expect(__any(high || low), 0)) another_e(u, before, nt);
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      const float x2 = u[x] * u[x], x4 = x2 * x2;
+      float w = x4 * x4 * x2;
+#pragma unroll
+      for (int k = 0; k < TERMS; ++k) {
+        const bf16 r = (bf16)w;
+        p[x / 8][k][x % 8] = r;
+        w -= (float)r;
+      }
+    }
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+      for (int k = 0; k < TERMS; ++k) z[nt] = mfma16x16x32(ones, p[hf][k], z[nt]);
+  }
+
   // One tile.  Its keys' and values' registers take the next tile's as soon as they have been used (`more`), so that
   // those loads are on their way over half of the work each.
   template <bool EDGE>
@@ -337,16 +373,7 @@ struct Unit {
           for (int i = 0; i < TERMS; ++i) s[nt] = mfma16x16x32(kf, q[nt][f][i], s[nt]);
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float c1 = raw.ks * unit[nt];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float x = __builtin_elementwise_maximum(fmaf(s[nt][i], c1, off[nt]), 0.0f);  // NaN stays
-          if (EDGE) x = key0 + 16 * g + 4 * t + i < lim[nt] ? x : 0.0f;
-          m[nt] = fmaxf(m[nt], x);
-          u[nt][4 * t + i] = x;
-        }
-      }
+      for (int nt = 0; nt < NT; ++nt) scores<EDGE>(s[nt], nt, t, raw.ks, key0, u[nt]);
     }
     if (more) {
       at = find(next, key0 + STEP);
@@ -355,26 +382,7 @@ struct Unit {
     }
     bf16x8 p[NT][2][TERMS];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const bool high = m[nt] > TOP && e[nt] < E_LAST, low = before[nt] == 0 && m[nt] > 0 && m[nt] < LOW;
-      if (__builtin_expect(__any(high || low), 0)) another_e(u[nt], before[nt], nt);
-#pragma unroll
-      for (int x = 0; x < 16; ++x) {
-        const float x2 = u[nt][x] * u[nt][x], x4 = x2 * x2;
-        float w = x4 * x4 * x2;
-#pragma unroll
-        for (int k = 0; k < TERMS; ++k) {
-          const bf16 r = (bf16)w;
-          p[nt][x / 8][k][x % 8] = r;
-          w -= (float)r;
-        }
-      }
-      // the weights' sum, over all lane groups: a product with ones
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-        for (int k = 0; k < TERMS; ++k) z[nt] = mfma16x16x32(ones, p[nt][hf][k], z[nt]);
-    }
+    for (int nt = 0; nt < NT; ++nt) weights(u[nt], before[nt], nt, p[nt]);
     if (EDGE) values_edge(raw, key0);
 #pragma unroll
     for (int j = 0; j < ND; ++j)
@@ -555,41 +563,44 @@ __global__ __launch_bounds__(256, resident(sizeof(T), DT, NT)) void unit_kernel(
   if (u.wave == 0) u.store();
 }
 
-// Pieces of units, one for each wave.  A sequence's tiles are cut alike for all its heads and row tiles, into as many
-// equal pieces as give every wave that the card has room for its share; neighbouring waves then have the same tokens
+// A workgroup's piece of a unit: the sequence, which of how many pieces its tiles are cut into, which of the sequence's
+// units, and the number of the item of all items; -1: none.
+struct Piece {
+  int b, tiles, piece, n, in, item, items;
+};
+
+// Pieces of units.  A sequence's tiles are cut alike for all its units (`each` of them: heads and row tiles), into as many
+// equal pieces as give every slot of the card its share; neighbouring items then have the same tokens
 // of neighbouring heads, which lie side by side in the pages: 64 sequences of up to 8192 tokens of random length,
 // 16 heads of 64, take 106 us, with shares cut through the line of all units 127.
-template <typename T, int DT, int NT>
-__global__ __launch_bounds__(64, resident(sizeof(T), DT, NT)) void piece_kernel(AttnArgs a) {
-  Unit<T, DT, NT, 1> u(a);
+__device__ __forceinline__ Piece piece_of(const AttnArgs& a, int lane, int each, int most_items) {
   const auto tiles_of_sequence = [&](int b) {
     const int64_t start = a.span.first(b);
     const int n = a.span.count(b);
     return tiles_of(start < 0 || start + n > a.c.capacity() || n == 0 ? 0 : (int)(start + n));
   };
-  const int per = (a.c.B + 63) / 64, b0 = u.lane * per, b1 = min(b0 + per, a.c.B);
+  const int per = (a.c.B + 63) / 64, b0 = lane * per, b1 = min(b0 + per, a.c.B);
   int64_t all = 0;
   for (int b = b0; b < b1; ++b) all += tiles_of_sequence(b);
   for (int o = 1; o < 64; o *= 2) all += __shfl_xor(all, o, 64);
   // With s tiles a piece there are at most all / s + B pieces, and half of B less as a rule.
-  const int each = a.c.H * a.R;  // waves a piece
   const float slots = (float)a.slots / each, room = fmaxf(slots - 0.5f * a.c.B, 0.6f * slots);
   int64_t s = max((int64_t)1, uniform((int64_t)ceilf((float)all / room)));
   const auto pieces_of = [&](int tiles) { return (int)((tiles + s - 1) / s); };
-  int sum, items;  // pieces of the sequences up to the end of each lane's; waves of all of them
+  int sum, items;  // pieces of the sequences up to the end of each lane's; items of all of them
   for (;; ++s) {   // (again only if fp32's rounding gave a piece more than there is room for)
     sum = 0;
     for (int b = b0; b < b1; ++b) sum += pieces_of(tiles_of_sequence(b));
     for (int o = 1; o < 64; o *= 2) {
       const int x = __shfl_up(sum, o, 64);
-      if (u.lane >= o) sum += x;
+      if (lane >= o) sum += x;
     }
     items = uniform(__shfl(sum, 63, 64)) * each;
-    if (items <= a.most_items) break;
+    if (items <= most_items) break;
   }
   // consecutive items on one XCD (workgroups go to the eight in turn)
   const int eighth = (items + 7) / 8, item = (int)blockIdx.x % 8 * eighth + (int)blockIdx.x / 8;
-  if ((int)blockIdx.x / 8 >= eighth || item >= items) return;
+  if ((int)blockIdx.x / 8 >= eighth || item >= items) return Piece{0, 0, 0, 0, 0, -1, items};
   const int line = item / each, group = __builtin_ctzll(__ballot(sum > line));
   int piece = line - (group ? uniform(__shfl(sum, group - 1, 64)) : 0), b = group * per, tiles, n;
   for (;;) {
@@ -597,14 +608,203 @@ __global__ __launch_bounds__(64, resident(sizeof(T), DT, NT)) void piece_kernel(
     if (piece < n) break;
     piece -= n, ++b;
   }
-  u.begin(b, item % each / a.R, item % a.R);
-  u.run((int)((int64_t)tiles * piece / n), (int)((int64_t)tiles * (piece + 1) / n));
+  return Piece{b, tiles, piece, n, item % each, item, items};
+}
+
+// One wave a piece.
+template <typename T, int DT, int NT>
+__global__ __launch_bounds__(64, resident(sizeof(T), DT, NT)) void piece_kernel(AttnArgs a) {
+  Unit<T, DT, NT, 1> u(a);
+  const Piece p = piece_of(a, u.lane, a.c.H * a.R, a.most_items);
+  if (p.item < 0) return;
+  const int h = p.in / a.R, rt = p.in % a.R;
+  u.begin(p.b, h, rt);
+  u.run((int)((int64_t)p.tiles * p.piece / p.n), (int)((int64_t)p.tiles * (p.piece + 1) / p.n));
   u.row_peaks();
-  if (n == 1) u.store();
-  else u.keep(item);
-  if (u.lane == 0) a.headers[item] = Header{b, item % each / a.R, item % a.R, piece, n};
+  if (p.n == 1) u.store();
+  else u.keep(p.item);
+  if (u.lane == 0) a.headers[p.item] = Header{p.b, h, rt, p.piece, p.n};
   // those that no item has, for the join
-  if (u.lane == 0 && item == items - 1) *a.items = items;
+  if (u.lane == 0 && p.item == p.items - 1) *a.items = p.items;
+}
+
+// Many rows: a unit is four row tiles, a wave each, that share their keys and values.  Every wave brings a quarter of the
+// next tile to LDS as the fragments that all of them read, in the order of their lanes: the bytes are loaded and turned to
+// bf16 once for 64 NT rows, not for 16 NT.  (Fragments read four ahead of their products: no faster with heads of 64 and 128,
+// spills with 256, of which a wave's results alone are half of its registers.)
+template <typename T, int DT, int NT>
+struct Sharing : Unit<T, DT, NT, 1> {
+  using U = Unit<T, DT, NT, 1>;
+  using P = Parts<DT>;
+  using U::a, U::lane, U::wave, U::g, U::r16, U::b, U::rt, U::n, U::start, U::q, U::acc, U::m, U::lim;
+  static constexpr int FRAGS = U::FRAGS, ND = U::ND, TERMS = U::TERMS, KEYS = 4 * FRAGS;
+  struct Tile {
+    u32x4 frag[KEYS + 2 * ND][64];
+    float ks[4];  // of the blocks
+    int odd[4];   // at an edge: whether a wave's values are not all finite
+  };
+  struct Quarter {  // as Raw
+    u32x4 k64[P::N64 ? P::N64 : 1], v[(ND + 3) / 4];
+    u32x2 k32;
+    unsigned k16;
+    float ks, vs;
+  };
+  __device__ __forceinline__ Sharing(const AttnArgs& args) : U(args) {}
+
+  __device__ __forceinline__ void ask(const typename U::At& at, Quarter& w) const {
+    w.ks = at.there ? two_to((int)a.c.k_scale[at.v] - 127) : __builtin_nanf("");
+    w.vs = two_to(min((int)a.c.v_scale[at.v], 247) - 127);
+    const uint8_t* p = a.c.k + (int64_t)at.k * (BLOCK * DT) + ((r16 & 3) + 4 * wave) * DT;
+#pragma unroll
+    for (int i = 0; i < P::N64; ++i) w.k64[i] = *reinterpret_cast<const u32x4*>(p + 64 * i + 16 * g);
+    if (P::N32) w.k32 = *reinterpret_cast<const u32x2*>(p + 64 * P::N64 + 8 * g);
+    if (P::N16) w.k16 = *reinterpret_cast<const unsigned*>(p + 64 * P::N64 + 32 * P::N32 + 4 * g);
+    const uint8_t* vb = a.c.v + (int64_t)at.v * (BLOCK * DT) + r16 * 16 + 256 * wave;
+#pragma unroll
+    for (int j = 0; j < ND; j += 4)
+      if (j + 3 < ND || j + wave < ND) w.v[j / 4] = *reinterpret_cast<const u32x4*>(vb + 256 * j);
+  }
+  __device__ __forceinline__ void put(const Quarter& w, Tile& tile, bool edge) const {
+    u32x4* keys = &tile.frag[wave * FRAGS][lane];
+#pragma unroll
+    for (int f = 0; f < FRAGS; ++f) {
+      bf16x8 x;
+      if (f < 2 * P::N64) {
+        const u32x4 c = w.k64[f / 2];
+        x = f % 2 ? eight(c[2], c[3], 1.0f) : eight(c[0], c[1], 1.0f);
+      } else if (P::N32 && f == 2 * P::N64) {
+        x = eight(w.k32[0], w.k32[1], 1.0f);
+      } else {
+        x = eight(w.k16, 0, 1.0f);
+      }
+      keys[64 * f] = __builtin_bit_cast(u32x4, x);
+    }
+    u32x4* values = &tile.frag[KEYS + 2 * wave][lane];
+    unsigned any = 0;
+#pragma unroll
+    for (int j = 0; j < ND; j += 4)
+      if (j + 3 < ND || j + wave < ND) {
+        const u32x4 c = w.v[j / 4];
+        values[64 * 2 * j] = __builtin_bit_cast(u32x4, eight(c[0], c[1], w.vs));
+        values[64 * (2 * j + 1)] = __builtin_bit_cast(u32x4, eight(c[2], c[3], w.vs));
+        if (edge)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) any |= not_finite(c[i], w.vs);
+      }
+    if (wave == 0 && r16 == 0) tile.ks[g] = w.ks;
+    if (edge && (any = __any(any != 0), lane == 0)) tile.odd[wave] = any;
+  }
+
+  template <bool EDGE>
+  __device__ __forceinline__ void compute(const Tile& tile, int key0) {
+    const float ks = tile.ks[g];
+    float u[NT][16], before[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) before[nt] = m[nt];
+    f32x4 s[NT];
+    each<KEYS>(tile.frag, [&](int i, bf16x8 k) {
+      const int t = i / FRAGS, f = i % FRAGS;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if (f == 0) s[nt] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int x = 0; x < TERMS; ++x) s[nt] = mfma16x16x32(k, q[nt][f][x], s[nt]);
+        if (f == FRAGS - 1) U::template scores<EDGE>(s[nt], nt, t, ks, key0, u[nt]);
+      }
+    });
+    bf16x8 p[NT][2][TERMS];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) U::weights(u[nt], before[nt], nt, p[nt]);
+    const auto add = [&](int i, bf16x8 v) {
+      const int j = i / 2, hf = i % 2;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < TERMS; ++x) acc[nt][j] = mfma16x16x32(v, p[nt][hf][x], acc[nt][j]);
+    };
+    if (EDGE && __builtin_expect(tile.odd[0] | tile.odd[1] | tile.odd[2] | tile.odd[3], 0)) {  // as values_edge
+      typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+      each<2 * ND>(tile.frag + KEYS, [&](int i, bf16x8 v) {
+        const u16x8 bits = __builtin_bit_cast(u16x8, v);
+        const u16x8 bad = __builtin_bit_cast(u16x8, (bits & 0x7f80) == 0x7f80);
+        const bf16x8 one = __builtin_bit_cast(bf16x8, bad & 0x3f80);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          bf16x8 sees;
+#pragma unroll
+          for (int x = 0; x < 8; ++x) sees[x] = (bf16)(key0 + 16 * g + 8 * (i % 2) + x < lim[nt] ? 1.0f : 0.0f);
+          const f32x4 hit = mfma16x16x32(one, sees, f32x4{0, 0, 0, 0});
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (hit[x] > 0) acc[nt][i / 2][x] = __builtin_nanf("");
+        }
+        add(i, __builtin_bit_cast(bf16x8, bits & ~bad));
+      });
+    } else {
+      each<2 * ND>(tile.frag + KEYS, add);
+    }
+  }
+  // f of N fragments in turn.
+  template <int N, typename F>
+  __device__ __forceinline__ void each(const u32x4 (*frag)[64], F f) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f(i, __builtin_bit_cast(bf16x8, frag[i][lane]));
+  }
+
+  // The tiles [t0, t1) of the unit; all four waves come here together.
+  __device__ __forceinline__ void run(int t0, int t1, Tile (&lds)[2]) {
+    const int keys = min(seen_by<4 * NT>(a, start, n, rt / 4), t1 * TILE), mine = min(seen_by<NT>(a, start, n, rt), keys);
+    // from here on, a tile is one that some row of the unit does not see whole
+    const int whole = a.causal ? (int)min(start + rt / 4 * (64 * NT) / a.G + 1, (int64_t)(1 << 30)) : keys;
+    int key0 = t0 * TILE;
+    if (key0 >= keys) return;
+    Quarter w;
+    typename U::Pages next = U::look(key0);
+    typename U::At at = U::find(next, key0);
+    next = U::look(key0 + TILE);
+    ask(at, w), put(w, lds[0], key0 + TILE > whole);
+    at = U::find(next, key0 + TILE), next = U::look(key0 + 2 * TILE);  // beside the keys: some page of the sequence
+    if (key0 + TILE < keys) ask(at, w);
+    __syncthreads();
+    for (int i = 0; key0 < keys; key0 += TILE, i ^= 1) {
+      if (key0 < mine) {
+        if (key0 + TILE > whole) compute<true>(lds[i], key0);
+        else compute<false>(lds[i], key0);
+      }
+      if (key0 + TILE < keys) {
+        put(w, lds[i ^ 1], key0 + 2 * TILE > whole);
+        at = U::find(next, key0 + 2 * TILE), next = U::look(key0 + 3 * TILE);
+        if (key0 + 2 * TILE < keys) ask(at, w);
+      }
+      __syncthreads();
+    }
+  }
+};
+
+template <typename T, int DT, int NT>
+__global__ __launch_bounds__(256, RESIDENT_SHARED) void shared_kernel(AttnArgs a) {
+  using S = Sharing<T, DT, NT>;
+  __shared__ typename S::Tile lds[2];
+  S u(a);
+  const int R = a.R / 4;
+  if (!a.most_items) {  // a workgroup a unit, the longest first
+    const int w = (int)place(blockIdx.x, gridDim.x), bh = w / R;
+    u.begin(bh / a.c.H, bh % a.c.H, 4 * (R - 1 - w % R) + u.wave);
+    u.run(0, 1 << 24, lds);
+    u.row_peaks();
+    u.store();
+    return;
+  }
+  const Piece p = piece_of(a, u.lane, a.c.H * R, a.most_items / 4);
+  if (p.item < 0) return;
+  const int h = p.in / R, rt = 4 * (p.in % R) + u.wave;
+  u.begin(p.b, h, rt);
+  u.run((int)((int64_t)p.tiles * p.piece / p.n), (int)((int64_t)p.tiles * (p.piece + 1) / p.n), lds);
+  u.row_peaks();
+  if (p.n == 1) u.store();
+  else u.keep(4 * p.item + u.wave);
+  if (u.lane == 0) a.headers[4 * p.item + u.wave] = Header{p.b, h, rt, p.piece, p.n};
+  if (threadIdx.x == 0 && p.item == p.items - 1) *a.items = 4 * p.items;
 }
 
 // Joins the units that were cut: the waves of a unit's n pieces, a.join_waves for each, have equal parts of its results.
@@ -657,6 +857,11 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
 }
 
 template <typename T, int DT, int NT>
+int join(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
+  join_kernel<T, DT, NT><<<dim3((unsigned)((p.items * p.join_waves + 3) / 4)), dim3(256), 0, st>>>(a);
+  return launch_status("cached_attn");
+}
+template <typename T, int DT, int NT>
 int run(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
   if (!p.items) {
     unit_kernel<T, DT, NT><<<dim3((unsigned)p.units), dim3(256), 0, st>>>(a);
@@ -664,11 +869,19 @@ int run(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
   }
   piece_kernel<T, DT, NT><<<dim3((unsigned)p.items), dim3(64), 0, st>>>(a);
   if (int rc = launch_status("cached_attn")) return rc;
-  join_kernel<T, DT, NT><<<dim3((unsigned)((p.items * p.join_waves + 3) / 4)), dim3(256), 0, st>>>(a);
-  return launch_status("cached_attn");
+  return join<T, DT, NT>(a, p, st);
+}
+template <typename T, int DT, int NT>
+int run_shared(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
+  shared_kernel<T, DT, NT><<<dim3((unsigned)(p.items ? p.items / 4 : p.units)), dim3(256), 0, st>>>(a);
+  const int rc = launch_status("cached_attn");
+  return rc || !p.items ? rc : join<T, DT, NT>(a, p, st);
 }
 template <typename T, int DT>
 int run_rows(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
+  if constexpr (sizeof(T) == 2 && DT <= 128) {
+    if (p.shared) return run_shared<T, DT, 2>(a, p, st);
+  }
   if constexpr (DT <= 128) {
     if (p.NT == 2) return run<T, DT, 2>(a, p, st);
   }

@@ -8,16 +8,24 @@ namespace {
 AttnPlan plan_of(int64_t B, int64_t H, int64_t G, int64_t N, int D, int64_t capacity, int bytes) {
   AttnPlan p = {};
   const int64_t rows = G * N;
-  p.NT = rows <= 16 || D > 128 ? 1 : 2;
+  const int64_t tiles = (capacity + TILE - 1) / TILE, tall = B * H * ((rows + 127) / 128);
+  // Waves that share their keys gain where turning these to bf16 is much of the work, heads of more than 64 columns, and
+  // where there are workgroups of 128 rows for the whole card.  bf16, in us, shared and not: 2 sequences of 8192 tokens, 16 heads
+  // of 128, 512 query tokens 133 and 175, with 80 query tokens 53 and 38; heads of 64 159 and 146; prompts of 512
+  // tokens and 8 heads of 128 16 of them 63 and 114, of 256 tokens behind 256 8 of them 47 and 33, 16 of them 47 and 64;
+  // prompts of 512 tokens and 4 heads of 64 64 of them 61 and 79, 16 of them 24.7 and 24.9, 8 of them 24 and 14.
+  p.shared = bytes == 2 && D <= 128 && rows >= 256 && (tiles > 8 ? D > 64 : tall >= (D > 64 ? 256 : 512));
+  p.NT = p.shared ? 2 : rows <= 16 || D > 128 ? 1 : 2;
   p.R = (int)((rows + 16 * p.NT - 1) / (16 * p.NT));
-  p.units = B * H * p.R;
-  const int64_t tiles = (capacity + TILE - 1) / TILE;
-  p.slots = 1024 * resident(bytes, D, p.NT);
+  const int waves = p.shared ? 4 : 1;  // of a unit that is cut
+  p.R = (p.R + waves - 1) / waves * waves;
+  p.units = B * H * p.R / waves;
+  p.slots = p.shared ? 256 * RESIDENT_SHARED : 1024 * resident(bytes, D, p.NT);
   p.slot_rows = (int)std::min<int64_t>(rows, 16 * p.NT);
   // One workgroup a unit where no cut can gain: short caches, whose few tiles cost less than the join's launch, and
   // enough units for the card to even out by itself.
-  if (tiles <= 8 || (p.R > 1 && p.units >= 2048) || p.units >= 4 * p.slots) return p;
-  p.items = (std::min(p.units * tiles, p.units + p.slots) + 7) / 8 * 8;
+  if (tiles <= 8 || p.units >= (p.shared ? 2 * p.slots : p.R > 1 ? 2048 : 4 * p.slots)) return p;
+  p.items = (std::min(p.units * tiles, p.units + p.slots) + 7) / 8 * 8 * waves;
   const auto round = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
   p.join_waves = std::min(8, (p.slot_rows * D + 255) / 256);  // of results, a unit has at least two pieces
   p.header_bytes = 256 + round(p.items * (int64_t)sizeof(Header));
