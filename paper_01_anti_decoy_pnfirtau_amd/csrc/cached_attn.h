@@ -810,28 +810,27 @@ __global__ __launch_bounds__(256, RESIDENT_SHARED) void shared_kernel(AttnArgs a
 // Joins the units that were cut: the waves of a unit's n pieces, a.join_waves for each, have equal parts of its results.
 // A lane has a result and, where there are fewer results than lanes, every so many of the pieces; it goes over them once,
 // the sums in units of the largest e so far, so that no load waits for another.
-template <typename T, int DT, int NT>
-__global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
+// Q: columns of a lane, 4 or, where the head size is no multiple of it, 1.
+template <typename T, int DT, int NT, int Q>
+__device__ __forceinline__ void join_part(const AttnArgs& a, const Header& u, int item, int part_wave, int lane) {
   constexpr int ROWS = 16 * NT;
-  const int wave = blockIdx.x * 4 + uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int item = wave / a.join_waves, items = *a.items;
-  const Header u = a.headers[min(item, a.most_items - 1)];
-  if (item >= items || u.n == 1) return;
-  const int each = a.c.H * a.R, me = u.piece * a.join_waves + wave % a.join_waves;
+  typedef float vec __attribute__((ext_vector_type(Q)));
+  const int each = a.c.H * a.R, me = u.piece * a.join_waves + part_wave, wide = a.c.d / Q;
   const int count = a.span.count(u.b);
   const int rows = min(ROWS, a.G * a.span.N - u.rt * ROWS), live = min(rows, a.G * count - u.rt * ROWS);
   const int64_t start = a.span.first(u.b);
   const bool refused = start < 0 || start + count > a.c.capacity();
   // no part of less than 16 results: pieces come in lines of the cache
-  const int all = rows * a.c.d, parts = min(u.n * a.join_waves, max(1, all / 16));
+  const int all = rows * wide, parts = min(u.n * a.join_waves, max(1, all * Q / 16));
   if (me >= parts) return;
   const int x0 = (int)((int64_t)all * me / parts), x1 = (int)((int64_t)all * (me + 1) / parts);
   int width = 1;  // results at a time
   while (width < 64 && width < x1 - x0) width *= 2;
   for (int base = x0; base < x1; base += width) {
-    const int x = base + (lane & (width - 1)), r = x / a.c.d, c = x % a.c.d;
-    float top = E_NONE, z = 0, m = 0, v = 0;
-    const auto add = [&](float e, float z1, float m1, float v1) {
+    const int x = base + (lane & (width - 1)), r = x / wide, c = x % wide * Q;
+    float top = E_NONE, z = 0, m = 0;
+    vec v = 0;
+    const auto add = [&](float e, float z1, float m1, const vec& v1) {
       const float to = fmaxf(top, e);
       const int was = (int)(top - to), is = (int)(e - to);
       const float fw = ldexpf(1.0f, 10 * was), fi = ldexpf(1.0f, 10 * is);
@@ -842,18 +841,37 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
       for (int i = lane / width; i < u.n; i += 64 / width) {
         const int64_t slot = item + (i - u.piece) * each;
         const float* st = a.stats + slot * 3 * a.slot_rows + r;
-        add(st[2 * a.slot_rows], st[0], st[a.slot_rows], a.acc[(slot * a.slot_rows + r) * DT + c]);
+        add(st[2 * a.slot_rows], st[0], st[a.slot_rows],
+            *reinterpret_cast<const vec*>(a.acc + (slot * a.slot_rows + r) * DT + c));
       }
     }
-    for (int o = width; o < 64; o *= 2)
-      add(__shfl_xor(top, o, 64), __shfl_xor(z, o, 64), __shfl_xor(m, o, 64), __shfl_xor(v, o, 64));
+    for (int o = width; o < 64; o *= 2) {
+      vec other;
+#pragma unroll
+      for (int y = 0; y < Q; ++y) other[y] = __shfl_xor((float)v[y], o, 64);
+      add(__shfl_xor(top, o, 64), __shfl_xor(z, o, 64), __shfl_xor(m, o, 64), other);
+    }
     if (lane < width && x < x1) {
-      v = r < live ? v * factor(a, z, m, (int)top) : 0.0f;  // no query token: zero
-      if (refused && r < live) v = __builtin_nanf("");
+      const float f = factor(a, z, m, (int)top);
       const int row = u.rt * ROWS + r;
-      static_cast<T*>(a.o)[u.b * a.osb + (u.h * a.G + row % a.G) * a.osh + row / a.G * a.osn + c] = from_f32<T>(v);
+      T* to = static_cast<T*>(a.o) + u.b * a.osb + (u.h * a.G + row % a.G) * a.osh + row / a.G * a.osn + c;
+#pragma unroll
+      for (int y = 0; y < Q; ++y) {
+        float w = r < live ? v[y] * f : 0.0f;  // no query token: zero
+        if (refused && r < live) w = __builtin_nanf("");
+        to[y] = from_f32<T>(w);
+      }
     }
   }
+}
+template <typename T, int DT, int NT>
+__global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
+  const int wave = blockIdx.x * 4 + uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int item = wave / a.join_waves, items = *a.items;
+  const Header u = a.headers[min(item, a.most_items - 1)];
+  if (item >= items || u.n == 1) return;
+  if (a.c.d % 4 == 0) join_part<T, DT, NT, 4>(a, u, item, wave % a.join_waves, lane);
+  else join_part<T, DT, NT, 1>(a, u, item, wave % a.join_waves, lane);
 }
 
 template <typename T, int DT, int NT>
