@@ -13,7 +13,8 @@
 // A unit of work is a sequence, a key head and 16 NT rows (the query heads that share the key head, times query
 // tokens).  A wave has a piece of one, which it finds by itself, as only the device knows the lengths; a second kernel
 // joins the pieces.  Short caches, and calls with enough units to fill the card evenly, do without: a workgroup of four
-// waves has a unit, takes its tiles in turn and adds up through LDS.
+// waves has a unit, takes its tiles in turn and adds up through LDS.  Of many rows, four waves have row tiles of their own
+// and share the keys and values, in LDS.
 //
 // The powers are taken of u 2^-e with one e a row: 0 or, where a row's first scores are below 1/4, less; raised (and the
 // sums scaled, exactly) when a score passes 2 2^e.  So weights stay below 2^10, and those down to 2^-100 of the
@@ -54,8 +55,8 @@ struct AttnArgs {
   int slot_rows, most_items, join_waves;
 };
 
-// How a call is cut: row tiles of 16 NT rows, R for each sequence and key head; items: the most pieces that units are
-// cut into (0: one workgroup a unit); join_waves: that join a piece's part; bytes of workspace.
+// How a call is cut: row tiles of 16 NT rows, R for each sequence and key head; items: the most pieces of row tiles that units
+// are cut into (0: one workgroup a unit); join_waves: that join a piece's part; bytes of workspace.
 struct AttnPlan {
   bool shared;  // workgroups of four waves share their keys through LDS, in units of four row tiles
   int NT, R, slots, slot_rows, join_waves;

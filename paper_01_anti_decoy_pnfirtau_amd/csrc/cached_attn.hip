@@ -10,10 +10,11 @@ AttnPlan plan_of(int64_t B, int64_t H, int64_t G, int64_t N, int D, int64_t capa
   const int64_t rows = G * N;
   const int64_t tiles = (capacity + TILE - 1) / TILE, tall = B * H * ((rows + 127) / 128);
   // Waves that share their keys gain where turning these to bf16 is much of the work, heads of more than 64 columns, and
-  // where there are workgroups of 128 rows for the whole card.  bf16, in us, shared and not: 2 sequences of 8192 tokens, 16 heads
-  // of 128, 512 query tokens 133 and 175, with 80 query tokens 53 and 38; heads of 64 159 and 146; prompts of 512
-  // tokens and 8 heads of 128 16 of them 63 and 114, of 256 tokens behind 256 8 of them 47 and 33, 16 of them 47 and 64;
-  // prompts of 512 tokens and 4 heads of 64 64 of them 61 and 79, 16 of them 24.7 and 24.9, 8 of them 24 and 14.
+  // where there are workgroups of 128 rows for the whole card.  bf16, in us, shared and not:
+  //   512 query tokens behind 7680, 2 sequences of 16 heads of 128: 131, 174; 4 of 16 heads of 64: 153, 136
+  //   80 query tokens behind 7680, one sequence of 16 heads of 128: 42, 35
+  //   prompts of 512 tokens, 16 of 8 heads of 128: 61, 113; 64 of 4 heads of 64: 61, 78; 16 of these: 24, 24; 8: 23, 14
+  //   256 query tokens behind 256, 16 sequences of 8 heads of 128: 49, 64; 8 of these: 47, 35
   p.shared = bytes == 2 && D <= 128 && rows >= 256 && (tiles > 8 ? D > 64 : tall >= (D > 64 ? 256 : 512));
   p.NT = p.shared ? 2 : rows <= 16 || D > 128 ? 1 : 2;
   p.R = (int)((rows + 16 * p.NT - 1) / (16 * p.NT));
