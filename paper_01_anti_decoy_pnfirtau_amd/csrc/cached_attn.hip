@@ -23,9 +23,11 @@ AttnPlan plan_of(int64_t B, int64_t H, int64_t G, int64_t N, int D, int64_t capa
   p.units = B * H * p.R / waves;
   p.slots = p.shared ? 256 * RESIDENT_SHARED : 1024 * resident(bytes, D, p.NT);
   p.slot_rows = (int)std::min<int64_t>(rows, 16 * p.NT);
-  // One workgroup a unit where no cut can gain: short caches, whose few tiles cost less than the join's launch, and
-  // enough units for the card to even out by itself.
-  if (tiles <= 8 || p.units >= (p.shared ? 2 * p.slots : p.R > 1 ? 2048 : 4 * p.slots)) return p;
+  // One workgroup a unit where no cut can gain: short caches, whose few tiles cost less than the join's launch (in us, whole and
+  // cut, heads of 64: one token of 4 heads behind 1023 11.3, 14.5, behind 2047 12.5, 14.8; 100 tokens of 8 heads, 4
+  // sequences behind 900 15, 20; 2048 tokens of 16 heads 127, 113), and enough units for the card to even out by itself
+  // (one token, 16 heads, behind up to 1500, 800 sequences 239, 251; 64 tokens, 200 sequences 209, 169).
+  if (tiles * std::max(D, 64) <= (p.R == 1 ? 2048 : 1024) || p.units >= (p.shared ? 2 : 4) * (int64_t)p.slots) return p;
   p.items = (std::min(p.units * tiles, p.units + p.slots) + 7) / 8 * 8 * waves;
   const auto round = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
   // a wave for half of 1024 results, as a unit has at least two pieces, four a lane: 7.9 us for 4 sequences of 512 query

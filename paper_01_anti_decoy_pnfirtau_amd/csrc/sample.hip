@@ -10,9 +10,10 @@
 // histogram of max z - z, then of the logits' bits within its bin; for top-p, the same with the weights' sums; then the
 // sum of each wave's 64 chunks, in the order of the row, the chunks in which u falls, and the token in them.
 //
-// Long bf16 rows have few different logits: with the magnitudes from 2^-32 to 2^16, 12289 of them.  Their weights are a
-// table in LDS, one exponential for each in place of one for each token, and one histogram of them settles both
-// thresholds: 256 rows of 131072 take 55 us (all weights one by one 150), one of 33278 takes 21 (37).
+// bf16 rows have few different logits: with the magnitudes from 2^-32 to 2^16, 12289 of them.  Their weights are a table
+// in LDS, one exponential for each that occurs, and one histogram of them settles both thresholds and the maximum: 256 rows of
+// 131072 take 49 us (all weights one by one 150), of 1000 with top-p 15 (31), one of 33278 takes 19 (37); 64 rows of 4000
+// by temperature alone 12 either way.
 //
 // Integers decide: weights are 64-bit fixed point, 2^S for the largest, so that sums are exact and the same in any
 // order (the histogram's atomics among them), and a token differs from the real numbers' only where u falls within about
@@ -342,7 +343,7 @@ struct Sampler {
   }
 };
 
-// The table of long bf16 rows: place 6144 for zero, those above it for the positive numbers from 2^-32 to 2^16, those
+// The table of bf16 rows: place 6144 for zero, those above it for the positive numbers from 2^-32 to 2^16, those
 // below for the negative ones; what is beyond -2^16 shares the first, as its weight is 0.
 constexpr int TINY = (127 - 32) << 7, HALF = 48 << 7, PLACES = 2 * HALF + 1;  // TINY: the bits of 2^-32
 constexpr int MINE = 2 * HALF / THREADS;  // places of a thread; place 0 is nobody's, and nothing is counted there
@@ -711,9 +712,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
 template <typename T>
 void sample_any(const SampleArgs& a, int64_t B, hipStream_t st) {
   const dim3 grid((unsigned)B), block(THREADS);
-  // a table pays where a thread has more logits than places of it
-  if (sizeof(T) == 2 && a.V > PLACES) sample_kernel<T, sizeof(T) == 2><<<grid, block, 0, st>>>(a);
-  else sample_kernel<T, false><<<grid, block, 0, st>>>(a);
+  sample_kernel<T, sizeof(T) == 2><<<grid, block, 0, st>>>(a);
 }
 
 }  // namespace

@@ -1,9 +1,10 @@
-"""Attention of many query rows over the 8-bit cache, where the waves of a workgroup share their keys."""
+"""Attention over the 8-bit cache: many query rows, where the waves of a workgroup share their keys, and long contexts in
+pieces at every head size."""
 import pytest
 import torch
 
 from paper_01_anti_decoy_pnfirtau_amd import KVCache, cached_attention
-from test_gpu_cache import BF16, check_attention, i32, random_cache
+from test_gpu_cache import BF16, F32, check_attention, i32, random_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +84,10 @@ def test_query_strides_and_a_captured_graph(dev):
         start.copy_(i32(s, dev))
         graph.replay()
         assert torch.equal(o, cached_attention(q, cache, start, tau, counts=counts))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d", [7, 16, 40, 64, 100, 128, 144, 200, 256])
+def test_long_contexts_in_pieces(dev, dtype, d):
+    check_attention(dev, 2, 2, 2, d, 1, [700, 2900], dtype=dtype, page=64)
+    check_attention(dev, 2, 1, 3, d, 9, [1500, 3], dtype=dtype, page=16, counts=[9, 4])
