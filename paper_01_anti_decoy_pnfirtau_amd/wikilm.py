@@ -300,8 +300,14 @@ class Decoder:
         self.most = 0  # tokens of the longest sequence
         self._captured = None
 
+    def _autocast(self):
+        """bf16 where ``amp``, without the cache of cast weights: inside a caller's autocast it outlives this context, and
+        a captured step would read its copies from outside the graph, after they are freed; they would not follow
+        weights that change in place either."""
+        return torch.autocast(self.rows.device.type, torch.bfloat16, enabled=self.amp, cache_enabled=False)
+
     def _run(self, idx, start, counts=None):
-        with torch.no_grad(), torch.autocast(idx.device.type, torch.bfloat16, enabled=self.amp):
+        with torch.no_grad(), self._autocast():
             return self.model.hidden_cached(idx, self.caches, start, counts)
 
     def prefill(self, prompt: torch.Tensor, lengths: torch.Tensor | None = None) -> None:
@@ -316,7 +322,7 @@ class Decoder:
         self.most = N
 
     def _step(self) -> None:
-        with torch.no_grad(), torch.autocast(self.rows.device.type, torch.bfloat16, enabled=self.amp):
+        with torch.no_grad(), self._autocast():
             token = sample_tokens(self.model.head(self.rows), self.u, **self.settings)
         h = self._run(token.clamp(min=0)[:, None], self.start)  # -1: a row of NaN has no token
         self.rows.copy_(h[:, 0])

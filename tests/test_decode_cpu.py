@@ -69,3 +69,20 @@ def test_generate_refuses():
     dec.step(torch.rand(1)), dec.step(torch.rand(1))
     with pytest.raises(ValueError):
         dec.step(torch.rand(1))
+
+
+def test_weights_that_change_inside_the_caller_s_autocast():
+    """A decoder's casts of the weights are its own: none is kept by a context around its calls."""
+    m, prompt = model(), torch.randint(0, 97, (2, 9))
+    with torch.autocast("cpu", torch.bfloat16):
+        dec = Decoder(m, 2, amp=True, temperature=0.0)
+        dec.prefill(prompt)
+        before = dec.rows.clone()
+        with torch.no_grad():
+            m.blocks[0].attn.out.weight.mul_(-3), m.embed.weight.mul_(0.5)
+        dec.prefill(prompt)
+        got = [dec.rows.clone(), dec.step(torch.rand(2)).clone(), dec.rows.clone()]
+    dec = Decoder(m, 2, amp=True, temperature=0.0)
+    dec.prefill(prompt)
+    want = [dec.rows.clone(), dec.step(torch.rand(2)).clone(), dec.rows.clone()]
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and not torch.equal(before, want[0])

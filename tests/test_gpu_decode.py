@@ -71,3 +71,34 @@ def test_decoders_side_by_side(dev):
         torch.cuda.synchronize()
         for i in range(2):
             assert torch.equal(torch.stack(got[i]), want[i])
+
+
+def test_captured_inside_the_caller_s_autocast(dev):
+    """The captured step goes on after that context has ended, its memory has other contents and weights have changed."""
+    m = model(dev)
+    g = torch.Generator().manual_seed(5)
+    prompt, u = torch.randint(0, 997, (2, 15), generator=g).to(dev), torch.rand(24, 2, generator=g).to(dev)
+
+    def run(graph, outer):
+        with torch.no_grad():
+            m.blocks[1].attn.out.weight.copy_(weight)
+        dec = Decoder(m, 2, amp=True, graph=graph, temperature=0.9)
+        with torch.autocast("cuda", torch.bfloat16, enabled=outer):
+            dec.prefill(prompt)
+            got = [dec.step(u[t]).clone() for t in range(3)]
+        for t in range(3, 24):
+            junk = [torch.full((n,), 7.0, device=dev, dtype=torch.bfloat16) for n in (997 * 128, 384 * 128, 128 * 128, 256 * 128)]
+            del junk
+            if t == 9:
+                with torch.no_grad():
+                    m.blocks[1].attn.out.weight.mul_(-2)
+            got.append(dec.step(u[t]).clone())
+        with torch.autocast("cuda", torch.bfloat16, enabled=outer):  # a replay inside another one
+            got.append(dec.step(u[0]).clone())
+        return torch.stack(got)
+
+    weight = m.blocks[1].attn.out.weight.detach().clone()
+    want = run(False, False)
+    assert torch.equal(run(False, True), want)
+    assert torch.equal(run(True, True), want)
+    assert torch.equal(run(True, False), want)
