@@ -203,9 +203,10 @@ def make_optimizer(model: nn.Module, cfg: WikiLMConfig, capturable: bool = False
 def lm_loss(model: nn.Module, x: torch.Tensor, amp: bool) -> torch.Tensor:
     """Next-token cross-entropy over the sequence, under bf16 autocast when ``amp``; without the logits
     where the model's config has ``fused_loss`` (each sequence's last row, which has no next token, is
-    ignored there)."""
+    ignored there).  The context keeps no casts of the weights: a caller's autocast around it would keep them over
+    optimizer steps, and beyond a captured step's memory."""
     vocab = model.head.weight.shape[0]
-    with torch.autocast(device_type=x.device.type, dtype=torch.bfloat16, enabled=amp):
+    with torch.autocast(device_type=x.device.type, dtype=torch.bfloat16, enabled=amp, cache_enabled=False):
         if getattr(getattr(model, "cfg", None), "fused_loss", False):
             target = torch.cat([x[:, 1:], x.new_full((x.shape[0], 1), -100)], 1)
             return linear_cross_entropy(model.hidden(x), model.head.weight, target)
