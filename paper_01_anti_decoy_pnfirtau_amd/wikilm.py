@@ -168,7 +168,7 @@ class WikiLM(nn.Module):
         """As ``hidden``, of the tokens idx [B, N] that follow those in the caches (which they join): positions start ..
         start + N - 1, of which a sequence has ``counts``.  In evaluation mode, under torch.no_grad()."""
         pos = torch.arange(idx.shape[1], device=idx.device) + (start[:, None] if torch.is_tensor(start) else start)
-        h = self.embed(idx) + self.pos(pos.clamp(max=self.cfg.max_seq - 1))
+        h = self.embed(idx) + self.pos(pos.clamp(0, self.cfg.max_seq - 1))
         for blk, cache in zip(self.blocks, caches):
             h = blk.forward_cached(h, cache, start, counts)
         return self.ln_f(h)

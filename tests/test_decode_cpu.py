@@ -86,3 +86,9 @@ def test_weights_that_change_inside_the_caller_s_autocast():
     dec.prefill(prompt)
     want = [dec.rows.clone(), dec.step(torch.rand(2)).clone(), dec.rows.clone()]
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and not torch.equal(before, want[0])
+
+
+def test_a_start_below_zero_is_refused_by_the_cache_not_met_by_the_embedding():
+    m = model()
+    with torch.no_grad(), pytest.raises(ValueError, match="append"):
+        m.hidden_cached(torch.randint(0, 97, (2, 3)), m.new_caches(2), torch.tensor([-1, 3]))

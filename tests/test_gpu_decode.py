@@ -105,3 +105,12 @@ def test_captured_inside_the_caller_s_autocast(dev):
     assert torch.equal(run(False, True), want)
     assert torch.equal(run(True, True), want)
     assert torch.equal(run(True, False), want)
+
+
+def test_sequences_that_begin_below_zero(dev):
+    """They get NaN, as from the cache, and their neighbours what they get alone."""
+    m, idx = model(dev), torch.randint(0, 997, (2, 3), generator=torch.Generator().manual_seed(6)).to(dev)
+    with torch.no_grad():
+        got = m.hidden_cached(idx, m.new_caches(2), torch.tensor([-7, 0], dtype=torch.int32, device=dev))
+        want = m.hidden_cached(idx, m.new_caches(2), 0)
+    assert got[0].isnan().all() and torch.equal(got[1], want[1])
