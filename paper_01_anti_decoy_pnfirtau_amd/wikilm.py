@@ -156,7 +156,10 @@ class WikiLM(nn.Module):
         return self.head(self.hidden(idx))
 
     def new_caches(self, batch: int, max_len: int | None = None, **kwargs) -> list[KVCache]:
-        """One empty cache for each layer, for sequences of up to max_len tokens, with one table."""
+        """One empty cache for each layer, for sequences of up to max_len tokens (at most, and by default, the model's
+        max_seq), with one table."""
+        if max_len is not None and max_len > self.cfg.max_seq:
+            raise ValueError(f"new_caches: {max_len} tokens of a model of {self.cfg.max_seq}")
         caches: list[KVCache] = []
         for blk in self.blocks:
             shared = {"table": caches[0].table, "pages": caches[0].k.shape[0]} if caches else {}
@@ -166,9 +169,15 @@ class WikiLM(nn.Module):
     def hidden_cached(self, idx: torch.Tensor, caches: list[KVCache], start: int | torch.Tensor,
                       counts: torch.Tensor | None = None) -> torch.Tensor:
         """As ``hidden``, of the tokens idx [B, N] that follow those in the caches (which they join): positions start ..
-        start + N - 1, of which a sequence has ``counts``.  In evaluation mode, under torch.no_grad()."""
+        start + N - 1, of which a sequence has ``counts``.  In evaluation mode, under torch.no_grad().  The model has no
+        positions from max_seq on: ValueError where the host knows, otherwise NaN for those tokens."""
+        most, known = self.cfg.max_seq, not torch.is_tensor(start) and counts is None
+        if known and start + idx.shape[1] > most:
+            raise ValueError(f"hidden_cached: tokens {start} .. {start + idx.shape[1] - 1} of a model of {most}")
         pos = torch.arange(idx.shape[1], device=idx.device) + (start[:, None] if torch.is_tensor(start) else start)
-        h = self.embed(idx) + self.pos(pos.clamp(0, self.cfg.max_seq - 1))
+        h = self.embed(idx) + self.pos(pos.clamp(0, most - 1))
+        if not known and any(c.capacity > most for c in caches):  # whole pages; beyond them the cache gives NaN
+            h = h.masked_fill((pos >= most)[..., None], torch.nan)
         for blk, cache in zip(self.blocks, caches):
             h = blk.forward_cached(h, cache, start, counts)
         return self.ln_f(h)

@@ -92,3 +92,17 @@ def test_a_start_below_zero_is_refused_by_the_cache_not_met_by_the_embedding():
     m = model()
     with torch.no_grad(), pytest.raises(ValueError, match="append"):
         m.hidden_cached(torch.randint(0, 97, (2, 3)), m.new_caches(2), torch.tensor([-1, 3]))
+
+
+def test_positions_that_the_model_does_not_have():
+    m, idx = model(), torch.randint(0, 97, (2, 3))  # max_seq = 40, in pages of 64
+    with pytest.raises(ValueError, match="new_caches"):
+        m.new_caches(2, 41)
+    with torch.no_grad():
+        with pytest.raises(ValueError, match="hidden_cached"):
+            m.hidden_cached(idx, m.new_caches(2), 38)
+        assert m.hidden_cached(idx, m.new_caches(2), 37).isfinite().all()
+        got = m.hidden_cached(idx, m.new_caches(2), torch.tensor([39, 4]))
+        assert got[0, 0].isfinite().all() and got[0, 1:].isnan().all() and got[1].isfinite().all()
+        got = m.hidden_cached(idx, m.new_caches(2), 38, counts=torch.tensor([2, 3]))
+        assert got[:, :2].isfinite().all() and got[1, 2].isnan().all()

@@ -114,3 +114,13 @@ def test_sequences_that_begin_below_zero(dev):
         got = m.hidden_cached(idx, m.new_caches(2), torch.tensor([-7, 0], dtype=torch.int32, device=dev))
         want = m.hidden_cached(idx, m.new_caches(2), 0)
     assert got[0].isnan().all() and torch.equal(got[1], want[1])
+
+
+def test_positions_that_the_model_does_not_have(dev):
+    m = WikiLM(97, WikiLMConfig(d_model=64, n_heads=2, n_layers=2, d_ff=96, max_seq=40, dropout=0.0)).eval().to(dev)
+    idx, start = torch.randint(0, 97, (2, 3), device=dev), torch.tensor([39, 4], dtype=torch.int32, device=dev)
+    with torch.no_grad():
+        got = m.hidden_cached(idx, m.new_caches(2), start)
+        with pytest.raises(ValueError, match="hidden_cached"):
+            m.hidden_cached(idx, m.new_caches(2), 38)
+    assert got[0, 0].isfinite().all() and got[0, 1:].isnan().all() and got[1].isfinite().all()
