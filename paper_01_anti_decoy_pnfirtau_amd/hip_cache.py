@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import functools
 import math
+import operator
 from dataclasses import dataclass
 
 import torch
@@ -47,14 +48,21 @@ def _each(what: str, x: int | torch.Tensor | None, batch: int) -> tuple[torch.Te
     if x is None:
         return None, 0
     if not torch.is_tensor(x):
+        x = operator.index(x)  # TypeError of what is no whole number
         if x < 0 or x >= 1 << 31:
             raise ValueError(f"{what} {x}")
-        return None, int(x)
+        return None, x
     if x.is_floating_point() or x.dtype == torch.bool:
         raise TypeError(f"{what} is {x.dtype}: whole numbers")
     if x.shape != (batch,):
         raise ValueError(f"{what} has shape {tuple(x.shape)} for {batch} sequences")
     return (x if x.dtype == torch.int32 else x.to(torch.int32)), 0
+
+
+def _counts(what: str, x: torch.Tensor | None, batch: int) -> torch.Tensor | None:
+    if x is not None and not torch.is_tensor(x):
+        raise TypeError(f"{what} is {type(x).__name__}: a tensor of one whole number for each sequence")
+    return _each(what, x, batch)[0]
 
 
 @dataclass
@@ -139,7 +147,7 @@ class KVCache:
     def _span(self, what: str, start, counts, N: int):
         B = self.table.shape[0]
         start, at = _each("start", start, B)
-        counts, _ = _each("counts", counts, B)
+        counts = _counts("counts", counts, B)
         if start is None and counts is None and at + N > self.capacity:
             raise ValueError(f"{what}: tokens {at} .. {at + N - 1} in pages for {self.capacity}")
         return start, at, counts
