@@ -340,7 +340,12 @@ class Decoder:
         self.token.copy_(token)
 
     def step(self, u: torch.Tensor) -> torch.Tensor:
-        """The next token of each sequence, drawn by u [B] in [0, 1); overwritten by the next call."""
+        """The next token of each sequence, drawn by u [B] in [0, 1); overwritten by the next call.  -1: a sequence whose
+        logits hold a NaN."""
+        if not self.most:
+            raise ValueError("Decoder: no prompts yet")
+        if u.shape != self.u.shape:
+            raise ValueError(f"Decoder: u has shape {tuple(u.shape)}, not {tuple(self.u.shape)}")
         if self.most + 1 > self.max_len:
             raise ValueError(f"Decoder: sequences of {self.max_len} tokens are full")
         self.most += 1

@@ -106,3 +106,15 @@ def test_positions_that_the_model_does_not_have():
         assert got[0, 0].isfinite().all() and got[0, 1:].isnan().all() and got[1].isfinite().all()
         got = m.hidden_cached(idx, m.new_caches(2), 38, counts=torch.tensor([2, 3]))
         assert got[:, :2].isfinite().all() and got[1, 2].isnan().all()
+
+
+def test_steps_without_prompts_and_with_other_numbers_of_u():
+    dec, prompt = Decoder(model(), 2, 12, temperature=0.0), torch.randint(0, 97, (2, 9))
+    with pytest.raises(ValueError, match="prompts"):
+        dec.step(torch.rand(2))
+    dec.prefill(prompt)
+    for u in (torch.rand(1), torch.rand(()), torch.rand(2, 1), torch.rand(3)):
+        with pytest.raises(ValueError, match="u has shape"):
+            dec.step(u)
+    for _ in range(3):  # a refused step takes no room
+        dec.step(torch.rand(2))
