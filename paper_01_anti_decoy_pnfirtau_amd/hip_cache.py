@@ -59,7 +59,8 @@ def _each(what: str, x: int | torch.Tensor | None, batch: int) -> tuple[torch.Te
     return (x if x.dtype == torch.int32 else x.to(torch.int32)), 0
 
 
-def _counts(what: str, x: torch.Tensor | None, batch: int) -> torch.Tensor | None:
+def whole_numbers(what: str, x: torch.Tensor | None, batch: int) -> torch.Tensor | None:
+    """x as int32 [batch]: a tensor of one whole number for each sequence, or none."""
     if x is not None and not torch.is_tensor(x):
         raise TypeError(f"{what} is {type(x).__name__}: a tensor of one whole number for each sequence")
     return _each(what, x, batch)[0]
@@ -147,7 +148,7 @@ class KVCache:
     def _span(self, what: str, start, counts, N: int):
         B = self.table.shape[0]
         start, at = _each("start", start, B)
-        counts = _counts("counts", counts, B)
+        counts = whole_numbers("counts", counts, B)
         if start is None and counts is None and at + N > self.capacity:
             raise ValueError(f"{what}: tokens {at} .. {at + N - 1} in pages for {self.capacity}")
         return start, at, counts

@@ -26,7 +26,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from .hip_cache import KVCache, sample_tokens
+from .hip_cache import KVCache, sample_tokens, whole_numbers
 from .hip_lm import gated_ffn, linear_cross_entropy
 from .pnfirtau_attention import PnFirConfig, PnFirTauFlashMHA, PnFirTauMHA, PnFirTauTritonMHA
 
@@ -321,14 +321,26 @@ class Decoder:
             return self.model.hidden_cached(idx, self.caches, start, counts)
 
     def prefill(self, prompt: torch.Tensor, lengths: torch.Tensor | None = None) -> None:
-        """Begins anew with the prompts [B, N], of which sequence b has lengths[b] tokens (at least one; null: N)."""
+        """Begins anew with the prompts [B, N], of which sequence b has lengths[b] tokens (null: N).  A length outside 1
+        .. N is a ValueError where it is on the host; nothing waits for the device to look at one there: such a sequence
+        gets -1 for every token."""
         B, N = prompt.shape
         if not 0 < N <= self.max_len or B != len(self.start):
             raise ValueError(f"Decoder: prompts {tuple(prompt.shape)} for {len(self.start)} sequences of {self.max_len}")
-        counts = torch.full_like(self.start, N) if lengths is None else lengths.to(self.start).clamp(1, N)
-        h = self._run(prompt, 0, None if lengths is None else counts)
-        self.rows.copy_(h.gather(1, (counts.long() - 1)[:, None, None].expand(B, 1, h.shape[2]))[:, 0])
-        self.start.copy_(counts)
+        counts = whole_numbers("lengths", lengths, B)
+        if counts is None:
+            h = self._run(prompt, 0)
+            self.rows.copy_(h[:, -1])
+            self.start.fill_(N)
+        else:
+            bad = (counts < 1) | (counts > N)
+            if not bad.is_cuda and bad.any():
+                raise ValueError(f"Decoder: lengths {lengths.tolist()} of prompts of {N} tokens")
+            counts, bad = counts.to(self.start.device), bad.to(self.start.device)
+            h = self._run(prompt, 0, counts)
+            last = (counts.clamp(1, N).long() - 1)[:, None, None].expand(B, 1, h.shape[2])
+            self.rows.copy_(h.gather(1, last)[:, 0].masked_fill(bad[:, None], torch.nan))
+            self.start.copy_(counts.masked_fill(bad, -(1 << 30)))  # below zero at every step: NaN from the caches
         self.most = N
 
     def _step(self) -> None:

@@ -118,3 +118,18 @@ def test_steps_without_prompts_and_with_other_numbers_of_u():
             dec.step(u)
     for _ in range(3):  # a refused step takes no room
         dec.step(torch.rand(2))
+
+
+def test_lengths_outside_their_prompts():
+    dec, prompt = Decoder(model(), 2, 12, temperature=0.0), torch.randint(0, 97, (2, 9))
+    for lengths in ([9, 0], [10, 3], [-1, 2]):
+        with pytest.raises(ValueError, match="lengths"):
+            dec.prefill(prompt, torch.tensor(lengths))
+    with pytest.raises(TypeError):
+        dec.prefill(prompt, torch.tensor([9.0, 2.5]))
+    with pytest.raises(TypeError):
+        dec.prefill(prompt, 4)
+    with pytest.raises(ValueError):
+        dec.prefill(prompt, torch.tensor([9]))
+    dec.prefill(prompt, torch.tensor([1, 9]))
+    assert dec.step(torch.rand(2)).min() >= 0

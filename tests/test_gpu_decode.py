@@ -124,3 +124,20 @@ def test_positions_that_the_model_does_not_have(dev):
         with pytest.raises(ValueError, match="hidden_cached"):
             m.hidden_cached(idx, m.new_caches(2), 38)
     assert got[0, 0].isfinite().all() and got[0, 1:].isnan().all() and got[1].isfinite().all()
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_lengths_outside_their_prompts(dev, graph):
+    """Known on the host: refused; on the device: -1 for those sequences, and their neighbours go on."""
+    m, g = model(dev), torch.Generator().manual_seed(8)
+    prompt, u = torch.randint(0, 997, (4, 9), generator=g).to(dev), torch.rand(6, 4, generator=g).to(dev)
+    dec = Decoder(m, 4, graph=graph)
+    with pytest.raises(ValueError, match="lengths"):
+        dec.prefill(prompt, torch.tensor([9, 0, 10, 2]))
+
+    def run(lengths):
+        dec.prefill(prompt, lengths)
+        return torch.stack([dec.step(x).clone() for x in u])
+
+    got, want = run(torch.tensor([9, 0, 10, 2], device=dev)), run(torch.tensor([9, 1, 9, 2]))
+    assert (got[:, 1:3] == -1).all() and torch.equal(got[:, [0, 3]], want[:, [0, 3]]) and want.min() >= 0
