@@ -1247,6 +1247,31 @@ std::tuple<Tensor, Tensor, Tensor> linear_xent_autograd(const Tensor& x, const T
   return {r[0], r[1], r[2]};
 }
 
+// The cache's operators have no derivative: a call that would record one, or that brings a tangent, is refused.
+void refuse_gradients(const char* what, std::initializer_list<const Tensor*> ts) {
+  TORCH_CHECK(!records(ts), what, " has no gradients: call it under torch.no_grad(), without tangents");
+}
+
+void cache_append_autograd(const Tensor& k, const Tensor& v, Tensor& ck, Tensor& cv, Tensor& k_scale, Tensor& v_scale,
+                           Tensor& raw, const Tensor& table, const OptTensor& start, int64_t start_all,
+                           const OptTensor& counts, const OptTensor& taps) {
+  const Tensor t = taps.value_or(Tensor());
+  refuse_gradients("cache_append", {&k, &v, &t});
+  at::AutoDispatchBelowAutograd guard;
+  static auto h = op("pnfx::cache_append").typed<decltype(cache_append_cuda)>();
+  h.call(k, v, ck, cv, k_scale, v_scale, raw, table, start, start_all, counts, taps);
+}
+
+Tensor cached_attn_autograd(const Tensor& q, const Tensor& ck, const Tensor& cv, const Tensor& k_scale,
+                            const Tensor& v_scale, const Tensor& table, const OptTensor& start, int64_t start_all,
+                            const OptTensor& counts, const Tensor& tau, double scale, double gamma, bool has_gamma,
+                            bool causal) {
+  refuse_gradients("cached_attn", {&q, &tau});
+  at::AutoDispatchBelowAutograd guard;
+  static auto h = op("pnfx::cached_attn").typed<decltype(cached_attn_cuda)>();
+  return h.call(q, ck, cv, k_scale, v_scale, table, start, start_all, counts, tau, scale, gamma, has_gamma, causal);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(pnfx, m) {
@@ -1324,4 +1349,6 @@ TORCH_LIBRARY_IMPL(pnfx, Autograd, m) {
   m.impl("gated_ffn", gated_ffn_autograd);
   m.impl("linear_xent", linear_xent_autograd);
   m.impl("flash_fwd", flash_fwd_autograd);
+  m.impl("cache_append", cache_append_autograd);
+  m.impl("cached_attn", cached_attn_autograd);
 }

@@ -10,7 +10,8 @@
 None has a counterpart in the reference, whose attention is over dense keys of equal length
 (src/triton_pnfirtau.py:814-983) and which does not generate.  GPU tensors, bf16 or fp32, run the HIP kernels
 (``pnfx::cache_append``, ``cache_read``, ``cached_attn``, ``sample_tokens``), none of which waits for the device; CPU
-tensors the same in torch operations.  None records gradients.
+tensors the same in torch operations.  None has gradients: writing and attention raise where one would be recorded, or forward
+mode's tangent carried.
 """
 from __future__ import annotations
 
@@ -21,6 +22,7 @@ from dataclasses import dataclass
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 BLOCK = 16         # tokens that share a scale
 RAW = 16           # keys before the FIR that are kept of each sequence
@@ -39,8 +41,10 @@ def _op(name: str):
 
 
 def _no_gradient(what: str, *tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no gradients: call it under torch.no_grad()")
+    """Of CPU tensors; the operators refuse for themselves."""
+    for t in tensors:
+        if t is not None and (torch.is_grad_enabled() and t.requires_grad or forward_ad.unpack_dual(t).tangent is not None):
+            raise RuntimeError(f"{what} has no gradients: call it under torch.no_grad(), without tangents")
 
 
 def _each(what: str, x: int | torch.Tensor | None, batch: int) -> tuple[torch.Tensor | None, int]:
@@ -163,12 +167,12 @@ class KVCache:
         a block, the tokens before its own are rounded again if the scale has to grow.  What is not finite becomes NaN.
         Appending again from an earlier ``start`` replaces what was there; with a FIR this needs the K - 1 keys before
         it among the last 16 that were appended."""
-        _no_gradient("KVCache.append", k, v)
         start, at, counts = self._span("append", start, counts, k.shape[2] if k.dim() == 4 else 0)
         if self.k.is_cuda:
             _op("cache_append")(k, v, self.k, self.v, self.k_scale, self.v_scale, self.raw, self.table, start, at, counts,
                                 taps)
         else:
+            _no_gradient("KVCache.append", k, v, taps)
             _append(self, k, v, at if start is None else start, taps, counts)
 
     def read(self, first: int | torch.Tensor, count: int,
@@ -198,7 +202,6 @@ def cached_attention(q: torch.Tensor, cache: KVCache, start: int | torch.Tensor,
     rounded to bf16 (2^-9 at most, relative) for their product with the values and normalised by the sum of the rounded
     ones; fp32 queries: 24 bits throughout.  They are normalised last: values beyond 2^117 over the number of keys may
     overflow.  Bitwise repeatable for one shape of call."""
-    _no_gradient("cached_attention", q, score_tau)
     if q.dim() != 4 or q.shape[3] != cache.raw.shape[3]:
         raise ValueError(f"cached_attention: q {tuple(q.shape)}, the cache's head size is {cache.raw.shape[3]}")
     if scale is None:
@@ -209,6 +212,7 @@ def cached_attention(q: torch.Tensor, cache: KVCache, start: int | torch.Tensor,
         return _op("cached_attn")(q, cache.k, cache.v, cache.k_scale, cache.v_scale, cache.table, start, at, counts,
                                   score_tau, float(scale), float(gamma) if has_gamma else 0.0, has_gamma,
                                   bool(causal_mask))
+    _no_gradient("cached_attention", q, score_tau)
     return _attend(q, cache, at if start is None else start, score_tau, scale, gamma if has_gamma else None,
                    causal_mask, counts)
 

@@ -1,6 +1,7 @@
 """Arguments of the 8-bit cache, attention over it and the draw that a call must not take for others, on CPU tensors."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from paper_01_anti_decoy_pnfirtau_amd import KVCache, cached_attention
 
@@ -36,3 +37,22 @@ def test_starts_of_a_compiled_call():
     compiled = torch.compile(step, backend="eager")
     for start in (3, 4, 5, 9):
         assert torch.equal(compiled(cache, k, start), step(same, k, start))
+
+
+def test_tangents_and_taps_that_ask_for_a_gradient():
+    cache, k = new(), torch.randn(2, 2, 3, 20)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        cache.append(k, k, 0, taps=torch.ones(3, requires_grad=True))
+    with forward_ad.dual_level(), torch.no_grad():
+        dual = forward_ad.make_dual(k, k)
+        tau, taps = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (TAU, torch.ones(3)))
+        for call in (lambda: cache.append(dual, k, 0), lambda: cache.append(k, dual, 0),
+                     lambda: cache.append(k, k, 0, taps=taps), lambda: cached_attention(dual, cache, 0, TAU),
+                     lambda: cached_attention(k, cache, 0, tau)):
+            with pytest.raises(RuntimeError, match="no gradients"):
+                call()
+        cache.append(k, k, 0)  # without one
+    with torch.no_grad(), pytest.raises(RuntimeError, match="no gradients"):
+        torch.func.jvp(lambda q: cached_attention(q, cache, 0, TAU), (k,), (k,))
+    with pytest.raises(RuntimeError, match="no gradients"):
+        torch.func.grad(lambda q: cached_attention(q, cache, 0, TAU).sum())(k)

@@ -1,0 +1,43 @@
+"""Arguments of the 8-bit cache, attention over it and the draw that a call must not take for others, on the GPU."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from paper_01_anti_decoy_pnfirtau_amd import KVCache, cached_attention
+
+pytestmark = pytest.mark.gpu
+
+
+def new(dev, B=2, H=2, d=20, max_len=64, **kw):
+    return KVCache.new(B, H, d, max_len, page=32, dtype=torch.float32, device=dev, **kw)
+
+
+def test_gradients_and_tangents_are_refused(dev):
+    """By the operators themselves, too."""
+    import paper_01_anti_decoy_pnfirtau_amd.ops  # noqa: F401
+
+    cache, k, tau0, taps0 = new(dev), torch.randn(2, 2, 3, 20, device=dev), torch.zeros(1, device=dev), torch.ones(3, device=dev)
+    c = (cache.k, cache.v, cache.k_scale, cache.v_scale)
+
+    def calls(wrap):
+        x, tau, taps = wrap(k), wrap(tau0), wrap(taps0)
+        P = torch.ops.pnfx
+        return (lambda: cache.append(x, k, 0), lambda: cache.append(k, x, 0), lambda: cache.append(k, k, 0, taps=taps),
+                lambda: cached_attention(x, cache, 0, tau0), lambda: cached_attention(k, cache, 0, tau),
+                lambda: P.cache_append(x, k, *c, cache.raw, cache.table, None, 0, None, None),
+                lambda: P.cached_attn(x, *c, cache.table, None, 0, None, tau0, 0.2, 0.5, True, True))
+
+    for call in calls(lambda t: t.clone().requires_grad_()):
+        with pytest.raises(RuntimeError, match="no gradients"):
+            call()
+    with forward_ad.dual_level(), torch.no_grad():
+        for call in calls(lambda t: forward_ad.make_dual(t, torch.ones_like(t))):
+            with pytest.raises(RuntimeError, match="no gradients"):
+                call()
+    with torch.no_grad(), pytest.raises(RuntimeError, match="no gradients"):
+        torch.func.jvp(lambda q: cached_attention(q, cache, 0, tau0), (k,), (k,))
+    assert not cache.k.any()
+    with torch.no_grad():
+        for call in calls(lambda t: t.clone().requires_grad_()):
+            call()
+    assert cache.k.any()
