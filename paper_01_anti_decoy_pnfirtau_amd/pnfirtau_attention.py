@@ -170,13 +170,15 @@ class PnFirTauMHA(nn.Module):
         """The layer's output for the next tokens x [B, N, D] of sequences whose earlier ones are in ``cache``, which
         these join: positions ``start`` .. start + N - 1, of which a sequence has ``counts`` (hip_cache.KVCache).  Keys
         and values are those of the cache, 8 bits; no dropout, no gradients.  Causal layers whose scores are the
-        kernels': p = 10 and the peak gate, where the layer's forward goes by its configuration."""
+        kernels': p = 10 and the peak gate or none, in so far as the layer's forward goes by its configuration."""
         from .hip_cache import cached_attention
 
         cfg = self.cfg
         if not cfg.causal_mask:
             raise ValueError("forward_cached: a layer that sees later tokens has no use for a cache")
-        if self._by_config and (cfg.p != 10.0 or (cfg.silence_gamma and cfg.silence_mode != "peak")):
+        gated = cfg.silence_gamma is not None and cfg.silence_gamma > 0
+        if ("p" in self._consulted and cfg.p != 10.0) or (
+                "silence_mode" in self._consulted and gated and cfg.silence_mode != "peak"):
             raise ValueError(f"forward_cached: p={cfg.p}, silence_mode={cfg.silence_mode}: p = 10 and the peak gate")
         B, N, D = x.shape
         q, k, v = (self._split_heads(t) for t in self.qkv(x).split(D, dim=-1))
@@ -185,15 +187,18 @@ class PnFirTauMHA(nn.Module):
                              counts=counts)
         return self.out(o.transpose(1, 2).reshape(B, N, D))
 
-    _by_config = True  # whether p and silence_mode are consulted
+    _consulted = ("p", "silence_mode")  # of the configuration's fields that forward may ignore, those that it does not
 
 
 class PnFirTauTritonMHA(PnFirTauMHA):
     """Materialised-score variant: HIP FIR + HIP row-fused score kernel (src/pnfirtau_attention.py:250-282).
 
     The class keeps the reference's name so that existing model code and
-    checkpoints switch over unchanged; nothing here uses Triton.
+    checkpoints switch over unchanged; nothing here uses Triton.  The row kernel's gate is the
+    peak's (cfg.silence_mode is not consulted).
     """
+
+    _consulted = ("p",)
 
     def forward(self, x: torch.Tensor, return_weights: bool = False):
         from .hip_pnfirtau import hip_causal_fir, hip_pn_fir_tau_scores, project
@@ -221,7 +226,7 @@ class PnFirTauFlashMHA(PnFirTauMHA):
     heads before the output projection is a view.
     """
 
-    _by_config = False
+    _consulted = ()
 
     def forward(self, x: torch.Tensor, return_weights: bool = False):
         if return_weights:

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from paper_01_anti_decoy_pnfirtau_amd import PnFirConfig, PnFirTauFlashMHA, PnFirTauMHA
+from paper_01_anti_decoy_pnfirtau_amd import PnFirConfig, PnFirTauFlashMHA, PnFirTauMHA, PnFirTauTritonMHA
 from paper_01_anti_decoy_pnfirtau_amd.wikilm import Decoder, WikiLM, WikiLMConfig, generate
 
 
@@ -133,3 +133,21 @@ def test_lengths_outside_their_prompts():
         dec.prefill(prompt, torch.tensor([9]))
     dec.prefill(prompt, torch.tensor([1, 9]))
     assert dec.step(torch.rand(2)).min() >= 0
+
+
+@pytest.mark.parametrize("cls", [PnFirTauMHA, PnFirTauTritonMHA, PnFirTauFlashMHA])
+def test_layers_that_have_a_cache_are_those_whose_forward_it_repeats(cls):
+    def runs(**kw):
+        layer = cls(PnFirConfig(d_model=32, n_heads=2, **kw))
+        with torch.no_grad():
+            try:
+                layer.forward_cached(torch.randn(1, 3, 32), layer.new_cache(1, 8, page=16), 0)
+            except ValueError:
+                return False
+        return True
+
+    eager, rows = cls is PnFirTauMHA, cls is not PnFirTauFlashMHA
+    assert runs(p=2.0) is not rows
+    assert runs(silence_mode="mass_pow") is not eager
+    for gamma in (None, 0.0, -1.0):  # no gate
+        assert runs(silence_mode="mass_pow", silence_gamma=gamma)
