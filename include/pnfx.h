@@ -358,15 +358,16 @@ int pnfx_xent_bwd(const float* dloss, const void* x, int64_t x_rs, const void* w
  * The 8-bit key and value cache, and attention over it.  No counterpart in the reference, which has dense attention
  * only.
  *
- * Tokens come in blocks of 16, blocks in pages of `page` tokens (a power of two from 16 on); row b of `table` names
- * the pages of sequence b in order.  D: the head size d rounded up to a multiple of 16; columns past d hold zeros.
+ * Tokens come in blocks of 16, blocks in pages of `page` tokens (a power of two from 16 to 65536); row b of `table`
+ * names the pages of sequence b in order.  D: the head size d rounded up to a multiple of 16; columns past d hold zeros.
  *   k        [pages, H, page, D]           keys behind the FIR, e4m3 bytes (no infinity; NaN: what was not finite)
  *   v        [pages, H, page / 16, D, 16]  values, the 16 tokens of a block side by side
  *   k_scale  [pages, H, page / 16]         exponent + 127 of the power of two that a block's bytes are times
  *   v_scale  likewise
  *   raw      [B, H, 16, d]                 the last 16 keys before the FIR, position p at p % 16, of the appended
  *                                          keys' type; may be null where no FIR is used
- * k and v 16-byte aligned; d <= 256; pages * H * page * D may pass 2^31.
+ * k and v 16-byte aligned; d <= 256; B < 2^24, H < 2^20; width * page <= 2^30 tokens a sequence; pages * H * page / 16
+ * < 2^31 blocks (their bytes may pass 2^32).
  *
  * Every call takes a position for each sequence, `start` int32 [B], or start_all for all where start is null, and
  * `counts` int32 [B]: how many of the call's N tokens a sequence has (null: all).

@@ -52,7 +52,7 @@ inline int cache_of(const pnfx_cache* c, const char* what, Cache* out) {
   PNFX_REQUIRE(c->d >= 1 && c->d <= PNFX_CACHE_MAX_HEAD && c->D == (c->d + 15) / 16 * 16,
                "%s: head size %lld in rows of %lld", what, (long long)c->d, (long long)c->D);
   PNFX_REQUIRE(c->page >= BLOCK && c->page <= (1 << 16) && (c->page & (c->page - 1)) == 0,
-               "%s: pages of %lld tokens (a power of two from 16 on)", what, (long long)c->page);
+               "%s: pages of %lld tokens (a power of two from 16 to 65536)", what, (long long)c->page);
   PNFX_REQUIRE(c->table_rs >= c->width, "%s: table's row stride %lld", what, (long long)c->table_rs);
   PNFX_REQUIRE(((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) == 0,
                "%s: keys and values must be 16-byte aligned", what);

@@ -29,6 +29,7 @@ RAW = 16           # keys before the FIR that are kept of each sequence
 LOWEST = -100      # smallest scale: 2^LOWEST
 MAX_HEAD_DIM = 256
 MAX_TAPS = 16
+MAX_PAGE, MAX_CAPACITY, MAX_BLOCKS = 1 << 16, 1 << 30, 1 << 31  # of a page's tokens, a sequence's, all heads' blocks
 MAX_VOCAB = 1 << 20
 
 
@@ -70,14 +71,20 @@ def whole_numbers(what: str, x: torch.Tensor | None, batch: int) -> torch.Tensor
     return _each(what, x, batch)[0]
 
 
+def _check_page(page: int) -> None:
+    if not BLOCK <= page <= MAX_PAGE or page & (page - 1):
+        raise ValueError(f"KVCache: pages of {page} tokens: a power of two from {BLOCK} to {MAX_PAGE}")
+
+
 @dataclass
 class KVCache:
     """Keys and values of one attention layer in 8 bits, of ``table.shape[0]`` sequences.
 
-    Tokens come in blocks of 16, blocks in pages of ``page`` tokens (a power of two); row b of ``table`` (int32
+    Tokens come in blocks of 16, blocks in pages of ``page`` tokens (a power of two up to 65536); row b of ``table`` (int32
     [B, n]) names the pages of sequence b in order, so that sequences of any lengths share one pool.  Layers may
     share a table, and several sequences the pages of a common beginning, as long as none of them appends there (a
-    page that two sequences append to in one call holds a mixture).  A block of one head has one scale, a power of two
+    page that two sequences append to in one call holds a mixture).  A sequence's pages hold at most 2^30 tokens; all
+    pages have less than 2^31 blocks of a head.  A block of one head has one scale, a power of two
     2^E, held as the byte E + 127; e4m3 times such a scale is exact in bf16.
 
         k        uint8 [pages, H, page, D]           D: head_dim rounded up to a multiple of 16, the rest zeros
@@ -105,8 +112,11 @@ class KVCache:
                              f"{tuple(self.table.shape)}")
         pages, H, page, D = self.k.shape
         B, d = self.table.shape[0], self.raw.shape[3]
-        if page < BLOCK or page & (page - 1):
-            raise ValueError(f"KVCache: pages of {page} tokens: a power of two from {BLOCK} on")
+        _check_page(page)
+        if not 1 <= H < 1 << 20 or B >= 1 << 24 or B and not (pages and self.table.shape[1]):
+            raise ValueError(f"KVCache: {pages} pages of {H} heads, table {tuple(self.table.shape)}")
+        if self.capacity > MAX_CAPACITY or pages * H * (page // BLOCK) >= MAX_BLOCKS:
+            raise ValueError(f"KVCache: {pages} pages of {page} tokens and {H} heads, {self.capacity} tokens a sequence")
         if not 1 <= d <= MAX_HEAD_DIM or D != -(-d // BLOCK) * BLOCK:
             raise ValueError(f"KVCache: head size {d} (at most {MAX_HEAD_DIM}) in rows of {D}")
         shapes = {"v": (pages, H, page // BLOCK, D, BLOCK), "k_scale": (pages, H, page // BLOCK),
@@ -130,6 +140,7 @@ class KVCache:
             table: torch.Tensor | None = None) -> "KVCache":
         """An empty cache for sequences of up to max_len tokens: each with pages of its own, or with a ``table`` and a
         number of ``pages`` in all.  ``dtype``: the type of the keys that will be appended."""
+        _check_page(page)
         width = -(-max_len // page)
         if table is None:
             table = torch.arange(batch * width, dtype=torch.int32, device=device).view(batch, width)

@@ -3,7 +3,8 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from paper_01_anti_decoy_pnfirtau_amd import KVCache, cached_attention
+from paper_01_anti_decoy_pnfirtau_amd import KVCache, _lib, cached_attention
+from test_cache_abi_cpu import append, cache as described
 
 TAU = torch.tensor(0.0)
 
@@ -56,3 +57,26 @@ def test_tangents_and_taps_that_ask_for_a_gradient():
         torch.func.jvp(lambda q: cached_attention(q, cache, 0, TAU), (k,), (k,))
     with pytest.raises(RuntimeError, match="no gradients"):
         torch.func.grad(lambda q: cached_attention(q, cache, 0, TAU).sum())(k)
+
+
+@pytest.mark.parametrize("B,H,max_len,kw", [
+    (1, 1, 1 << 17, dict(page=1 << 17)), (1, 1, 64, dict(page=0)), (1, 1, 64, dict(page=-16)), (1, 1, 64, dict(page=8)),
+    (1, 1, (1 << 30) + 1, {}), (2, 1 << 17, 1 << 17, {}), (1, 1 << 20, 16, {}), (1, 0, 16, {}), (1, 2, 0, {}),
+    (1, 2, 64, dict(pages=0)), (1 << 24, 1, 16, dict(pages=1))], ids=str)
+def test_caches_that_no_kernel_takes(B, H, max_len, kw):
+    """Shapes alone are looked at: nothing is allocated."""
+    with pytest.raises(ValueError, match="KVCache"):
+        KVCache.new(B, H, 16, max_len, device="meta", **kw)
+
+
+def test_the_largest_caches():
+    assert KVCache.new(1, 1, 16, 1 << 16, device="meta", page=1 << 16).capacity == 1 << 16
+    assert KVCache.new(1, 1, 16, 1 << 30, device="meta").capacity == 1 << 30
+    KVCache.new(1, 2 ** 20 - 1, 16, 16, device="meta", page=16)
+    KVCache.new(2 ** 24 - 1, 1, 16, 16, device="meta", page=16)
+    KVCache.new(0, 2, 16, 16, device="meta")
+
+
+def test_the_c_entry_names_both_ends_of_the_page_size():
+    assert append(described(page=1 << 17)) != 0
+    assert b"131072" in _lib.lib().pnfx_last_error() and b"16 to 65536" in _lib.lib().pnfx_last_error()
