@@ -45,7 +45,7 @@ struct AttnArgs {
   const float* tau;
   float scale, gamma;
   int has_gamma, causal, vec;  // vec: query rows of whole 8-byte parts, heads of whole 8 elements
-  int Hq, G, R;       // query heads, those of a key head, row tiles
+  int G, R;           // query heads of a key head, row tiles
   int slots;          // waves that the card has room for
   // Of the pieces: how many there are, headers, [items][slot_rows][D] sums and [items][3][slot_rows]: the weights' sum,
   // peak, exponent

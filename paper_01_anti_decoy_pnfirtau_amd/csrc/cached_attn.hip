@@ -80,7 +80,7 @@ extern "C" int pnfx_cached_attn(const pnfx_cache* cache, const void* q, int64_t 
   a.vec = a.c.d % 8 == 0 && qsb % parts == 0 && qsh % parts == 0 && qsn % parts == 0 &&
           (reinterpret_cast<uintptr_t>(q) & 7) == 0;
   a.tau = tau, a.scale = scale, a.gamma = gamma, a.has_gamma = has_gamma, a.causal = causal;
-  a.Hq = (int)Hq, a.G = (int)Hq / a.c.H, a.R = p.R, a.slots = p.slots, a.slot_rows = p.slot_rows;
+  a.G = (int)Hq / a.c.H, a.R = p.R, a.slots = p.slots, a.slot_rows = p.slot_rows;
   a.most_items = (int)p.items, a.join_waves = p.join_waves;
   char* ws = static_cast<char*>(workspace);
   a.items = reinterpret_cast<int*>(ws);
