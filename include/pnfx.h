@@ -366,7 +366,7 @@ int pnfx_xent_bwd(const float* dloss, const void* x, int64_t x_rs, const void* w
  *   v_scale  likewise
  *   raw      [B, H, 16, d]                 the last 16 keys before the FIR, position p at p % 16, of the appended
  *                                          keys' type; may be null where no FIR is used
- * k and v 16-byte aligned; d <= 256; B < 2^24, H < 2^20; width * page <= 2^30 tokens a sequence; pages * H * page / 16
+ * k and v 16-byte aligned; d <= 256; B < 2^24, H < 2^20, B * H < 2^31; width * page <= 2^30 tokens a sequence; pages * H * page / 16
  * < 2^31 blocks (their bytes may pass 2^32).
  *
  * Every call takes a position for each sequence, `start` int32 [B], or start_all for all where start is null, and

@@ -46,7 +46,7 @@ __device__ __forceinline__ float two_to(int e) {  // -126 <= e <= 127
 inline int cache_of(const pnfx_cache* c, const char* what, Cache* out) {
   PNFX_REQUIRE(c && c->k && c->v && c->k_scale && c->v_scale && c->table, "%s: null pointer in the cache", what);
   PNFX_REQUIRE(c->B >= 1 && c->H >= 1 && c->pages >= 1 && c->width >= 1 && c->B < (1 << 24) && c->H < (1 << 20) &&
-                   c->pages < (1ll << 31) && c->width < (1ll << 31),
+                   c->B * c->H < (1ll << 31) && c->pages < (1ll << 31) && c->width < (1ll << 31),
                "%s: cache of B=%lld H=%lld pages=%lld width=%lld", what, (long long)c->B, (long long)c->H,
                (long long)c->pages, (long long)c->width);
   PNFX_REQUIRE(c->d >= 1 && c->d <= PNFX_CACHE_MAX_HEAD && c->D == (c->d + 15) / 16 * 16,

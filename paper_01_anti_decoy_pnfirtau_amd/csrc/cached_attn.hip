@@ -67,10 +67,10 @@ extern "C" int pnfx_cached_attn(const pnfx_cache* cache, const void* q, int64_t 
   PNFX_REQUIRE(dtype == PNFX_F32 || dtype == PNFX_BF16, "cached_attn: dtype %d", dtype);
   PNFX_REQUIRE(Hq >= a.c.H && Hq % a.c.H == 0 && Hq < (1 << 20), "cached_attn: %lld query heads for %d key heads",
                (long long)Hq, a.c.H);
-  PNFX_REQUIRE(N >= 1 && Hq / a.c.H * N < (1ll << 31) - 64, "cached_attn: N=%lld", (long long)N);
+  PNFX_REQUIRE(N >= 1 && Hq / a.c.H * N < (1ll << 31) - 256, "cached_attn: N=%lld", (long long)N);
   PNFX_REQUIRE(start || (start_all >= 0 && start_all < (1ll << 31)), "cached_attn: start %lld", (long long)start_all);
   const AttnPlan p = plan_of(a.c.B, a.c.H, Hq / a.c.H, N, a.c.D, a.c.capacity(), dtype == PNFX_F32 ? 4 : 2);
-  PNFX_REQUIRE(p.units * 256 < (1ll << 32), "cached_attn: %lld row tiles in one call", (long long)p.units);
+  PNFX_REQUIRE(p.units < (1ll << 24), "cached_attn: %lld row tiles in one call", (long long)p.units);
   PNFX_REQUIRE(!p.bytes() || (workspace && workspace_bytes >= p.bytes() &&
                               (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
                "cached_attn: workspace needs %lld bytes, 16-byte aligned", (long long)p.bytes());

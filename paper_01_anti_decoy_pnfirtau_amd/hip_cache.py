@@ -113,7 +113,7 @@ class KVCache:
         pages, H, page, D = self.k.shape
         B, d = self.table.shape[0], self.raw.shape[3]
         _check_page(page)
-        if not 1 <= H < 1 << 20 or B >= 1 << 24 or B and not (pages and self.table.shape[1]):
+        if not 1 <= H < 1 << 20 or B >= 1 << 24 or B * H >= 1 << 31 or B and not (pages and self.table.shape[1]):
             raise ValueError(f"KVCache: {pages} pages of {H} heads, table {tuple(self.table.shape)}")
         if self.capacity > MAX_CAPACITY or pages * H * (page // BLOCK) >= MAX_BLOCKS:
             raise ValueError(f"KVCache: {pages} pages of {page} tokens and {H} heads, {self.capacity} tokens a sequence")

@@ -4,7 +4,7 @@ import torch
 from torch.autograd import forward_ad
 
 from paper_01_anti_decoy_pnfirtau_amd import KVCache, _lib, cached_attention
-from test_cache_abi_cpu import append, cache as described
+from test_cache_abi_cpu import append, attend, cache as described
 
 TAU = torch.tensor(0.0)
 
@@ -80,3 +80,16 @@ def test_the_largest_caches():
 def test_the_c_entry_names_both_ends_of_the_page_size():
     assert append(described(page=1 << 17)) != 0
     assert b"131072" in _lib.lib().pnfx_last_error() and b"16 to 65536" in _lib.lib().pnfx_last_error()
+
+
+def test_numbers_of_blocks_and_rows_beyond_64_bits():
+    """2 * 2^23 * 2^19 * 2^21 groups of blocks, 2^42 * 2^14 row tiles of 256 threads: both were 0 of 2^64."""
+    c = described(B=1 << 23, H=1 << 19, pages=1)
+    assert append(c, N=(1 << 26) - 30) != 0
+    assert b"B=8388608 H=524288" in _lib.lib().pnfx_last_error()
+    assert attend(c, Hq=1 << 19, N=1 << 19) != 0
+    assert b"B=8388608 H=524288" in _lib.lib().pnfx_last_error()
+    assert attend(described(B=1 << 12, H=1 << 18, pages=1), Hq=1 << 18, N=1 << 19) != 0
+    assert b"row tiles in one call" in _lib.lib().pnfx_last_error()
+    assert attend(described(), N=(1 << 31) - 200) != 0
+    assert b"N=2147483448" in _lib.lib().pnfx_last_error()
