@@ -133,10 +133,11 @@ __device__ __forceinline__ unsigned not_finite(unsigned w, float scale) {
   return ((w & 0x7f7f7f7fu) + (scale < two_to(120) ? 0x01010101u : 0x08080808u)) & 0x80808080u;
 }
 
-// What the weighted sum of a row is multiplied by: gate / (sum + 1e-12), both sums in units of 2^(10 e).
+// What the weighted sum of a row is multiplied by: gate / (sum + 1e-12), both sums in units of 2^(10 e).  A row without
+// scores has the gate 0, whatever fp32 makes of a small gamma.
 __device__ __forceinline__ float factor(const AttnArgs& a, float z, float m, int e) {
   const float peak = ldexpf(m, e);
-  const float gate = a.has_gamma ? peak / (peak + a.gamma) : 1.0f;
+  const float gate = !a.has_gamma ? 1.0f : peak > 0 ? peak / (peak + a.gamma) : 0.0f;
   return gate / (z + ldexpf(1e-12f, -10 * e));
 }
 

@@ -394,7 +394,7 @@ def _attend(q, cache: KVCache, start, tau, scale, gamma, causal, counts) -> torc
     w = ((x * x) ** 2 * x) ** 2
     w = w / (w.sum(-1, keepdim=True) + 1e-12 / peak.double() ** 10).float()
     if gamma is not None:
-        w = w * (peak / (peak + gamma))
+        w = w * torch.where(peak > 0, peak / (peak + gamma), 0.0)  # gamma may be 0 in fp32
     bad = ~v.isfinite()
     y = w @ torch.where(bad, 0.0, v)
     if bad.any():  # those count where they are seen only

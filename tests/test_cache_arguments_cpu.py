@@ -93,3 +93,11 @@ def test_numbers_of_blocks_and_rows_beyond_64_bits():
     assert b"row tiles in one call" in _lib.lib().pnfx_last_error()
     assert attend(described(), N=(1 << 31) - 200) != 0
     assert b"N=2147483448" in _lib.lib().pnfx_last_error()
+
+
+def test_rows_without_scores_under_a_gamma_that_fp32_does_not_hold():
+    cache, k = new(), torch.randn(2, 2, 5, 20)
+    cache.append(k, k, 0)
+    assert cached_attention(k, cache, 0, torch.tensor(1e9), gamma=1e-50).eq(0).all()
+    want = cached_attention(k, cache, 0, TAU, gamma=None)
+    assert torch.equal(cached_attention(k, cache, 0, TAU, gamma=1e-50), want)

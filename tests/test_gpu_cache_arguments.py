@@ -41,3 +41,15 @@ def test_gradients_and_tangents_are_refused(dev):
         for call in calls(lambda t: t.clone().requires_grad_()):
             call()
     assert cache.k.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,max_len", [(5, 64), (5, 9000), (300, 9000)])
+def test_rows_without_scores_under_a_gamma_that_fp32_does_not_hold(dev, dtype, N, max_len):
+    cache = KVCache.new(2, 2, 72, max_len, dtype=dtype, device=dev)
+    k = torch.randn(2, 2, N, 72, generator=torch.Generator().manual_seed(0)).to(dev, dtype)
+    cache.append(k, k, 0)
+    tau = lambda x: torch.tensor(x, device=dev)  # noqa: E731
+    assert cached_attention(k, cache, 0, tau(1e9), gamma=1e-50).eq(0).all()
+    want = cached_attention(k, cache, 0, tau(0.0), gamma=None)
+    assert torch.equal(cached_attention(k, cache, 0, tau(0.0), gamma=1e-50), want) and want.isfinite().all()
