@@ -48,6 +48,13 @@ def _no_gradient(what: str, *tensors: torch.Tensor | None) -> None:
             raise RuntimeError(f"{what} has no gradients: call it under torch.no_grad(), without tangents")
 
 
+def _int32(x: torch.Tensor) -> torch.Tensor:
+    """Whole numbers in 32 bits: those beyond become the first or last of them, which no sequence or row has either."""
+    if x.dtype in (torch.int32, torch.int16, torch.int8, torch.uint8):
+        return x.to(torch.int32)
+    return x.to(torch.int64).clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)
+
+
 def _each(what: str, x: int | torch.Tensor | None, batch: int) -> tuple[torch.Tensor | None, int]:
     """A whole number for each sequence: an int32 tensor [batch], or one for all."""
     if x is None:
@@ -61,7 +68,7 @@ def _each(what: str, x: int | torch.Tensor | None, batch: int) -> tuple[torch.Te
         raise TypeError(f"{what} is {x.dtype}: whole numbers")
     if x.shape != (batch,):
         raise ValueError(f"{what} has shape {tuple(x.shape)} for {batch} sequences")
-    return (x if x.dtype == torch.int32 else x.to(torch.int32)), 0
+    return _int32(x), 0
 
 
 def whole_numbers(what: str, x: torch.Tensor | None, batch: int) -> torch.Tensor | None:
@@ -260,12 +267,12 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: float | to
                 raise ValueError(f"sample_tokens: {name} has shape {tuple(x.shape)}, the rows {tuple(rows)}")
             if x.is_floating_point() == (name == "top_k"):
                 raise TypeError(f"sample_tokens: {name} is {x.dtype}")
-            each[name] = x.to(torch.int32 if name == "top_k" else torch.float32).reshape(-1)
-        elif not x >= 0:
+            each[name] = (_int32(x) if name == "top_k" else x.to(torch.float32)).reshape(-1)
+        elif not x >= 0 or (name == "top_k" and x % 1 != 0):
             raise ValueError(f"sample_tokens: {name} {x}")
         else:
             one[name] = x
-    args = (one["temperature"], int(one["top_k"]), one["top_p"], one["min_p"], each["temperature"], each["top_k"],
+    args = (one["temperature"], int(min(one["top_k"], MAX_VOCAB)), one["top_p"], one["min_p"], each["temperature"], each["top_k"],
             each["top_p"], each["min_p"])
     z, u = logits.detach().reshape(-1, V), u.detach().reshape(-1)
     return (_op("sample_tokens") if z.is_cuda else _sample)(z, u, *args).view(rows)

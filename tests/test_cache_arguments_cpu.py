@@ -3,7 +3,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from paper_01_anti_decoy_pnfirtau_amd import KVCache, _lib, cached_attention
+from paper_01_anti_decoy_pnfirtau_amd import KVCache, _lib, cached_attention, sample_tokens
 from test_cache_abi_cpu import append, attend, cache as described
 
 TAU = torch.tensor(0.0)
@@ -101,3 +101,20 @@ def test_rows_without_scores_under_a_gamma_that_fp32_does_not_hold():
     assert cached_attention(k, cache, 0, torch.tensor(1e9), gamma=1e-50).eq(0).all()
     want = cached_attention(k, cache, 0, TAU, gamma=None)
     assert torch.equal(cached_attention(k, cache, 0, TAU, gamma=1e-50), want)
+
+
+def test_whole_numbers_of_more_than_32_bits():
+    cache, k, far = new(), torch.randn(2, 2, 5, 20), 1 << 32
+    with pytest.raises(ValueError, match="beside"):
+        cache.append(k, k, torch.tensor([0, far + 3]))
+    with pytest.raises(ValueError, match="beside"):
+        cached_attention(k, cache, torch.tensor([0, -far]), TAU)
+    cache.append(k, k, 0, counts=torch.tensor([far + 2, 5]))  # more than the call's: all of them
+    assert cache.read(torch.tensor([0, far]), 5)[0][0].any(-1).all() and not cache.read(torch.tensor([0, far]), 5)[0][1].any()
+    z, u = torch.randn(3, 50), torch.rand(3)
+    every = sample_tokens(z, u).tolist()
+    assert sample_tokens(z, u, top_k=torch.tensor([far + 1, far, 1 << 62])).tolist() == every
+    assert sample_tokens(z, u, top_k=1 << 70).tolist() == every and sample_tokens(z, u, top_k=50.0).tolist() == every
+    for k in (0.5, 2.5, float("inf")):
+        with pytest.raises(ValueError, match="top_k"):
+            sample_tokens(z, u, top_k=k)

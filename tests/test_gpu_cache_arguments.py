@@ -3,7 +3,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from paper_01_anti_decoy_pnfirtau_amd import KVCache, cached_attention
+from paper_01_anti_decoy_pnfirtau_amd import KVCache, cached_attention, sample_tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +53,18 @@ def test_rows_without_scores_under_a_gamma_that_fp32_does_not_hold(dev, dtype, N
     assert cached_attention(k, cache, 0, tau(1e9), gamma=1e-50).eq(0).all()
     want = cached_attention(k, cache, 0, tau(0.0), gamma=None)
     assert torch.equal(cached_attention(k, cache, 0, tau(0.0), gamma=1e-50), want) and want.isfinite().all()
+
+
+def test_whole_numbers_of_more_than_32_bits(dev):
+    """Sequences so far away do not fit their pages; a top_k so large keeps all."""
+    cache, far = new(dev), 1 << 32
+    k = torch.randn(2, 2, 5, 20, device=dev)
+    cache.append(k, k, torch.tensor([0, far + 3], device=dev), counts=torch.tensor([far + 2, 5], device=dev))
+    got = cache.read(0, 64)[0]
+    assert got[0, :, :5].any(-1).all() and not got[1].any()
+    o = cached_attention(k, cache, torch.tensor([0, -far], device=dev), torch.zeros(1, device=dev))
+    assert o[0].isfinite().all() and o[1].isnan().all()
+    z, u = torch.randn(3, 50, device=dev), torch.rand(3, device=dev)
+    every = sample_tokens(z, u).tolist()
+    assert sample_tokens(z, u, top_k=torch.tensor([far + 1, far, 1 << 62], device=dev)).tolist() == every
+    assert sample_tokens(z, u, top_k=1 << 70).tolist() == every
