@@ -292,9 +292,9 @@ def _checked(cache: KVCache, what: str, x: torch.Tensor, start, counts) -> tuple
         raise ValueError(f"{what}: a tensor on {x.device}, the cache on {cache.k.device}")
     start = torch.as_tensor(start).long().expand(B)
     n = torch.full((B,), x.shape[2]) if counts is None else counts.long().clamp(0, x.shape[2])
-    if (start < 0).any() or (start + n > cache.capacity).any():
+    if ((n > 0) & ((start < 0) | (start + n > cache.capacity))).any():
         raise ValueError(f"{what}: tokens beside the {cache.capacity} that a sequence's pages hold")
-    return start, n
+    return torch.where(n > 0, start, 0), n  # of no tokens: anywhere
 
 
 def _at(cache: KVCache, pos: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -385,7 +385,7 @@ def _attend(q, cache: KVCache, start, tau, scale, gamma, causal, counts) -> torc
     B, Hq, N, d = q.shape
     start, n = _checked(cache, "cached_attention", q, start, counts)
     o = q.new_zeros(B, N, Hq, d).transpose(1, 2)
-    if not q.numel():
+    if not q.numel() or not n.any():
         return o
     H, L = cache.raw.shape[1], int((start + n).max())
     k, v = (t.repeat_interleave(Hq // H, 1) for t in _read(cache, 0, L, torch.float32))

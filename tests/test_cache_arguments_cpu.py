@@ -118,3 +118,22 @@ def test_whole_numbers_of_more_than_32_bits():
     for k in (0.5, 2.5, float("inf")):
         with pytest.raises(ValueError, match="top_k"):
             sample_tokens(z, u, top_k=k)
+
+
+@pytest.mark.parametrize("at", [0, -9, 64, 1 << 30])
+def test_sequences_without_tokens_may_be_anywhere(at):
+    """Of an empty cache, too, and of pages that do not exist; their rows are zeros."""
+    cache, k = new(), torch.randn(2, 2, 5, 20)
+    none, some = torch.tensor([0, 0]), torch.tensor([0, 5])
+    cache.table[0, :] = -1
+    start = torch.tensor([at, 0])
+    cache.append(k, k, start, counts=none)
+    assert cached_attention(k, cache, start, TAU, counts=none).eq(0).all() and not cache.k.any()
+    cache.append(k, k, start, counts=some)
+    for causal in (True, False):
+        o = cached_attention(k, cache, start, TAU, counts=some, causal_mask=causal)
+        alone = new(1)
+        alone.append(k[1:], k[1:], 0)
+        assert o[0].eq(0).all() and torch.equal(o[1:], cached_attention(k[1:], alone, 0, TAU, causal_mask=causal))
+    with pytest.raises(ValueError):
+        cached_attention(k, cache, start, TAU, counts=torch.tensor([1, 5]))
