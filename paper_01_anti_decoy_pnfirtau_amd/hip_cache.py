@@ -426,9 +426,11 @@ def _sample(z, u, temperature, top_k, top_p, min_p, temperature_each, top_k_each
     w, order = torch.nan_to_num(w).gather(1, (by := z.sort(dim=1, descending=True, stable=True).indices)), by
     w = torch.where(torch.arange(V) < k, w, 0.0)
     before = w.cumsum(1) - w
-    keep = (w >= least) & ((p >= 1) | (before < p * w.sum(1, keepdim=True)))
+    keep = ~(w < least) & (~(p < 1) | (before < p * w.sum(1, keepdim=True)))  # a NaN cuts nothing off
     keep[:, 0] = True
     c = torch.zeros_like(w).scatter_(1, order, torch.where(keep, w, 0.0)).cumsum(1)
-    token = (c <= u.double()[:, None] * c[:, -1:]).sum(1).clamp(max=V - 1)
+    at = torch.nan_to_num(u.double(), nan=0.0).clamp(0, 1)[:, None] * c[:, -1:]
+    last = (c < c[:, -1:]).sum(1)  # the last one that is kept: u may be 1, rounded from more bits
+    token = (c <= at).sum(1).minimum(last)
     lost = z.isnan().any(1) | (z == -torch.inf).all(1)
     return torch.where(lost, -1, token)

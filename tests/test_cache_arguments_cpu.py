@@ -137,3 +137,15 @@ def test_sequences_without_tokens_may_be_anywhere(at):
         assert o[0].eq(0).all() and torch.equal(o[1:], cached_attention(k[1:], alone, 0, TAU, causal_mask=causal))
     with pytest.raises(ValueError):
         cached_attention(k, cache, start, TAU, counts=torch.tensor([1, 5]))
+
+
+def test_random_numbers_and_settings_beside_their_range():
+    """A token that is not kept is never drawn; what is no number is 0, or cuts nothing off."""
+    z = torch.tensor([[-torch.inf, 1.0, 3.0, 2.0, -torch.inf, 0.0]]).repeat(5, 1)
+    u = torch.tensor([1.0, 7.0, -0.5, float("nan"), 0.0])
+    assert sample_tokens(z, u, top_k=2).tolist() == [3, 3, 2, 2, 2]
+    assert sample_tokens(z, u).tolist() == [5, 5, 1, 1, 1]
+    nan, u = torch.full((5,), float("nan")), torch.tensor([0.05, 0.3, 0.6, 0.9, 0.99])
+    every = sample_tokens(z, u).tolist()
+    assert sample_tokens(z, u, top_p=nan).tolist() == every and sample_tokens(z, u, min_p=nan).tolist() == every
+    assert sample_tokens(z, u, temperature=nan).tolist() == [2] * 5

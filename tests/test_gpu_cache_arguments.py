@@ -68,3 +68,16 @@ def test_whole_numbers_of_more_than_32_bits(dev):
     every = sample_tokens(z, u).tolist()
     assert sample_tokens(z, u, top_k=torch.tensor([far + 1, far, 1 << 62], device=dev)).tolist() == every
     assert sample_tokens(z, u, top_k=1 << 70).tolist() == every
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_random_numbers_and_settings_beside_their_range(dev, dtype):
+    """As on CPU tensors."""
+    z = torch.tensor([[-torch.inf, 1.0, 3.0, 2.0, -torch.inf, 0.0]], device=dev, dtype=dtype).repeat(5, 1)
+    u = torch.tensor([1.0, 7.0, -0.5, float("nan"), 0.0], device=dev)
+    assert sample_tokens(z, u, top_k=2).tolist() == [3, 3, 2, 2, 2]
+    assert sample_tokens(z, u).tolist() == [5, 5, 1, 1, 1]
+    nan, u = torch.full((5,), float("nan"), device=dev), torch.tensor([0.05, 0.3, 0.6, 0.9, 0.99], device=dev)
+    every = sample_tokens(z, u).tolist()
+    assert sample_tokens(z, u, top_p=nan).tolist() == every and sample_tokens(z, u, min_p=nan).tolist() == every
+    assert sample_tokens(z, u, temperature=nan).tolist() == [2] * 5
