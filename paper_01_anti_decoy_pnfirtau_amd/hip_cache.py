@@ -383,6 +383,9 @@ def _read(cache: KVCache, first, count: int, dtype: torch.dtype) -> tuple[torch.
 
 def _attend(q, cache: KVCache, start, tau, scale, gamma, causal, counts) -> torch.Tensor:
     B, Hq, N, d = q.shape
+    if tau.numel() != 1:
+        raise ValueError(f"cached_attention: score_tau of shape {tuple(tau.shape)}, not one value")
+    tau = tau.reshape(())
     start, n = _checked(cache, "cached_attention", q, start, counts)
     o = q.new_zeros(B, N, Hq, d).transpose(1, 2)
     if not q.numel() or not n.any():

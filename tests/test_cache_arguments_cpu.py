@@ -149,3 +149,13 @@ def test_random_numbers_and_settings_beside_their_range():
     every = sample_tokens(z, u).tolist()
     assert sample_tokens(z, u, top_p=nan).tolist() == every and sample_tokens(z, u, min_p=nan).tolist() == every
     assert sample_tokens(z, u, temperature=nan).tolist() == [2] * 5
+
+
+def test_tau_is_one_value():
+    cache, k = new(), torch.randn(2, 2, 5, 20)
+    cache.append(k, k, 0)
+    want = cached_attention(k, cache, 0, TAU + 0.3)
+    assert torch.equal(cached_attention(k, cache, 0, torch.full((1, 1, 1, 1, 1), 0.3)), want)
+    for shape in (5, 2, 0, (2, 1, 1)):
+        with pytest.raises(ValueError, match="score_tau"):
+            cached_attention(k, cache, 0, torch.full((shape,) if isinstance(shape, int) else shape, 0.3))
