@@ -254,15 +254,16 @@ class GraphedStep:
         if any(len(st) for st in opt.state.values()):
             raise ValueError("GraphedStep: the optimizer already has state")
         saved = [t.detach().clone() for t in list(model.parameters()) + list(model.buffers())]
-        side = torch.cuda.Stream()
-        side.wait_stream(torch.cuda.current_stream())
-        with torch.cuda.stream(side):
-            for _ in range(warmup):
-                self._step()
-        torch.cuda.current_stream().wait_stream(side)
-        self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
-            self.loss = self._step()
+        with torch.cuda.device(x.device):  # a capture is of the current device's streams
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                for _ in range(warmup):
+                    self._step()
+            torch.cuda.current_stream().wait_stream(side)
+            self.graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(self.graph):
+                self.loss = self._step()
         # capture records the step without running it: undo the warm-up steps in place, so
         # the captured addresses stay the live ones
         with torch.no_grad():
@@ -366,21 +367,25 @@ class Decoder:
             self._step()
             return self.token
         if self._captured is None:
-            # the warm-up runs on what a step overwrites: the caches' next token, written again by the replay, and state
-            # that is put back
-            saved = self.rows.clone(), self.start.clone()
-            side = torch.cuda.Stream(self.u.device)
-            side.wait_stream(torch.cuda.current_stream(self.u.device))
-            with torch.cuda.stream(side):
-                self._step()
-                self.rows.copy_(saved[0]), self.start.copy_(saved[1])
-            torch.cuda.current_stream(self.u.device).wait_stream(side)
-            graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph):
-                self._step()
-            self._captured = graph
+            with torch.cuda.device(self.u.device):  # a capture is of the current device's streams
+                self._capture()
         self._captured.replay()
         return self.token
+
+    def _capture(self) -> None:
+        # the warm-up runs on what a step overwrites: the caches' next token, written again by the replay, and state
+        # that is put back
+        saved = self.rows.clone(), self.start.clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            self._step()
+            self.rows.copy_(saved[0]), self.start.copy_(saved[1])
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            self._step()
+        self._captured = graph
 
 
 def generate(model: WikiLM, prompt: torch.Tensor, max_new: int, lengths: torch.Tensor | None = None,
