@@ -387,7 +387,8 @@ int pnfx_xent_bwd(const float* dloss, const void* x, int64_t x_rs, const void* w
  * [B, Hq, N, d] (Hq a multiple of H: query head h reads key head h / (Hq / H)), over the sequence's keys 0 .. start +
  * count - 1, for causal != 0 those up to the token's own.  Rows past a sequence's count are zeros.  Sequences that
  * append leaves alone, and rows that see a page which the table does not name, are NaN.  Workspace: 16-byte aligned,
- * as large as pnfx_cached_attn_workspace_size says.  Bitwise repeatable.
+ * as large as pnfx_cached_attn_workspace_size says.  Bitwise repeatable for the same arguments: all sequences' lengths and
+ * the capacity go into how the keys are cut and summed.
  */
 #define PNFX_CACHE_MAX_HEAD 256
 typedef struct pnfx_cache {
