@@ -420,7 +420,8 @@ int pnfx_cached_attn(const pnfx_cache* cache, const void* q, int64_t qsb, int64_
  * first, by index, at which the running weight of the kept ones is above u times their whole weight.  temperature <= 0:
  * the first of the order.  Settings of one row each (`*_each`, on the device) take the place of the others where they are
  * not null.  -infinity is never drawn; a row with a NaN, or of nothing else, gets -1.  Weights are taken in 64 bits and
- * summed in 64-bit fixed point, so that results do not depend on any order.  V <= 2^20.
+ * summed in 64-bit fixed point, the largest as 2^S with S = min(50, 62 - ceil(log2 V)), so that results do not depend on any
+ * order; a border is off by V * 2^-(S+1) of the largest weight at most.  V <= 2^20.
  */
 typedef struct pnfx_sampling {
   double temperature, top_p, min_p;

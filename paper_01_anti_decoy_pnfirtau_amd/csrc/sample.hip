@@ -5,10 +5,10 @@
 // threshold logit, and of the tokens that equal it those up to an index.  The token is the first by index at which
 // the kept ones' running weight passes u times their whole weight.
 //
-// One workgroup of 16 waves has a row and goes over it several times, the next chunks on their way (a row held in
-// registers gained nothing: 37 us either way for 33278 bf16 logits): the maximum; for top-k, the threshold by a
-// histogram of max z - z, then of the logits' bits within its bin; for top-p, the same with the weights' sums; then the
-// sum of each wave's 64 chunks, in the order of the row, the chunks in which u falls, and the token in them.
+// One workgroup of 16 waves has a row and goes over it several times, the next chunks on their way: the maximum; for
+// top-k, the threshold by a histogram of max z - z, then of the logits' bits within its bin; for top-p, the same with the
+// weights' sums; then the sum of each wave's 64 chunks, in the order of the row, the chunks in which u falls, and the
+// token in them.
 //
 // bf16 rows have few different logits: with the magnitudes from 2^-32 to 2^16, 12289 of them.  Their weights are a table
 // in LDS, one exponential for each that occurs, and one histogram of them settles both thresholds and the maximum: 256 rows of
@@ -16,9 +16,12 @@
 // by temperature alone 12 either way.
 //
 // Integers decide: weights are 64-bit fixed point, 2^S for the largest, so that sums are exact and the same in any
-// order (the histogram's atomics among them), and a token differs from the real numbers' only where u falls within about
-// 2^-46 of a border.  For that the exponential is a table of 256 steps an octave times a cubic, in fp64 (1.4e-13,
-// relative): one of fp32 is off by enough to move some border past u every few hundred rows of 10^5 tokens.
+// order (the histogram's atomics among them).  S is 50, or 62 less the bits of V: 45 for 131072 tokens, 42 for 2^20.  The
+// exponential is a table of 256 steps an octave times a cubic, in fp64 (1.4e-13, relative), and a weight is rounded by half
+// a unit at most, so a border is off by no more than V 2^-(S+1) of the largest weight and 1.4e-13 of its own sum: 2^-29 of
+// the largest in all for 131072 tokens, 2^-23 for 2^20, if every rounding falls to one side.  A token differs from the real
+// numbers' only where u times the kept weight is as near to a border.  (An fp32 exponential moves some border past u every few
+// hundred rows of 10^5 tokens.)
 #include "pnfx_common.h"
 
 #include <cmath>

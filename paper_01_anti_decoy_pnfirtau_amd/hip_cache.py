@@ -248,9 +248,10 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: float | to
     The token is the first, by index, at which the running weight of the kept ones is above u times their whole weight.
     temperature 0 takes the first of the order.  Each setting is one value or a tensor [...] of one for each row.
 
-    Minus infinity is never drawn; a row that holds a NaN, or nothing else, gets -1.  Weights are taken in 64 bits and
-    summed as 64-bit fixed point, of which the largest has 2^42 to 2^50: the result depends on no order of sums, and a
-    token of a smaller part is not drawn.  V <= 2^20."""
+    Minus infinity is never drawn; a row that holds a NaN, or nothing else, gets -1.  GPU: weights are taken in 64 bits
+    (1.4e-13) and summed as 64-bit fixed point, the largest as 2^S with S = min(50, 62 - ceil(log2 V)): the result depends on
+    no order of sums, a border is off by V 2^-(S+1) of the largest weight at most, and a token of less than half a unit is
+    not drawn.  A u beside [0, 1) is taken as the nearest, NaN as 0.  V <= 2^20."""
     V = logits.shape[-1] if logits.dim() else 0
     if not logits.dim() or not 1 <= V <= MAX_VOCAB:
         raise ValueError(f"sample_tokens: logits {tuple(logits.shape)}: rows of 1 to {MAX_VOCAB}")
