@@ -50,8 +50,8 @@ def _no_gradient(what: str, *tensors: torch.Tensor | None) -> None:
 
 def _int32(x: torch.Tensor) -> torch.Tensor:
     """Whole numbers in 32 bits: those beyond become the first or last of them, which no sequence or row has either."""
-    if x.dtype in (torch.int32, torch.int16, torch.int8, torch.uint8):
-        return x.to(torch.int32)
+    if x.dtype == torch.int32:
+        return x
     return x.to(torch.int64).clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)
 
 
