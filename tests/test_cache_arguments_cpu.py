@@ -159,3 +159,13 @@ def test_tau_is_one_value():
     for shape in (5, 2, 0, (2, 1, 1)):
         with pytest.raises(ValueError, match="score_tau"):
             cached_attention(k, cache, 0, torch.full((shape,) if isinstance(shape, int) else shape, 0.3))
+
+
+def test_a_single_row_of_logits():
+    z, u = torch.randn(40), torch.rand(1)
+    want = sample_tokens(z[None], u, top_k=7, temperature=0.5)
+    got = sample_tokens(z, u[0], top_k=torch.tensor(7), temperature=torch.tensor(0.5))
+    assert got.shape == () and got == want[0]
+    many = z.expand(5, 40)
+    assert sample_tokens(many, u.expand(5), top_k=7, temperature=0.5).tolist() == want.tolist() * 5
+    assert sample_tokens(many.t().contiguous().t(), u.expand(5), top_k=7, temperature=0.5).tolist() == want.tolist() * 5

@@ -81,3 +81,13 @@ def test_random_numbers_and_settings_beside_their_range(dev, dtype):
     every = sample_tokens(z, u).tolist()
     assert sample_tokens(z, u, top_p=nan).tolist() == every and sample_tokens(z, u, min_p=nan).tolist() == every
     assert sample_tokens(z, u, temperature=nan).tolist() == [2] * 5
+
+
+def test_a_single_row_of_logits(dev):
+    z, u = torch.randn(40, device=dev), torch.rand(1, device=dev)
+    want = sample_tokens(z[None], u, top_k=7, temperature=0.5)
+    got = sample_tokens(z, u[0], top_k=torch.tensor(7, device=dev), temperature=torch.tensor(0.5, device=dev))
+    assert got.shape == () and got == want[0]
+    many = z.expand(5, 40)
+    assert sample_tokens(many, u.expand(5), top_k=7, temperature=0.5).tolist() == want.tolist() * 5
+    assert sample_tokens(many.t().contiguous().t(), u.expand(5), top_k=7, temperature=0.5).tolist() == want.tolist() * 5
