@@ -64,11 +64,23 @@ struct AttnPlan {
   int64_t bytes() const { return header_bytes + acc_bytes + stat_bytes; }
 };
 
-// Waves of a kernel that a SIMD holds, by its registers: the card has 1024 times as many slots.
+// Waves of a kernel that a SIMD holds, by its registers: the card has 1024 times as many slots.  In us with 1, 2, 3 and 4
+// waves, the rule's own in brackets; one: a token of 64 sequences and 8 heads behind 500 MB of cache (NT = 1), rows: 100
+// tokens of 8 sequences and 16 heads behind 4096 (NT = 2 up to 128 columns, else 1):
+//   bf16   16, one 276 200 170 [161], rows 50 39 40 [42];   32, 162 100 84 [85], 54 41 [41] 52;   64, 110 85 [86] 86,
+//   60 [50] 61 202;   80, 126 [97] 148 265, [77] 72 250 406;   128, 106 [90] 258 371, [94] 282 637 857;   144, [101] 135 301
+//   424, [130] 136 521 774;   256, [94] 305 420 630, [216] 921 1390 2197
+//   fp32   16, 336 231 202 [193], 65 56 57 [81];   32, 162 125 110 [108], 71 [60] 61 100;   64, 116 [90] 91 126, 88 [75] 139 355;
+//   80, 122 [103] 246 401, [110] 195 462 729;   112, 111 [142] 331 474, [134] 359 718 1080;   128, 100 [153] 329 470,
+//   [145] 444 924 1253;   256, [123] 372 549 735, [310] 1101 2004 2423
+// The rule counts bf16's registers.  fp32's operands take three times as many: heads of 112 and 128 spill 80 and 110 of them
+// with two waves (one token) where one wave would be faster, 16 columns 133 with four (many rows).
 constexpr int resident(int bytes, int D, int NT) {
   return D * NT <= 32 ? 4 : bytes == 2 && D * NT <= 64 ? 3 : D * NT <= 128 ? 2 : 1;
 }
-// The same of the kernel whose waves share their keys: 256 times as many workgroups.
+// The same of the kernel whose waves share their keys: 256 times as many workgroups.  512 query tokens behind 7680, 2
+// sequences of 16 heads, with 1, 2 and 3 (us): heads of 80 164, 107, 116; 96 160, 108, 131; 112 189, 117, 218; 128 201, 120,
+// 233, although 32 and 109 registers spill with two in heads of 112 and 128, none with one.
 constexpr int RESIDENT_SHARED = 2;
 
 // The kernels, by the type of the queries and the head size in the cache.
@@ -574,7 +586,9 @@ struct Piece {
 // Pieces of units.  A sequence's tiles are cut alike for all its units (`each` of them: heads and row tiles), into as many
 // equal pieces as give every slot of the card its share; neighbouring items then have the same tokens
 // of neighbouring heads, which lie side by side in the pages: 64 sequences of up to 8192 tokens of random length,
-// 16 heads of 64, take 106 us, with shares cut through the line of all units 127.
+// 16 heads of 64, one token each, take 106 us, with shares cut through the line of all units 127.  Of many rows and few
+// sequences this is coarse (4 sequences of 512 query tokens and 16 heads of 64: 256 units each, for 2048 slots): behind 7680
+// tokens each a billion pairs take 0.50 ms, behind random numbers of up to 7680 0.63 to 0.87.
 __device__ __forceinline__ Piece piece_of(const AttnArgs& a, int lane, int each, int most_items) {
   const auto tiles_of_sequence = [&](int b) {
     const int64_t start = a.span.first(b);
