@@ -16,7 +16,7 @@
 // 16384 rows 29 us (93), of which summing the partial tiles takes 6; 256 x 256 17 (93); 768 x 256
 // over 65536 rows 66 (240), 390 TFLOP/s.  Bound by the partial tiles' traffic at few rows and by the
 // transposing LDS reads (one per two MFMAs and operand) at many; where a weight has tiles enough to
-// fill the chip the library's larger tiles are faster (3072 x 1024 over 65536 rows 1272 against 492).
+// fill the chip the library's larger tiles are faster (3 * 1024 x 1024 over 65536 rows 1272 against 492).
 #include "tiles_bf16.h"
 
 namespace pnfx {

@@ -94,7 +94,7 @@ def split_wgrad_applies(rows: int, out_features: int, in_features: int, wide: bo
     one workgroup per output tile leaves the chip idle.  Measured on MI355X (us, this kernel against
     the library product and its cast to fp32): 768x256 over 16384 rows 29 / 93, over 2048 12 / 17,
     over 512 9.8 / 10.0; 1536x512 over 8192 42 / 55, over 2048 24 / 19; 768x768 over 8192 36 / 51,
-    over 2048 22 / 18; 1024x1024 over 8192 34 / 56; 2304x768 over 16384 127 / 124; 3072x1024 over
+    over 2048 22 / 18; 1024x1024 over 8192 34 / 56; 2304x768 over 16384 127 / 124; (3 * 1024)x1024 over
     65536 1272 / 492.  A bf16 weight (not ``wide``), whose library product needs no cast, from 768
     rows on (64x64 over 300 rows 9.2 / 6.9, over 512 7.8 / 7.5, 192x64 over 777 9.1 / 15.5).  No side
     below 32, a quarter of the kernel's tile (65536x8 over 8192 rows 1327 / 180, 24x8 over 1024 7.4 /
