@@ -19,7 +19,8 @@
 // The powers are taken of u 2^-e with one e a row: 0 or, where a row's first scores are below 1/4, less; raised (and the
 // sums scaled, exactly) when a score passes 2 2^e.  So weights stay below 2^10, and those down to 2^-100 of the
 // largest are within fp32; values are summed with them as they are, so that 2^117 over the number of keys is the largest
-// that cannot overflow.  With 2^8 in place of 2 it would be 2^47, and no faster.
+// that cannot overflow.  With 2^8 in place of 2 it would be 2^47, and no faster.  e is -60 at least, for which keys of up to
+// 2^60 (their scale times 2^60) and scores of up to 2^67 stay within fp32.
 //
 // bf16 queries: the weights are rounded to bf16 for the product and the same rounded values are summed, as the dense
 // kernels do.  fp32 queries: queries and weights as three bf16 parts each (24 bits), keys and values are exact in one.

@@ -217,9 +217,10 @@ def cached_attention(q: torch.Tensor, cache: KVCache, start: int | torch.Tensor,
     ``counts`` are zeros.  scale defaults to 1/sqrt(head_dim).
 
     Keys and values are what their bytes stand for, exactly; scores and sums are fp32.  bf16 queries: the weights are
-    rounded to bf16 (2^-9 at most, relative) for their product with the values and normalised by the sum of the rounded
+    rounded to bf16 (2^-8 at most, relative) for their product with the values and normalised by the sum of the rounded
     ones; fp32 queries: 24 bits throughout.  They are normalised last: values beyond 2^117 over the number of keys may
-    overflow.  Bitwise repeatable for the same arguments; a sequence's last bits may be others beside other sequences, or
+    overflow.  On the GPU a row whose first scores are far below 1 takes its powers in their unit, down to 2^-60: keys beyond
+    2^60 or scores beyond 2^67 further on may then give NaN.  Bitwise repeatable for the same arguments; a sequence's last bits may be others beside other sequences, or
     in a cache of another capacity, as all lengths go into how the keys are cut and summed."""
     if q.dim() != 4 or q.shape[3] != cache.raw.shape[3]:
         raise ValueError(f"cached_attention: q {tuple(q.shape)}, the cache's head size is {cache.raw.shape[3]}")
